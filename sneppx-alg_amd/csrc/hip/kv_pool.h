@@ -1,0 +1,66 @@
+// kv_pool.h - a paged key-value pool and the rows' block tables as the kernels
+// see them (see include/sneppx_kv.h for the layout).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sneppx_kv.h"
+
+namespace snx {
+
+struct KVPool {
+    uint8_t *k, *v;
+    float *ks, *vs, *weights;
+    int32_t* positions;
+    const int32_t* tables;
+    uint32_t width, pages, heads, page_size;
+    uint32_t mul, shift;       // slot / page_size = slot * mul >> shift
+    uint32_t dim;
+
+    // Slot / page_size for slots below 2^31: with 2^(l-1) < d <= 2^l and
+    // mul = ceil(2^(31+l) / d), slot * mul / 2^(31+l) is the quotient plus less
+    // than slot * 2^l / (d 2^(31+l)) < 1 / d.
+    __device__ __forceinline__ uint32_t page_of(uint32_t slot) const {
+        return (uint32_t)(((uint64_t)slot * mul) >> shift);
+    }
+
+    // Row of the pool (of head_dim values, and of each plane) that holds slot
+    // `slot` of head h in row b's pages; false where that page is not there.
+    __device__ __forceinline__ bool row(uint32_t b, uint32_t h, uint32_t slot, uint32_t& r) const {
+        const uint32_t e = page_of(slot);
+        const uint32_t page = (uint32_t)tables[(size_t)b * width + e];
+        r = (page * heads + h) * page_size + (slot - e * page_size);
+        return page < pages;
+    }
+};
+
+inline KVPool kv_pool(const SNEPPXKVCache* c, const int32_t* tables, size_t width) {
+    KVPool p;
+    p.k = static_cast<uint8_t*>(c->k);
+    p.v = static_cast<uint8_t*>(c->v);
+    p.ks = c->k_scales;
+    p.vs = c->v_scales;
+    p.weights = c->weights;
+    p.positions = c->positions;
+    p.tables = tables;
+    p.width = (uint32_t)width;
+    p.pages = (uint32_t)c->pages;
+    p.heads = (uint32_t)c->kv_heads;
+    p.page_size = (uint32_t)c->page_size;
+    p.dim = (uint32_t)c->head_dim;
+    uint32_t l = 0;
+    while (((uint64_t)1 << l) < c->page_size) l++;
+    p.shift = 31 + l;
+    p.mul = (uint32_t)((((uint64_t)1 << p.shift) + c->page_size - 1) / c->page_size);
+    return p;
+}
+
+// a row's slots in use, of at most `most`
+__device__ __forceinline__ uint32_t kv_length(const int32_t* lengths, uint32_t b, uint32_t most) {
+    const int32_t n = lengths[b];
+    return n < 0 ? 0u : (uint32_t)n < most ? (uint32_t)n : most;
+}
+
+}  // namespace snx

@@ -30,6 +30,7 @@ LIB_PATH = os.path.join(HERE, "libsneppx_quant.so")
 SNEPPX_FLOAT32 = 0
 SNEPPX_FLOAT16 = 2
 SNEPPX_BFLOAT16 = 3
+SNEPPX_INT8 = 8
 
 _f32p = np.ctypeslib.ndpointer(np.float32, flags="C")
 _i8p = np.ctypeslib.ndpointer(np.int8, flags="C")
@@ -141,6 +142,11 @@ EXPORTS = {
     "SNEPPX_qlinear_mx_gemm_bs": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _sz, _sz, _sz,
                                             _vp]),
     "SNEPPX_mx_to_mfma": (C.c_int, [_vp, _vp, _vp, _vp, _sz, _sz, C.c_int, _vp, _vp]),
+    # paged key-value cache (include/sneppx_kv.h)
+    "SNEPPX_kv_append": (C.c_int, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _sz, _vp]),
+    "SNEPPX_kv_attention": (C.c_int, [_vp, _vp, _sz, _vp, _sz, C.c_int, _vp, _sz, _vp, _sz, _sz, _sz, C.c_float,
+                                      C.c_int, _vp]),
+    "SNEPPX_kv_evict": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
     # thin HIP ABI
     "snx_hip_device_count": (C.c_int, [C.POINTER(C.c_int)]),
     "snx_hip_event_create": (C.c_int, [C.POINTER(_vp)]),
@@ -594,6 +600,24 @@ class Library:
             _ptr(rounded), self._stream(stream)), "mx_to_mfma")
         return out_p, out_s, rounded
 
+    # ---------------- paged key-value cache ----------------------------------
+    def kv_cache(self, pages, page_size, kv_heads, head_dim, dtype="bf16", weights=False, positions=False,
+                 device="cuda"):
+        """A KVCache of `pages` pages in new memory ("bf16" or "int8");
+        weights / positions: with the planes that eviction goes by."""
+        if dtype not in ("bf16", "int8"):
+            raise ValueError(f"dtype must be 'bf16' or 'int8', got {dtype!r}")
+        shape, planes = (pages, kv_heads, page_size, head_dim), (pages, kv_heads, page_size)
+        k, v = (torch.empty(shape, dtype=torch.int8 if dtype == "int8" else torch.bfloat16, device=device)
+                for _ in range(2))
+        ks, vs = (torch.zeros(planes, device=device) if dtype == "int8" else None for _ in range(2))
+        return KVCache(self, k, v, ks, vs, torch.zeros(planes, device=device) if weights else None,
+                       torch.zeros(planes, dtype=torch.int32, device=device) if positions else None)
+
+    def kv_cache_from(self, k, v, k_scales=None, v_scales=None, weights=None, positions=None):
+        """A KVCache over tensors that the caller has (layouts of include/sneppx_kv.h)."""
+        return KVCache(self, k, v, k_scales, v_scales, weights, positions)
+
     # ---------------- HIP events on an explicit stream ----------------------
     def event(self):
         e = C.c_void_p()
@@ -761,6 +785,111 @@ class QStoreWriter:
         h, self.h = self.h, None
         if h:
             self.L.check(self.L.fn["SNEPPX_qstore_writer_close"](h), "qstore_writer_close")
+
+
+class _KVCacheStruct(C.Structure):
+    """SNEPPXKVCache (include/sneppx_kv.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scales", _vp), ("v_scales", _vp), ("weights", _vp), ("positions", _vp),
+                ("dtype", C.c_int), ("pages", _sz), ("page_size", _sz), ("kv_heads", _sz), ("head_dim", _sz)]
+
+
+class KVCache:
+    """A paged key-value pool (include/sneppx_kv.h): k, v [pages, kv_heads,
+    page_size, head_dim] in bf16 or int8; k_scales, v_scales (int8), weights
+    (fp32) and positions (int32) [pages, kv_heads, page_size].
+
+    Calls take the rows' block tables (int32 [rows, width]) and lengths (int32
+    [rows], the call's new tokens included) on the device, and run on torch's
+    current stream unless one is given."""
+
+    def __init__(self, lib, k, v, k_scales=None, v_scales=None, weights=None, positions=None):
+        if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in (torch.bfloat16, torch.int8):
+            raise ValueError("k must be a bf16 or int8 tensor [pages, kv_heads, page_size, head_dim]")
+        self.L, self.device = lib, k.device
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        i8 = k.dtype == torch.int8
+        planes = k.shape[:3]
+        for t, name, dtype, shape, needed in (
+                (k, "k", k.dtype, k.shape, True), (v, "v", k.dtype, k.shape, True),
+                (k_scales, "k_scales", torch.float32, planes, i8), (v_scales, "v_scales", torch.float32, planes, i8),
+                (weights, "weights", torch.float32, planes, False),
+                (positions, "positions", torch.int32, planes, False)):
+            if t is None and not needed:
+                continue
+            self._check(t, name, dtype, shape)
+        if not i8 and (k_scales is not None or v_scales is not None):
+            raise ValueError("a bf16 cache has no scales")
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.weights, self.positions = weights, positions
+        self._c = _KVCacheStruct(*(None if t is None else t.data_ptr()
+                                   for t in (k, v, k_scales, v_scales, weights, positions)),
+                                 SNEPPX_INT8 if i8 else SNEPPX_BFLOAT16, *(k.shape[i] for i in (0, 2, 1, 3)))
+        self._p = C.cast(C.pointer(self._c), _vp)
+        self._append, self._attention, self._evict = (
+            lib.fn[f"SNEPPX_kv_{n}"] for n in ("append", "attention", "evict"))
+
+    def _check(self, t, name, dtype, shape):
+        """A contiguous tensor of this type and shape on the cache's device."""
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != self.device \
+                or not t.is_contiguous():
+            got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
+            raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {self.device}, got {got}")
+        return t.data_ptr()
+
+    def _rows(self, t, name, heads, dtypes):
+        """[n, heads, head_dim] whose rows are contiguous; returns the row stride."""
+        if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != self.device or t.dim() != 3 \
+                or t.shape[2] != self.head_dim or heads and t.shape[1] != heads \
+                or t.stride(2) != 1 or t.shape[1] > 1 and t.stride(1) != self.head_dim:
+            got = f"{t.dtype} {tuple(t.shape)} (strides {t.stride()}) on {t.device}" \
+                if isinstance(t, torch.Tensor) else repr(t)
+            raise ValueError(f"{name} must be [n, {heads or 'q_heads'}, {self.head_dim}] with contiguous rows, "
+                             f"{' or '.join(map(str, dtypes))}, on {self.device}; got {got}")
+        return t.stride(0)
+
+    def _tables(self, tables, lengths):
+        if not isinstance(tables, torch.Tensor) or tables.dim() != 2:
+            raise ValueError("tables must be an int32 tensor [rows, width]")
+        n, width = tables.shape
+        return self._check(tables, "tables", torch.int32, (n, width)), width, \
+            self._check(lengths, "lengths", torch.int32, (n,)), n
+
+    def append(self, k, v, tables, lengths, next_pos=None, starts=None, k_stored=None, v_stored=None, stream=None):
+        """SNEPPX_kv_append: k, v bf16 [tokens, kv_heads, head_dim], slices of
+        wider rows among them; starts int32 [rows + 1], without it one token
+        per row; k_stored, v_stored bf16 [tokens, kv_heads, head_dim]."""
+        ks, vs = (self._rows(t, n, self.kv_heads, (torch.bfloat16,)) for t, n in ((k, "k"), (v, "v")))
+        tb, width, ln, n = self._tables(tables, lengths)
+        if v.shape != k.shape:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        np_ = None if next_pos is None else self._check(next_pos, "next_pos", torch.int32, (n,))
+        st = None if starts is None else self._check(starts, "starts", torch.int32, (n + 1,))
+        ko, vo = (None if t is None else self._check(t, name, torch.bfloat16, k.shape)
+                  for t, name in ((k_stored, "k_stored"), (v_stored, "v_stored")))
+        self.L.check(self._append(self._p, k.data_ptr(), ks, v.data_ptr(), vs, k.shape[0], st, ko, vo, tb, width, ln,
+                                  np_, n, self.L._stream(stream)), "kv_append")
+
+    def attention(self, q, out, tables, lengths, max_length, scale=None, accumulate=False, stream=None):
+        """SNEPPX_kv_attention: q bf16 [rows, q_heads, head_dim], out the same
+        in bf16 or fp32; scale 1 / sqrt(head_dim) unless given."""
+        qs = self._rows(q, "q", 0, (torch.bfloat16,))
+        os_ = self._rows(out, "out", q.shape[1], (torch.bfloat16, torch.float32))
+        tb, width, ln, n = self._tables(tables, lengths)
+        if q.shape[0] != n or out.shape[0] != n:
+            raise ValueError(f"q has {q.shape[0]} rows and out {out.shape[0]}, tables {n}")
+        self.L.check(self._attention(
+            self._p, q.data_ptr(), qs, out.data_ptr(), os_,
+            SNEPPX_FLOAT32 if out.dtype == torch.float32 else SNEPPX_BFLOAT16, tb, width, ln, n, q.shape[1],
+            max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate), self.L._stream(stream)),
+            "kv_attention")
+
+    def evict(self, tables, lengths, next_pos, new_lengths, max_length, budget, recent, stream=None):
+        """SNEPPX_kv_evict; new_lengths int32 [rows] or None."""
+        tb, width, ln, n = self._tables(tables, lengths)
+        np_ = self._check(next_pos, "next_pos", torch.int32, (n,))
+        nl = None if new_lengths is None else self._check(new_lengths, "new_lengths", torch.int32, (n,))
+        self.L.check(self._evict(self._p, tb, width, ln, np_, nl, n, max_length, budget, recent,
+                                 self.L._stream(stream)), "kv_evict")
 
 
 class QLayer:
