@@ -542,7 +542,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     const KVPool p = kv_pool(c, tables, width);
     const Plan n = plan(c, rows, q_heads, max_length, accumulate);
     const size_t blocks = rows * c->kv_heads * n.tiles * n.splits;
-    if (blocks > 0x7fffffff) {
+    if (blocks > 0xffffff) {          // a grid has below 2^32 threads
         snx_set_error("kv_attention: %zu rows of up to %zu tokens are too many", rows, max_length);
         return -1;
     }

@@ -26,26 +26,33 @@ struct NewRows {
     size_t k_stride, v_stride;
     uint16_t *k_stored, *v_stored;
     const int32_t *starts, *lengths, *next_pos;
-    uint32_t tokens, rows;
+    uint32_t tokens, rows, slots;
+    int aligned, stored_aligned;
 };
 
-// One wave per (token, key or value, head): its head_dim values, up to 4 per
-// lane.
-template <bool I8>
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// LR lanes per (token, key or value, head), eight of its values each: one pass
+// with the row in registers, 16-byte loads and (int8: 8-byte) stores.  What
+// bounds it: at a decode batch the launch (16 tokens of 8 heads of 128: 3 us),
+// at a prompt the reads and writes.
+template <bool I8, int LR>
 __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows n) {
-    const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const uint32_t t = (uint32_t)(item / (2 * p.heads));
+    const uint64_t first = (uint64_t)blockIdx.x * (256 / LR);
+    const uint32_t per = 2 * p.heads, t0 = (uint32_t)(first / per);
+    const uint32_t rest = (uint32_t)(first - (uint64_t)t0 * per) + threadIdx.x / LR;
+    const uint32_t t = t0 + rest / per;
     if (t >= n.tokens) return;
-    const uint32_t rest = (uint32_t)(item - (uint64_t)t * (2 * p.heads));
-    const bool is_v = rest >= p.heads;
-    const uint32_t h = is_v ? rest - p.heads : rest;
+    const uint32_t which = rest % per, d = 8 * (threadIdx.x % LR);
+    const bool is_v = which >= p.heads;
+    const uint32_t h = is_v ? which - p.heads : which;
 
     // the row of token t: the last one whose tokens start at or before it
     uint32_t b = t;
     int32_t back = 1;
     if (n.starts) {
-        uint32_t lo = 0, hi = n.rows;          // starts[lo] <= t < starts[hi], if in any row
+        uint32_t lo = 0, hi = n.rows;
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) >> 1;
             if (n.starts[mid] <= (int32_t)t) lo = mid;
@@ -57,30 +64,51 @@ __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows
     }
     const int32_t slot = n.lengths[b] - back;
     uint32_t r;
-    if (slot < 0 || (uint64_t)slot >= (uint64_t)p.width * p.page_size || !p.row(b, h, (uint32_t)slot, r)) return;
+    if (slot < 0 || (uint32_t)slot >= n.slots || !p.row(b, h, (uint32_t)slot, r)) return;
 
-    const uint16_t* x = (is_v ? n.v + t * n.v_stride : n.k + t * n.k_stride) + (size_t)h * p.dim;
-    uint8_t* pool = is_v ? p.v : p.k;
-    uint16_t* stored = is_v ? n.v_stored : n.k_stored;
-    if (stored) stored += ((size_t)t * p.heads + h) * p.dim;
-    if (I8) {
-        float m = 0.0f;
-        for (uint32_t d = lane; d < p.dim; d += 64) m = nanless_max(m, fabsf(bf16_to_f32(x[d])));
-        for (int o = 32; o > 0; o >>= 1) m = nanless_max(m, __shfl_xor(m, o));
-        const float s = m < FLT_MIN ? 1.0f : m / 127.0f, inv = 1.0f / s;
-        for (uint32_t d = lane; d < p.dim; d += 64) {
-            const int q = clampi(round_i32(bf16_to_f32(x[d]) * inv), -128, 127);
-            reinterpret_cast<int8_t*>(pool)[(size_t)r * p.dim + d] = (int8_t)q;
-            if (stored) stored[d] = bf16_out((float)q * s);
-        }
-        if (lane == 0) (is_v ? p.vs : p.ks)[r] = s;
-    } else {
-        for (uint32_t d = lane; d < p.dim; d += 64) {
-            reinterpret_cast<uint16_t*>(pool)[(size_t)r * p.dim + d] = x[d];
-            if (stored) stored[d] = x[d];
-        }
+    const uint16_t* x = (is_v ? n.v + t * n.v_stride : n.k + t * n.k_stride) + (size_t)h * p.dim + d;
+    u32x4 w = {0u, 0u, 0u, 0u};
+    const bool in = d < p.dim;
+    if (in) {
+        if (n.aligned) w = *reinterpret_cast<const u32x4*>(x);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = x[2 * e] | (uint32_t)x[2 * e + 1] << 16;
     }
-    if (lane == 0 && !is_v) {
+    if (I8) {
+        float f[8], m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            f[2 * e] = u2f(w[e] << 16);
+            f[2 * e + 1] = u2f(w[e] & 0xFFFF0000u);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = nanless_max(m, fabsf(f[e]));
+#pragma unroll
+        for (int o = LR / 2; o > 0; o >>= 1) m = nanless_max(m, __shfl_xor(m, o));
+        const float s = m < FLT_MIN ? 1.0f : m / 127.0f, inv = 1.0f / s;
+        u32x2 q = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int c = clampi(round_i32(f[e] * inv), -128, 127);
+            q[e >> 2] |= (uint32_t)(c & 0xFF) << (8 * (e & 3));
+            f[e] = (float)c * s;
+        }
+        if (in) *reinterpret_cast<u32x2*>((is_v ? p.v : p.k) + (size_t)r * p.dim + d) = q;
+        if (d == 0) (is_v ? p.vs : p.ks)[r] = s;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = bf16x2_out(f[2 * e], f[2 * e + 1]);
+    } else if (in) {
+        *reinterpret_cast<u32x4*>((is_v ? p.v : p.k) + ((size_t)r * p.dim + d) * 2) = w;
+    }
+    if (n.k_stored && in) {
+        uint16_t* to = (is_v ? n.v_stored : n.k_stored) + ((size_t)t * p.heads + h) * p.dim + d;
+        if (n.stored_aligned) *reinterpret_cast<u32x4*>(to) = w;
+        else
+#pragma unroll
+            for (int e = 0; e < 8; e++) to[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    }
+    if (d == 0 && !is_v) {
         if (p.weights) p.weights[r] = 0.0f;
         if (p.positions) p.positions[r] = n.next_pos[b] - back;
     }
@@ -98,148 +126,263 @@ __device__ __forceinline__ uint32_t rank_key(float w, int32_t pos, int32_t recen
 
 constexpr int kCutWaves = 16;
 constexpr int kCutThreads = 64 * kCutWaves;
+constexpr int kBins = 2048;              // digits of 11, 11 and 10 bits
+constexpr uint32_t kMoveAtOnce = 64;     // moves that the workgroup which finds them makes itself
 
-// exclusive prefix over the waves of a per-wave count; *total gets the sum
-__device__ __forceinline__ uint32_t wave_prefix(uint32_t count, uint32_t* sh, uint32_t& total) {
+// two counts per wave -> their exclusive prefixes over the waves, and the totals
+__device__ __forceinline__ void wave_prefix(uint32_t& x, uint32_t& y, uint2* sh, uint2& total) {
     const int w = threadIdx.x >> 6;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[w] = count;
+    if ((threadIdx.x & 63) == 0) sh[w] = make_uint2(x, y);
     __syncthreads();
-    uint32_t before = 0, all = 0;
+    x = y = 0;
+    total = make_uint2(0, 0);
+#pragma unroll
     for (int i = 0; i < kCutWaves; i++) {
-        if (i < w) before += sh[i];
-        all += sh[i];
+        const uint2 v = sh[i];
+        if (i < w) {
+            x += v.x;
+            y += v.y;
+        }
+        total.x += v.x;
+        total.y += v.y;
     }
-    total = all;
-    return before;
 }
 
-// One workgroup per (row, head): finds the budget-th largest key by its digits
-// of 8 bits, from the top (a histogram of the keys that agree with the digits
-// found so far), then lists the free slots below the budget and the kept ones
-// from it on, both in ascending order, as rows of the pool.
-// moves [rows][heads][2][most], counts [rows][heads].
-__global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const int32_t* __restrict__ lengths,
-                                                        const int32_t* __restrict__ next_pos,
-                                                        int32_t* __restrict__ new_lengths, uint32_t max_length,
-                                                        uint32_t budget, uint32_t recent, uint32_t most,
-                                                        uint32_t* __restrict__ counts, uint32_t* __restrict__ moves) {
-    __shared__ uint32_t hist[256], sh[kCutWaves], found[2];
+// rows of the pool: k, v and the planes, from row `of` to row `to`, for `n`
+// moves by `threads` threads of which this is `me`
+__device__ __forceinline__ void move_rows(const KVPool& p, uint32_t row_bytes, const uint32_t* to, const uint32_t* of,
+                                          uint32_t n, uint32_t me, uint32_t threads) {
+    const uint32_t per = row_bytes / 16, chunks = n * per;
+    constexpr int U = 4;
+    for (uint32_t i0 = me; i0 < chunks; i0 += U * threads) {
+        u32x4 a[U], b[U];
+        size_t at[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + u * threads;
+            if (i >= chunks) continue;
+            const uint32_t m = i / per, c = 16 * (i - m * per);
+            const size_t from = (size_t)of[m] * row_bytes + c;
+            at[u] = (size_t)to[m] * row_bytes + c;
+            a[u] = *reinterpret_cast<const u32x4*>(p.k + from);
+            b[u] = *reinterpret_cast<const u32x4*>(p.v + from);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i0 + u * threads >= chunks) continue;
+            *reinterpret_cast<u32x4*>(p.k + at[u]) = a[u];
+            *reinterpret_cast<u32x4*>(p.v + at[u]) = b[u];
+        }
+    }
+    for (uint32_t m = me; m < n; m += threads) {
+        const uint32_t t = to[m], f = of[m];
+        const float w = p.weights[f];
+        const int32_t pos = p.positions[f];
+        if (p.ks) {
+            const float x = p.ks[f], y = p.vs[f];
+            p.ks[t] = x;
+            p.vs[t] = y;
+        }
+        p.weights[t] = w;
+        p.positions[t] = pos;
+    }
+}
+
+struct Cut {
+    const int32_t *lengths, *next_pos;
+    int32_t* new_lengths;
+    uint32_t max_length, budget, recent, most, row_bytes;
+    uint32_t* counts;          // [rows * heads] moves of each row and head (unless moved at once)
+    uint32_t* moves;           // [rows * heads][2][most] targets, then sources
+    uint32_t* keys;            // [rows * heads][max_length] where they do not fit in registers
+};
+
+// One workgroup per (row, head): the budget-th largest key by its digits from
+// the top (each time a histogram of the keys that agree with the digits found
+// so far), then the free slots below the budget and the kept ones from it on,
+// both in ascending order.  Each wave has consecutive slots, so that order by
+// (wave, step, lane) is order by slot.  KPT keys per thread stay in registers;
+// KPT = 0: in a workspace, any number.  MOVE: with so few moves that the
+// workgroup makes them at once.
+template <int KPT, bool MOVE>
+__global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
+    __shared__ uint32_t hist[kBins], found[3];
+    __shared__ uint2 sh[kCutWaves];
+    __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t L = kv_length(lengths, b, max_length);
-    uint32_t* const count = counts + blockIdx.x;
+    const uint32_t L = kv_length(a.lengths, b, a.max_length), budget = a.budget;
+    const uint32_t steps = (L + kCutThreads - 1) / kCutThreads;       // slots of a thread, up to KPT
+    const uint32_t t0 = wave * steps * 64 + lane;
+    uint32_t* const far_keys = KPT ? nullptr : a.keys + (size_t)blockIdx.x * a.max_length;
+
+    uint32_t kept_keys[KPT ? KPT : 1];
     bool gone = false;
     if (L > budget) {
-        const uint32_t used = p.page_of(L - 1) + 1;
-        for (uint32_t e = tid; e < used; e += kCutThreads)
-            gone |= (uint32_t)p.tables[(size_t)b * p.width + e] >= p.pages;
-    }
-    gone = __syncthreads_or(gone);
-    if (tid == 0 && h == 0 && new_lengths) new_lengths[b] = (int32_t)(L > budget && !gone ? budget : L);
-    if (L <= budget || gone) {
-        if (tid == 0) *count = 0;
-        return;
-    }
-    const int32_t from = (int32_t)((int64_t)next_pos[b] - (int64_t)recent < INT32_MIN
-                                       ? INT32_MIN : (int64_t)next_pos[b] - (int64_t)recent);
-    auto key = [&](uint32_t t) {
-        uint32_t r;
-        (void)p.row(b, h, t, r);
-        return rank_key(p.weights[r], p.positions[r], from);
-    };
-
-    uint32_t prefix = 0, want = budget;      // the want-th largest among the keys that share the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-        for (uint32_t t = tid; t < L; t += kCutThreads) {
-            const uint32_t q = key(t);
-            if ((q & mask) == prefix) atomicAdd(&hist[(q >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t above = 0;
-            int d = 255;
-            while (above + hist[d] < want) above += hist[d--];
-            found[0] = prefix | (uint32_t)d << shift;
-            found[1] = want - above;
-        }
-        __syncthreads();
-        prefix = found[0];
-        want = found[1];
-        __syncthreads();
-    }
-
-    // each wave takes consecutive slots, so that order by (wave, step, lane) is
-    // order by slot
-    const uint32_t per = (L + kCutThreads - 1) / kCutThreads * 64;
-    const uint32_t t0 = wave * per, t1 = t0 + per < L ? t0 + per : L;
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    uint32_t n = 0, total;
-    for (uint32_t t = t0; t < t1; t += 64)
-        n += __popcll(__ballot(t + lane < t1 && key(t + lane) == prefix));
-    const uint32_t ties = wave_prefix(n, sh, total);
-
-    uint32_t holes = 0, far = 0, seen = ties;
-    for (int pass = 0; pass < 2; pass++) {
-        uint32_t hole_at = 0, far_at = 0;
-        if (pass == 1) {
-            hole_at = wave_prefix(holes, sh, total);
-            far_at = wave_prefix(far, sh, total);
-            if (tid == 0) *count = total;
-            seen = ties;
-        }
-        for (uint32_t t = t0; t < t1; t += 64) {
-            const uint32_t s = t + lane;
-            const bool in = s < t1;
-            const uint32_t q = in ? key(s) : 0u;
-            const bool tie = in && q == prefix;
-            const uint64_t tb = __ballot(tie);
-            const bool keep = in && (q > prefix || (tie && seen + __popcll(tb & below) < want));
-            seen += __popcll(tb);
-            const bool hole = in && !keep && s < budget, come = keep && s >= budget;
-            const uint64_t hb = __ballot(hole), fb = __ballot(come);
-            if (pass == 0) {
-                holes += __popcll(hb);
-                far += __popcll(fb);
-            } else {
-                uint32_t r;
-                uint32_t* list = moves + (size_t)blockIdx.x * 2 * most;
-                if (hole || come) {
-                    (void)p.row(b, h, s, r);
-                    if (hole) list[hole_at + __popcll(hb & below)] = r;
-                    else list[most + far_at + __popcll(fb & below)] = r;
+        const int64_t from64 = (int64_t)a.next_pos[b] - (int64_t)a.recent;
+        const int32_t from = (int32_t)(from64 < INT32_MIN ? INT32_MIN : from64);
+        if (KPT) {
+            constexpr int G = KPT % 8 == 0 ? 8 : KPT % 6 == 0 ? 6 : 4;       // loads in flight
+#pragma unroll
+            for (int i0 = 0; i0 < KPT; i0 += G) {
+                uint32_t rows[G];
+#pragma unroll
+                for (int i = 0; i < G; i++) {
+                    const uint32_t t = t0 + 64 * (i0 + i);
+                    rows[i] = 0;
+                    if ((uint32_t)(i0 + i) < steps && t < L && !p.row(b, h, t, rows[i])) {
+                        gone = true;
+                        rows[i] = 0;
+                    }
                 }
-                hole_at += __popcll(hb);
-                far_at += __popcll(fb);
+#pragma unroll
+                for (int i = 0; i < G; i++) kept_keys[KPT ? i0 + i : 0] = rank_key(p.weights[rows[i]], p.positions[rows[i]], from);
+            }
+        } else {
+            for (uint32_t i = 0; i < steps; i++) {
+                const uint32_t t = t0 + 64 * i;
+                uint32_t r;
+                if (t >= L) continue;
+                if (!p.row(b, h, t, r)) gone = true;
+                else far_keys[t] = rank_key(p.weights[r], p.positions[r], from);
             }
         }
     }
+    gone = __syncthreads_or(gone);
+    if (tid == 0 && h == 0 && a.new_lengths) a.new_lengths[b] = (int32_t)(L > budget && !gone ? budget : L);
+    if (L <= budget || gone) {
+        if (!MOVE && tid == 0) a.counts[blockIdx.x] = 0;
+        return;
+    }
+    // (a workspace's keys are read by the thread that wrote them)
+    auto key = [&](uint32_t i) { return KPT ? kept_keys[KPT ? i : 0] : t0 + 64 * i < L ? far_keys[t0 + 64 * i] : 0u; };
+    auto each = [&](auto f) {
+        if (KPT) {
+#pragma unroll
+            for (int i = 0; i < KPT; i++)
+                if ((uint32_t)i < steps) f((uint32_t)i);
+        } else {
+            for (uint32_t i = 0; i < steps; i++) f(i);
+        }
+    };
+
+    uint32_t prefix = 0, want = budget, tied = 0;    // the want-th largest of the `tied` keys that share the prefix
+#pragma unroll
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t bins = pass == 2 ? 1024 : kBins, mask = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
+        hist[tid] = hist[tid + kCutThreads] = 0;
+        __syncthreads();
+        each([&](uint32_t i) {
+            const uint32_t q = key(i), digit = (q >> shift) & (bins - 1);
+            const bool in = t0 + 64 * i < L && (q & mask) == prefix;
+            const uint64_t who = __ballot(in);
+            if (!who) return;
+            // many alike (zeros, recent ones) are counted at once
+            const uint32_t one = __builtin_amdgcn_readlane(digit, __builtin_ctzll(who));
+            if (__ballot(in && digit == one) == who) {
+                if (lane == __builtin_ctzll(who)) atomicAdd(&hist[one], (uint32_t)__popcll(who));
+            } else if (in) {
+                atomicAdd(&hist[digit], 1u);
+            }
+        });
+        __syncthreads();
+        // from the top: thread i has bins 2 i and 2 i + 1 below it
+        const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
+        uint32_t sum = hi + lo;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 63) sh[wave].x = sum;
+        __syncthreads();
+        uint32_t before = sum - hi - lo;
+#pragma unroll
+        for (int w = 0; w < kCutWaves; w++)
+            if (w < wave) before += sh[w].x;
+        const bool at_hi = before < want && want <= before + hi;
+        const bool at_lo = !at_hi && before + hi < want && want <= before + hi + lo;
+        if (at_hi || at_lo) {
+            found[0] = (uint32_t)(kBins - 1 - 2 * tid) - (at_lo ? 1u : 0u);
+            found[1] = want - before - (at_lo ? hi : 0u);
+            found[2] = at_hi ? hi : lo;
+        }
+        __syncthreads();
+        prefix |= found[0] << shift;
+        want = found[1];
+        tied = found[2];
+    }
+
+    // of the keys equal to the threshold the first `want` stay
+    uint2 total;
+    uint32_t ties = 0, none = 0;
+    if (want < tied) {
+        each([&](uint32_t i) { ties += __popcll(__ballot(t0 + 64 * i < L && key(i) == prefix)); });
+        wave_prefix(ties, none, sh, total);
+    }
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    uint32_t seen = ties;
+    auto stays = [&](uint32_t i) {
+        const uint32_t q = key(i);
+        const bool in = t0 + 64 * i < L, tie = in && q == prefix;
+        if (want == tied) return in && q >= prefix;
+        const uint64_t tb = __ballot(tie);
+        const bool keep = in && (q > prefix || (tie && seen + __popcll(tb & below) < want));
+        seen += __popcll(tb);
+        return keep;
+    };
+    uint32_t holes = 0, far = 0;
+    each([&](uint32_t i) {
+        const uint32_t t = t0 + 64 * i;
+        const bool keep = stays(i);
+        holes += __popcll(__ballot(!keep && t < budget));
+        far += __popcll(__ballot(keep && t >= budget));
+    });
+    wave_prefix(holes, far, sh, total);
+    seen = ties;
+    uint32_t* const to = MOVE ? list : a.moves + (size_t)blockIdx.x * 2 * a.most;
+    uint32_t* const of = to + (MOVE ? kMoveAtOnce : a.most);
+    each([&](uint32_t i) {
+        const uint32_t t = t0 + 64 * i;
+        const bool keep = stays(i), hole = !keep && t < budget, come = keep && t >= budget;
+        const uint64_t hb = __ballot(hole), fb = __ballot(come);
+        if (hole || come) {
+            uint32_t r;
+            (void)p.row(b, h, t, r);
+            if (hole) to[holes + __popcll(hb & below)] = r;
+            else of[far + __popcll(fb & below)] = r;
+        }
+        holes += __popcll(hb);
+        far += __popcll(fb);
+    });
+    if (MOVE) {
+        __syncthreads();
+        move_rows(p, a.row_bytes, to, of, total.x, tid, kCutThreads);
+    } else if (tid == 0) {
+        a.counts[blockIdx.x] = total.x;
+    }
 }
 
-// The moves, one wave each: rows of k and v and the planes.  Sources lie in
-// slots from the budget on and targets below it, so all are independent.
-__global__ void __launch_bounds__(256) k_kv_move(const KVPool p, uint32_t row_bytes, uint32_t most,
-                                                 const uint32_t* __restrict__ counts,
-                                                 const uint32_t* __restrict__ moves) {
-    const uint32_t bh = blockIdx.y, n = counts[bh];
-    const int lane = threadIdx.x & 63;
-    const uint32_t* list = moves + (size_t)bh * 2 * most;
-    for (uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += gridDim.x * 4) {
-        const size_t to = list[i], of = list[most + i];
-        for (uint32_t c = lane * 16; c < row_bytes; c += 64 * 16) {
-            *reinterpret_cast<uint4*>(p.k + to * row_bytes + c) = *reinterpret_cast<const uint4*>(p.k + of * row_bytes + c);
-            *reinterpret_cast<uint4*>(p.v + to * row_bytes + c) = *reinterpret_cast<const uint4*>(p.v + of * row_bytes + c);
-        }
-        if (lane == 0) {
-            p.weights[to] = p.weights[of];
-            p.positions[to] = p.positions[of];
-            if (p.ks) p.ks[to] = p.ks[of];
-            if (p.vs) p.vs[to] = p.vs[of];
-        }
-    }
+// The moves that k_kv_cut listed.  Sources lie in slots from the budget on and
+// targets below it, so all are independent.
+__global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a) {
+    const uint32_t bh = blockIdx.y, n = a.counts[bh];
+    const uint32_t* to = a.moves + (size_t)bh * 2 * a.most;
+    move_rows(p, a.row_bytes, to, to + a.most, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+}
+
+template <int LR>
+void append(bool i8, unsigned blocks, const KVPool& p, const NewRows& n, hipStream_t s) {
+    if (i8) k_kv_append<true, LR><<<blocks, 256, 0, s>>>(p, n);
+    else k_kv_append<false, LR><<<blocks, 256, 0, s>>>(p, n);
+}
+
+template <int KPT>
+void cut(bool at_once, unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
+    if (at_once) k_kv_cut<KPT, true><<<blocks, kCutThreads, 0, s>>>(p, a);
+    else k_kv_cut<KPT, false><<<blocks, kCutThreads, 0, s>>>(p, a);
 }
 
 uint32_t most_moves(size_t max_length, size_t budget) {
@@ -256,43 +399,76 @@ int snx_k_kv_append(const SNEPPXKVCache* c, const uint16_t* k, size_t k_stride, 
                     const int32_t* tables, size_t width, const int32_t* lengths, const int32_t* next_pos,
                     size_t rows, void* st) {
     const KVPool p = kv_pool(c, tables, width);
-    const NewRows n{k, v, k_stride, v_stride, k_stored, v_stored, starts, lengths, next_pos, (uint32_t)tokens, (uint32_t)rows};
-    const size_t blocks = (tokens * 2 * c->kv_heads + 3) / 4;
-    if (blocks > 0x7fffffff) {
+    NewRows n;
+    n.k = k;
+    n.v = v;
+    n.k_stride = k_stride;
+    n.v_stride = v_stride;
+    n.k_stored = k_stored;
+    n.v_stored = v_stored;
+    n.starts = starts;
+    n.lengths = lengths;
+    n.next_pos = next_pos;
+    n.tokens = (uint32_t)tokens;
+    n.rows = (uint32_t)rows;
+    n.slots = (uint32_t)(width * c->page_size);
+    n.aligned = (((uintptr_t)k | (uintptr_t)v) & 15u) == 0 && (tokens < 2 || (k_stride % 8 == 0 && v_stride % 8 == 0));
+    n.stored_aligned = (((uintptr_t)k_stored | (uintptr_t)v_stored) & 15u) == 0;
+    const int lr = c->head_dim <= 64 ? 8 : c->head_dim <= 128 ? 16 : 32;
+    const size_t blocks = (tokens * 2 * c->kv_heads * lr + 255) / 256;
+    if (blocks > 0xffffff) {          // a grid has below 2^32 threads
         snx_set_error("kv_append: %zu tokens of %zu heads are too many", tokens, c->kv_heads);
         return -1;
     }
-    if (c->dtype == SNEPPX_INT8)
-        k_kv_append<true><<<(unsigned)blocks, 256, 0, S(st)>>>(p, n);
-    else
-        k_kv_append<false><<<(unsigned)blocks, 256, 0, S(st)>>>(p, n);
+    const bool i8 = c->dtype == SNEPPX_INT8;
+    if (lr == 8) append<8>(i8, (unsigned)blocks, p, n, S(st));
+    else if (lr == 16) append<16>(i8, (unsigned)blocks, p, n, S(st));
+    else append<32>(i8, (unsigned)blocks, p, n, S(st));
     return snx_launch_check("k_kv_append");
 }
 
+// Keys that do not fit in the registers of a workgroup
+static bool keys_far(size_t max_length) { return max_length > 32 * (size_t)kCutThreads; }
+
 size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, size_t budget) {
-    return rows * c->kv_heads * (1 + 2 * (size_t)most_moves(max_length, budget)) * sizeof(uint32_t);
+    const size_t most = most_moves(max_length, budget), bh = rows * c->kv_heads;
+    return bh * sizeof(uint32_t) *
+           ((most > kMoveAtOnce ? 1 + 2 * most : 0) + (keys_far(max_length) && most ? max_length : 0));
 }
 
 int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, const int32_t* lengths,
                    const int32_t* next_pos, int32_t* new_lengths, size_t rows, size_t max_length, size_t budget,
                    size_t recent, void* ws, void* st) {
     const KVPool p = kv_pool(c, tables, width);
-    const uint32_t most = most_moves(max_length, budget);
     const size_t bh = rows * c->kv_heads;
-    uint32_t* counts = static_cast<uint32_t*>(ws);
-    uint32_t* moves = counts + bh;
-    k_kv_cut<<<(unsigned)bh, kCutThreads, 0, S(st)>>>(p, lengths, next_pos, new_lengths, (uint32_t)max_length,
-                                                      (uint32_t)budget, (uint32_t)(recent < INT32_MAX ? recent : INT32_MAX),
-                                                      most, counts, moves);
+    Cut a;
+    a.lengths = lengths;
+    a.next_pos = next_pos;
+    a.new_lengths = new_lengths;
+    a.max_length = (uint32_t)max_length;
+    a.budget = (uint32_t)budget;
+    a.recent = (uint32_t)(recent < INT32_MAX ? recent : INT32_MAX);
+    a.most = most_moves(max_length, budget);
+    a.row_bytes = (uint32_t)(c->head_dim * (c->dtype == SNEPPX_INT8 ? 1 : 2));
+    const bool at_once = a.most <= kMoveAtOnce;
+    a.counts = static_cast<uint32_t*>(ws);
+    a.moves = a.counts + bh;
+    a.keys = at_once ? a.counts : a.moves + bh * 2 * a.most;
+    // with nothing to cut every workgroup ends at once: any form does
+    const size_t keys = a.most ? max_length : 1;
+    if (keys <= 4 * (size_t)kCutThreads) cut<4>(at_once, (unsigned)bh, p, a, S(st));
+    else if (keys <= 12 * (size_t)kCutThreads) cut<12>(at_once, (unsigned)bh, p, a, S(st));
+    else if (!keys_far(keys)) cut<32>(at_once, (unsigned)bh, p, a, S(st));
+    else cut<0>(at_once, (unsigned)bh, p, a, S(st));
     if (snx_launch_check("k_kv_cut")) return -1;
-    if (!most) return 0;
-    const uint32_t row_bytes = (uint32_t)(c->head_dim * (c->dtype == SNEPPX_INT8 ? 1 : 2));
-    const uint32_t gx = (most + 3) / 4;
+    if (at_once) return 0;
+    const size_t chunks = (size_t)a.most * (a.row_bytes / 16), gx = (chunks + 1023) / 1024;
     for (size_t at = 0; at < bh; at += 65535) {
         const size_t n = bh - at < 65535 ? bh - at : 65535;
-        k_kv_move<<<dim3(gx < 65536 ? gx : 65536, (unsigned)n), 256, 0, S(st)>>>(p, row_bytes, most, counts + at,
-                                                                                moves + at * 2 * most);
+        k_kv_move<<<dim3((unsigned)(gx < 65536 ? gx : 65536), (unsigned)n), 256, 0, S(st)>>>(p, a);
         if (snx_launch_check("k_kv_move")) return -1;
+        a.counts += n;
+        a.moves += n * 2 * a.most;
     }
     return 0;
 }

@@ -20,6 +20,8 @@
 
 /* slots of a row are counted in 32 bits on the device, with room to round up */
 #define MAX_SLOTS ((size_t)1 << 30)
+/* a workgroup of 1024 for each row and head: a grid has below 2^32 threads */
+#define MAX_PAIRS (((size_t)1 << 22) - 1)
 
 static int aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
@@ -34,9 +36,7 @@ static int cache_ok(const char* who, const SNEPPXKVCache* c) {
     const size_t step = c->dtype == SNEPPX_INT8 ? 16 : 8;
     REQUIRE(c->head_dim <= 256 && c->head_dim % step == 0, "%s: head_dim %zu is not a multiple of %zu up to 256", who,
             c->head_dim, step);
-    /* token rows of the pool are numbered in 32 bits (at 2^32 rows of 16 bytes
-     * and more, the pool is beyond what a GPU holds of both k and v at
-     * useful head sizes) */
+    /* token rows of the pool are numbered in 32 bits */
     REQUIRE(c->page_size <= MAX_SLOTS && c->pages <= INT32_MAX && c->kv_heads <= 65535 &&
                 c->pages <= (size_t)UINT32_MAX / c->page_size / c->kv_heads,
             "%s: pages * kv_heads * page_size = %zu * %zu * %zu is too large", who, c->pages, c->kv_heads, c->page_size);
@@ -49,7 +49,7 @@ static int rows_ok(const char* who, const SNEPPXKVCache* c, const int32_t* table
     REQUIRE(width, "%s: empty block_tables", who);
     REQUIRE(width <= MAX_SLOTS / c->page_size, "%s: table_width %zu * page_size %zu is too large", who, width,
             c->page_size);
-    REQUIRE(rows <= 0x7fffffff / c->kv_heads, "%s: %zu rows are too many", who, rows);
+    REQUIRE(rows <= MAX_PAIRS / c->kv_heads, "%s: %zu rows of %zu heads are too many", who, rows, c->kv_heads);
     return 0;
 }
 
@@ -87,7 +87,6 @@ int SNEPPX_kv_attention(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_
     const size_t n = q_heads * cache->head_dim;
     REQUIRE(rows < 2 || (q_stride >= n && out_stride >= n), "kv_attention: strides %zu, %zu are below q_heads * head_dim = %zu",
             q_stride, out_stride, n);
-    REQUIRE(rows <= 0x7fffffff / q_heads, "kv_attention: %zu rows are too many", rows);
     REQUIRE(!accumulate || cache->weights, "kv_attention: accumulate needs the cache's weights");
     snx_clear_error();
     if (!rows) return 0;

@@ -828,6 +828,11 @@ class KVCache:
         self._append, self._attention, self._evict = (
             lib.fn[f"SNEPPX_kv_{n}"] for n in ("append", "attention", "evict"))
 
+    def _stream(self, stream):
+        # torch's current stream as a number: current_stream() makes an object
+        # of it, 2.8 us where this takes 0.2
+        return stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device.index or 0)
+
     def _check(self, t, name, dtype, shape):
         """A contiguous tensor of this type and shape on the cache's device."""
         if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != self.device \
@@ -867,7 +872,7 @@ class KVCache:
         ko, vo = (None if t is None else self._check(t, name, torch.bfloat16, k.shape)
                   for t, name in ((k_stored, "k_stored"), (v_stored, "v_stored")))
         self.L.check(self._append(self._p, k.data_ptr(), ks, v.data_ptr(), vs, k.shape[0], st, ko, vo, tb, width, ln,
-                                  np_, n, self.L._stream(stream)), "kv_append")
+                                  np_, n, self._stream(stream)), "kv_append")
 
     def attention(self, q, out, tables, lengths, max_length, scale=None, accumulate=False, stream=None):
         """SNEPPX_kv_attention: q bf16 [rows, q_heads, head_dim], out the same
@@ -880,7 +885,7 @@ class KVCache:
         self.L.check(self._attention(
             self._p, q.data_ptr(), qs, out.data_ptr(), os_,
             SNEPPX_FLOAT32 if out.dtype == torch.float32 else SNEPPX_BFLOAT16, tb, width, ln, n, q.shape[1],
-            max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate), self.L._stream(stream)),
+            max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate), self._stream(stream)),
             "kv_attention")
 
     def evict(self, tables, lengths, next_pos, new_lengths, max_length, budget, recent, stream=None):
@@ -889,7 +894,7 @@ class KVCache:
         np_ = self._check(next_pos, "next_pos", torch.int32, (n,))
         nl = None if new_lengths is None else self._check(new_lengths, "new_lengths", torch.int32, (n,))
         self.L.check(self._evict(self._p, tb, width, ln, np_, nl, n, max_length, budget, recent,
-                                 self.L._stream(stream)), "kv_evict")
+                                 self._stream(stream)), "kv_evict")
 
 
 class QLayer:
