@@ -119,8 +119,8 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&piece)[3]) 
 // spread over all banks.
 template <int RB, bool I8>
 __device__ __forceinline__ int v_chunk(int r, int c) {
-    if (I8) {
-        constexpr int per = 256 / RB;                                  // rows in 256 bytes
+    if constexpr (I8) {
+        constexpr int per = RB < 256 ? 256 / RB : 1;                   // rows in 256 bytes
         const int f = (r / per) ^ ((r >> 4) << 1);
         return r * (RB / 16) + (c ^ (f & (RB / 16 - 1)));
     } else {

@@ -48,6 +48,17 @@ __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows
     const bool is_v = which >= p.heads;
     const uint32_t h = is_v ? which - p.heads : which;
 
+    // (loaded ahead of the look-ups, which depend on one another)
+    const uint16_t* x = (is_v ? n.v + t * n.v_stride : n.k + t * n.k_stride) + (size_t)h * p.dim + d;
+    u32x4 w = {0u, 0u, 0u, 0u};
+    const bool in = d < p.dim;
+    if (in) {
+        if (n.aligned) w = *reinterpret_cast<const u32x4*>(x);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = x[2 * e] | (uint32_t)x[2 * e + 1] << 16;
+    }
+
     // the row of token t: the last one whose tokens start at or before it
     uint32_t b = t;
     int32_t back = 1;
@@ -66,15 +77,6 @@ __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows
     uint32_t r;
     if (slot < 0 || (uint32_t)slot >= n.slots || !p.row(b, h, (uint32_t)slot, r)) return;
 
-    const uint16_t* x = (is_v ? n.v + t * n.v_stride : n.k + t * n.k_stride) + (size_t)h * p.dim + d;
-    u32x4 w = {0u, 0u, 0u, 0u};
-    const bool in = d < p.dim;
-    if (in) {
-        if (n.aligned) w = *reinterpret_cast<const u32x4*>(x);
-        else
-#pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = x[2 * e] | (uint32_t)x[2 * e + 1] << 16;
-    }
     if (I8) {
         float f[8], m = 0.0f;
 #pragma unroll
@@ -126,7 +128,8 @@ __device__ __forceinline__ uint32_t rank_key(float w, int32_t pos, int32_t recen
 
 constexpr int kCutWaves = 16;
 constexpr int kCutThreads = 64 * kCutWaves;
-constexpr int kBins = 2048;              // digits of 11, 11 and 10 bits
+constexpr int kPasses = 4;               // digits of 9, 8, 8 and 7 bits: sign and exponent first
+constexpr int kShift[kPasses] = {23, 15, 7, 0}, kBins[kPasses] = {512, 256, 256, 256};
 constexpr uint32_t kMoveAtOnce = 64;     // moves that the workgroup which finds them makes itself
 
 // two counts per wave -> their exclusive prefixes over the waves, and the totals
@@ -149,34 +152,55 @@ __device__ __forceinline__ void wave_prefix(uint32_t& x, uint32_t& y, uint2* sh,
     }
 }
 
-// rows of the pool: k, v and the planes, from row `of` to row `to`, for `n`
-// moves by `threads` threads of which this is `me`
-__device__ __forceinline__ void move_rows(const KVPool& p, uint32_t row_bytes, const uint32_t* to, const uint32_t* of,
-                                          uint32_t n, uint32_t me, uint32_t threads) {
+// inclusive prefix sum over the lanes
+__device__ __forceinline__ uint32_t lane_prefix(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);       // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+
+// rows of the pool (k, v and the planes) of slots of[i] to those of slots
+// to[i], for `n` moves, by `threads` threads of which this is `me`
+__device__ __forceinline__ void move_rows(const KVPool& p, uint32_t b, uint32_t h, uint32_t row_bytes,
+                                          const uint32_t* to, const uint32_t* of, uint32_t n, uint32_t me,
+                                          uint32_t threads) {
     const uint32_t per = row_bytes / 16, chunks = n * per;
     constexpr int U = 4;
     for (uint32_t i0 = me; i0 < chunks; i0 += U * threads) {
-        u32x4 a[U], b[U];
-        size_t at[U];
+        u32x4 x[U], y[U];
+        uint32_t src[U], dst[U], c[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const uint32_t i = i0 + u * threads;
-            if (i >= chunks) continue;
-            const uint32_t m = i / per, c = 16 * (i - m * per);
-            const size_t from = (size_t)of[m] * row_bytes + c;
-            at[u] = (size_t)to[m] * row_bytes + c;
-            a[u] = *reinterpret_cast<const u32x4*>(p.k + from);
-            b[u] = *reinterpret_cast<const u32x4*>(p.v + from);
+            const uint32_t i = i0 + u * threads < chunks ? i0 + u * threads : i0, m = i / per;
+            c[u] = 16 * (i - m * per);
+            src[u] = of[m];
+            dst[u] = to[m];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            (void)p.row(b, h, src[u], src[u]);
+            (void)p.row(b, h, dst[u], dst[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            x[u] = *reinterpret_cast<const u32x4*>(p.k + (size_t)src[u] * row_bytes + c[u]);
+            y[u] = *reinterpret_cast<const u32x4*>(p.v + (size_t)src[u] * row_bytes + c[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (i0 + u * threads >= chunks) continue;
-            *reinterpret_cast<u32x4*>(p.k + at[u]) = a[u];
-            *reinterpret_cast<u32x4*>(p.v + at[u]) = b[u];
+            *reinterpret_cast<u32x4*>(p.k + (size_t)dst[u] * row_bytes + c[u]) = x[u];
+            *reinterpret_cast<u32x4*>(p.v + (size_t)dst[u] * row_bytes + c[u]) = y[u];
         }
     }
     for (uint32_t m = me; m < n; m += threads) {
-        const uint32_t t = to[m], f = of[m];
+        uint32_t t, f;
+        (void)p.row(b, h, to[m], t);
+        (void)p.row(b, h, of[m], f);
         const float w = p.weights[f];
         const int32_t pos = p.positions[f];
         if (p.ks) {
@@ -194,58 +218,74 @@ struct Cut {
     int32_t* new_lengths;
     uint32_t max_length, budget, recent, most, row_bytes;
     uint32_t* counts;          // [rows * heads] moves of each row and head (unless moved at once)
-    uint32_t* moves;           // [rows * heads][2][most] targets, then sources
+    uint32_t* moves;           // [rows * heads][2][most] slots: targets, then sources
     uint32_t* keys;            // [rows * heads][max_length] where they do not fit in registers
 };
 
 // One workgroup per (row, head): the budget-th largest key by its digits from
 // the top (each time a histogram of the keys that agree with the digits found
-// so far), then the free slots below the budget and the kept ones from it on,
-// both in ascending order.  Each wave has consecutive slots, so that order by
-// (wave, step, lane) is order by slot.  KPT keys per thread stay in registers;
-// KPT = 0: in a workspace, any number.  MOVE: with so few moves that the
-// workgroup makes them at once.
+// so far, read by every wave for itself), then the free slots below the budget
+// and the kept ones from it on, both in ascending order.  Each wave has
+// consecutive slots, so that order by (wave, step, lane) is order by slot.  KPT
+// keys per thread stay in registers; KPT = 0: in a workspace, any number.
+// MOVE: with so few moves that the workgroup makes them at once.
 template <int KPT, bool MOVE>
 __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
-    __shared__ uint32_t hist[kBins], found[3];
+    constexpr int kHist = kBins[0] + kBins[1] + kBins[2] + kBins[3];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kHist];
     __shared__ uint2 sh[kCutWaves];
     __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t L = kv_length(a.lengths, b, a.max_length), budget = a.budget;
     const uint32_t steps = (L + kCutThreads - 1) / kCutThreads;       // slots of a thread, up to KPT
-    const uint32_t t0 = wave * steps * 64 + lane;
+    const uint32_t w0 = wave * steps * 64, t0 = w0 + lane;
     uint32_t* const far_keys = KPT ? nullptr : a.keys + (size_t)blockIdx.x * a.max_length;
 
+    for (int i = tid; i < kHist; i += kCutThreads) hist[i] = 0;
     uint32_t kept_keys[KPT ? KPT : 1];
     bool gone = false;
     if (L > budget) {
         const int64_t from64 = (int64_t)a.next_pos[b] - (int64_t)a.recent;
         const int32_t from = (int32_t)(from64 < INT32_MIN ? INT32_MIN : from64);
+        // G slots at once (past the length: its last one), so that their look-ups
+        // and loads are in flight together; key 0 past the length
+        constexpr int G = KPT == 0 ? 8 : KPT % 16 == 0 ? 16 : KPT;
+        const uint32_t groups = (steps + G - 1) / G;
+        auto group = [&](uint32_t i0, uint32_t (&q)[G]) {
+            uint32_t rows[G];
+            float w[G];
+            int32_t pos[G];
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                const uint32_t t = t0 + 64 * (i0 + i);
+                const bool there = p.row(b, h, t < L ? t : L - 1, rows[i]);
+                gone |= !there;
+                if (!there) rows[i] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < G; i++) {
+                w[i] = p.weights[rows[i]];
+                pos[i] = p.positions[rows[i]];
+            }
+#pragma unroll
+            for (int i = 0; i < G; i++) q[i] = t0 + 64 * (i0 + i) < L ? rank_key(w[i], pos[i], from) : 0u;
+        };
         if (KPT) {
-            constexpr int G = KPT % 8 == 0 ? 8 : KPT % 6 == 0 ? 6 : 4;       // loads in flight
 #pragma unroll
             for (int i0 = 0; i0 < KPT; i0 += G) {
-                uint32_t rows[G];
+                uint32_t q[G] = {};
+                if ((uint32_t)i0 < steps) group(i0, q);
 #pragma unroll
-                for (int i = 0; i < G; i++) {
-                    const uint32_t t = t0 + 64 * (i0 + i);
-                    rows[i] = 0;
-                    if ((uint32_t)(i0 + i) < steps && t < L && !p.row(b, h, t, rows[i])) {
-                        gone = true;
-                        rows[i] = 0;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < G; i++) kept_keys[KPT ? i0 + i : 0] = rank_key(p.weights[rows[i]], p.positions[rows[i]], from);
+                for (int i = 0; i < G; i++) kept_keys[KPT ? i0 + i : 0] = q[i];
             }
         } else {
-            for (uint32_t i = 0; i < steps; i++) {
-                const uint32_t t = t0 + 64 * i;
-                uint32_t r;
-                if (t >= L) continue;
-                if (!p.row(b, h, t, r)) gone = true;
-                else far_keys[t] = rank_key(p.weights[r], p.positions[r], from);
+            for (uint32_t i0 = 0; i0 < groups * G; i0 += G) {
+                uint32_t q[G];
+                group(i0, q);
+#pragma unroll
+                for (int i = 0; i < G; i++)
+                    if (i0 + i < steps && t0 + 64 * (i0 + i) < L) far_keys[t0 + 64 * (i0 + i)] = q[i];
             }
         }
     }
@@ -255,7 +295,9 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         if (!MOVE && tid == 0) a.counts[blockIdx.x] = 0;
         return;
     }
-    // (a workspace's keys are read by the thread that wrote them)
+    // Slots past the length have the lowest key and come after all others: no
+    // test keeps them out below.  (A workspace's keys are read by the thread that
+    // wrote them.)
     auto key = [&](uint32_t i) { return KPT ? kept_keys[KPT ? i : 0] : t0 + 64 * i < L ? far_keys[t0 + 64 * i] : 0u; };
     auto each = [&](auto f) {
         if (KPT) {
@@ -268,98 +310,128 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     };
 
     uint32_t prefix = 0, want = budget, tied = 0;    // the want-th largest of the `tied` keys that share the prefix
+    uint32_t* hp = hist;
 #pragma unroll
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t bins = pass == 2 ? 1024 : kBins, mask = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
-        hist[tid] = hist[tid + kCutThreads] = 0;
-        __syncthreads();
+    for (int pass = 0; pass < kPasses; pass++) {
+        const int shift = kShift[pass], bins = kBins[pass], width = pass + 1 < kPasses ? kShift[pass ? pass - 1 : 0] - shift : 7;
+        const uint32_t digits = pass == 0 ? 511u : (1u << width) - 1u;
         each([&](uint32_t i) {
-            const uint32_t q = key(i), digit = (q >> shift) & (bins - 1);
-            const bool in = t0 + 64 * i < L && (q & mask) == prefix;
-            const uint64_t who = __ballot(in);
-            if (!who) return;
+            const uint32_t q = key(i), digit = (q >> shift) & digits;
+            const uint64_t who = pass == 0 ? ~0ull : __ballot((q >> (shift + width)) == (prefix >> (shift + width)));
+            if (who == 0) return;
             // many alike (zeros, recent ones) are counted at once
-            const uint32_t one = __builtin_amdgcn_readlane(digit, __builtin_ctzll(who));
-            if (__ballot(in && digit == one) == who) {
-                if (lane == __builtin_ctzll(who)) atomicAdd(&hist[one], (uint32_t)__popcll(who));
-            } else if (in) {
-                atomicAdd(&hist[digit], 1u);
+            if (who == ~0ull && __ballot(digit != (uint32_t)__builtin_amdgcn_readfirstlane(digit)) == 0) {
+                if (lane == 0) atomicAdd(&hp[digit], 64u);
+            } else if (who >> lane & 1) {
+                atomicAdd(&hp[digit], 1u);
             }
         });
         __syncthreads();
-        // from the top: thread i has bins 2 i and 2 i + 1 below it
-        const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
-        uint32_t sum = hi + lo;
+        // from the top: lane i has the i-th bins / 64 of them, the last the highest
+        constexpr int most = 8;
+        uint32_t n[most];
+        const int per = bins / 64;
+        uint32_t sum = 0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t v = __shfl_up(sum, o);
-            if (lane >= o) sum += v;
-        }
-        if (lane == 63) sh[wave].x = sum;
-        __syncthreads();
-        uint32_t before = sum - hi - lo;
+        for (int j = 0; j < per; j += 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(hp + bins - per * (lane + 1) + j);
 #pragma unroll
-        for (int w = 0; w < kCutWaves; w++)
-            if (w < wave) before += sh[w].x;
-        const bool at_hi = before < want && want <= before + hi;
-        const bool at_lo = !at_hi && before + hi < want && want <= before + hi + lo;
-        if (at_hi || at_lo) {
-            found[0] = (uint32_t)(kBins - 1 - 2 * tid) - (at_lo ? 1u : 0u);
-            found[1] = want - before - (at_lo ? hi : 0u);
-            found[2] = at_hi ? hi : lo;
+            for (int e = 0; e < 4; e++) {
+                n[j + e] = v[e];
+                sum += v[e];
+            }
         }
-        __syncthreads();
-        prefix |= found[0] << shift;
-        want = found[1];
-        tied = found[2];
+        const uint32_t upto = lane_prefix(sum);
+        uint32_t above = upto - sum, digit = 0, count = 0, rest = 0;
+        const uint64_t mine = __ballot(above < want && want <= upto);
+#pragma unroll
+        for (int j = per - 1; j >= 0; j--) {
+            if (above < want && want <= above + n[j]) {
+                digit = bins - per * (lane + 1) + j;
+                rest = want - above;
+                count = n[j];
+            }
+            above += n[j];
+        }
+        const int at = __builtin_ctzll(mine);
+        prefix |= (uint32_t)__builtin_amdgcn_readlane(digit, at) << shift;
+        want = __builtin_amdgcn_readlane(rest, at);
+        tied = __builtin_amdgcn_readlane(count, at);
+        hp += bins;
     }
 
     // of the keys equal to the threshold the first `want` stay
     uint2 total;
     uint32_t ties = 0, none = 0;
     if (want < tied) {
-        each([&](uint32_t i) { ties += __popcll(__ballot(t0 + 64 * i < L && key(i) == prefix)); });
+        each([&](uint32_t i) { ties += __popcll(__ballot(key(i) == prefix)); });
         wave_prefix(ties, none, sh, total);
     }
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
     uint32_t seen = ties;
-    auto stays = [&](uint32_t i) {
-        const uint32_t q = key(i);
-        const bool in = t0 + 64 * i < L, tie = in && q == prefix;
-        if (want == tied) return in && q >= prefix;
-        const uint64_t tb = __ballot(tie);
-        const bool keep = in && (q > prefix || (tie && seen + __popcll(tb & below) < want));
-        seen += __popcll(tb);
-        return keep;
+    auto lane_rank = [&](uint64_t m) {
+        return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
     };
-    uint32_t holes = 0, far = 0;
-    each([&](uint32_t i) {
-        const uint32_t t = t0 + 64 * i;
-        const bool keep = stays(i);
-        holes += __popcll(__ballot(!keep && t < budget));
-        far += __popcll(__ballot(keep && t >= budget));
-    });
-    wave_prefix(holes, far, sh, total);
+    // lanes whose slot of step i stays
+    auto stay = [&](uint32_t i) -> uint64_t {
+        const uint32_t q = key(i);
+        if (want == tied) return __ballot(q >= prefix);
+        const uint64_t tb = __ballot(q == prefix);
+        const uint64_t s = __ballot(q > prefix || (q == prefix && seen + lane_rank(tb) < want));
+        seen += __popcll(tb);
+        return s;
+    };
+    // Up to 64 steps from i0 at once, lane i with step i0 + i: the slots below the
+    // budget that are left free, those from it on that stay, and the numbers of
+    // both before them in the block (the latter in the upper half).
+    auto block = [&](uint32_t i0, uint64_t& hole, uint64_t& far) {
+        uint32_t lo = 0, hi = 0;
+        auto put = [&](uint32_t i) {
+            const uint64_t s = stay(i);
+            const bool me = (uint32_t)lane == i - i0;
+            lo = me ? (uint32_t)s : lo;
+            hi = me ? (uint32_t)(s >> 32) : hi;
+        };
+        if (KPT) each(put);
+        else
+            for (uint32_t i = i0; i < i0 + 64 && i < steps; i++) put(i);
+        const uint64_t s = (uint64_t)hi << 32 | lo;
+        const uint32_t at = w0 + 64 * (i0 + lane);
+        const uint64_t low = i0 + lane >= steps || at >= budget ? 0 : budget - at >= 64 ? ~0ull : ((uint64_t)1 << (budget - at)) - 1;
+        hole = low & ~s;
+        far = s & ~low;
+    };
+    uint32_t holes = 0, fars = 0;
+    uint64_t hole, far;
+    for (uint32_t i0 = 0; i0 < steps; i0 += 64) {
+        block(i0, hole, far);
+        const uint32_t sum = __builtin_amdgcn_readlane(lane_prefix(__popcll(hole) | __popcll(far) << 16), 63);
+        holes += sum & 0xFFFF;
+        fars += sum >> 16;
+    }
+    wave_prefix(holes, fars, sh, total);
     seen = ties;
     uint32_t* const to = MOVE ? list : a.moves + (size_t)blockIdx.x * 2 * a.most;
     uint32_t* const of = to + (MOVE ? kMoveAtOnce : a.most);
-    each([&](uint32_t i) {
-        const uint32_t t = t0 + 64 * i;
-        const bool keep = stays(i), hole = !keep && t < budget, come = keep && t >= budget;
-        const uint64_t hb = __ballot(hole), fb = __ballot(come);
-        if (hole || come) {
-            uint32_t r;
-            (void)p.row(b, h, t, r);
-            if (hole) to[holes + __popcll(hb & below)] = r;
-            else of[far + __popcll(fb & below)] = r;
+    for (uint32_t i0 = 0; i0 < steps; i0 += 64) {
+        if (!KPT) block(i0, hole, far);
+        const uint32_t own = __popcll(hole) | __popcll(far) << 16, upto = lane_prefix(own), before = upto - own;
+        const uint32_t end = i0 + 64 < steps ? 64 : steps - i0;
+        for (uint32_t i = 0; i < end; i++) {
+            const uint64_t hb = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(hole >> 32), i) << 32 |
+                                (uint32_t)__builtin_amdgcn_readlane((uint32_t)hole, i);
+            const uint64_t fb = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(far >> 32), i) << 32 |
+                                (uint32_t)__builtin_amdgcn_readlane((uint32_t)far, i);
+            const uint32_t at = __builtin_amdgcn_readlane(before, i), t = t0 + 64 * (i0 + i);
+            if (hb >> lane & 1) to[holes + (at & 0xFFFF) + lane_rank(hb)] = t;
+            if (fb >> lane & 1) of[fars + (at >> 16) + lane_rank(fb)] = t;
         }
-        holes += __popcll(hb);
-        far += __popcll(fb);
-    });
+        const uint32_t sum = __builtin_amdgcn_readlane(upto, 63);
+        holes += sum & 0xFFFF;
+        fars += sum >> 16;
+    }
     if (MOVE) {
         __syncthreads();
-        move_rows(p, a.row_bytes, to, of, total.x, tid, kCutThreads);
+        move_rows(p, b, h, a.row_bytes, to, of, total.x, tid, kCutThreads);
     } else if (tid == 0) {
         a.counts[blockIdx.x] = total.x;
     }
@@ -367,10 +439,10 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
 
 // The moves that k_kv_cut listed.  Sources lie in slots from the budget on and
 // targets below it, so all are independent.
-__global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a) {
-    const uint32_t bh = blockIdx.y, n = a.counts[bh];
+__global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a, uint32_t first) {
+    const uint32_t bh = first + blockIdx.y, b = bh / p.heads, n = a.counts[bh];
     const uint32_t* to = a.moves + (size_t)bh * 2 * a.most;
-    move_rows(p, a.row_bytes, to, to + a.most, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    move_rows(p, b, bh - b * p.heads, a.row_bytes, to, to + a.most, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 template <int LR>
@@ -465,10 +537,8 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
     const size_t chunks = (size_t)a.most * (a.row_bytes / 16), gx = (chunks + 1023) / 1024;
     for (size_t at = 0; at < bh; at += 65535) {
         const size_t n = bh - at < 65535 ? bh - at : 65535;
-        k_kv_move<<<dim3((unsigned)(gx < 65536 ? gx : 65536), (unsigned)n), 256, 0, S(st)>>>(p, a);
+        k_kv_move<<<dim3((unsigned)(gx < 65536 ? gx : 65536), (unsigned)n), 256, 0, S(st)>>>(p, a, (uint32_t)at);
         if (snx_launch_check("k_kv_move")) return -1;
-        a.counts += n;
-        a.moves += n * 2 * a.most;
     }
     return 0;
 }
