@@ -130,6 +130,7 @@ constexpr int kCutWaves = 16;
 constexpr int kCutThreads = 64 * kCutWaves;
 constexpr int kPasses = 4;               // digits of 9, 8, 8 and 7 bits: sign and exponent first
 constexpr int kShift[kPasses] = {23, 15, 7, 0}, kBins[kPasses] = {512, 256, 256, 256};
+constexpr uint32_t kSome = 4096;         // keys that share the first digit and are kept apart
 constexpr uint32_t kMoveAtOnce = 64;     // moves that the workgroup which finds them makes itself
 
 // two counts per wave -> their exclusive prefixes over the waves, and the totals
@@ -233,6 +234,7 @@ template <int KPT, bool MOVE>
 __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
     constexpr int kHist = kBins[0] + kBins[1] + kBins[2] + kBins[3];
     __shared__ __attribute__((aligned(16))) uint32_t hist[kHist];
+    __shared__ uint32_t some[KPT == 4 ? 1 : kSome], some_n;
     __shared__ uint2 sh[kCutWaves];
     __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
@@ -243,6 +245,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     uint32_t* const far_keys = KPT ? nullptr : a.keys + (size_t)blockIdx.x * a.max_length;
 
     for (int i = tid; i < kHist; i += kCutThreads) hist[i] = 0;
+    if (tid == 0) some_n = 0;
     uint32_t kept_keys[KPT ? KPT : 1];
     bool gone = false;
     if (L > budget) {
@@ -309,23 +312,52 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         }
     };
 
+    auto lane_rank = [&](uint64_t m) {
+        return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+    };
+
     uint32_t prefix = 0, want = budget, tied = 0;    // the want-th largest of the `tied` keys that share the prefix
+    bool few = false;                                // these are in `some`
     uint32_t* hp = hist;
 #pragma unroll
     for (int pass = 0; pass < kPasses; pass++) {
-        const int shift = kShift[pass], bins = kBins[pass], width = pass + 1 < kPasses ? kShift[pass ? pass - 1 : 0] - shift : 7;
-        const uint32_t digits = pass == 0 ? 511u : (1u << width) - 1u;
-        each([&](uint32_t i) {
-            const uint32_t q = key(i), digit = (q >> shift) & digits;
-            const uint64_t who = pass == 0 ? ~0ull : __ballot((q >> (shift + width)) == (prefix >> (shift + width)));
-            if (who == 0) return;
-            // many alike (zeros, recent ones) are counted at once
-            if (who == ~0ull && __ballot(digit != (uint32_t)__builtin_amdgcn_readfirstlane(digit)) == 0) {
-                if (lane == 0) atomicAdd(&hp[digit], 64u);
-            } else if (who >> lane & 1) {
-                atomicAdd(&hp[digit], 1u);
+        if (want == tied) break;                     // all of them stay, whatever their other digits are
+        const int shift = kShift[pass], bins = kBins[pass], width = pass == 0 ? 9 : pass == 3 ? 7 : 8;
+        const uint32_t digits = (1u << width) - 1u, above_shift = (shift + width) & 31;
+        // One pass over all keys puts those that are left aside, if there is room
+        // (8192 x 8 heads x 8 rows: 17 -> XX us).
+        if (KPT != 4 && pass == 1 && tied <= kSome) {
+            few = true;
+            each([&](uint32_t i) {
+                const uint32_t q = key(i);
+                const bool in = q >> above_shift == prefix >> above_shift;
+                const uint64_t who = __ballot(in);
+                if (who == 0) return;
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&some_n, (uint32_t)__popcll(who));
+                at = __builtin_amdgcn_readfirstlane(at);
+                if (in) some[at + lane_rank(who)] = q;
+            });
+            __syncthreads();
+        }
+        if (few) {
+            for (uint32_t i = tid; i < kSome && i < some_n; i += kCutThreads) {
+                const uint32_t q = some[i];
+                if (q >> above_shift == prefix >> above_shift) atomicAdd(&hp[(q >> shift) & digits], 1u);
             }
-        });
+        } else {
+            each([&](uint32_t i) {
+                const uint32_t q = key(i), digit = (q >> shift) & digits;
+                const uint64_t who = pass == 0 ? ~0ull : __ballot(q >> above_shift == prefix >> above_shift);
+                if (who == 0) return;
+                // many alike (zeros, recent ones) are counted at once
+                if (who == ~0ull && __ballot(digit != (uint32_t)__builtin_amdgcn_readfirstlane(digit)) == 0) {
+                    if (lane == 0) atomicAdd(&hp[digit], 64u);
+                } else if (who >> lane & 1) {
+                    atomicAdd(&hp[digit], 1u);
+                }
+            });
+        }
         __syncthreads();
         // from the top: lane i has the i-th bins / 64 of them, the last the highest
         constexpr int most = 8;
@@ -368,9 +400,6 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         wave_prefix(ties, none, sh, total);
     }
     uint32_t seen = ties;
-    auto lane_rank = [&](uint64_t m) {
-        return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-    };
     // lanes whose slot of step i stays
     auto stay = [&](uint32_t i) -> uint64_t {
         const uint32_t q = key(i);
