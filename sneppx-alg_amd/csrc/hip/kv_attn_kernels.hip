@@ -19,6 +19,7 @@
 
 #include <cstdint>
 
+
 #include "codec.h"
 #include "kv_pool.h"
 #include "launch.h"
@@ -38,21 +39,94 @@ typedef __attribute__((address_space(3))) uint8_t* lds_t;
 
 hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
+constexpr int SLOT_KV_ATTN = 7;       // of the stream's workspaces
 constexpr int TILE = 32;              // tokens of a wave's step
 constexpr int WAVES = 4;
 constexpr int STEP = TILE * WAVES;    // tokens of a workgroup's step: chunks are multiples of it
+
+// Workgroups of a CU (waves of a SIMD) for token rows of `bytes`: what the
+// registers allow of a tile's keys, values, queries and outputs.  At three for
+// rows of 256 bytes some of them spill (131072 tokens in bf16: 98 us at two, 113
+// at three), at two for 512 bytes (XX at one, XX at two).
+constexpr int resident(int bytes) { return bytes <= 128 ? 3 : bytes <= 256 ? 2 : 1; }
 
 struct Attn {
     const uint16_t* q;
     void* out;
     size_t q_stride, out_stride;
     const int32_t* lengths;
-    float* part;              // [rows][q_heads][splits][dim]
-    float2* ml;               // [rows][q_heads][splits]: maximum, sum
+    uint32_t* arrivals;       // [rows * kv_heads * tiles], zero, or NULL: k_kv_join follows
+    float* part;              // [chunks of all rows][kv_heads * tiles][heads][dim]
+    float2* ml;               // [chunks of all rows][kv_heads * tiles][heads]: maximum, sum
     float* logits;            // [rows][q_heads][logit_stride], or NULL
-    uint32_t q_heads, max_length, splits, chunk, tiles, logit_stride, pairs;
+    uint32_t rows, q_heads, max_length, tiles, heads, share, logit_stride;
     float scale_log2;
-    int out_f32, q_aligned, direct;
+    int out_f32, q_aligned;
+};
+
+// ------------------------------------------------------------- the division
+// A row's tokens are cut into chunks of the same number of steps for all rows,
+// as many as make `share` chunks of all rows' tokens together (a row has one at
+// least, 256 at most).  The lengths are known on the device alone, so every wave
+// works this out for itself: from max_length, which may be far above them, the
+// host could not (16 rows of 0 to 4096 tokens in chunks of max_length / 8: 45 us;
+// so: XX).
+struct Row {
+    uint32_t b, chunk0, n, len;    // the row, its first chunk's number, its chunks (0: no such row), its length
+};
+
+struct Division {
+    const Attn& a;
+    uint32_t len0, per;            // length of row `lane`; steps of a chunk
+    __device__ __forceinline__ explicit Division(const Attn& attn) : a(attn) {
+        const uint32_t lane = threadIdx.x & 63;
+        uint32_t total = 0, longest = 0;
+        len0 = length(lane);
+        for (uint32_t r0 = 0; r0 < a.rows; r0 += 64) {
+            const uint32_t n = steps(r0 ? length(r0 + lane) : len0);
+            total += n;
+            longest = n > longest ? n : longest;
+        }
+        total = __builtin_amdgcn_readlane(lane_prefix(total), 63);
+        per = (total + a.share - 1) / a.share;
+        const uint32_t least = (lane_max(longest) + 255) / 256;
+        per = per > least ? per : least;
+        per = per > 1 ? per : 1;
+    }
+    __device__ __forceinline__ uint32_t length(uint32_t r) const { return r < a.rows ? kv_length(a.lengths, r, a.max_length) : 0; }
+    static __device__ __forceinline__ uint32_t steps(uint32_t len) { return (len + STEP - 1) / STEP; }
+    // chunks of up to 64 rows from r0, one per lane
+    __device__ __forceinline__ uint32_t chunks(uint32_t r0, uint32_t& len) const {
+        const uint32_t r = r0 + (threadIdx.x & 63);
+        len = r0 ? length(r) : len0;
+        const uint32_t n = (steps(len) + per - 1) / per;
+        return r < a.rows ? n > 1 ? n : 1 : 0;
+    }
+    __device__ __forceinline__ Row pick(uint32_t r0, uint32_t base, uint32_t n, uint32_t upto, uint32_t len, int lane) const {
+        return Row{r0 + lane, base + (uint32_t)__builtin_amdgcn_readlane(upto - n, lane),
+                   (uint32_t)__builtin_amdgcn_readlane(n, lane), (uint32_t)__builtin_amdgcn_readlane(len, lane)};
+    }
+    // the row that has chunk number c
+    __device__ __forceinline__ Row of_chunk(uint32_t c) const {
+        uint32_t base = 0;
+        for (uint32_t r0 = 0; r0 < a.rows; r0 += 64) {
+            uint32_t len;
+            const uint32_t n = chunks(r0, len), upto = lane_prefix(n);
+            const uint64_t behind = __ballot(base + upto > c);
+            if (behind) return pick(r0, base, n, upto, len, __builtin_ctzll(behind));
+            base += __builtin_amdgcn_readlane(upto, 63);
+        }
+        return Row{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ Row of_row(uint32_t b) const {
+        uint32_t base = 0;
+        for (uint32_t r0 = 0;; r0 += 64) {
+            uint32_t len;
+            const uint32_t n = chunks(r0, len), upto = lane_prefix(n);
+            if (b < r0 + 64) return pick(r0, base, n, upto, len, (int)(b - r0));
+            base += __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
 };
 
 // max / sum over the four lanes that differ in bits 4 and 5
@@ -113,30 +187,122 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&piece)[3]) 
     for (int i = 0; i < 3; i++) piece[i] = __builtin_bit_cast(bf16x8, o[i]);
 }
 
-// Where 16-byte chunk c of token row r lies in a wave's value tile (rows of
-// RB bytes).  The transposed reads take 32 (int8: 16) bytes of the same
-// columns from 8 (16) rows at once, the writes one chunk of 16 rows: both
-// spread over all banks.
-template <int RB, bool I8>
-__device__ __forceinline__ int v_chunk(int r, int c) {
-    if constexpr (I8) {
-        constexpr int per = RB < 256 ? 256 / RB : 1;                   // rows in 256 bytes
-        const int f = (r / per) ^ ((r >> 4) << 1);
-        return r * (RB / 16) + (c ^ (f & (RB / 16 - 1)));
-    } else {
-        const int f = RB == 128 ? ((r >> 1) & 1) | ((r >> 3) & 1) << 1 : (r & 3) | ((r >> 3) & 1) << 2;
-        return r * (RB / 16) + ((((c >> 1) ^ f) << 1) | ((c & 1) ^ (r >> 4)));
-    }
-}
-
+// A wave's value tile in LDS: token rows of RB bytes.  The transposed reads take
+// 32 bytes (int8: 16) of the same columns from 8 (16) rows at once, the writes
+// 16 bytes of 16 rows; the row stride and the order of the rows spread both over
+// all banks, and leave every address a lane's own base plus a constant.
 template <int DP, bool I8>
 struct Lds {
     static constexpr int RB = DP * (I8 ? 1 : 2);                // bytes of a token's row
-    static constexpr int V = TILE * RB;                         // a wave's value tile
+    static constexpr int STRIDE = RB + (I8 ? 16 : 32);
+    static constexpr int UPPER = I8 ? 64 : 16;                  // rows from 16 on lie this much further
+    static constexpr int V = TILE * STRIDE + UPPER;             // a wave's value tile
     static constexpr int WAVE = V + (I8 ? 2 * TILE * 4 : 0);    // and its scales
     static constexpr int OS = DP + 4;                           // floats of a head's row at the end
     static constexpr int END = WAVES * 16 * OS * 4;
     static constexpr int ALL = END > WAVES * WAVE ? END : WAVES * WAVE;
+    // bf16: tokens 0 - 3, 8 - 11, 4 - 7, 12 - 15 (and so the upper half)
+    static __device__ __forceinline__ int row(int tok) {
+        const int at = I8 ? tok : (tok & 19) | ((tok >> 1) & 4) | ((tok << 1) & 8);
+        return at * STRIDE + (tok >> 4) * UPPER;
+    }
+};
+
+// ------------------------------------------------------ the chunks' results
+// Of each chunk and query head the weighted values, maximum and sum.  They are
+// stored past the L2s, which the XCDs do not share, and read so, for the
+// workgroup that arrives last may join them within the launch.
+constexpr int kSysCoherent = 1 | 16;            // buffer cache policy sc0 sc1
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, -1, 0x00020000);
+}
+
+struct Parts {
+    const Attn& a;
+    __amdgpu_buffer_rsrc_t part, ml;
+    uint32_t dim, units, unit;     // unit: key-value head and tile of 16 query heads
+    __device__ __forceinline__ Parts(const Attn& attn, uint32_t d, uint32_t n, uint32_t u)
+        : a(attn), part(rsrc(attn.part)), ml(rsrc(attn.ml)), dim(d), units(n), unit(u) {}
+    __device__ __forceinline__ uint32_t at(uint32_t chunk, uint32_t head) const { return (chunk * units + unit) * a.heads + head; }
+    __device__ __forceinline__ void put(uint32_t chunk, uint32_t head, uint32_t d, f32x4 v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at(chunk, head) * dim + d) * 4, 0, kSysCoherent);
+    }
+    __device__ __forceinline__ void put_ml(uint32_t chunk, uint32_t head, float m, float l) const {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{f2u(m), f2u(l)}, ml, at(chunk, head) * 8, 0, kSysCoherent);
+    }
+    __device__ __forceinline__ f32x4 get(uint32_t chunk, uint32_t head, uint32_t d) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, (at(chunk, head) * dim + d) * 4, 0, kSysCoherent));
+    }
+    __device__ __forceinline__ float2 get_ml(uint32_t chunk, uint32_t head) const {
+        const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(ml, at(chunk, head) * 8, 0, kSysCoherent);
+        return make_float2(u2f(r[0]), u2f(r[1]));
+    }
+
+    // maximum and 1 / sum of a query head over its row's chunks, by one wave: 0
+    // for no tokens, NaN where there are tokens and every logit is -inf
+    __device__ __forceinline__ float2 whole(const Row& w, uint32_t head) const {
+        const uint32_t lane = threadIdx.x & 63;
+        float2 e[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            e[j] = 64 * j + lane < w.n ? get_ml(w.chunk0 + 64 * j + lane, head) : make_float2(-INFINITY, 0.0f);
+        float top = fmaxf(fmaxf(e[0].x, e[1].x), fmaxf(e[2].x, e[3].x));
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        float total = 0.0f, plain = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            total += (e[j].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e[j].x - top)) * e[j].y;
+            plain += e[j].y;
+        }
+        for (int o = 32; o > 0; o >>= 1) {
+            total += __shfl_xor(total, o);
+            plain += __shfl_xor(plain, o);
+        }
+        return make_float2(top, top == -INFINITY ? plain == 0.0f ? 0.0f : NAN : 1.0f / total);
+    }
+
+    // One wave joins the chunks of a query head and writes its result: 4 elements
+    // per lane, the chunks in 64 / span turns, added in a fixed order.
+    __device__ __forceinline__ void join(const Row& w, uint32_t head, uint32_t hq) const {
+        constexpr int U = 16;             // loads in flight
+        const uint32_t lane = threadIdx.x & 63;
+        const uint32_t span = dim <= 64 ? 16 : dim <= 128 ? 32 : 64, ways = 64 / span;
+        const uint32_t d = 4 * (lane & (span - 1)), way = lane / span;
+        const float2 st = whole(w, head);
+        const bool in = d < dim;
+        f32x4 v = {};
+        for (uint32_t i0 = way; i0 < w.n; i0 += U * ways) {
+            f32x4 x[U];
+            float m[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const bool on = i0 + u * ways < w.n;
+                const uint32_t c = w.chunk0 + (on ? i0 + u * ways : 0);
+                x[u] = get(c, head, in ? d : 0);
+                m[u] = get_ml(c, head).x;
+                if (!on) m[u] = -INFINITY;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float f = m[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[u] - st.x);
+                if (i0 + u * ways < w.n) v += f * x[u];
+            }
+        }
+        for (uint32_t o = span; o < 64; o <<= 1)
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += __shfl_xor(v[j], o);
+        if (way == 0 && in) store(w.b, hq, d, v, st.y);
+    }
+
+    __device__ __forceinline__ void store(uint32_t b, uint32_t hq, uint32_t d, f32x4 v, float inv) const {
+        const size_t to = b * a.out_stride + (size_t)hq * dim + d;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (a.out_f32) static_cast<float*>(a.out)[to + j] = v[j] * inv;
+            else static_cast<uint16_t*>(a.out)[to + j] = bf16_out(v[j] * inv);
+        }
+    }
 };
 
 // Lane l = 16 g + r.  Keys are the A operand of 16x16x32 products (token rows)
@@ -152,8 +318,8 @@ struct Lds {
 // A wave's tile is read while it computes the one before: keys into the
 // registers that the first product has just used, values into those that
 // went to LDS.
-template <int DP, bool I8, bool SAVE>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+template <int DP, bool I8, bool SAVE, bool FULL>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(resident(DP * (I8 ? 1 : 2)))))
 k_kv_attn(const KVPool p, const Attn a) {
     typedef Lds<DP, I8> L;
     constexpr int NC = L::RB / 64;        // 16-byte chunks of a row per lane
@@ -161,22 +327,27 @@ k_kv_attn(const KVPool p, const Attn a) {
     constexpr int DT = DP / 16;           // tiles of 16 output elements
     __shared__ __attribute__((aligned(16))) uint8_t lds[L::ALL];
     __shared__ float2 ends[WAVES][16];
+    __shared__ uint32_t arrived;
 
-    uint32_t x = blockIdx.x;
-    const uint32_t ht = x % a.tiles;
-    x /= a.tiles;
-    const uint32_t split = x % a.splits, bh = x / a.splits;
-    const uint32_t b = bh / p.heads, h = bh - b * p.heads;
-    const uint32_t len = kv_length(a.lengths, b, a.max_length);
-    const uint32_t first = split * a.chunk, last = first + a.chunk < len ? first + a.chunk : len;
-    if (first >= len && !(a.direct && split == 0)) return;
+    // The units of a chunk, then the next chunk: workgroups go to the XCDs in turn,
+    // and so every XCD gets chunks of all rows.
+    const uint32_t units = p.heads * a.tiles, number = blockIdx.x / units, unit = blockIdx.x - number * units;
+    const Division cut(a);
+    const Row w = cut.of_chunk(number);
+    if (w.n == 0) return;
+    const uint32_t b = w.b, h = unit / a.tiles, ht = unit - h * a.tiles;
+    // its steps are dealt out evenly (below 2^24 steps, 256 chunks)
+    const uint32_t i = number - w.chunk0, steps = Division::steps(w.len);
+    const uint32_t first = i * steps / w.n * STEP, end = (i + 1) * steps / w.n * STEP;
+    const uint32_t last = end < w.len ? end : w.len;
+    const Parts parts(a, FULL ? DP : p.dim, units, unit);
 
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t group = a.q_heads / p.heads;
     const uint32_t nh = group - ht * 16 < 16 ? group - ht * 16 : 16;
     const uint32_t hq = h * group + ht * 16;             // the first of the tile's query heads
-    const uint32_t row_bytes = p.dim * (I8 ? 1 : 2);
+    const uint32_t dim = FULL ? DP : p.dim, row_bytes = dim * (I8 ? 1 : 2);
     uint8_t* const vt = lds + wave * L::WAVE;
     float* const sc = reinterpret_cast<float*>(vt + L::V);
 
@@ -185,8 +356,8 @@ k_kv_attn(const KVPool p, const Attn a) {
     for (int s = 0; s < KS; s++) {
         const uint32_t d = I8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 8 * (g + 4 * s);
         u32x4 w = {0u, 0u, 0u, 0u};
-        if ((uint32_t)r < nh && d < p.dim) {
-            const uint16_t* src = a.q + b * a.q_stride + (size_t)(hq + r) * p.dim + d;
+        if ((uint32_t)r < nh && d < dim) {
+            const uint16_t* src = a.q + b * a.q_stride + (size_t)(hq + r) * dim + d;
             if (a.q_aligned) w = *reinterpret_cast<const u32x4*>(src);
             else
 #pragma unroll
@@ -222,7 +393,7 @@ k_kv_attn(const KVPool p, const Attn a) {
     float ksc[2], vsc[2];
     auto chunk_at = [&](const uint8_t* pool, int t, int i) {
         const uint32_t c = 16 * (g + 4 * i);
-        return *reinterpret_cast<const u32x4*>(pool + (size_t)row[t] * row_bytes + (c < row_bytes ? c : 0));
+        return *reinterpret_cast<const u32x4*>(pool + (size_t)row[t] * row_bytes + (FULL || c < row_bytes ? c : 0));
     };
     auto load_k = [&] {
 #pragma unroll
@@ -266,7 +437,7 @@ k_kv_attn(const KVPool p, const Attn a) {
                 if (I8) kf = (i & 1) ? bytes_to_bf16(w[2], w[3]) : bytes_to_bf16(w[0], w[1]);
                 else kf = __builtin_bit_cast(bf16x8, w);
                 // past the head's end the lane has other elements, maybe NaN
-                if (p.dim != DP && (I8 ? 16 * (g + 4 * (i >> 1)) : 8 * (g + 4 * i)) >= (int)p.dim)
+                if (!FULL && (I8 ? 16 * (g + 4 * (i >> 1)) : 8 * (g + 4 * i)) >= (int)dim)
                     kf = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
                 s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i], s[t], 0, 0, 0);
             }
@@ -287,7 +458,7 @@ k_kv_attn(const KVPool p, const Attn a) {
             for (int i = 0; i < NC; i++) {
                 u32x4 w = vc[t][i];
                 if (!whole && !ok[t]) w = u32x4{0u, 0u, 0u, 0u};
-                *reinterpret_cast<u32x4*>(vt + 16 * v_chunk<L::RB, I8>(tok, g + 4 * i)) = w;
+                *reinterpret_cast<u32x4*>(vt + L::row(tok) + 16 * (g + 4 * i)) = w;
             }
             if (I8 && g == 0) sc[TILE + tok] = ok[t] ? vsc[t] : 0.0f;
         }
@@ -339,15 +510,15 @@ k_kv_attn(const KVPool p, const Attn a) {
             bf16x8 vf;
             if (I8) {
                 const int tok = 8 * g + (r >> 1);
-                const lds_t at = (lds_t)(vt + 16 * v_chunk<L::RB, true>(tok, dt) + 8 * (r & 1));
+                const lds_t at = (lds_t)(vt + L::row(tok) + 8 * (r & 1) + 16 * dt);
                 const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)at);
                 vf = bytes_to_bf16((uint32_t)w[0], (uint32_t)w[1]);
             } else {
                 s16x4 w[2];
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const int tok = 8 * g + 4 * t + (r >> 2), c = 2 * dt + ((r >> 1) & 1);
-                    const lds_t at = (lds_t)(vt + 16 * v_chunk<L::RB, false>(tok, c) + 8 * (r & 1));
+                    const int tok = 8 * g + 4 * t + (r >> 2);
+                    const lds_t at = (lds_t)(vt + L::row(tok) + 8 * (r & 3) + 32 * dt);
                     w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
                 }
                 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -371,14 +542,13 @@ k_kv_attn(const KVPool p, const Attn a) {
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f32x4*>(ow + r * L::OS + 16 * dt + 4 * g) = o[dt];
     __syncthreads();
-    const uint32_t quads = p.dim / 4;
+    const uint32_t quads = dim / 4;
     for (uint32_t i = tid; i < nh * quads; i += 256) {
         const uint32_t hd = i / quads, d = 4 * (i - hd * quads);
-        float top = -INFINITY, total = 0.0f;
+        float top = -INFINITY, total = 0.0f, plain = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) top = fmaxf(top, ends[w][hd].x);
         f32x4 v = {};
-        float plain = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
             const float2 e = ends[w][hd];
@@ -388,137 +558,90 @@ k_kv_attn(const KVPool p, const Attn a) {
             v += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds) + (w * 16 + hd) * L::OS + d);
         }
         if (top == -INFINITY) total = plain > 1.0f ? 1.0f : plain;
-        if (a.direct) {
-            const float inv = top == -INFINITY ? total == 0.0f ? 0.0f : NAN : 1.0f / total;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const size_t at = b * a.out_stride + (size_t)(hq + hd) * p.dim + d + j;
-                if (a.out_f32) static_cast<float*>(a.out)[at] = v[j] * inv;
-                else static_cast<uint16_t*>(a.out)[at] = bf16_out(v[j] * inv);
-            }
+        if (!SAVE && w.n == 1) {
+            parts.store(b, hq + hd, d, v, top == -INFINITY ? total == 0.0f ? 0.0f : NAN : 1.0f / total);
         } else {
-            const size_t at = ((size_t)b * a.q_heads + hq + hd) * a.splits + split;
-            *reinterpret_cast<f32x4*>(a.part + at * p.dim + d) = v;
-            if (d == 0) a.ml[at] = make_float2(top, total);
+            parts.put(number, hd, d, v);
+            if (d == 0) parts.put_ml(number, hd, top, total);
         }
     }
+    if (SAVE || w.n == 1 || !a.arrivals) return;
+    // the last of the row's chunks to arrive joins them
+    __builtin_amdgcn_s_waitcnt(0x0f70);              // vmcnt(0): this wave's stores are out
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t* const mine = a.arrivals + (size_t)b * units + unit;
+        const uint32_t c = atomicAdd(mine, 1u);
+        if (c == w.n - 1) atomicExch(mine, 0u);      // ready for the next call
+        arrived = c;
+    }
+    __syncthreads();
+    if (arrived != w.n - 1) return;
+    for (uint32_t j = wave; j < nh; j += WAVES) parts.join(w, j, hq + j);
 }
 
-// One workgroup per (row, key-value head, x): joins the chunks of the group's
-// query heads x, x + gridDim.x, .. and, with logits, adds the attention weights
-// of tokens 256 x .., every 256 gridDim.x.
-__global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a) {
+// After k_kv_attn, workgroups x of every (row, key-value head): the first
+// `joins` join the chunks of four query heads of the group, one a wave, where
+// there are several or (with logits) anyhow; with logits the others add the
+// attention weights of 256 tokens each.
+__global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, uint32_t joins) {
     __shared__ float2 stat[256];      // of a head: maximum, 1 / sum
-    __shared__ float red[256];
     const uint32_t bh = blockIdx.y + blockIdx.z * 65535u;
-    if (bh >= a.pairs) return;
+    if (bh >= a.rows * p.heads) return;
     const uint32_t b = bh / p.heads, h = bh - b * p.heads;
     const uint32_t group = a.q_heads / p.heads;
-    const uint32_t len = kv_length(a.lengths, b, a.max_length);
-    const uint32_t n = (len + a.chunk - 1) / a.chunk;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    auto parts = [&](uint32_t j) { return Parts(a, p.dim, p.heads * a.tiles, h * a.tiles + j / 16); };
 
-    // maximum and 1 / sum of a query head over its chunks, by one wave: 0 for
-    // no tokens, NaN where there are tokens and every logit is -inf
-    auto whole = [&](uint32_t hq) {
-        const float2* ml = a.ml + ((size_t)b * a.q_heads + hq) * a.splits;
-        float top = -INFINITY, total = 0.0f, plain = 0.0f;
-        for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, ml[i].x);
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        for (uint32_t i = lane; i < n; i += 64) {
-            const float2 e = ml[i];
-            total += (e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top)) * e.y;
-            plain += e.y;
-        }
-        for (int o = 32; o > 0; o >>= 1) {
-            total += __shfl_xor(total, o);
-            plain += __shfl_xor(plain, o);
-        }
-        return make_float2(top, top == -INFINITY ? plain == 0.0f ? 0.0f : NAN : 1.0f / total);
-    };
-
-    const uint32_t threads = p.dim <= 64 ? 64 : p.dim <= 128 ? 128 : 256, ways = 256 / threads;
-    const uint32_t d = tid % threads, way = tid / threads;
-    for (uint32_t j = blockIdx.x; j < group; j += gridDim.x) {
-        const uint32_t hq = h * group + j;
-        const float2 st = whole(hq);
-        const size_t at = ((size_t)b * a.q_heads + hq) * a.splits;
-        float v = 0.0f;
-        if (d < p.dim)
-#pragma unroll 4
-            for (uint32_t i = way; i < n; i += ways) {
-                const float mx = a.ml[at + i].x;
-                v += (mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - st.x)) * a.part[(at + i) * p.dim + d];
-            }
-        red[tid] = v;
+    if (blockIdx.x < joins) {
+        const Row w = Division(a).of_row(b);
+        if (a.logits || w.n > 1)
+            for (uint32_t j = 4 * blockIdx.x + wave; j < group; j += 4 * joins) parts(j).join(w, j % 16, h * group + j);
+        return;
+    }
+    // what does not depend on the chunks is loaded first
+    constexpr int G = 8;
+    const uint32_t t = (blockIdx.x - joins) * 256 + tid, len = kv_length(a.lengths, b, a.max_length);
+    if ((blockIdx.x - joins) * 256 >= len) return;
+    uint32_t row = 0;
+    const bool ok = t < len && p.row(b, h, t, row);
+    const float* const s = a.logits + ((size_t)b * a.q_heads + h * group) * a.logit_stride + (ok ? t : 0);
+    float v[G], before = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < G; j++) v[j] = s[(size_t)((uint32_t)j < group ? j : 0) * a.logit_stride];
+    if (ok) before = p.weights[row];
+    const Row w = Division(a).of_row(b);
+    for (uint32_t j0 = 0; j0 < group; j0 += 256) {
+        const uint32_t nj = group - j0 < 256 ? group - j0 : 256;
         __syncthreads();
-        if (way == 0 && d < p.dim) {
-            for (uint32_t w = 1; w < ways; w++) v += red[w * threads + d];
-            const size_t to = b * a.out_stride + (size_t)hq * p.dim + d;
-            if (a.out_f32) static_cast<float*>(a.out)[to] = v * st.y;
-            else static_cast<uint16_t*>(a.out)[to] = bf16_out(v * st.y);
+        for (uint32_t j = wave; j < nj; j += 4) {
+            const float2 st = parts(j0 + j).whole(w, (j0 + j) % 16);
+            if (lane == 0) stat[j] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y);
         }
         __syncthreads();
-    }
-    if (!a.logits || !len) return;
-    for (uint32_t t0 = blockIdx.x * 256; t0 < len; t0 += gridDim.x * 256) {
-        const uint32_t t = t0 + tid;
-        uint32_t row = 0;
-        const bool ok = t < len && p.row(b, h, t, row);
-        float w = 0.0f;
-        for (uint32_t j0 = 0; j0 < group; j0 += 256) {
-            const uint32_t nj = group - j0 < 256 ? group - j0 : 256;
-            __syncthreads();
-            for (uint32_t j = wave; j < nj; j += 4) {
-                const float2 st = whole(h * group + j0 + j);
-                if (lane == 0) stat[j] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y);
-            }
-            __syncthreads();
-            if (ok) {
-                const float* s = a.logits + ((size_t)b * a.q_heads + h * group + j0) * a.logit_stride + t;
-#pragma unroll 4
-                for (uint32_t j = 0; j < nj; j++)
-                    w += __builtin_amdgcn_exp2f(s[(size_t)j * a.logit_stride] - stat[j].x) * stat[j].y;
-            }
+        for (uint32_t j1 = 0; j1 < nj; j1 += G) {
+            if (j0 + j1)
+#pragma unroll
+                for (int j = 0; j < G; j++) v[j] = s[(size_t)(j1 + j < nj ? j0 + j1 + j : 0) * a.logit_stride];
+#pragma unroll
+            for (int j = 0; j < G; j++)
+                if (j1 + j < nj) sum += __builtin_amdgcn_exp2f(v[j] - stat[j1 + j].x) * stat[j1 + j].y;
         }
-        if (ok) p.weights[row] += w;
     }
+    if (ok) p.weights[row] = before + sum;
 }
 
 uint32_t div_up(size_t a, size_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// How a call is cut: chunks of the longest row, and its parts of the workspace.
-struct Plan {
-    uint32_t tiles, chunk, splits, logit_stride;
-    size_t part, ml, logits;
-    bool direct;
-    size_t bytes() const { return part + ml + logits; }
-};
-
-Plan plan(const SNEPPXKVCache* c, size_t rows, size_t q_heads, size_t max_length, int accumulate) {
-    Plan n;
-    const size_t group = q_heads / c->kv_heads;
-    n.tiles = div_up(group, 16);
-    const size_t units = rows * c->kv_heads * n.tiles;
-    const size_t want = (size_t)4 * cu_count();
-    size_t splits = (want + units - 1) / units;
-    const size_t most = max_length ? div_up(max_length, STEP) : 1;
-    if (splits > most) splits = most;
-    if (splits > 256) splits = 256;
-    n.chunk = max_length ? div_up(div_up(max_length, splits), STEP) * STEP : STEP;
-    n.splits = max_length ? div_up(max_length, n.chunk) : 1;
-    n.direct = n.splits == 1 && !accumulate;
-    n.logit_stride = accumulate ? n.splits * n.chunk : 0;
-    n.part = n.direct ? 0 : rows * q_heads * n.splits * c->head_dim * sizeof(float);
-    n.ml = n.direct ? 0 : rows * q_heads * n.splits * sizeof(float2);
-    n.logits = accumulate ? rows * q_heads * (size_t)n.logit_stride * sizeof(float) : 0;
-    return n;
-}
-
 template <int DP, bool I8>
 void launch(unsigned grid, bool save, const KVPool& p, const Attn& a, hipStream_t s) {
-    if (save) k_kv_attn<DP, I8, true><<<grid, 256, 0, s>>>(p, a);
-    else k_kv_attn<DP, I8, false><<<grid, 256, 0, s>>>(p, a);
+    if (p.dim == DP) {
+        if (save) k_kv_attn<DP, I8, true, true><<<grid, 256, 0, s>>>(p, a);
+        else k_kv_attn<DP, I8, false, true><<<grid, 256, 0, s>>>(p, a);
+    } else {
+        if (save) k_kv_attn<DP, I8, true, false><<<grid, 256, 0, s>>>(p, a);
+        else k_kv_attn<DP, I8, false, false><<<grid, 256, 0, s>>>(p, a);
+    }
 }
 
 template <bool I8>
@@ -532,19 +655,39 @@ void launch(unsigned grid, bool save, const KVPool& p, const Attn& a, hipStream_
 
 extern "C" {
 
-size_t snx_kv_attention_ws(const SNEPPXKVCache* c, size_t rows, size_t q_heads, size_t max_length, int accumulate) {
-    return plan(c, rows, q_heads, max_length, accumulate).bytes();
-}
-
 int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, void* out, size_t out_stride,
                        int out_f32, const int32_t* tables, size_t width, const int32_t* lengths, size_t rows,
-                       size_t q_heads, size_t max_length, float scale, int accumulate, void* ws, void* st) {
+                       size_t q_heads, size_t max_length, float scale, int accumulate, void* st) {
     const KVPool p = kv_pool(c, tables, width);
-    const Plan n = plan(c, rows, q_heads, max_length, accumulate);
-    const size_t blocks = rows * c->kv_heads * n.tiles * n.splits;
-    if (blocks > 0xffffff) {          // a grid has below 2^32 threads
+    const size_t group = q_heads / c->kv_heads, tiles = (group + 15) / 16, units = c->kv_heads * tiles;
+    const size_t heads = group < 16 ? group : 16;
+    const int row_bytes = (c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256) * (c->dtype == SNEPPX_INT8 ? 1 : 2);
+
+    // chunks of all rows: `share` of their tokens, and what rows round up; no more
+    // than a step each
+    const size_t share = ((size_t)resident(row_bytes) * cu_count() + units - 1) / units, steps = (max_length + STEP - 1) / STEP;
+    size_t chunks = share + rows;
+    if (chunks > rows * (steps ? steps : 1)) chunks = rows * (steps ? steps : 1);
+    const size_t blocks = chunks * units;
+    const size_t part = blocks * heads * c->head_dim * sizeof(float), ml = blocks * heads * sizeof(float2);
+    const size_t logit_stride = accumulate ? steps * STEP : 0, logits = rows * q_heads * logit_stride * sizeof(float);
+    // (a grid has below 2^32 threads; offsets of the parts and counts of steps are of 32 bits)
+    if (blocks > 0xffffff || part > 0xffffffffu || steps * rows > 0x7fffffffu || steps >= 0x1000000) {
         snx_set_error("kv_attention: %zu rows of up to %zu tokens are too many", rows, max_length);
         return -1;
+    }
+    // Joined within the launch, unless weights are added (by all CUs, after all
+    // maxima are known) or the call is recorded: a graph may be replayed beside
+    // other calls, and must not leave arrival counters that they would find.
+    void* ws = nullptr;
+    uint32_t* arrivals = nullptr;
+    if (steps > 1 || accumulate) {
+        if (!accumulate && !snx_stream_capturing(st)) {
+            if (snx_span_workspaces(part + ml, rows * units * sizeof(uint32_t), st, &ws, &arrivals)) return -1;
+        } else {
+            ws = snx_workspace(part + ml + logits, SLOT_KV_ATTN, st);
+            if (!ws) return -1;
+        }
     }
     Attn a;
     a.q = q;
@@ -553,29 +696,28 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.out_stride = out_stride;
     a.lengths = lengths;
     uint8_t* w = static_cast<uint8_t*>(ws);
+    a.arrivals = arrivals;
     a.part = reinterpret_cast<float*>(w);
-    a.logits = accumulate ? reinterpret_cast<float*>(w + n.part) : nullptr;
-    a.ml = reinterpret_cast<float2*>(w + n.part + n.logits);
+    a.logits = accumulate ? reinterpret_cast<float*>(w + part) : nullptr;
+    a.ml = reinterpret_cast<float2*>(w + part + logits);
+    a.rows = (uint32_t)rows;
     a.q_heads = (uint32_t)q_heads;
     a.max_length = (uint32_t)max_length;
-    a.splits = n.splits;
-    a.chunk = n.chunk;
-    a.tiles = n.tiles;
-    a.logit_stride = n.logit_stride;
-    a.pairs = (uint32_t)(rows * c->kv_heads);
+    a.tiles = (uint32_t)tiles;
+    a.heads = (uint32_t)heads;
+    a.share = (uint32_t)share;
+    a.logit_stride = (uint32_t)logit_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.out_f32 = out_f32;
     a.q_aligned = ((uintptr_t)q & 15u) == 0 && (rows < 2 || q_stride % 8 == 0);
-    a.direct = n.direct;
     if (c->dtype == SNEPPX_INT8) launch<true>((unsigned)blocks, accumulate != 0, p, a, S(st));
     else launch<false>((unsigned)blocks, accumulate != 0, p, a, S(st));
     if (snx_launch_check("k_kv_attn")) return -1;
-    if (n.direct) return 0;
-    const uint32_t group = (uint32_t)(q_heads / c->kv_heads);
-    uint32_t gx = group;
-    if (accumulate && div_up(max_length, 256) > gx) gx = div_up(max_length, 256);
+    if (!ws || arrivals) return 0;
+    const uint32_t joins = div_up(group, 4);
+    const size_t gx = joins + (accumulate ? steps * STEP / 256 + 1 : 0);
     const size_t bh = rows * c->kv_heads;
-    k_kv_join<<<dim3(gx < 65536 ? gx : 65536, (unsigned)(bh < 65535 ? bh : 65535), div_up(bh, 65535)), 256, 0, S(st)>>>(p, a);
+    k_kv_join<<<dim3((unsigned)gx, (unsigned)(bh < 65535 ? bh : 65535), div_up(bh, 65535)), 256, 0, S(st)>>>(p, a, joins);
     return snx_launch_check("k_kv_join");
 }
 

@@ -153,17 +153,6 @@ __device__ __forceinline__ void wave_prefix(uint32_t& x, uint32_t& y, uint2* sh,
     }
 }
 
-// inclusive prefix sum over the lanes
-__device__ __forceinline__ uint32_t lane_prefix(uint32_t x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);       // row_shr 1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast 15, 31
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-    return x;
-}
-
 // rows of the pool (k, v and the planes) of slots of[i] to those of slots
 // to[i], for `n` moves, by `threads` threads of which this is `me`
 __device__ __forceinline__ void move_rows(const KVPool& p, uint32_t b, uint32_t h, uint32_t row_bytes,

@@ -63,4 +63,27 @@ __device__ __forceinline__ uint32_t kv_length(const int32_t* lengths, uint32_t b
     return n < 0 ? 0u : (uint32_t)n < most ? (uint32_t)n : most;
 }
 
+// inclusive prefix sum over the lanes
+__device__ __forceinline__ uint32_t lane_prefix(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);       // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast 15, 31
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+
+// maximum over the lanes
+__device__ __forceinline__ uint32_t lane_max(uint32_t x) {
+    auto step = [&](uint32_t y) { x = y > x ? y : x; };
+    step(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return (uint32_t)__builtin_amdgcn_readlane(x, 63);
+}
+
 }  // namespace snx

@@ -7,7 +7,6 @@
 #include "sneppx_kv.h"
 #include "../snx_internal.h"
 
-#define SLOT_KV_ATTN 7
 #define SLOT_KV_MOVES 8
 
 #define REQUIRE(cond, ...)               \
@@ -92,11 +91,8 @@ int SNEPPX_kv_attention(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_
     if (!rows) return 0;
     const size_t slots = table_width * cache->page_size;
     if (max_length > slots) max_length = slots;
-    const size_t bytes = snx_kv_attention_ws(cache, rows, q_heads, max_length, accumulate);
-    void* ws = bytes ? snx_workspace(bytes, SLOT_KV_ATTN, stream) : NULL;
-    if (bytes && !ws) return -1;
     return snx_k_kv_attention(cache, q, q_stride, out, out_stride, out_dtype == SNEPPX_FLOAT32, block_tables, table_width,
-                              lengths, rows, q_heads, max_length, scale, accumulate != 0, ws, stream);
+                              lengths, rows, q_heads, max_length, scale, accumulate != 0, stream);
 }
 
 int SNEPPX_kv_evict(const SNEPPXKVCache* cache, const int32_t* block_tables, size_t table_width,

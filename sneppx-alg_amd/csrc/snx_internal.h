@@ -279,16 +279,16 @@ int snx_k_fp8_gemm(const uint8_t* A, const uint8_t* W, const float* sA, const fl
                    void* stream);
 
 /* ---- paged key-value cache (kv_attn_kernels.hip, kv_cache_kernels.hip) ----
- * checked arguments; max_length within the table, budget <= max_length; ws of
- * the bytes that the *_ws functions say */
+ * checked arguments; max_length within the table, budget <= max_length; the
+ * attention takes its workspaces itself, the eviction gets one of
+ * snx_kv_evict_ws bytes */
 int snx_k_kv_append(const SNEPPXKVCache* c, const uint16_t* k, size_t k_stride, const uint16_t* v, size_t v_stride,
                     size_t tokens, const int32_t* starts, uint16_t* k_stored, uint16_t* v_stored,
                     const int32_t* tables, size_t width, const int32_t* lengths, const int32_t* next_pos,
                     size_t rows, void* stream);
-size_t snx_kv_attention_ws(const SNEPPXKVCache* c, size_t rows, size_t q_heads, size_t max_length, int accumulate);
 int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, void* out, size_t out_stride,
                        int out_f32, const int32_t* tables, size_t width, const int32_t* lengths, size_t rows,
-                       size_t q_heads, size_t max_length, float scale, int accumulate, void* ws, void* stream);
+                       size_t q_heads, size_t max_length, float scale, int accumulate, void* stream);
 size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, size_t budget);
 int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, const int32_t* lengths,
                    const int32_t* next_pos, int32_t* new_lengths, size_t rows, size_t max_length, size_t budget,
