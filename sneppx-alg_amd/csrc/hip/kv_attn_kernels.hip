@@ -44,11 +44,16 @@ constexpr int TILE = 32;              // tokens of a wave's step
 constexpr int WAVES = 4;
 constexpr int STEP = TILE * WAVES;    // tokens of a workgroup's step: chunks are multiples of it
 
-// Workgroups of a CU (waves of a SIMD) for token rows of `bytes`: what the
-// registers allow of a tile's keys, values, queries and outputs.  At three for
-// rows of 256 bytes some of them spill (131072 tokens in bf16: 98 us at two, 113
-// at three), at two for 512 bytes (XX at one, XX at two).
-constexpr int resident(int bytes) { return bytes <= 128 ? 3 : bytes <= 256 ? 2 : 1; }
+// Waves of a SIMD that the registers allow with heads padded to `dim`: of a tile's
+// keys, values, queries and outputs.  (bf16 heads of 128 at three spill some:
+// 131072 tokens 138 us, 98 at two.)
+constexpr int resident(int dim, bool i8) { return dim <= 64 ? 4 : dim <= 128 ? (i8 ? 3 : 2) : i8 ? 2 : 1; }
+// Workgroups of a CU that a call is divided among, at most: us at 2 / 3 / 4 for
+// 131072 tokens of 128 in bf16 98 / 102 / 104, in int8 59 / 63 / 68, 64 rows of 0
+// to 8192 in int8 108 / 111 / 123, 16 rows of 4096 of 64 30 / 33 / 31 (all at the
+// residency above).
+constexpr int shares_of_cu(int dim, bool i8) { return resident(dim, i8) < 2 ? 1 : 2; }
+constexpr int padded(size_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 struct Attn {
     const uint16_t* q;
@@ -56,75 +61,81 @@ struct Attn {
     size_t q_stride, out_stride;
     const int32_t* lengths;
     uint32_t* arrivals;       // [rows * kv_heads * tiles], zero, or NULL: k_kv_join follows
-    float* part;              // [chunks of all rows][kv_heads * tiles][heads][dim]
-    float2* ml;               // [chunks of all rows][kv_heads * tiles][heads]: maximum, sum
+    float* part;              // [2 * shares][kv_heads * tiles][heads][dim]
+    float2* ml;               // [2 * shares][kv_heads * tiles][heads]: maximum, sum
     float* logits;            // [rows][q_heads][logit_stride], or NULL
-    uint32_t rows, q_heads, max_length, tiles, heads, share, logit_stride;
+    uint32_t rows, q_heads, max_length, tiles, heads, shares, logit_stride;
     float scale_log2;
     int out_f32, q_aligned;
 };
 
 // ------------------------------------------------------------- the division
-// A row's tokens are cut into chunks of the same number of steps for all rows,
-// as many as make `share` chunks of all rows' tokens together (a row has one at
-// least, 256 at most).  The lengths are known on the device alone, so every wave
-// works this out for itself: from max_length, which may be far above them, the
-// host could not (16 rows of 0 to 4096 tokens in chunks of max_length / 8: 45 us;
-// so: XX).
+// All rows' steps (one at least for each row), one row after the other, are cut
+// into equal shares; a workgroup takes one, with the end of a row, whole rows
+// and the beginning of another in it, and so all end together.  Where a share is
+// only a few steps, changing the row costs more than that evens out, and every
+// row begins with a new share.  The lengths are known on the device alone, so
+// every wave works this out for itself.  (us of shares across rows / by rows: 16
+// rows of 0 to 4096 tokens, 4 steps a share, 32 / 28; 128 of 0 to 2000, 16 steps,
+// 101 / 109; 64 of 0 to 8192, 32 steps, 183 / 210.  A grid for the longest row
+// that the host allows for leaves most of it idle: 45 for the first.)
 struct Row {
-    uint32_t b, chunk0, n, len;    // the row, its first chunk's number, its chunks (0: no such row), its length
+    uint32_t b, at, len;           // the row, its first step, its length in tokens
+    __device__ __forceinline__ uint32_t steps() const { return len > STEP ? (len + STEP - 1) / STEP : 1; }
 };
+
+// the shares that a row's steps lie in, and where each left its result
+struct Shares {
+    uint32_t first, n, inside;     // inside: the row begins within its first share
+    __device__ __forceinline__ Shares(const Row& w, uint32_t per) {
+        first = w.at / per;
+        n = (w.at + w.steps() - 1) / per - first + 1;
+        inside = w.at != first * per;
+    }
+    __device__ __forceinline__ uint32_t slot(uint32_t i) const { return 2 * (first + i) + (i == 0 ? inside : 0); }
+};
+constexpr uint32_t kMostShares = 256;     // of a row
+
+constexpr uint32_t kFewSteps = 8;         // of a share
 
 struct Division {
     const Attn& a;
-    uint32_t len0, per;            // length of row `lane`; steps of a chunk
+    uint32_t len0, total, per;     // length of row `lane`; steps of all rows, of a share
+    bool by_row;
     __device__ __forceinline__ explicit Division(const Attn& attn) : a(attn) {
         const uint32_t lane = threadIdx.x & 63;
-        uint32_t total = 0, longest = 0;
+        uint32_t sum = 0, longest = 0;
         len0 = length(lane);
         for (uint32_t r0 = 0; r0 < a.rows; r0 += 64) {
-            const uint32_t n = steps(r0 ? length(r0 + lane) : len0);
-            total += n;
+            const uint32_t n = steps(r0 + lane, r0 ? length(r0 + lane) : len0);
+            sum += n;
             longest = n > longest ? n : longest;
         }
-        total = __builtin_amdgcn_readlane(lane_prefix(total), 63);
-        per = (total + a.share - 1) / a.share;
-        const uint32_t least = (lane_max(longest) + 255) / 256;
+        total = __builtin_amdgcn_readlane(lane_prefix(sum), 63);
+        per = (total + a.shares - 1) / a.shares;
+        // a row has part of its first and last share
+        const uint32_t least = (lane_max(longest) + kMostShares - 3) / (kMostShares - 2);
         per = per > least ? per : least;
-        per = per > 1 ? per : 1;
+        by_row = per <= kFewSteps;
     }
     __device__ __forceinline__ uint32_t length(uint32_t r) const { return r < a.rows ? kv_length(a.lengths, r, a.max_length) : 0; }
-    static __device__ __forceinline__ uint32_t steps(uint32_t len) { return (len + STEP - 1) / STEP; }
-    // chunks of up to 64 rows from r0, one per lane
-    __device__ __forceinline__ uint32_t chunks(uint32_t r0, uint32_t& len) const {
-        const uint32_t r = r0 + (threadIdx.x & 63);
-        len = r0 ? length(r) : len0;
-        const uint32_t n = (steps(len) + per - 1) / per;
-        return r < a.rows ? n > 1 ? n : 1 : 0;
-    }
-    __device__ __forceinline__ Row pick(uint32_t r0, uint32_t base, uint32_t n, uint32_t upto, uint32_t len, int lane) const {
-        return Row{r0 + lane, base + (uint32_t)__builtin_amdgcn_readlane(upto - n, lane),
-                   (uint32_t)__builtin_amdgcn_readlane(n, lane), (uint32_t)__builtin_amdgcn_readlane(len, lane)};
-    }
-    // the row that has chunk number c
-    __device__ __forceinline__ Row of_chunk(uint32_t c) const {
-        uint32_t base = 0;
-        for (uint32_t r0 = 0; r0 < a.rows; r0 += 64) {
-            uint32_t len;
-            const uint32_t n = chunks(r0, len), upto = lane_prefix(n);
-            const uint64_t behind = __ballot(base + upto > c);
-            if (behind) return pick(r0, base, n, upto, len, __builtin_ctzll(behind));
-            base += __builtin_amdgcn_readlane(upto, 63);
-        }
-        return Row{0, 0, 0, 0};
-    }
-    __device__ __forceinline__ Row of_row(uint32_t b) const {
+    __device__ __forceinline__ uint32_t steps(uint32_t r, uint32_t len) const { return r < a.rows ? Row{r, 0, len}.steps() : 0; }
+    // what a row takes of the steps: whole shares by row
+    __device__ __forceinline__ uint32_t extent(uint32_t steps) const { return by_row ? (steps + per - 1) / per * per : steps; }
+    // the row that step `at` belongs to, or row `b`
+    template <bool STEPS>
+    __device__ __forceinline__ Row find(uint32_t x) const {
         uint32_t base = 0;
         for (uint32_t r0 = 0;; r0 += 64) {
-            uint32_t len;
-            const uint32_t n = chunks(r0, len), upto = lane_prefix(n);
-            if (b < r0 + 64) return pick(r0, base, n, upto, len, (int)(b - r0));
+            const uint32_t r = r0 + (threadIdx.x & 63), len = r0 ? length(r) : len0, n = extent(steps(r, len)), upto = lane_prefix(n);
+            const uint64_t behind = STEPS ? __ballot(base + upto > x) : __ballot(r == x);
+            if (behind) {
+                const int lane = __builtin_ctzll(behind);
+                return Row{r0 + lane, base + (uint32_t)__builtin_amdgcn_readlane(upto - n, lane),
+                           (uint32_t)__builtin_amdgcn_readlane(len, lane)};
+            }
             base += __builtin_amdgcn_readlane(upto, 63);
+            if (r0 + 64 >= a.rows) return Row{a.rows, base, 0};          // no such step
         }
     }
 };
@@ -224,29 +235,29 @@ struct Parts {
     uint32_t dim, units, unit;     // unit: key-value head and tile of 16 query heads
     __device__ __forceinline__ Parts(const Attn& attn, uint32_t d, uint32_t n, uint32_t u)
         : a(attn), part(rsrc(attn.part)), ml(rsrc(attn.ml)), dim(d), units(n), unit(u) {}
-    __device__ __forceinline__ uint32_t at(uint32_t chunk, uint32_t head) const { return (chunk * units + unit) * a.heads + head; }
-    __device__ __forceinline__ void put(uint32_t chunk, uint32_t head, uint32_t d, f32x4 v) const {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at(chunk, head) * dim + d) * 4, 0, kSysCoherent);
+    __device__ __forceinline__ uint32_t at(uint32_t slot, uint32_t head) const { return (slot * units + unit) * a.heads + head; }
+    __device__ __forceinline__ void put(uint32_t slot, uint32_t head, uint32_t d, f32x4 v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at(slot, head) * dim + d) * 4, 0, kSysCoherent);
     }
-    __device__ __forceinline__ void put_ml(uint32_t chunk, uint32_t head, float m, float l) const {
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{f2u(m), f2u(l)}, ml, at(chunk, head) * 8, 0, kSysCoherent);
+    __device__ __forceinline__ void put_ml(uint32_t slot, uint32_t head, float m, float l) const {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{f2u(m), f2u(l)}, ml, at(slot, head) * 8, 0, kSysCoherent);
     }
-    __device__ __forceinline__ f32x4 get(uint32_t chunk, uint32_t head, uint32_t d) const {
-        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, (at(chunk, head) * dim + d) * 4, 0, kSysCoherent));
+    __device__ __forceinline__ f32x4 get(uint32_t slot, uint32_t head, uint32_t d) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, (at(slot, head) * dim + d) * 4, 0, kSysCoherent));
     }
-    __device__ __forceinline__ float2 get_ml(uint32_t chunk, uint32_t head) const {
-        const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(ml, at(chunk, head) * 8, 0, kSysCoherent);
+    __device__ __forceinline__ float2 get_ml(uint32_t slot, uint32_t head) const {
+        const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(ml, at(slot, head) * 8, 0, kSysCoherent);
         return make_float2(u2f(r[0]), u2f(r[1]));
     }
 
     // maximum and 1 / sum of a query head over its row's chunks, by one wave: 0
     // for no tokens, NaN where there are tokens and every logit is -inf
-    __device__ __forceinline__ float2 whole(const Row& w, uint32_t head) const {
+    __device__ __forceinline__ float2 whole(const Shares& w, uint32_t head) const {
         const uint32_t lane = threadIdx.x & 63;
-        float2 e[4];
+        float2 e[kMostShares / 64];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            e[j] = 64 * j + lane < w.n ? get_ml(w.chunk0 + 64 * j + lane, head) : make_float2(-INFINITY, 0.0f);
+        for (int j = 0; j < (int)kMostShares / 64; j++)
+            e[j] = 64 * j + lane < w.n ? get_ml(w.slot(64 * j + lane), head) : make_float2(-INFINITY, 0.0f);
         float top = fmaxf(fmaxf(e[0].x, e[1].x), fmaxf(e[2].x, e[3].x));
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
         float total = 0.0f, plain = 0.0f;
@@ -264,8 +275,8 @@ struct Parts {
 
     // One wave joins the chunks of a query head and writes its result: 4 elements
     // per lane, the chunks in 64 / span turns, added in a fixed order.
-    __device__ __forceinline__ void join(const Row& w, uint32_t head, uint32_t hq) const {
-        constexpr int U = 16;             // loads in flight
+    __device__ __forceinline__ void join(const Shares& w, uint32_t b, uint32_t head, uint32_t hq) const {
+        constexpr int U = 8;              // loads in flight
         const uint32_t lane = threadIdx.x & 63;
         const uint32_t span = dim <= 64 ? 16 : dim <= 128 ? 32 : 64, ways = 64 / span;
         const uint32_t d = 4 * (lane & (span - 1)), way = lane / span;
@@ -278,7 +289,7 @@ struct Parts {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const bool on = i0 + u * ways < w.n;
-                const uint32_t c = w.chunk0 + (on ? i0 + u * ways : 0);
+                const uint32_t c = w.slot(on ? i0 + u * ways : 0);
                 x[u] = get(c, head, in ? d : 0);
                 m[u] = get_ml(c, head).x;
                 if (!on) m[u] = -INFINITY;
@@ -292,7 +303,7 @@ struct Parts {
         for (uint32_t o = span; o < 64; o <<= 1)
 #pragma unroll
             for (int j = 0; j < 4; j++) v[j] += __shfl_xor(v[j], o);
-        if (way == 0 && in) store(w.b, hq, d, v, st.y);
+        if (way == 0 && in) store(b, hq, d, v, st.y);
     }
 
     __device__ __forceinline__ void store(uint32_t b, uint32_t hq, uint32_t d, f32x4 v, float inv) const {
@@ -319,7 +330,7 @@ struct Parts {
 // registers that the first product has just used, values into those that
 // went to LDS.
 template <int DP, bool I8, bool SAVE, bool FULL>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(resident(DP * (I8 ? 1 : 2)))))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(resident(DP, I8))))
 k_kv_attn(const KVPool p, const Attn a) {
     typedef Lds<DP, I8> L;
     constexpr int NC = L::RB / 64;        // 16-byte chunks of a row per lane
@@ -329,20 +340,24 @@ k_kv_attn(const KVPool p, const Attn a) {
     __shared__ float2 ends[WAVES][16];
     __shared__ uint32_t arrived;
 
-    // The units of a chunk, then the next chunk: workgroups go to the XCDs in turn,
-    // and so every XCD gets chunks of all rows.
+    // The units of a share, then the next share: workgroups go to the XCDs in turn,
+    // and so every XCD gets shares of all rows.
     const uint32_t units = p.heads * a.tiles, number = blockIdx.x / units, unit = blockIdx.x - number * units;
     const Division cut(a);
-    const Row w = cut.of_chunk(number);
-    if (w.n == 0) return;
-    const uint32_t b = w.b, h = unit / a.tiles, ht = unit - h * a.tiles;
-    // its steps are dealt out evenly (below 2^24 steps, 256 chunks)
-    const uint32_t i = number - w.chunk0, steps = Division::steps(w.len);
-    const uint32_t first = i * steps / w.n * STEP, end = (i + 1) * steps / w.n * STEP;
-    const uint32_t last = end < w.len ? end : w.len;
+    uint32_t at = number * cut.per;
+    if (!cut.by_row && at >= cut.total) return;
+    Row w = cut.find<true>(at);
+    if (w.b == a.rows) return;
+    const uint32_t row_end = w.at + w.steps(), share_end = at + cut.per;
+    const uint32_t stop = cut.by_row ? (share_end < row_end ? share_end : row_end) : share_end < cut.total ? share_end : cut.total;
+    const uint32_t h = unit / a.tiles, ht = unit - h * a.tiles;
     const Parts parts(a, FULL ? DP : p.dim, units, unit);
 
-    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    for (;;) {
+    // (opaque, so that what follows from it is not kept in registers from row to row)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t group = a.q_heads / p.heads;
     const uint32_t nh = group - ht * 16 < 16 ? group - ht * 16 : 16;
@@ -350,6 +365,11 @@ k_kv_attn(const KVPool p, const Attn a) {
     const uint32_t dim = FULL ? DP : p.dim, row_bytes = dim * (I8 ? 1 : 2);
     uint8_t* const vt = lds + wave * L::WAVE;
     float* const sc = reinterpret_cast<float*>(vt + L::V);
+
+    const uint32_t b = w.b, ends_at = w.at + w.steps() < stop ? w.at + w.steps() : stop;
+    const uint32_t first = (at - w.at) * STEP, upto = (ends_at - w.at) * STEP, last = upto < w.len ? upto : w.len;
+    const Shares shares(w, cut.per);
+    const uint32_t next_len = ends_at < stop ? cut.length(b + 1) : 0;
 
     bf16x8 q[KS];
 #pragma unroll
@@ -432,7 +452,9 @@ k_kv_attn(const KVPool p, const Attn a) {
             s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < KS; i++) {
-                const u32x4 w = kc[t][I8 ? i >> 1 : i];
+                u32x4 w = kc[t][I8 ? i >> 1 : i];
+                // (or the compiler converts when it loads, and keeps twice the registers)
+                if (I8) asm volatile("" : "+v"(w));
                 bf16x8 kf;
                 if (I8) kf = (i & 1) ? bytes_to_bf16(w[2], w[3]) : bytes_to_bf16(w[0], w[1]);
                 else kf = __builtin_bit_cast(bf16x8, w);
@@ -466,6 +488,7 @@ k_kv_attn(const KVPool p, const Attn a) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 
+        __builtin_amdgcn_sched_barrier(0);
         // softmax of the tile's eight logits of this lane's head
         float e[8];
         float top = -INFINITY;
@@ -505,6 +528,7 @@ k_kv_attn(const KVPool p, const Attn a) {
         }
         bf16x8 pc[3];
         split3(e, pc);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             bf16x8 vf;
@@ -525,6 +549,7 @@ k_kv_attn(const KVPool p, const Attn a) {
             }
 #pragma unroll
             for (int i = 0; i < 3; i++) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pc[i], o[dt], 0, 0, 0);
+            if (dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -558,26 +583,33 @@ k_kv_attn(const KVPool p, const Attn a) {
             v += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds) + (w * 16 + hd) * L::OS + d);
         }
         if (top == -INFINITY) total = plain > 1.0f ? 1.0f : plain;
-        if (!SAVE && w.n == 1) {
+        if (!SAVE && shares.n == 1) {
             parts.store(b, hq + hd, d, v, top == -INFINITY ? total == 0.0f ? 0.0f : NAN : 1.0f / total);
         } else {
-            parts.put(number, hd, d, v);
-            if (d == 0) parts.put_ml(number, hd, top, total);
+            const uint32_t slot = 2 * number + (at != number * cut.per);
+            parts.put(slot, hd, d, v);
+            if (d == 0) parts.put_ml(slot, hd, top, total);
         }
     }
-    if (SAVE || w.n == 1 || !a.arrivals) return;
-    // the last of the row's chunks to arrive joins them
-    __builtin_amdgcn_s_waitcnt(0x0f70);              // vmcnt(0): this wave's stores are out
-    __syncthreads();
-    if (tid == 0) {
-        uint32_t* const mine = a.arrivals + (size_t)b * units + unit;
-        const uint32_t c = atomicAdd(mine, 1u);
-        if (c == w.n - 1) atomicExch(mine, 0u);      // ready for the next call
-        arrived = c;
+    if (!SAVE && shares.n > 1 && a.arrivals) {
+        // the last of the row's shares to arrive joins them
+        __builtin_amdgcn_s_waitcnt(0x0f70);              // vmcnt(0): this wave's stores are out
+        __syncthreads();
+        if (tid == 0) {
+            uint32_t* const mine = a.arrivals + (size_t)b * units + unit;
+            const uint32_t c = atomicAdd(mine, 1u);
+            if (c == shares.n - 1) atomicExch(mine, 0u);      // ready for the next call
+            arrived = c;
+        }
+        __syncthreads();
+        if (arrived == shares.n - 1)
+            for (uint32_t j = wave; j < nh; j += WAVES) parts.join(shares, b, j, hq + j);
     }
-    __syncthreads();
-    if (arrived != w.n - 1) return;
-    for (uint32_t j = wave; j < nh; j += WAVES) parts.join(w, j, hq + j);
+    at = ends_at;
+    if (at >= stop) break;
+    w = Row{b + 1, at, next_len};
+    __syncthreads();                                     // the next row's tiles reuse the LDS
+    }
 }
 
 // After k_kv_attn, workgroups x of every (row, key-value head): the first
@@ -594,9 +626,10 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
     auto parts = [&](uint32_t j) { return Parts(a, p.dim, p.heads * a.tiles, h * a.tiles + j / 16); };
 
     if (blockIdx.x < joins) {
-        const Row w = Division(a).of_row(b);
+        const Division cut(a);
+        const Shares w(cut.find<false>(b), cut.per);
         if (a.logits || w.n > 1)
-            for (uint32_t j = 4 * blockIdx.x + wave; j < group; j += 4 * joins) parts(j).join(w, j % 16, h * group + j);
+            for (uint32_t j = 4 * blockIdx.x + wave; j < group; j += 4 * joins) parts(j).join(w, b, j % 16, h * group + j);
         return;
     }
     // what does not depend on the chunks is loaded first
@@ -610,7 +643,8 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
 #pragma unroll
     for (int j = 0; j < G; j++) v[j] = s[(size_t)((uint32_t)j < group ? j : 0) * a.logit_stride];
     if (ok) before = p.weights[row];
-    const Row w = Division(a).of_row(b);
+    const Division cut(a);
+    const Shares w(cut.find<false>(b), cut.per);
     for (uint32_t j0 = 0; j0 < group; j0 += 256) {
         const uint32_t nj = group - j0 < 256 ? group - j0 : 256;
         __syncthreads();
@@ -646,8 +680,8 @@ void launch(unsigned grid, bool save, const KVPool& p, const Attn& a, hipStream_
 
 template <bool I8>
 void launch(unsigned grid, bool save, const KVPool& p, const Attn& a, hipStream_t s) {
-    if (p.dim <= 64) launch<64, I8>(grid, save, p, a, s);
-    else if (p.dim <= 128) launch<128, I8>(grid, save, p, a, s);
+    if (padded(p.dim) == 64) launch<64, I8>(grid, save, p, a, s);
+    else if (padded(p.dim) == 128) launch<128, I8>(grid, save, p, a, s);
     else launch<256, I8>(grid, save, p, a, s);
 }
 
@@ -661,15 +695,14 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     const KVPool p = kv_pool(c, tables, width);
     const size_t group = q_heads / c->kv_heads, tiles = (group + 15) / 16, units = c->kv_heads * tiles;
     const size_t heads = group < 16 ? group : 16;
-    const int row_bytes = (c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256) * (c->dtype == SNEPPX_INT8 ? 1 : 2);
-
-    // chunks of all rows: `share` of their tokens, and what rows round up; no more
-    // than a step each
-    const size_t share = ((size_t)resident(row_bytes) * cu_count() + units - 1) / units, steps = (max_length + STEP - 1) / STEP;
-    size_t chunks = share + rows;
-    if (chunks > rows * (steps ? steps : 1)) chunks = rows * (steps ? steps : 1);
-    const size_t blocks = chunks * units;
-    const size_t part = blocks * heads * c->head_dim * sizeof(float), ml = blocks * heads * sizeof(float2);
+    // as many shares as the CUs hold workgroups at once, and one more for each row
+    // (see Division); no more than there are steps
+    const size_t steps = (max_length + STEP - 1) / STEP;
+    const size_t shares = ((size_t)shares_of_cu(padded(c->head_dim), c->dtype == SNEPPX_INT8) * cu_count() + units - 1) / units;
+    size_t blocks = shares + rows;
+    if (blocks > rows * (steps ? steps : 1)) blocks = rows * (steps ? steps : 1);
+    blocks *= units;
+    const size_t part = 2 * blocks * heads * c->head_dim * sizeof(float), ml = 2 * blocks * heads * sizeof(float2);
     const size_t logit_stride = accumulate ? steps * STEP : 0, logits = rows * q_heads * logit_stride * sizeof(float);
     // (a grid has below 2^32 threads; offsets of the parts and counts of steps are of 32 bits)
     if (blocks > 0xffffff || part > 0xffffffffu || steps * rows > 0x7fffffffu || steps >= 0x1000000) {
@@ -705,7 +738,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.max_length = (uint32_t)max_length;
     a.tiles = (uint32_t)tiles;
     a.heads = (uint32_t)heads;
-    a.share = (uint32_t)share;
+    a.shares = (uint32_t)shares;
     a.logit_stride = (uint32_t)logit_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.out_f32 = out_f32;
