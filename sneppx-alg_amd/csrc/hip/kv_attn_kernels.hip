@@ -250,55 +250,64 @@ struct Parts {
         return make_float2(u2f(r[0]), u2f(r[1]));
     }
 
-    // maximum and 1 / sum of a query head over its row's chunks, by one wave: 0
-    // for no tokens, NaN where there are tokens and every logit is -inf
-    __device__ __forceinline__ float2 whole(const Shares& w, uint32_t head) const {
-        const uint32_t lane = threadIdx.x & 63;
+    // maxima and sums of a query head in its row's shares, one per lane and 64
+    struct Ends {
         float2 e[kMostShares / 64];
+    };
+    __device__ __forceinline__ Ends ends(const Shares& w, uint32_t head) const {
+        const uint32_t lane = threadIdx.x & 63;
+        Ends x;
 #pragma unroll
-        for (int j = 0; j < (int)kMostShares / 64; j++)
-            e[j] = 64 * j + lane < w.n ? get_ml(w.slot(64 * j + lane), head) : make_float2(-INFINITY, 0.0f);
-        float top = fmaxf(fmaxf(e[0].x, e[1].x), fmaxf(e[2].x, e[3].x));
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        float total = 0.0f, plain = 0.0f;
+        for (int j = 0; j < (int)kMostShares / 64; j++) {
+            x.e[j] = make_float2(-INFINITY, 0.0f);
+            if (64 * j + lane < w.n) x.e[j] = get_ml(w.slot(64 * j + lane), head);
+        }
+        return x;
+    }
+    // Their maximum and 1 / sum, by one wave: 0 for no tokens, NaN where there are
+    // tokens and every logit is -inf; to `factors` each share's weight.
+    __device__ __forceinline__ float2 whole(const Ends& x, const Shares& w, float* factors) const {
+        const uint32_t lane = threadIdx.x & 63;
+        float top = -INFINITY, total = 0.0f, plain = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            total += (e[j].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e[j].x - top)) * e[j].y;
-            plain += e[j].y;
+        for (int j = 0; j < (int)kMostShares / 64; j++) top = fmaxf(top, x.e[j].x);
+        top = lane_max(top);
+#pragma unroll
+        for (int j = 0; j < (int)kMostShares / 64; j++) {
+            const float f = x.e[j].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.e[j].x - top);
+            total += f * x.e[j].y;
+            plain += x.e[j].y;
+            if (factors && 64 * j < w.n) factors[64 * j + lane] = f;
         }
-        for (int o = 32; o > 0; o >>= 1) {
-            total += __shfl_xor(total, o);
-            plain += __shfl_xor(plain, o);
-        }
+        total = lane_sum(total);
+        plain = lane_sum(plain);
         return make_float2(top, top == -INFINITY ? plain == 0.0f ? 0.0f : NAN : 1.0f / total);
     }
 
-    // One wave joins the chunks of a query head and writes its result: 4 elements
-    // per lane, the chunks in 64 / span turns, added in a fixed order.
-    __device__ __forceinline__ void join(const Shares& w, uint32_t b, uint32_t head, uint32_t hq) const {
+    // One wave joins a row's shares of a query head and writes the result: 4
+    // elements per lane, the shares in 64 / span turns, added in a fixed order.
+    // factors: LDS of the wave, kMostShares floats.
+    __device__ __forceinline__ void join(const Shares& w, uint32_t b, uint32_t head, uint32_t hq, float* factors) const {
         constexpr int U = 8;              // loads in flight
         const uint32_t lane = threadIdx.x & 63;
         const uint32_t span = dim <= 64 ? 16 : dim <= 128 ? 32 : 64, ways = 64 / span;
         const uint32_t d = 4 * (lane & (span - 1)), way = lane / span;
-        const float2 st = whole(w, head);
         const bool in = d < dim;
+        const Ends e = ends(w, head);
         f32x4 v = {};
-        for (uint32_t i0 = way; i0 < w.n; i0 += U * ways) {
+        float2 st = {};
+        for (uint32_t i0 = way; i0 < way + (w.n + ways - 1) / ways * ways; i0 += U * ways) {
             f32x4 x[U];
-            float m[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const bool on = i0 + u * ways < w.n;
-                const uint32_t c = w.slot(on ? i0 + u * ways : 0);
-                x[u] = get(c, head, in ? d : 0);
-                m[u] = get_ml(c, head).x;
-                if (!on) m[u] = -INFINITY;
+            for (int u = 0; u < U; u++) x[u] = get(w.slot(i0 + u * ways < w.n ? i0 + u * ways : 0), head, in ? d : 0);
+            if (i0 == way) {
+                st = whole(e, w, factors);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
             }
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const float f = m[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[u] - st.x);
-                if (i0 + u * ways < w.n) v += f * x[u];
-            }
+            for (int u = 0; u < U; u++)
+                if (i0 + u * ways < w.n) v += factors[i0 + u * ways] * x[u];
         }
         for (uint32_t o = span; o < 64; o <<= 1)
 #pragma unroll
@@ -371,21 +380,6 @@ k_kv_attn(const KVPool p, const Attn a) {
     const Shares shares(w, cut.per);
     const uint32_t next_len = ends_at < stop ? cut.length(b + 1) : 0;
 
-    bf16x8 q[KS];
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
-        const uint32_t d = I8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 8 * (g + 4 * s);
-        u32x4 w = {0u, 0u, 0u, 0u};
-        if ((uint32_t)r < nh && d < dim) {
-            const uint16_t* src = a.q + b * a.q_stride + (size_t)(hq + r) * dim + d;
-            if (a.q_aligned) w = *reinterpret_cast<const u32x4*>(src);
-            else
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
-        }
-        q[s] = __builtin_bit_cast(bf16x8, w);
-    }
-
     f32x4 o[DT] = {};
     float m = -INFINITY, sum = 0.0f;
     bool any = false;
@@ -433,8 +427,23 @@ k_kv_attn(const KVPool p, const Attn a) {
     };
 
     uint32_t base = first + wave * TILE;
+    if (base < last) look(base);
+    bf16x8 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const uint32_t d = I8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 8 * (g + 4 * s);
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if ((uint32_t)r < nh && d < dim) {
+            const uint16_t* src = a.q + b * a.q_stride + (size_t)(hq + r) * dim + d;
+            if (a.q_aligned) w = *reinterpret_cast<const u32x4*>(src);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
+        }
+        q[s] = __builtin_bit_cast(bf16x8, w);
+    }
+
     if (base < last) {
-        look(base);
         find(base);
         look(base + STEP);
         load_k();
@@ -603,7 +612,8 @@ k_kv_attn(const KVPool p, const Attn a) {
         }
         __syncthreads();
         if (arrived == shares.n - 1)
-            for (uint32_t j = wave; j < nh; j += WAVES) parts.join(shares, b, j, hq + j);
+            for (uint32_t j = wave; j < nh; j += WAVES)
+                parts.join(shares, b, j, hq + j, reinterpret_cast<float*>(lds) + wave * kMostShares);
     }
     at = ends_at;
     if (at >= stop) break;
@@ -618,6 +628,7 @@ k_kv_attn(const KVPool p, const Attn a) {
 // attention weights of 256 tokens each.
 __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, uint32_t joins) {
     __shared__ float2 stat[256];      // of a head: maximum, 1 / sum
+    __shared__ float factors[4][kMostShares];
     const uint32_t bh = blockIdx.y + blockIdx.z * 65535u;
     if (bh >= a.rows * p.heads) return;
     const uint32_t b = bh / p.heads, h = bh - b * p.heads;
@@ -629,7 +640,8 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
         const Division cut(a);
         const Shares w(cut.find<false>(b), cut.per);
         if (a.logits || w.n > 1)
-            for (uint32_t j = 4 * blockIdx.x + wave; j < group; j += 4 * joins) parts(j).join(w, b, j % 16, h * group + j);
+            for (uint32_t j = 4 * blockIdx.x + wave; j < group; j += 4 * joins)
+                parts(j).join(w, b, j % 16, h * group + j, factors[wave]);
         return;
     }
     // what does not depend on the chunks is loaded first
@@ -649,7 +661,8 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
         const uint32_t nj = group - j0 < 256 ? group - j0 : 256;
         __syncthreads();
         for (uint32_t j = wave; j < nj; j += 4) {
-            const float2 st = parts(j0 + j).whole(w, (j0 + j) % 16);
+            const Parts pt = parts(j0 + j);
+            const float2 st = pt.whole(pt.ends(w, (j0 + j) % 16), w, nullptr);
             if (lane == 0) stat[j] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y);
         }
         __syncthreads();

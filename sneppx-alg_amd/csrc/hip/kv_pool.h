@@ -63,27 +63,38 @@ __device__ __forceinline__ uint32_t kv_length(const int32_t* lengths, uint32_t b
     return n < 0 ? 0u : (uint32_t)n < most ? (uint32_t)n : most;
 }
 
-// inclusive prefix sum over the lanes
-__device__ __forceinline__ uint32_t lane_prefix(uint32_t x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);       // row_shr 1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast 15, 31
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-    return x;
+// Over the lanes of a wave: a step takes each row of 16 from the lanes `ctrl`
+// says (row_shr 1, 2, 4, 8, then row_bcast 15 and 31), `none` where there is none.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T lane_step(T x, T none) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, x), CTRL,
+                                                             ROWS, 0xf, false));
 }
-
-// maximum over the lanes
+// inclusive prefixes of an associative operation
+template <typename T, typename F>
+__device__ __forceinline__ T lane_scan(T x, T none, F op) {
+    x = op(x, lane_step<0x111, 0xf>(x, none));
+    x = op(x, lane_step<0x112, 0xf>(x, none));
+    x = op(x, lane_step<0x114, 0xf>(x, none));
+    x = op(x, lane_step<0x118, 0xf>(x, none));
+    x = op(x, lane_step<0x142, 0xa>(x, none));
+    return op(x, lane_step<0x143, 0xc>(x, none));
+}
+template <typename T>
+__device__ __forceinline__ T last_lane(T x) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ uint32_t lane_prefix(uint32_t x) {
+    return lane_scan(x, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+}
 __device__ __forceinline__ uint32_t lane_max(uint32_t x) {
-    auto step = [&](uint32_t y) { x = y > x ? y : x; };
-    step(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));
-    step(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));
-    step(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));
-    step(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));
-    step(__builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
-    step(__builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
-    return (uint32_t)__builtin_amdgcn_readlane(x, 63);
+    return last_lane(lane_scan(x, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
+}
+__device__ __forceinline__ float lane_max(float x) {
+    return last_lane(lane_scan(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); }));
+}
+__device__ __forceinline__ float lane_sum(float x) {
+    return last_lane(lane_scan(x, 0.0f, [](float a, float b) { return a + b; }));
 }
 
 }  // namespace snx
