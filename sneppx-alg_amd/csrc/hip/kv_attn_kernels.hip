@@ -65,6 +65,7 @@ struct Attn {
     float2* ml;               // [2 * shares][kv_heads * tiles][heads]: maximum, sum
     float* logits;            // [rows][q_heads][logit_stride], or NULL
     uint32_t rows, q_heads, max_length, tiles, heads, shares, logit_stride;
+    Divider by_eights, by_heads;      // by 8 tiles and by kv_heads
     float scale_log2;
     int out_f32, q_aligned;
 };
@@ -349,17 +350,20 @@ k_kv_attn(const KVPool p, const Attn a) {
     __shared__ float2 ends[WAVES][16];
     __shared__ uint32_t arrived;
 
-    // The units of a share, then the next share: workgroups go to the XCDs in turn,
-    // and so every XCD gets shares of all rows.
-    const uint32_t units = p.heads * a.tiles, number = blockIdx.x / units, unit = blockIdx.x - number * units;
+    // The heads of a share, then the next share: workgroups go to the XCDs in turn,
+    // and so every XCD gets shares of all rows.  The tiles of one head and share
+    // are 8 workgroups apart, on one XCD, whose L2 has their tokens then (16 rows of
+    // 4096, 32 query heads to a key-value head: XX us side by side, XX so).
+    const uint32_t units = p.heads * a.tiles, eights = a.by_eights(blockIdx.x), rest = blockIdx.x - eights * 8 * a.tiles;
+    const uint32_t ht = rest / 8, pair = eights * 8 + rest % 8, number = a.by_heads(pair), h = pair - number * p.heads;
+    const uint32_t unit = h * a.tiles + ht;
     const Division cut(a);
+    if ((uint64_t)number * cut.per >= (cut.by_row ? 0xFFFFFFFFu : cut.total)) return;
     uint32_t at = number * cut.per;
-    if (!cut.by_row && at >= cut.total) return;
     Row w = cut.find<true>(at);
     if (w.b == a.rows) return;
     const uint32_t row_end = w.at + w.steps(), share_end = at + cut.per;
     const uint32_t stop = cut.by_row ? (share_end < row_end ? share_end : row_end) : share_end < cut.total ? share_end : cut.total;
-    const uint32_t h = unit / a.tiles, ht = unit - h * a.tiles;
     const Parts parts(a, FULL ? DP : p.dim, units, unit);
 
     for (;;) {
@@ -714,7 +718,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     const size_t shares = ((size_t)shares_of_cu(padded(c->head_dim), c->dtype == SNEPPX_INT8) * cu_count() + units - 1) / units;
     size_t blocks = shares + rows;
     if (blocks > rows * (steps ? steps : 1)) blocks = rows * (steps ? steps : 1);
-    blocks *= units;
+    blocks = (blocks * c->kv_heads + 7) / 8 * 8 * tiles;
     const size_t part = 2 * blocks * heads * c->head_dim * sizeof(float), ml = 2 * blocks * heads * sizeof(float2);
     const size_t logit_stride = accumulate ? steps * STEP : 0, logits = rows * q_heads * logit_stride * sizeof(float);
     // (a grid has below 2^32 threads; offsets of the parts and counts of steps are of 32 bits)
@@ -751,6 +755,8 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.max_length = (uint32_t)max_length;
     a.tiles = (uint32_t)tiles;
     a.heads = (uint32_t)heads;
+    a.by_eights = divider(8 * tiles);
+    a.by_heads = divider(c->kv_heads);
     a.shares = (uint32_t)shares;
     a.logit_stride = (uint32_t)logit_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;

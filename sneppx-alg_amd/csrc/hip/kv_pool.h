@@ -10,21 +10,27 @@
 
 namespace snx {
 
+// Division of numbers below 2^31 by d: with 2^(l-1) < d <= 2^l and mul =
+// ceil(2^(31+l) / d), x * mul / 2^(31+l) is the quotient plus less than
+// x * 2^l / (d 2^(31+l)) < 1 / d.
+struct Divider {
+    uint32_t mul, shift;
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
+};
+inline Divider divider(size_t d) {
+    uint32_t l = 0;
+    while (((uint64_t)1 << l) < d) l++;
+    return Divider{(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), 31 + l};
+}
+
 struct KVPool {
     uint8_t *k, *v;
     float *ks, *vs, *weights;
     int32_t* positions;
     const int32_t* tables;
     uint32_t width, pages, heads, page_size;
-    uint32_t mul, shift;       // slot / page_size = slot * mul >> shift
+    Divider page_of;           // of a slot (below 2^30)
     uint32_t dim;
-
-    // Slot / page_size for slots below 2^31: with 2^(l-1) < d <= 2^l and
-    // mul = ceil(2^(31+l) / d), slot * mul / 2^(31+l) is the quotient plus less
-    // than slot * 2^l / (d 2^(31+l)) < 1 / d.
-    __device__ __forceinline__ uint32_t page_of(uint32_t slot) const {
-        return (uint32_t)(((uint64_t)slot * mul) >> shift);
-    }
 
     // Row of the pool (of head_dim values, and of each plane) that holds slot
     // `slot` of head h in row b's pages; false where that page is not there.
@@ -50,10 +56,7 @@ inline KVPool kv_pool(const SNEPPXKVCache* c, const int32_t* tables, size_t widt
     p.heads = (uint32_t)c->kv_heads;
     p.page_size = (uint32_t)c->page_size;
     p.dim = (uint32_t)c->head_dim;
-    uint32_t l = 0;
-    while (((uint64_t)1 << l) < c->page_size) l++;
-    p.shift = 31 + l;
-    p.mul = (uint32_t)((((uint64_t)1 << p.shift) + c->page_size - 1) / c->page_size);
+    p.page_of = divider(c->page_size);
     return p;
 }
 

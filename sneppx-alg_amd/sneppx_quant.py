@@ -843,14 +843,18 @@ class KVCache:
 
     def _rows(self, t, name, heads, dtypes):
         """[n, heads, head_dim] whose rows are contiguous; returns the row stride."""
-        if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != self.device or t.dim() != 3 \
-                or t.shape[2] != self.head_dim or heads and t.shape[1] != heads \
-                or t.stride(2) != 1 or t.shape[1] > 1 and t.stride(1) != self.head_dim:
+        try:
+            (n, h, d), (step, s1, s2) = t.shape, t.stride()
+            good = d == self.head_dim and s2 == 1 and (s1 == d or h == 1) and (h == heads or not heads) \
+                and t.dtype in dtypes and t.device == self.device
+        except (AttributeError, ValueError):
+            good = False
+        if not good:
             got = f"{t.dtype} {tuple(t.shape)} (strides {t.stride()}) on {t.device}" \
                 if isinstance(t, torch.Tensor) else repr(t)
             raise ValueError(f"{name} must be [n, {heads or 'q_heads'}, {self.head_dim}] with contiguous rows, "
                              f"{' or '.join(map(str, dtypes))}, on {self.device}; got {got}")
-        return t.stride(0)
+        return step
 
     def _tables(self, tables, lengths):
         if not isinstance(tables, torch.Tensor) or tables.dim() != 2:
