@@ -63,13 +63,26 @@ __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows
     uint32_t b = t;
     int32_t back = 1;
     if (n.starts) {
-        uint32_t lo = 0, hi = n.rows;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (n.starts[mid] <= (int32_t)t) lo = mid;
-            else hi = mid;
+        b = 0;
+        uint32_t left = n.rows;
+        if (__ballot(t == (uint32_t)__builtin_amdgcn_readfirstlane(t)) == ~0ull) {
+            // one token in the wave: 64 rows are asked at once
+            const uint32_t lane = threadIdx.x & 63;
+            while (left > 1) {
+                const uint32_t step = (left + 63) / 64, at = lane * step;
+                const uint32_t k = __popcll(__ballot(at < left && n.starts[b + (at < left ? at : 0)] <= (int32_t)t));
+                const uint32_t skip = k ? (k - 1) * step : 0;
+                b += skip;
+                left = left - skip < step ? left - skip : step;
+            }
+        } else {
+            while (left > 1) {
+                const uint32_t half = left / 2;
+                const bool up = n.starts[b + half] <= (int32_t)t;
+                b += up ? half : 0;
+                left = up ? left - half : half;
+            }
         }
-        b = lo;
         back = n.starts[b + 1] - (int32_t)t;
         if (back <= 0 || n.starts[b] > (int32_t)t) return;
     }
@@ -89,10 +102,18 @@ __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows
 #pragma unroll
         for (int o = LR / 2; o > 0; o >>= 1) m = nanless_max(m, __shfl_xor(m, o));
         const float s = m < FLT_MIN ? 1.0f : m / 127.0f, inv = 1.0f / s;
+        // Numbers below 128 round half away by adding the number below 1/2 and
+        // cutting; what the rule gives for others (an infinity or NaN in the row, a
+        // scale whose reciprocal is infinite) takes the long way.
+        float all = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) all += fabsf(f[e]);
+        const bool plain = all < INFINITY && m < INFINITY && inv < INFINITY;
         u32x2 q = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const int c = clampi(round_i32(f[e] * inv), -128, 127);
+            const float v = f[e] * inv;
+            const int c = plain ? (int)(v + copysignf(0.49999997f, v)) : clampi(round_i32(v), -128, 127);
             q[e >> 2] |= (uint32_t)(c & 0xFF) << (8 * (e & 3));
             f[e] = (float)c * s;
         }
