@@ -181,18 +181,21 @@ __device__ __forceinline__ bf16x8 bytes_to_bf16(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(bf16x8, o);
 }
 
-// Eight fp32 as three bf16 pieces each, exactly (24 significant bits cut into
-// 8 + 8 + 8): the products with bf16 values then sum as fp32 ones would.
+// Eight weights (not negative) as three bf16 pieces each, exactly (24 significant
+// bits cut into 8 + 8 + 8): the products with bf16 values then sum as fp32 ones
+// would.  The second and third are 2^-126 at least: a zero among them would make
+// NaN of an infinite value.
 __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&piece)[3]) {
     u32x4 o[3];
+    const float least = u2f(0x00800000u);
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
         float a = x[e], b = x[e + 1];
 #pragma unroll
         for (int i = 0; i < 3; i++) {
             o[i][e >> 1] = __builtin_amdgcn_perm(f2u(b), f2u(a), 0x07060302u);
-            a -= u2f(f2u(a) & 0xFFFF0000u);
-            b -= u2f(f2u(b) & 0xFFFF0000u);
+            a = fmaxf(a - u2f(f2u(a) & 0xFFFF0000u), least);
+            b = fmaxf(b - u2f(f2u(b) & 0xFFFF0000u), least);
         }
     }
 #pragma unroll

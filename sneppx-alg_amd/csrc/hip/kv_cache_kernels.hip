@@ -4,11 +4,13 @@
 // divisions and without contraction.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cfloat>
 #include <cstdint>
 
 #include "codec.h"
 #include "kv_pool.h"
+#include "launch.h"
 #include "../snx_internal.h"
 
 using namespace snx;
@@ -230,42 +232,44 @@ struct Cut {
     uint32_t max_length, budget, recent, most, row_bytes;
     uint32_t* counts;          // [rows * heads] moves of each row and head (unless moved at once)
     uint32_t* moves;           // [rows * heads][2][most] slots: targets, then sources
-    uint32_t* keys;            // [rows * heads][max_length] where they do not fit in registers
+    uint32_t* keys;            // [rows * heads][max_length] where they do not fit in LDS
 };
 
 // One workgroup per (row, head): the budget-th largest key by its digits from
 // the top (each time a histogram of the keys that agree with the digits found
 // so far, read by every wave for itself), then the free slots below the budget
 // and the kept ones from it on, both in ascending order.  Each wave has
-// consecutive slots, so that order by (wave, step, lane) is order by slot.  KPT
-// keys per thread stay in registers; KPT = 0: in a workspace, any number.
-// MOVE: with so few moves that the workgroup makes them at once.
-template <int KPT, bool MOVE>
+// consecutive slots, so that order by (wave, step, lane) is order by slot.  NEAR:
+// the keys in LDS (in registers the loops over them have to be unrolled, and
+// reading that much code once took longer: XX us for 30001 slots, XX so); else
+// in a workspace, any number.  MOVE: with so few moves that the workgroup makes
+// them at once.
+template <bool NEAR, bool MOVE>
 __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
-    constexpr int kHist = kBins[0] + kBins[1] + kBins[2] + kBins[3];
+    constexpr int kCopies = 4;        // of the first histogram: most keys share a few exponents
+    constexpr int kHist = kCopies * kBins[0] + kBins[1] + kBins[2] + kBins[3];
+    extern __shared__ uint32_t near_keys[];
     __shared__ __attribute__((aligned(16))) uint32_t hist[kHist];
-    __shared__ uint32_t some[KPT == 4 ? 1 : kSome], some_n;
+    __shared__ uint32_t some[kSome], some_n;
     __shared__ uint2 sh[kCutWaves];
     __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t L = kv_length(a.lengths, b, a.max_length), budget = a.budget;
-    const uint32_t steps = (L + kCutThreads - 1) / kCutThreads;       // slots of a thread, up to KPT
+    const uint32_t steps = (L + 4 * kCutThreads - 1) / (4 * kCutThreads) * 4;       // slots of a thread, by fours
     const uint32_t w0 = wave * steps * 64, t0 = w0 + lane;
-    uint32_t* const far_keys = KPT ? nullptr : a.keys + (size_t)blockIdx.x * a.max_length;
+    uint32_t* const keys = NEAR ? near_keys : a.keys + (size_t)blockIdx.x * a.max_length;
 
     for (int i = tid; i < kHist; i += kCutThreads) hist[i] = 0;
     if (tid == 0) some_n = 0;
-    uint32_t kept_keys[KPT ? KPT : 1];
     bool gone = false;
     if (L > budget) {
         const int64_t from64 = (int64_t)a.next_pos[b] - (int64_t)a.recent;
         const int32_t from = (int32_t)(from64 < INT32_MIN ? INT32_MIN : from64);
         // G slots at once (past the length: its last one), so that their look-ups
         // and loads are in flight together; key 0 past the length
-        constexpr int G = KPT == 0 ? 8 : KPT % 16 == 0 ? 16 : KPT;
-        const uint32_t groups = (steps + G - 1) / G;
-        auto group = [&](uint32_t i0, uint32_t (&q)[G]) {
+        constexpr int G = 8;
+        for (uint32_t i0 = 0; i0 < steps; i0 += G) {
             uint32_t rows[G];
             float w[G];
             int32_t pos[G];
@@ -282,23 +286,9 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
                 pos[i] = p.positions[rows[i]];
             }
 #pragma unroll
-            for (int i = 0; i < G; i++) q[i] = t0 + 64 * (i0 + i) < L ? rank_key(w[i], pos[i], from) : 0u;
-        };
-        if (KPT) {
-#pragma unroll
-            for (int i0 = 0; i0 < KPT; i0 += G) {
-                uint32_t q[G] = {};
-                if ((uint32_t)i0 < steps) group(i0, q);
-#pragma unroll
-                for (int i = 0; i < G; i++) kept_keys[KPT ? i0 + i : 0] = q[i];
-            }
-        } else {
-            for (uint32_t i0 = 0; i0 < groups * G; i0 += G) {
-                uint32_t q[G];
-                group(i0, q);
-#pragma unroll
-                for (int i = 0; i < G; i++)
-                    if (i0 + i < steps && t0 + 64 * (i0 + i) < L) far_keys[t0 + 64 * (i0 + i)] = q[i];
+            for (int i = 0; i < G; i++) {
+                const uint32_t t = t0 + 64 * (i0 + i), q = t < L ? rank_key(w[i], pos[i], from) : 0u;
+                if (i0 + i < steps && (NEAR || t < L)) keys[t] = q;
             }
         }
     }
@@ -309,18 +299,20 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         return;
     }
     // Slots past the length have the lowest key and come after all others: no
-    // test keeps them out below.  (A workspace's keys are read by the thread that
-    // wrote them.)
-    auto key = [&](uint32_t i) { return KPT ? kept_keys[KPT ? i : 0] : t0 + 64 * i < L ? far_keys[t0 + 64 * i] : 0u; };
-    auto each = [&](auto f) {
-        if (KPT) {
+    // test keeps them out below.  (Keys are read by the thread that wrote them.)
+    auto each_of = [&](uint32_t i0, uint32_t end, auto f) {
+        for (uint32_t i = i0; i < end; i += 4) {
+            uint32_t q[4];
 #pragma unroll
-            for (int i = 0; i < KPT; i++)
-                if ((uint32_t)i < steps) f((uint32_t)i);
-        } else {
-            for (uint32_t i = 0; i < steps; i++) f(i);
+            for (int u = 0; u < 4; u++) {
+                const uint32_t t = t0 + 64 * (i + u);
+                q[u] = NEAR || t < L ? keys[t] : 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) f(i + u, q[u]);
         }
     };
+    auto each = [&](auto f) { each_of(0, steps, f); };
 
     auto lane_rank = [&](uint64_t m) {
         return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
@@ -336,17 +328,17 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         const uint32_t digits = (1u << width) - 1u, above_shift = (shift + width) & 31;
         // One pass over all keys puts those that are left aside, if there is room
         // (8192 x 8 heads x 8 rows: 17 -> XX us).
-        if (KPT != 4 && pass == 1 && tied <= kSome) {
+        if (pass == 1 && tied <= kSome) {
             few = true;
-            each([&](uint32_t i) {
-                const uint32_t q = key(i);
-                const bool in = q >> above_shift == prefix >> above_shift;
-                const uint64_t who = __ballot(in);
-                if (who == 0) return;
-                uint32_t at = 0;
-                if (lane == 0) at = atomicAdd(&some_n, (uint32_t)__popcll(who));
-                at = __builtin_amdgcn_readfirstlane(at);
-                if (in) some[at + lane_rank(who)] = q;
+            uint32_t own = 0;
+            each([&](uint32_t, uint32_t q) { own += __popcll(__ballot(q >> above_shift == prefix >> above_shift)); });
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(&some_n, own);
+            at = __builtin_amdgcn_readfirstlane(at);
+            each([&](uint32_t, uint32_t q) {
+                const uint64_t who = __ballot(q >> above_shift == prefix >> above_shift);
+                if (who >> lane & 1) some[at + lane_rank(who)] = q;
+                at += __popcll(who);
             });
             __syncthreads();
         }
@@ -356,15 +348,16 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
                 if (q >> above_shift == prefix >> above_shift) atomicAdd(&hp[(q >> shift) & digits], 1u);
             }
         } else {
-            each([&](uint32_t i) {
-                const uint32_t q = key(i), digit = (q >> shift) & digits;
+            each([&](uint32_t, uint32_t q) {
+                const uint32_t digit = (q >> shift) & digits;
+                const uint32_t to = pass == 0 ? digit * kCopies + lane % kCopies : digit;
                 const uint64_t who = pass == 0 ? ~0ull : __ballot(q >> above_shift == prefix >> above_shift);
                 if (who == 0) return;
                 // many alike (zeros, recent ones) are counted at once
                 if (who == ~0ull && __ballot(digit != (uint32_t)__builtin_amdgcn_readfirstlane(digit)) == 0) {
-                    if (lane == 0) atomicAdd(&hp[digit], 64u);
+                    if (lane == 0) atomicAdd(&hp[to], 64u);
                 } else if (who >> lane & 1) {
-                    atomicAdd(&hp[digit], 1u);
+                    atomicAdd(&hp[to], 1u);
                 }
             });
         }
@@ -374,13 +367,22 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         uint32_t n[most];
         const int per = bins / 64;
         uint32_t sum = 0;
+        if (pass == 0) {                             // a bin's copies at once
 #pragma unroll
-        for (int j = 0; j < per; j += 4) {
-            const u32x4 v = *reinterpret_cast<const u32x4*>(hp + bins - per * (lane + 1) + j);
+            for (int j = 0; j < per; j++) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(hp + 4 * (bins - per * (lane + 1) + j));
+                n[j] = v[0] + v[1] + v[2] + v[3];
+                sum += n[j];
+            }
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                n[j + e] = v[e];
-                sum += v[e];
+            for (int j = 0; j < per; j += 4) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(hp + bins - per * (lane + 1) + j);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    n[j + e] = v[e];
+                    sum += v[e];
+                }
             }
         }
         const uint32_t upto = lane_prefix(sum);
@@ -399,21 +401,21 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         prefix |= (uint32_t)__builtin_amdgcn_readlane(digit, at) << shift;
         want = __builtin_amdgcn_readlane(rest, at);
         tied = __builtin_amdgcn_readlane(count, at);
-        hp += bins;
+        hp += pass == 0 ? kCopies * bins : bins;
     }
 
     // of the keys equal to the threshold the first `want` stay
     uint2 total;
     uint32_t ties = 0, none = 0;
     if (want < tied) {
-        each([&](uint32_t i) { ties += __popcll(__ballot(key(i) == prefix)); });
+        each([&](uint32_t, uint32_t q) { ties += __popcll(__ballot(q == prefix)); });
         wave_prefix(ties, none, sh, total);
     }
     uint32_t seen = ties;
-    // lanes whose slot of step i stays
-    auto stay = [&](uint32_t i) -> uint64_t {
-        const uint32_t q = key(i);
-        if (want == tied) return __ballot(q >= prefix);
+    // lanes whose slot stays
+    const bool ranked = want < tied;
+    auto stay = [&](uint32_t q) -> uint64_t {
+        if (!ranked) return __ballot(q >= prefix);
         const uint64_t tb = __ballot(q == prefix);
         const uint64_t s = __ballot(q > prefix || (q == prefix && seen + lane_rank(tb) < want));
         seen += __popcll(tb);
@@ -424,15 +426,12 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     // both before them in the block (the latter in the upper half).
     auto block = [&](uint32_t i0, uint64_t& hole, uint64_t& far) {
         uint32_t lo = 0, hi = 0;
-        auto put = [&](uint32_t i) {
-            const uint64_t s = stay(i);
+        each_of(i0, i0 + 64 < steps ? i0 + 64 : steps, [&](uint32_t i, uint32_t q) {
+            const uint64_t s = stay(q);
             const bool me = (uint32_t)lane == i - i0;
             lo = me ? (uint32_t)s : lo;
             hi = me ? (uint32_t)(s >> 32) : hi;
-        };
-        if (KPT) each(put);
-        else
-            for (uint32_t i = i0; i < i0 + 64 && i < steps; i++) put(i);
+        });
         const uint64_t s = (uint64_t)hi << 32 | lo;
         const uint32_t at = w0 + 64 * (i0 + lane);
         const uint64_t low = i0 + lane >= steps || at >= budget ? 0 : budget - at >= 64 ? ~0ull : ((uint64_t)1 << (budget - at)) - 1;
@@ -452,17 +451,19 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     uint32_t* const to = MOVE ? list : a.moves + (size_t)blockIdx.x * 2 * a.most;
     uint32_t* const of = to + (MOVE ? kMoveAtOnce : a.most);
     for (uint32_t i0 = 0; i0 < steps; i0 += 64) {
-        if (!KPT) block(i0, hole, far);
+        if (steps > 64) block(i0, hole, far);      // (else it is the one above)
         const uint32_t own = __popcll(hole) | __popcll(far) << 16, upto = lane_prefix(own), before = upto - own;
         const uint32_t end = i0 + 64 < steps ? 64 : steps - i0;
         for (uint32_t i = 0; i < end; i++) {
-            const uint64_t hb = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(hole >> 32), i) << 32 |
-                                (uint32_t)__builtin_amdgcn_readlane((uint32_t)hole, i);
-            const uint64_t fb = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(far >> 32), i) << 32 |
-                                (uint32_t)__builtin_amdgcn_readlane((uint32_t)far, i);
-            const uint32_t at = __builtin_amdgcn_readlane(before, i), t = t0 + 64 * (i0 + i);
-            if (hb >> lane & 1) to[holes + (at & 0xFFFF) + lane_rank(hb)] = t;
-            if (fb >> lane & 1) of[fars + (at >> 16) + lane_rank(fb)] = t;
+            const uint32_t t = t0 + 64 * (i0 + i), before_i = __builtin_amdgcn_readlane(before, i);
+            auto write = [&](uint64_t mine, uint32_t* to, uint32_t at) {
+                const uint64_t m = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(mine >> 32), i) << 32 |
+                                   (uint32_t)__builtin_amdgcn_readlane((uint32_t)mine, i);
+                if (m >> lane & 1) to[at + lane_rank(m)] = t;
+            };
+            // a step lies below the budget, or from it on, or has it within
+            if (w0 + 64 * (i0 + i) < budget) write(hole, to, holes + (before_i & 0xFFFF));
+            if (w0 + 64 * (i0 + i) + 64 > budget) write(far, of, fars + (before_i >> 16));
         }
         const uint32_t sum = __builtin_amdgcn_readlane(upto, 63);
         holes += sum & 0xFFFF;
@@ -490,10 +491,21 @@ void append(bool i8, unsigned blocks, const KVPool& p, const NewRows& n, hipStre
     else k_kv_append<false, LR><<<blocks, 256, 0, s>>>(p, n);
 }
 
-template <int KPT>
-void cut(bool at_once, unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
-    if (at_once) k_kv_cut<KPT, true><<<blocks, kCutThreads, 0, s>>>(p, a);
-    else k_kv_cut<KPT, false><<<blocks, kCutThreads, 0, s>>>(p, a);
+template <bool NEAR, bool MOVE>
+int cut(unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
+    // with nothing to cut every workgroup ends at once
+    const int bytes = NEAR && a.most ? (int)((a.max_length + 4 * kCutThreads - 1) / (4 * kCutThreads) * (4 * kCutThreads) * sizeof(uint32_t)) : 0;
+    static std::atomic<uint64_t> done{0};
+    if (bytes > 32768 && lds_optin(reinterpret_cast<const void*>(&k_kv_cut<NEAR, MOVE>), 32 * kCutThreads * sizeof(uint32_t), done) != hipSuccess) {
+        snx_set_error("kv_evict: cannot reserve %d bytes of LDS", bytes);
+        return -1;
+    }
+    k_kv_cut<NEAR, MOVE><<<blocks, kCutThreads, bytes, s>>>(p, a);
+    return snx_launch_check("k_kv_cut");
+}
+template <bool NEAR>
+int cut(bool at_once, unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
+    return at_once ? cut<NEAR, true>(blocks, p, a, s) : cut<NEAR, false>(blocks, p, a, s);
 }
 
 uint32_t most_moves(size_t max_length, size_t budget) {
@@ -538,7 +550,7 @@ int snx_k_kv_append(const SNEPPXKVCache* c, const uint16_t* k, size_t k_stride, 
     return snx_launch_check("k_kv_append");
 }
 
-// Keys that do not fit in the registers of a workgroup
+// keys that do not fit in the LDS of a workgroup
 static bool keys_far(size_t max_length) { return max_length > 32 * (size_t)kCutThreads; }
 
 size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, size_t budget) {
@@ -565,13 +577,8 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
     a.counts = static_cast<uint32_t*>(ws);
     a.moves = a.counts + bh;
     a.keys = at_once ? a.counts : a.moves + bh * 2 * a.most;
-    // with nothing to cut every workgroup ends at once: any form does
-    const size_t keys = a.most ? max_length : 1;
-    if (keys <= 4 * (size_t)kCutThreads) cut<4>(at_once, (unsigned)bh, p, a, S(st));
-    else if (keys <= 12 * (size_t)kCutThreads) cut<12>(at_once, (unsigned)bh, p, a, S(st));
-    else if (!keys_far(keys)) cut<32>(at_once, (unsigned)bh, p, a, S(st));
-    else cut<0>(at_once, (unsigned)bh, p, a, S(st));
-    if (snx_launch_check("k_kv_cut")) return -1;
+    const bool near = !a.most || !keys_far(max_length);
+    if (near ? cut<true>(at_once, (unsigned)bh, p, a, S(st)) : cut<false>(at_once, (unsigned)bh, p, a, S(st))) return -1;
     if (at_once) return 0;
     const size_t chunks = (size_t)a.most * (a.row_bytes / 16), gx = (chunks + 1023) / 1024;
     for (size_t at = 0; at < bh; at += 65535) {

@@ -199,6 +199,31 @@ def test_nonfinite_values_are_the_rows_own(lib):
     assert bool(torch.isfinite(o[3]).all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "int8"])
+@pytest.mark.parametrize("n", [1, 2, 100])
+def test_infinite_values_with_short_weights(lib, n, dtype):
+    """Equal weights, which as powers of two have few significant bits: an infinite
+    value (int8: an infinite scale) times any part of them is infinite."""
+    print(f"[gpu] kv_attention infinite values n={n} {dtype}", flush=True)
+    c, ref, tables, dtab, dlen = build(lib, [n], 1, 64, 16, dtype, 37, garbage=False)
+    c.k.zero_()
+    page, off = int(tables[0, (n - 1) // 16]), (n - 1) % 16
+    if dtype == "int8":
+        c.v[page, 0, off] = 1
+        c.v[page, 0, off, 7] = -1
+        c.v_scales[page, 0, off] = math.inf
+    else:
+        c.v[page, 0, off, 5] = math.inf
+        c.v[page, 0, off, 7] = -math.inf
+    out = torch.empty((1, 4, 64), device=DEV)
+    c.attention(torch.ones((1, 4, 64), dtype=torch.bfloat16, device=DEV), out, dtab, dlen, 112)
+    torch.cuda.synchronize()
+    o = out.cpu()
+    assert bool((o[0, :, 5] == math.inf).all()) and bool((o[0, :, 7] == -math.inf).all())
+    rest = torch.tensor([d for d in range(64) if d not in (5, 7)])
+    assert bool(torch.isfinite(o[0][:, rest]).all() if dtype == "bf16" else (o[0][:, rest] == math.inf).all())
+
+
 def test_all_logits_minus_infinity(lib):
     """Tokens are there and every logit is -inf: 0 / 0, as the softmax has it; a
     row without tokens beside it stays zero."""
