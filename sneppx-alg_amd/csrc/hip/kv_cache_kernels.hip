@@ -239,18 +239,19 @@ struct Cut {
 // the top (each time a histogram of the keys that agree with the digits found
 // so far, read by every wave for itself), then the free slots below the budget
 // and the kept ones from it on, both in ascending order.  Each wave has
-// consecutive slots, so that order by (wave, step, lane) is order by slot.  NEAR:
-// the keys in LDS (in registers the loops over them have to be unrolled, and
-// reading that much code once took longer: XX us for 30001 slots, XX so); else
-// in a workspace, any number.  MOVE: with so few moves that the workgroup makes
-// them at once.
-template <bool NEAR, bool MOVE>
+// consecutive slots, so that order by (wave, step, lane) is order by slot.
+// KEYS: up to 4 of each thread in registers (16 rows of 2049 slots: XX us, in LDS
+// XX), up to 32 in LDS, else in a workspace.  MOVE: with so few moves that the
+// workgroup makes them at once.
+enum { kRegisters, kLds, kWorkspace };
+template <int KEYS, bool MOVE>
 __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
-    constexpr int kCopies = 4;        // of the first histogram: most keys share a few exponents
+    // most keys share a few exponents: with many, the first histogram is in copies
+    constexpr int kCopies = KEYS == kRegisters ? 1 : 4;
     constexpr int kHist = kCopies * kBins[0] + kBins[1] + kBins[2] + kBins[3];
     extern __shared__ uint32_t near_keys[];
     __shared__ __attribute__((aligned(16))) uint32_t hist[kHist];
-    __shared__ uint32_t some[kSome], some_n;
+    __shared__ uint32_t some[KEYS == kRegisters ? 1 : kSome], some_n;
     __shared__ uint2 sh[kCutWaves];
     __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
@@ -258,18 +259,19 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     const uint32_t L = kv_length(a.lengths, b, a.max_length), budget = a.budget;
     const uint32_t steps = (L + 4 * kCutThreads - 1) / (4 * kCutThreads) * 4;       // slots of a thread, by fours
     const uint32_t w0 = wave * steps * 64, t0 = w0 + lane;
-    uint32_t* const keys = NEAR ? near_keys : a.keys + (size_t)blockIdx.x * a.max_length;
+    uint32_t* const keys = KEYS == kLds ? near_keys : a.keys + (size_t)blockIdx.x * a.max_length;
 
     for (int i = tid; i < kHist; i += kCutThreads) hist[i] = 0;
     if (tid == 0) some_n = 0;
     bool gone = false;
+    uint32_t own_keys[4];
     if (L > budget) {
         const int64_t from64 = (int64_t)a.next_pos[b] - (int64_t)a.recent;
         const int32_t from = (int32_t)(from64 < INT32_MIN ? INT32_MIN : from64);
         // G slots at once (past the length: its last one), so that their look-ups
         // and loads are in flight together; key 0 past the length
-        constexpr int G = 8;
-        for (uint32_t i0 = 0; i0 < steps; i0 += G) {
+        constexpr int G = KEYS == kRegisters ? 4 : 8;
+        for (uint32_t i0 = 0; i0 < (KEYS == kRegisters ? 4 : steps); i0 += G) {
             uint32_t rows[G];
             float w[G];
             int32_t pos[G];
@@ -288,7 +290,8 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
 #pragma unroll
             for (int i = 0; i < G; i++) {
                 const uint32_t t = t0 + 64 * (i0 + i), q = t < L ? rank_key(w[i], pos[i], from) : 0u;
-                if (i0 + i < steps && (NEAR || t < L)) keys[t] = q;
+                if (KEYS == kRegisters) own_keys[i & 3] = q;
+                else if (i0 + i < steps && (KEYS == kLds || t < L)) keys[t] = q;
             }
         }
     }
@@ -301,12 +304,12 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     // Slots past the length have the lowest key and come after all others: no
     // test keeps them out below.  (Keys are read by the thread that wrote them.)
     auto each_of = [&](uint32_t i0, uint32_t end, auto f) {
-        for (uint32_t i = i0; i < end; i += 4) {
+        for (uint32_t i = i0; i < (KEYS == kRegisters ? 4 : end); i += 4) {
             uint32_t q[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const uint32_t t = t0 + 64 * (i + u);
-                q[u] = NEAR || t < L ? keys[t] : 0u;
+                q[u] = KEYS == kRegisters ? own_keys[u] : KEYS == kLds || t < L ? keys[t] : 0u;
             }
 #pragma unroll
             for (int u = 0; u < 4; u++) f(i + u, q[u]);
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         const uint32_t digits = (1u << width) - 1u, above_shift = (shift + width) & 31;
         // One pass over all keys puts those that are left aside, if there is room
         // (8192 x 8 heads x 8 rows: 17 -> XX us).
-        if (pass == 1 && tied <= kSome) {
+        if (KEYS != kRegisters && pass == 1 && tied <= kSome) {
             few = true;
             uint32_t own = 0;
             each([&](uint32_t, uint32_t q) { own += __popcll(__ballot(q >> above_shift == prefix >> above_shift)); });
@@ -367,7 +370,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         uint32_t n[most];
         const int per = bins / 64;
         uint32_t sum = 0;
-        if (pass == 0) {                             // a bin's copies at once
+        if (pass == 0 && kCopies == 4) {             // a bin's copies at once
 #pragma unroll
             for (int j = 0; j < per; j++) {
                 const u32x4 v = *reinterpret_cast<const u32x4*>(hp + 4 * (bins - per * (lane + 1) + j));
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     uint32_t* const to = MOVE ? list : a.moves + (size_t)blockIdx.x * 2 * a.most;
     uint32_t* const of = to + (MOVE ? kMoveAtOnce : a.most);
     for (uint32_t i0 = 0; i0 < steps; i0 += 64) {
-        if (steps > 64) block(i0, hole, far);      // (else it is the one above)
+        if (KEYS == kWorkspace && steps > 64) block(i0, hole, far);      // (else it is the one above)
         const uint32_t own = __popcll(hole) | __popcll(far) << 16, upto = lane_prefix(own), before = upto - own;
         const uint32_t end = i0 + 64 < steps ? 64 : steps - i0;
         for (uint32_t i = 0; i < end; i++) {
@@ -491,21 +494,20 @@ void append(bool i8, unsigned blocks, const KVPool& p, const NewRows& n, hipStre
     else k_kv_append<false, LR><<<blocks, 256, 0, s>>>(p, n);
 }
 
-template <bool NEAR, bool MOVE>
+template <int KEYS, bool MOVE>
 int cut(unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
-    // with nothing to cut every workgroup ends at once
-    const int bytes = NEAR && a.most ? (int)((a.max_length + 4 * kCutThreads - 1) / (4 * kCutThreads) * (4 * kCutThreads) * sizeof(uint32_t)) : 0;
+    const int bytes = KEYS == kLds ? (int)((a.max_length + 4 * kCutThreads - 1) / (4 * kCutThreads) * (4 * kCutThreads) * sizeof(uint32_t)) : 0;
     static std::atomic<uint64_t> done{0};
-    if (bytes > 32768 && lds_optin(reinterpret_cast<const void*>(&k_kv_cut<NEAR, MOVE>), 32 * kCutThreads * sizeof(uint32_t), done) != hipSuccess) {
+    if (bytes && lds_optin(reinterpret_cast<const void*>(&k_kv_cut<KEYS, MOVE>), 32 * kCutThreads * sizeof(uint32_t), done) != hipSuccess) {
         snx_set_error("kv_evict: cannot reserve %d bytes of LDS", bytes);
         return -1;
     }
-    k_kv_cut<NEAR, MOVE><<<blocks, kCutThreads, bytes, s>>>(p, a);
+    k_kv_cut<KEYS, MOVE><<<blocks, kCutThreads, bytes, s>>>(p, a);
     return snx_launch_check("k_kv_cut");
 }
-template <bool NEAR>
+template <int KEYS>
 int cut(bool at_once, unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
-    return at_once ? cut<NEAR, true>(blocks, p, a, s) : cut<NEAR, false>(blocks, p, a, s);
+    return at_once ? cut<KEYS, true>(blocks, p, a, s) : cut<KEYS, false>(blocks, p, a, s);
 }
 
 uint32_t most_moves(size_t max_length, size_t budget) {
@@ -577,8 +579,10 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
     a.counts = static_cast<uint32_t*>(ws);
     a.moves = a.counts + bh;
     a.keys = at_once ? a.counts : a.moves + bh * 2 * a.most;
-    const bool near = !a.most || !keys_far(max_length);
-    if (near ? cut<true>(at_once, (unsigned)bh, p, a, S(st)) : cut<false>(at_once, (unsigned)bh, p, a, S(st))) return -1;
+    const int rc = !a.most || max_length <= 4 * (size_t)kCutThreads ? cut<kRegisters>(at_once, (unsigned)bh, p, a, S(st))
+                   : !keys_far(max_length)                          ? cut<kLds>(at_once, (unsigned)bh, p, a, S(st))
+                                                                    : cut<kWorkspace>(at_once, (unsigned)bh, p, a, S(st));
+    if (rc) return -1;
     if (at_once) return 0;
     const size_t chunks = (size_t)a.most * (a.row_bytes / 16), gx = (chunks + 1023) / 1024;
     for (size_t at = 0; at < bh; at += 65535) {
