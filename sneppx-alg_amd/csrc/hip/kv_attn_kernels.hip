@@ -76,10 +76,10 @@ struct Attn {
 // and the beginning of another in it, and so all end together.  Where a share is
 // only a few steps, changing the row costs more than that evens out, and every
 // row begins with a new share.  The lengths are known on the device alone, so
-// every wave works this out for itself.  (us of shares across rows / by rows: 16
-// rows of 0 to 4096 tokens, 4 steps a share, 32 / 28; 128 of 0 to 2000, 16 steps,
-// 101 / 109; 64 of 0 to 8192, 32 steps, 183 / 210.  A grid for the longest row
-// that the host allows for leaves most of it idle: 45 for the first.)
+// every wave works this out for itself.  (us of shares across rows / by rows, 8 heads
+// of 128 in bf16: 16 rows of 0 to 4096 tokens, 4 steps a share, 32 / 28; 24 rows, 6
+// steps, 46 / 54; 64 rows, 16 steps, 100 / 118.  A grid for the longest row that
+// the host allows for leaves most of it idle: 45 for the first.)
 struct Row {
     uint32_t b, at, len;           // the row, its first step, its length in tokens
     __device__ __forceinline__ uint32_t steps() const { return len > STEP ? (len + STEP - 1) / STEP : 1; }
@@ -97,7 +97,7 @@ struct Shares {
 };
 constexpr uint32_t kMostShares = 256;     // of a row
 
-constexpr uint32_t kFewSteps = 8;         // of a share
+constexpr uint32_t kFewSteps = 4;         // of a share
 
 struct Division {
     const Attn& a;

@@ -109,6 +109,50 @@ def test_attention(lib, case, accumulate):
     compare(c, ref, tables, dtab, dlen, lengths, q, out, 1 / math.sqrt(dim), accumulate=accumulate)
 
 
+@pytest.mark.parametrize("lengths,heads,dim,dtype", [
+    ([3000, 0, 1, 2500, 1200, 700, 4000], 64, 16, "bf16"),       # shares of several steps that go across rows
+    ([128] * 40 + [0] * 30 + list(range(0, 400, 5)), 32, 8, "bf16"),      # 150 rows, many of one step or none
+    ([513, 0, 77, 1024, 300] * 30, 64, 16, "int8"),
+    ([20000], 1, 16, "int8"),                                    # more shares of a row than a wave has lanes
+    ([40001, 300], 1, 16, "bf16"),                               # and as many as a row may have
+    ([1] * 300, 2, 32, "bf16"),
+])
+def test_division_of_rows(lib, lengths, heads, dim, dtype):
+    """How rows are cut depends on all their lengths: shares of whole steps that
+    end and begin within rows, or rows that begin shares."""
+    print(f"[gpu] kv_attention division of {len(lengths)} rows {heads} {dim} {dtype}", flush=True)
+    c, ref, tables, dtab, dlen = build(lib, lengths, heads, dim, 64, dtype, 50 + dim)
+    g = torch.Generator(device=DEV).manual_seed(heads)
+    q = torch.randn((len(lengths), heads, dim), device=DEV, generator=g).to(torch.bfloat16)
+    out = torch.full((len(lengths), heads, dim), 7.0, device=DEV)
+    compare(c, ref, tables, dtab, dlen, lengths, q, out, 1 / math.sqrt(dim))
+    # the same through the second launch (as recorded calls join), bit for bit
+    st = torch.cuda.Stream()
+    again = torch.full_like(out, 5.0)
+    torch.cuda.synchronize()
+    rec = lib.capture(lambda: c.attention(q, again, dtab, dlen, dtab.shape[1] * 64, 1 / math.sqrt(dim),
+                                          stream=st.cuda_stream), stream=st.cuda_stream)
+    lib.graph_launch(rec, stream=st.cuda_stream)
+    st.synchronize()
+    assert torch.equal(again.view(torch.int32), out.view(torch.int32))
+    lib.graph_destroy(rec)
+    lib.fn["SNEPPX_qlinear_release_workspaces"](st.cuda_stream)
+
+
+def test_calls_of_many_divisions_in_turn(lib):
+    """One stream's scratch and counters serve calls of every size in turn."""
+    print("[gpu] kv_attention sizes in turn", flush=True)
+    cases = [([700, 30], 8, 64, "bf16"), ([5], 1, 128, "int8"), ([2000, 0, 900, 1], 4, 256, "bf16"), ([300] * 9, 16, 32, "int8")]
+    made = []
+    for i, (lengths, heads, dim, dtype) in enumerate(cases):
+        c, ref, tables, dtab, dlen = build(lib, lengths, heads, dim, 16, dtype, 60 + i)
+        g = torch.Generator(device=DEV).manual_seed(i)
+        q = torch.randn((len(lengths), 2 * heads, dim), device=DEV, generator=g).to(torch.bfloat16)
+        made.append((c, ref, tables, dtab, dlen, lengths, q, torch.empty(q.shape, device=DEV), 1 / math.sqrt(dim)))
+    for m in made + made[::-1]:
+        compare(*m)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "int8"])
 @pytest.mark.parametrize("page,absent", [(16, [(0, 0, -1), (0, 7, 1 << 30), (1, 3, -5), (2, 0, -1)]), (3, [(0, 40, -1)]),
                                          (64, [(0, 4, -1), (1, 0, 999999)])])
