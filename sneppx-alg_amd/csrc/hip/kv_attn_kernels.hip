@@ -6,19 +6,23 @@
 // for the group of query heads that share a key-value head.  Every key and
 // value is used for `group` products only, so reading the cache is what bounds
 // it, and the kernel is built around reading it once:
-//  * k_kv_attn: a workgroup per (row, key-value head, up to 16 of its query
-//    heads, chunk of the length).  Its four waves take tiles of 32 tokens in
-//    turn, each wave with its own running maximum, sum and output, and meet
-//    once at the end.  Heads are the columns of the matrix cores' tiles (a
-//    group of fewer leaves columns empty: even at one head the matrix cores
-//    have 8 times the work that the reads allow, so that costs nothing).
-//  * k_kv_join: with more than one chunk, the chunks' outputs weighted by
-//    their maxima and sums, in the order of the chunks; and the sums of the
-//    attention weights, from the logits that the first kernel wrote.
+//  * k_kv_attn: the tokens of all rows are cut into equal shares, as many as the
+//    CUs hold workgroups; a workgroup takes a share of one key-value head and up
+//    to 16 of its query heads.  Its four waves take tiles of 32 tokens in turn,
+//    each wave with its own running maximum, sum and output, and meet at the
+//    row's end.  Heads are the columns of the matrix cores' tiles (a group of
+//    fewer leaves columns empty: 16 rows of 4096 tokens take 52, 53 and 57 us at
+//    1, 4 and 16 query heads to a key-value head).
+//  * A row in several shares is joined, in the order of its shares, by the last of
+//    them to arrive, or by k_kv_join after them, which also adds the attention
+//    weights, from the logits that the first kernel wrote.
+// Reached: 131072 tokens of 8 heads of 128 in bf16 (537 MB) 98 us, 5.5 TB/s, where a
+// copy of 256 MB runs at 5.4; 64 rows of 0 to 8192 in int8 (532 MB) 105 us.  A call
+// is about 8 us and what it reads at 5.8 TB/s: the look-ups, the first tile, the
+// meeting and the join follow one another.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
-
 
 #include "codec.h"
 #include "kv_pool.h"
@@ -42,7 +46,7 @@ hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 constexpr int SLOT_KV_ATTN = 7;       // of the stream's workspaces
 constexpr int TILE = 32;              // tokens of a wave's step
 constexpr int WAVES = 4;
-constexpr int STEP = TILE * WAVES;    // tokens of a workgroup's step: chunks are multiples of it
+constexpr int STEP = TILE * WAVES;    // tokens of a workgroup's step
 
 // Waves of a SIMD that the registers allow with heads padded to `dim`: of a tile's
 // keys, values, queries and outputs.  (bf16 heads of 128 at three spill some:
@@ -64,6 +68,7 @@ struct Attn {
     float* part;              // [2 * shares][kv_heads * tiles][heads][dim]
     float2* ml;               // [2 * shares][kv_heads * tiles][heads]: maximum, sum
     float* logits;            // [rows][q_heads][logit_stride], or NULL
+    float2* whole;            // with logits, [rows][q_heads] of rows in one share: maximum, 1 / sum
     uint32_t rows, q_heads, max_length, tiles, heads, shares, logit_stride;
     Divider by_eights, by_heads;      // by 8 tiles and by kv_heads
     float scale_log2;
@@ -119,16 +124,23 @@ struct Division {
         per = per > least ? per : least;
         by_row = per <= kFewSteps;
     }
-    __device__ __forceinline__ uint32_t length(uint32_t r) const { return r < a.rows ? kv_length(a.lengths, r, a.max_length) : 0; }
-    __device__ __forceinline__ uint32_t steps(uint32_t r, uint32_t len) const { return r < a.rows ? Row{r, 0, len}.steps() : 0; }
+    __device__ __forceinline__ uint32_t length(uint32_t r) const {
+        return r < a.rows ? kv_length(a.lengths, r, a.max_length) : 0;
+    }
+    __device__ __forceinline__ uint32_t steps(uint32_t r, uint32_t len) const {
+        return r < a.rows ? Row{r, 0, len}.steps() : 0;
+    }
     // what a row takes of the steps: whole shares by row
-    __device__ __forceinline__ uint32_t extent(uint32_t steps) const { return by_row ? (steps + per - 1) / per * per : steps; }
+    __device__ __forceinline__ uint32_t extent(uint32_t steps) const {
+        return by_row ? (steps + per - 1) / per * per : steps;
+    }
     // the row that step `at` belongs to, or row `b`
     template <bool STEPS>
     __device__ __forceinline__ Row find(uint32_t x) const {
         uint32_t base = 0;
         for (uint32_t r0 = 0;; r0 += 64) {
-            const uint32_t r = r0 + (threadIdx.x & 63), len = r0 ? length(r) : len0, n = extent(steps(r, len)), upto = lane_prefix(n);
+            const uint32_t r = r0 + (threadIdx.x & 63), len = r0 ? length(r) : len0;
+            const uint32_t n = extent(steps(r, len)), upto = lane_prefix(n);
             const uint64_t behind = STEPS ? __ballot(base + upto > x) : __ballot(r == x);
             if (behind) {
                 const int lane = __builtin_ctzll(behind);
@@ -241,13 +253,15 @@ struct Parts {
         : a(attn), part(rsrc(attn.part)), ml(rsrc(attn.ml)), dim(d), units(n), unit(u) {}
     __device__ __forceinline__ uint32_t at(uint32_t slot, uint32_t head) const { return (slot * units + unit) * a.heads + head; }
     __device__ __forceinline__ void put(uint32_t slot, uint32_t head, uint32_t d, f32x4 v) const {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at(slot, head) * dim + d) * 4, 0, kSysCoherent);
+        const u32x4 x = __builtin_bit_cast(u32x4, v);
+        __builtin_amdgcn_raw_buffer_store_b128(x, part, (at(slot, head) * dim + d) * 4, 0, kSysCoherent);
     }
     __device__ __forceinline__ void put_ml(uint32_t slot, uint32_t head, float m, float l) const {
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{f2u(m), f2u(l)}, ml, at(slot, head) * 8, 0, kSysCoherent);
     }
     __device__ __forceinline__ f32x4 get(uint32_t slot, uint32_t head, uint32_t d) const {
-        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, (at(slot, head) * dim + d) * 4, 0, kSysCoherent));
+        const uint32_t off = (at(slot, head) * dim + d) * 4;
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, off, 0, kSysCoherent));
     }
     __device__ __forceinline__ float2 get_ml(uint32_t slot, uint32_t head) const {
         const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(ml, at(slot, head) * 8, 0, kSysCoherent);
@@ -356,7 +370,7 @@ k_kv_attn(const KVPool p, const Attn a) {
     // The heads of a share, then the next share: workgroups go to the XCDs in turn,
     // and so every XCD gets shares of all rows.  The tiles of one head and share
     // are 8 workgroups apart, on one XCD, whose L2 has their tokens then (16 rows of
-    // 4096, 32 query heads to a key-value head: XX us side by side, XX so).
+    // 4096, 32 query heads to a key-value head: 88 us side by side, 73 so).
     const uint32_t units = p.heads * a.tiles, eights = a.by_eights(blockIdx.x), rest = blockIdx.x - eights * 8 * a.tiles;
     const uint32_t ht = rest / 8, pair = eights * 8 + rest % 8, number = a.by_heads(pair), h = pair - number * p.heads;
     const uint32_t unit = h * a.tiles + ht;
@@ -366,273 +380,276 @@ k_kv_attn(const KVPool p, const Attn a) {
     Row w = cut.find<true>(at);
     if (w.b == a.rows) return;
     const uint32_t row_end = w.at + w.steps(), share_end = at + cut.per;
-    const uint32_t stop = cut.by_row ? (share_end < row_end ? share_end : row_end) : share_end < cut.total ? share_end : cut.total;
+    const uint32_t most = cut.by_row ? row_end : cut.total, stop = share_end < most ? share_end : most;
     const Parts parts(a, FULL ? DP : p.dim, units, unit);
 
     for (;;) {
-    // (opaque, so that what follows from it is not kept in registers from row to row)
-    int tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));
-    const int lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t group = a.q_heads / p.heads;
-    const uint32_t nh = group - ht * 16 < 16 ? group - ht * 16 : 16;
-    const uint32_t hq = h * group + ht * 16;             // the first of the tile's query heads
-    const uint32_t dim = FULL ? DP : p.dim, row_bytes = dim * (I8 ? 1 : 2);
-    uint8_t* const vt = lds + wave * L::WAVE;
-    float* const sc = reinterpret_cast<float*>(vt + L::V);
+        // (opaque, so that what follows from it is not kept in registers from row to row)
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, r = lane & 15, g = lane >> 4;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const uint32_t group = a.q_heads / p.heads;
+        const uint32_t nh = group - ht * 16 < 16 ? group - ht * 16 : 16;
+        const uint32_t hq = h * group + ht * 16;             // the first of the tile's query heads
+        const uint32_t dim = FULL ? DP : p.dim, row_bytes = dim * (I8 ? 1 : 2);
+        uint8_t* const vt = lds + wave * L::WAVE;
+        float* const sc = reinterpret_cast<float*>(vt + L::V);
 
-    const uint32_t b = w.b, ends_at = w.at + w.steps() < stop ? w.at + w.steps() : stop;
-    const uint32_t first = (at - w.at) * STEP, upto = (ends_at - w.at) * STEP, last = upto < w.len ? upto : w.len;
-    const Shares shares(w, cut.per);
-    const uint32_t next_len = ends_at < stop ? cut.length(b + 1) : 0;
+        const uint32_t b = w.b, ends_at = w.at + w.steps() < stop ? w.at + w.steps() : stop;
+        const uint32_t first = (at - w.at) * STEP, upto = (ends_at - w.at) * STEP, last = upto < w.len ? upto : w.len;
+        const Shares shares(w, cut.per);
+        const uint32_t next_len = ends_at < stop ? cut.length(b + 1) : 0;
 
-    f32x4 o[DT] = {};
-    float m = -INFINITY, sum = 0.0f;
-    bool any = false;
+        f32x4 o[DT] = {};
+        float m = -INFINITY, sum = 0.0f;
+        bool any = false;
 
-    // this lane's two tokens of a tile: the page table's entries, then their rows
-    // of the pool (a token that is not there: row 0, read but not used)
-    uint32_t entry[2], row[2];
-    bool ok[2], ok_next[2];
-    auto look = [&](uint32_t base) {
+        // this lane's two tokens of a tile: the page table's entries, then their rows
+        // of the pool (a token that is not there: row 0, read but not used)
+        uint32_t entry[2], row[2];
+        bool ok[2], ok_next[2];
+        auto look = [&](uint32_t base) {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint32_t tok = base + 8 * (r >> 2) + 4 * t + (r & 3);
-            entry[t] = tok < last ? (uint32_t)p.tables[(size_t)b * p.width + p.page_of(tok)] : 0xFFFFFFFFu;
-        }
-    };
-    auto find = [&](uint32_t base) {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint32_t tok = base + 8 * (r >> 2) + 4 * t + (r & 3);
-            ok_next[t] = entry[t] < p.pages;
-            row[t] = ok_next[t] ? (entry[t] * p.heads + h) * p.page_size + (tok - p.page_of(tok) * p.page_size) : 0;
-        }
-    };
-    u32x4 kc[2][NC], vc[2][NC];
-    float ksc[2], vsc[2];
-    auto chunk_at = [&](const uint8_t* pool, int t, int i) {
-        const uint32_t c = 16 * (g + 4 * i);
-        return *reinterpret_cast<const u32x4*>(pool + (size_t)row[t] * row_bytes + (FULL || c < row_bytes ? c : 0));
-    };
-    auto load_k = [&] {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int i = 0; i < NC; i++) kc[t][i] = chunk_at(p.k, t, i);
-            if (I8) ksc[t] = p.ks[row[t]];
-        }
-    };
-    auto load_v = [&] {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int i = 0; i < NC; i++) vc[t][i] = chunk_at(p.v, t, i);
-            if (I8) vsc[t] = p.vs[row[t]];
-        }
-    };
-
-    uint32_t base = first + wave * TILE;
-    if (base < last) look(base);
-    bf16x8 q[KS];
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
-        const uint32_t d = I8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 8 * (g + 4 * s);
-        u32x4 w = {0u, 0u, 0u, 0u};
-        if ((uint32_t)r < nh && d < dim) {
-            const uint16_t* src = a.q + b * a.q_stride + (size_t)(hq + r) * dim + d;
-            if (a.q_aligned) w = *reinterpret_cast<const u32x4*>(src);
-            else
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
-        }
-        q[s] = __builtin_bit_cast(bf16x8, w);
-    }
-
-    if (base < last) {
-        find(base);
-        look(base + STEP);
-        load_k();
-        load_v();
-    }
-    while (base < last) {
-        const uint32_t next = base + STEP;
-        ok[0] = ok_next[0];
-        ok[1] = ok_next[1];
-        const uint64_t t0 = __ballot(ok[0]), t1 = __ballot(ok[1]);      // lanes whose tokens are there
-        const bool whole = (t0 & t1) == ~0ull, more = next < last;
-        f32x4 s[2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < KS; i++) {
-                u32x4 w = kc[t][I8 ? i >> 1 : i];
-                // (or the compiler converts when it loads, and keeps twice the registers)
-                if (I8) asm volatile("" : "+v"(w));
-                bf16x8 kf;
-                if (I8) kf = (i & 1) ? bytes_to_bf16(w[2], w[3]) : bytes_to_bf16(w[0], w[1]);
-                else kf = __builtin_bit_cast(bf16x8, w);
-                // past the head's end the lane has other elements, maybe NaN
-                if (!FULL && (I8 ? 16 * (g + 4 * (i >> 1)) : 8 * (g + 4 * i)) >= (int)dim)
-                    kf = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i], s[t], 0, 0, 0);
+            for (int t = 0; t < 2; t++) {
+                const uint32_t tok = base + 8 * (r >> 2) + 4 * t + (r & 3);
+                entry[t] = tok < last ? (uint32_t)p.tables[(size_t)b * p.width + p.page_of(tok)] : 0xFFFFFFFFu;
             }
-        }
-        if (I8 && g == 0)
+        };
+        auto find = [&](uint32_t base) {
 #pragma unroll
-            for (int t = 0; t < 2; t++) sc[8 * (r >> 2) + 4 * t + (r & 3)] = ksc[t];
-        if (more) {
-            find(next);
-            look(next + STEP);
+            for (int t = 0; t < 2; t++) {
+                const uint32_t tok = base + 8 * (r >> 2) + 4 * t + (r & 3);
+                ok_next[t] = entry[t] < p.pages;
+                row[t] = ok_next[t] ? (entry[t] * p.heads + h) * p.page_size + (tok - p.page_of(tok) * p.page_size) : 0;
+            }
+        };
+        u32x4 kc[2][NC], vc[2][NC];
+        float ksc[2], vsc[2];
+        auto chunk_at = [&](const uint8_t* pool, int t, int i) {
+            const uint32_t c = 16 * (g + 4 * i);
+            return *reinterpret_cast<const u32x4*>(pool + (size_t)row[t] * row_bytes + (FULL || c < row_bytes ? c : 0));
+        };
+        auto load_k = [&] {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int i = 0; i < NC; i++) kc[t][i] = chunk_at(p.k, t, i);
+                if (I8) ksc[t] = p.ks[row[t]];
+            }
+        };
+        auto load_v = [&] {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int i = 0; i < NC; i++) vc[t][i] = chunk_at(p.v, t, i);
+                if (I8) vsc[t] = p.vs[row[t]];
+            }
+        };
+
+        uint32_t base = first + wave * TILE;
+        if (base < last) look(base);
+        bf16x8 q[KS];
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const uint32_t d = I8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 8 * (g + 4 * s);
+            u32x4 w = {0u, 0u, 0u, 0u};
+            if ((uint32_t)r < nh && d < dim) {
+                const uint16_t* src = a.q + b * a.q_stride + (size_t)(hq + r) * dim + d;
+                if (a.q_aligned) w = *reinterpret_cast<const u32x4*>(src);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
+            }
+            q[s] = __builtin_bit_cast(bf16x8, w);
+        }
+
+        if (base < last) {
+            find(base);
+            look(base + STEP);
             load_k();
+            load_v();
         }
-        // values to LDS by rows, those of absent tokens as zeros (0 * NaN)
+        while (base < last) {
+            const uint32_t next = base + STEP;
+            ok[0] = ok_next[0];
+            ok[1] = ok_next[1];
+            const uint64_t t0 = __ballot(ok[0]), t1 = __ballot(ok[1]);      // lanes whose tokens are there
+            const bool whole = (t0 & t1) == ~0ull, more = next < last;
+            f32x4 s[2];
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const int tok = 8 * (r >> 2) + 4 * t + (r & 3);
+            for (int t = 0; t < 2; t++) {
+                s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < NC; i++) {
-                u32x4 w = vc[t][i];
-                if (!whole && !ok[t]) w = u32x4{0u, 0u, 0u, 0u};
-                *reinterpret_cast<u32x4*>(vt + L::row(tok) + 16 * (g + 4 * i)) = w;
-            }
-            if (I8 && g == 0) sc[TILE + tok] = ok[t] ? vsc[t] : 0.0f;
-        }
-        if (more) load_v();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-
-        __builtin_amdgcn_sched_barrier(0);
-        // softmax of the tile's eight logits of this lane's head
-        float e[8];
-        float top = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float v = s[t][j] * a.scale_log2;
-                if (I8) v *= sc[8 * g + 4 * t + j];
-                if (!whole && !((t ? t1 : t0) >> (4 * g + j) & 1)) v = -INFINITY;
-                e[4 * t + j] = v;
-                top = fmaxf(top, v);
-            }
-        if (SAVE && (uint32_t)r < nh) {
-            float* dst = a.logits + ((size_t)b * a.q_heads + hq + r) * a.logit_stride + base + 8 * g;
-            *reinterpret_cast<f32x4*>(dst) = f32x4{e[0], e[1], e[2], e[3]};
-            *reinterpret_cast<f32x4*>(dst + 4) = f32x4{e[4], e[5], e[6], e[7]};
-        }
-        any |= (t0 | t1) != 0;
-        top = quad_max(top);
-        // The reference point moves only when a logit passes it by 8 (weights
-        // up to 2^8 are no harm): after the first tile hardly ever.
-        if (__any(top > m + 8.0f)) {
-            const float to = fmaxf(m, top);
-            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
-            m = to;
-            sum *= f;
-#pragma unroll
-            for (int i = 0; i < DT; i++) o[i] *= f;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            e[i] = __builtin_amdgcn_exp2f(e[i] - ref);
-            sum += e[i];
-            if (I8) e[i] *= sc[TILE + 8 * g + i];
-        }
-        bf16x8 pc[3];
-        split3(e, pc);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-            bf16x8 vf;
-            if (I8) {
-                const int tok = 8 * g + (r >> 1);
-                const lds_t at = (lds_t)(vt + L::row(tok) + 8 * (r & 1) + 16 * dt);
-                const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)at);
-                vf = bytes_to_bf16((uint32_t)w[0], (uint32_t)w[1]);
-            } else {
-                s16x4 w[2];
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const int tok = 8 * g + 4 * t + (r >> 2);
-                    const lds_t at = (lds_t)(vt + L::row(tok) + 8 * (r & 3) + 32 * dt);
-                    w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                for (int i = 0; i < KS; i++) {
+                    u32x4 w = kc[t][I8 ? i >> 1 : i];
+                    // (or the compiler converts when it loads, and keeps twice the registers)
+                    if (I8) asm volatile("" : "+v"(w));
+                    bf16x8 kf;
+                    if (I8) kf = (i & 1) ? bytes_to_bf16(w[2], w[3]) : bytes_to_bf16(w[0], w[1]);
+                    else kf = __builtin_bit_cast(bf16x8, w);
+                    // past the head's end the lane has other elements, maybe NaN
+                    if (!FULL && (I8 ? 16 * (g + 4 * (i >> 1)) : 8 * (g + 4 * i)) >= (int)dim)
+                        kf = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[i], s[t], 0, 0, 0);
                 }
-                vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
             }
+            if (I8 && g == 0)
 #pragma unroll
-            for (int i = 0; i < 3; i++) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pc[i], o[dt], 0, 0, 0);
-            if (dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        base = next;
-    }
+                for (int t = 0; t < 2; t++) sc[8 * (r >> 2) + 4 * t + (r & 3)] = ksc[t];
+            if (more) {
+                find(next);
+                look(next + STEP);
+                load_k();
+            }
+            // values to LDS by rows, those of absent tokens as zeros (0 * NaN)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int tok = 8 * (r >> 2) + 4 * t + (r & 3);
+#pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    u32x4 w = vc[t][i];
+                    if (!whole && !ok[t]) w = u32x4{0u, 0u, 0u, 0u};
+                    *reinterpret_cast<u32x4*>(vt + L::row(tok) + 16 * (g + 4 * i)) = w;
+                }
+                if (I8 && g == 0) sc[TILE + tok] = ok[t] ? vsc[t] : 0.0f;
+            }
+            if (more) load_v();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 
-    // the waves meet: a maximum of -inf with tokens there is told from no tokens
-    // by a sum of 1 (its outputs are zero)
-    sum = quad_sum(sum);
-    if (m == -INFINITY && any && sum == 0.0f) sum = 1.0f;
-    __syncthreads();
-    if (g == 0) ends[wave][r] = make_float2(m, sum);
-    float* const ow = reinterpret_cast<float*>(lds) + wave * 16 * L::OS;
-    if ((uint32_t)r < nh)
+            // (the phases are kept apart, which keeps registers few)
+            __builtin_amdgcn_sched_barrier(0);
+            // softmax of the tile's eight logits of this lane's head
+            float e[8];
+            float top = -INFINITY;
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f32x4*>(ow + r * L::OS + 16 * dt + 4 * g) = o[dt];
-    __syncthreads();
-    const uint32_t quads = dim / 4;
-    for (uint32_t i = tid; i < nh * quads; i += 256) {
-        const uint32_t hd = i / quads, d = 4 * (i - hd * quads);
-        float top = -INFINITY, total = 0.0f, plain = 0.0f;
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) top = fmaxf(top, ends[w][hd].x);
-        f32x4 v = {};
+                for (int j = 0; j < 4; j++) {
+                    float v = s[t][j] * a.scale_log2;
+                    if (I8) v *= sc[8 * g + 4 * t + j];
+                    if (!whole && !((t ? t1 : t0) >> (4 * g + j) & 1)) v = -INFINITY;
+                    e[4 * t + j] = v;
+                    top = fmaxf(top, v);
+                }
+            if (SAVE && (uint32_t)r < nh) {
+                float* dst = a.logits + ((size_t)b * a.q_heads + hq + r) * a.logit_stride + base + 8 * g;
+                *reinterpret_cast<f32x4*>(dst) = f32x4{e[0], e[1], e[2], e[3]};
+                *reinterpret_cast<f32x4*>(dst + 4) = f32x4{e[4], e[5], e[6], e[7]};
+            }
+            any |= (t0 | t1) != 0;
+            top = quad_max(top);
+            // The reference point moves only when a logit passes it by 8 (weights
+            // up to 2^8 are no harm): after the first tile hardly ever.
+            if (__any(top > m + 8.0f)) {
+                const float to = fmaxf(m, top);
+                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                sum *= f;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float2 e = ends[w][hd];
-            const float f = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
-            total += f * e.y;
-            plain += e.y;
-            v += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds) + (w * 16 + hd) * L::OS + d);
+                for (int i = 0; i < DT; i++) o[i] *= f;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                e[i] = __builtin_amdgcn_exp2f(e[i] - ref);
+                sum += e[i];
+                if (I8) e[i] *= sc[TILE + 8 * g + i];
+            }
+            bf16x8 pc[3];
+            split3(e, pc);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                bf16x8 vf;
+                if (I8) {
+                    const int tok = 8 * g + (r >> 1);
+                    const lds_t at = (lds_t)(vt + L::row(tok) + 8 * (r & 1) + 16 * dt);
+                    const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)at);
+                    vf = bytes_to_bf16((uint32_t)w[0], (uint32_t)w[1]);
+                } else {
+                    s16x4 w[2];
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const int tok = 8 * g + 4 * t + (r >> 2);
+                        const lds_t at = (lds_t)(vt + L::row(tok) + 8 * (r & 3) + 32 * dt);
+                        w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                    }
+                    vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+#pragma unroll
+                for (int i = 0; i < 3; i++) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pc[i], o[dt], 0, 0, 0);
+                if (dt % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            base = next;
         }
-        if (top == -INFINITY) total = plain > 1.0f ? 1.0f : plain;
-        if (!SAVE && shares.n == 1) {
-            parts.store(b, hq + hd, d, v, top == -INFINITY ? total == 0.0f ? 0.0f : NAN : 1.0f / total);
-        } else {
-            const uint32_t slot = 2 * number + (at != number * cut.per);
-            parts.put(slot, hd, d, v);
-            if (d == 0) parts.put_ml(slot, hd, top, total);
-        }
-    }
-    if (!SAVE && shares.n > 1 && a.arrivals) {
-        // the last of the row's shares to arrive joins them
-        __builtin_amdgcn_s_waitcnt(0x0f70);              // vmcnt(0): this wave's stores are out
+
+        // the waves meet: a maximum of -inf with tokens there is told from no tokens
+        // by a sum of 1 (its outputs are zero)
+        sum = quad_sum(sum);
+        if (m == -INFINITY && any && sum == 0.0f) sum = 1.0f;
         __syncthreads();
-        if (tid == 0) {
-            uint32_t* const mine = a.arrivals + (size_t)b * units + unit;
-            const uint32_t c = atomicAdd(mine, 1u);
-            if (c == shares.n - 1) atomicExch(mine, 0u);      // ready for the next call
-            arrived = c;
-        }
+        if (g == 0) ends[wave][r] = make_float2(m, sum);
+        float* const ow = reinterpret_cast<float*>(lds) + wave * 16 * L::OS;
+        if ((uint32_t)r < nh)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f32x4*>(ow + r * L::OS + 16 * dt + 4 * g) = o[dt];
         __syncthreads();
-        if (arrived == shares.n - 1)
-            for (uint32_t j = wave; j < nh; j += WAVES)
-                parts.join(shares, b, j, hq + j, reinterpret_cast<float*>(lds) + wave * kMostShares);
-    }
-    at = ends_at;
-    if (at >= stop) break;
-    w = Row{b + 1, at, next_len};
-    __syncthreads();                                     // the next row's tiles reuse the LDS
+        const uint32_t quads = dim / 4;
+        for (uint32_t i = tid; i < nh * quads; i += 256) {
+            const uint32_t hd = i / quads, d = 4 * (i - hd * quads);
+            float top = -INFINITY, total = 0.0f, plain = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) top = fmaxf(top, ends[w][hd].x);
+            f32x4 v = {};
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float2 e = ends[w][hd];
+                const float f = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
+                total += f * e.y;
+                plain += e.y;
+                v += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds) + (w * 16 + hd) * L::OS + d);
+            }
+            if (top == -INFINITY) total = plain > 1.0f ? 1.0f : plain;
+            if (shares.n == 1) {
+                const float inv = top == -INFINITY ? total == 0.0f ? 0.0f : NAN : 1.0f / total;
+                parts.store(b, hq + hd, d, v, inv);
+                if (SAVE && d == 0) a.whole[(size_t)b * a.q_heads + hq + hd] = make_float2(top, inv);
+            } else {
+                const uint32_t slot = 2 * number + (at != number * cut.per);
+                parts.put(slot, hd, d, v);
+                if (d == 0) parts.put_ml(slot, hd, top, total);
+            }
+        }
+        if (!SAVE && shares.n > 1 && a.arrivals) {
+            // the last of the row's shares to arrive joins them
+            __builtin_amdgcn_s_waitcnt(0x0f70);              // vmcnt(0): this wave's stores are out
+            __syncthreads();
+            if (tid == 0) {
+                uint32_t* const mine = a.arrivals + (size_t)b * units + unit;
+                const uint32_t c = atomicAdd(mine, 1u);
+                if (c == shares.n - 1) atomicExch(mine, 0u);      // ready for the next call
+                arrived = c;
+            }
+            __syncthreads();
+            if (arrived == shares.n - 1)
+                for (uint32_t j = wave; j < nh; j += WAVES)
+                    parts.join(shares, b, j, hq + j, reinterpret_cast<float*>(lds) + wave * kMostShares);
+        }
+        at = ends_at;
+        if (at >= stop) break;
+        w = Row{b + 1, at, next_len};
+        __syncthreads();                                     // the next row's tiles reuse the LDS
     }
 }
 
 // After k_kv_attn, workgroups x of every (row, key-value head): the first
-// `joins` join the chunks of four query heads of the group, one a wave, where
-// there are several or (with logits) anyhow; with logits the others add the
-// attention weights of 256 tokens each.
+// `joins` join the shares of four query heads of the group, one a wave, where
+// there are several; with logits the others add the attention weights of 256
+// tokens each.
 __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, uint32_t joins) {
     __shared__ float2 stat[256];      // of a head: maximum, 1 / sum
     __shared__ float factors[4][kMostShares];
@@ -646,12 +663,12 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
     if (blockIdx.x < joins) {
         const Division cut(a);
         const Shares w(cut.find<false>(b), cut.per);
-        if (a.logits || w.n > 1)
+        if (w.n > 1)
             for (uint32_t j = 4 * blockIdx.x + wave; j < group; j += 4 * joins)
                 parts(j).join(w, b, j % 16, h * group + j, factors[wave]);
         return;
     }
-    // what does not depend on the chunks is loaded first
+    // what does not depend on the shares is loaded first
     constexpr int G = 8;
     const uint32_t t = (blockIdx.x - joins) * 256 + tid, len = kv_length(a.lengths, b, a.max_length);
     if ((blockIdx.x - joins) * 256 >= len) return;
@@ -669,7 +686,8 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
         __syncthreads();
         for (uint32_t j = wave; j < nj; j += 4) {
             const Parts pt = parts(j0 + j);
-            const float2 st = pt.whole(pt.ends(w, (j0 + j) % 16), w, nullptr);
+            const float2 st = w.n == 1 ? a.whole[(size_t)b * a.q_heads + h * group + j0 + j]
+                                       : pt.whole(pt.ends(w, (j0 + j) % 16), w, nullptr);
             if (lane == 0) stat[j] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y);
         }
         __syncthreads();
@@ -715,15 +733,19 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     const KVPool p = kv_pool(c, tables, width);
     const size_t group = q_heads / c->kv_heads, tiles = (group + 15) / 16, units = c->kv_heads * tiles;
     const size_t heads = group < 16 ? group : 16;
-    // as many shares as the CUs hold workgroups at once, and one more for each row
-    // (see Division); no more than there are steps
+    // As many shares as the CUs hold workgroups at once; where rows begin shares, one
+    // more for each row, but a row has a step at least, and they are up to
+    // kFewSteps for each share then.  No more than there are steps.
     const size_t steps = (max_length + STEP - 1) / STEP;
-    const size_t shares = ((size_t)shares_of_cu(padded(c->head_dim), c->dtype == SNEPPX_INT8) * cu_count() + units - 1) / units;
+    const int of_cu = shares_of_cu(padded(c->head_dim), c->dtype == SNEPPX_INT8);
+    const size_t shares = ((size_t)of_cu * cu_count() + units - 1) / units;
     size_t blocks = shares + rows;
+    if (blocks > kFewSteps * shares) blocks = kFewSteps * shares;
     if (blocks > rows * (steps ? steps : 1)) blocks = rows * (steps ? steps : 1);
     blocks = (blocks * c->kv_heads + 7) / 8 * 8 * tiles;
     const size_t part = 2 * blocks * heads * c->head_dim * sizeof(float), ml = 2 * blocks * heads * sizeof(float2);
     const size_t logit_stride = accumulate ? steps * STEP : 0, logits = rows * q_heads * logit_stride * sizeof(float);
+    const size_t whole = accumulate ? rows * q_heads * sizeof(float2) : 0;
     // (a grid has below 2^32 threads; offsets of the parts and counts of steps are of 32 bits)
     if (blocks > 0xffffff || part > 0xffffffffu || steps * rows > 0x7fffffffu || steps >= 0x1000000) {
         snx_set_error("kv_attention: %zu rows of up to %zu tokens are too many", rows, max_length);
@@ -738,7 +760,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
         if (!accumulate && !snx_stream_capturing(st)) {
             if (snx_span_workspaces(part + ml, rows * units * sizeof(uint32_t), st, &ws, &arrivals)) return -1;
         } else {
-            ws = snx_workspace(part + ml + logits, SLOT_KV_ATTN, st);
+            ws = snx_workspace(part + ml + logits + whole, SLOT_KV_ATTN, st);
             if (!ws) return -1;
         }
     }
@@ -753,6 +775,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.part = reinterpret_cast<float*>(w);
     a.logits = accumulate ? reinterpret_cast<float*>(w + part) : nullptr;
     a.ml = reinterpret_cast<float2*>(w + part + logits);
+    a.whole = reinterpret_cast<float2*>(w + part + logits + ml);
     a.rows = (uint32_t)rows;
     a.q_heads = (uint32_t)q_heads;
     a.max_length = (uint32_t)max_length;

@@ -116,16 +116,21 @@ def test_attention(lib, case, accumulate):
     ([20000], 1, 16, "int8"),                                    # more shares of a row than a wave has lanes
     ([40001, 300], 1, 16, "bf16"),                               # and as many as a row may have
     ([1] * 300, 2, 32, "bf16"),
+    (list(range(300)), 32, 8, "bf16"),                           # a share of many whole rows
 ])
 def test_division_of_rows(lib, lengths, heads, dim, dtype):
     """How rows are cut depends on all their lengths: shares of whole steps that
     end and begin within rows, or rows that begin shares."""
     print(f"[gpu] kv_attention division of {len(lengths)} rows {heads} {dim} {dtype}", flush=True)
-    c, ref, tables, dtab, dlen = build(lib, lengths, heads, dim, 64, dtype, 50 + dim)
+    c, ref, tables, dtab, dlen = build(lib, lengths, heads, dim, 64, dtype, 50 + dim, weights=True)
     g = torch.Generator(device=DEV).manual_seed(heads)
     q = torch.randn((len(lengths), heads, dim), device=DEV, generator=g).to(torch.bfloat16)
     out = torch.full((len(lengths), heads, dim), 7.0, device=DEV)
     compare(c, ref, tables, dtab, dlen, lengths, q, out, 1 / math.sqrt(dim))
+    # the same with the weights added
+    both = torch.full_like(out, 5.0)
+    compare(c, ref, tables, dtab, dlen, lengths, q, both, 1 / math.sqrt(dim), accumulate=True)
+    assert torch.equal(both.view(torch.int32), out.view(torch.int32))
     # the same through the second launch (as recorded calls join), bit for bit
     st = torch.cuda.Stream()
     again = torch.full_like(out, 5.0)
