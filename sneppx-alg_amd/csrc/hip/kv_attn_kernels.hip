@@ -503,15 +503,19 @@ k_kv_attn(const KVPool p, const Attn a) {
                 load_k();
             }
             // values to LDS by rows, those of absent tokens as zeros (0 * NaN)
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < NC; i++)
+                        if (!ok[t]) vc[t][i] = u32x4{0u, 0u, 0u, 0u};
+                __builtin_amdgcn_sched_barrier(0);       // (a branch, not a select for each register)
+            }
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 const int tok = 8 * (r >> 2) + 4 * t + (r & 3);
 #pragma unroll
-                for (int i = 0; i < NC; i++) {
-                    u32x4 w = vc[t][i];
-                    if (!whole && !ok[t]) w = u32x4{0u, 0u, 0u, 0u};
-                    *reinterpret_cast<u32x4*>(vt + L::row(tok) + 16 * (g + 4 * i)) = w;
-                }
+                for (int i = 0; i < NC; i++) *reinterpret_cast<u32x4*>(vt + L::row(tok) + 16 * (g + 4 * i)) = vc[t][i];
                 if (I8 && g == 0) sc[TILE + tok] = ok[t] ? vsc[t] : 0.0f;
             }
             if (more) load_v();
@@ -529,10 +533,16 @@ k_kv_attn(const KVPool p, const Attn a) {
                 for (int j = 0; j < 4; j++) {
                     float v = s[t][j] * a.scale_log2;
                     if (I8) v *= sc[8 * g + 4 * t + j];
-                    if (!whole && !((t ? t1 : t0) >> (4 * g + j) & 1)) v = -INFINITY;
                     e[4 * t + j] = v;
-                    top = fmaxf(top, v);
                 }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (!((i < 4 ? t0 : t1) >> (4 * g + (i & 3)) & 1)) e[i] = -INFINITY;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, e[i]);
             if (SAVE && (uint32_t)r < nh) {
                 float* dst = a.logits + ((size_t)b * a.q_heads + hq + r) * a.logit_stride + base + 8 * g;
                 *reinterpret_cast<f32x4*>(dst) = f32x4{e[0], e[1], e[2], e[3]};
