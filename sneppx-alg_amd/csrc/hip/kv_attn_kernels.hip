@@ -39,6 +39,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+// of any alignment that their elements have
+typedef u32x4 bf16_load8 __attribute__((aligned(2)));
+typedef u32x2 bf16_store4 __attribute__((aligned(2)));
+typedef f32x4 f32_store4 __attribute__((aligned(4)));
 typedef __attribute__((address_space(3))) uint8_t* lds_t;
 
 hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
@@ -70,9 +74,9 @@ struct Attn {
     float* logits;            // [rows][q_heads][logit_stride], or NULL
     float2* whole;            // with logits, [rows][q_heads] of rows in one share: maximum, 1 / sum
     uint32_t rows, q_heads, max_length, tiles, heads, shares, logit_stride;
-    Divider by_eights, by_heads;      // by 8 tiles and by kv_heads
+    Divider by_eights, by_heads, by_shares;      // by 8 tiles, kv_heads and shares
     float scale_log2;
-    int out_f32, q_aligned;
+    int out_f32;
 };
 
 // ------------------------------------------------------------- the division
@@ -90,13 +94,26 @@ struct Row {
     __device__ __forceinline__ uint32_t steps() const { return len > STEP ? (len + STEP - 1) / STEP : 1; }
 };
 
+// Division by a number that only the device knows, in fewer instructions than the
+// integer one: the reciprocal is good to 40 bits, and (x + 1/2) / d is at least
+// 1 / 2d away from the next whole number, which is 2^-33 of it or more.
+struct By {
+    uint32_t d;
+    double inv;
+    __device__ __forceinline__ explicit By(uint32_t by) : d(by) {
+        const double y = (double)by, r = __builtin_amdgcn_rcp(y);
+        inv = __builtin_fma(r, __builtin_fma(-y, r, 1.0), r);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)(((double)x + 0.5) * inv); }
+};
+
 // the shares that a row's steps lie in, and where each left its result
 struct Shares {
     uint32_t first, n, inside;     // inside: the row begins within its first share
-    __device__ __forceinline__ Shares(const Row& w, uint32_t per) {
-        first = w.at / per;
-        n = (w.at + w.steps() - 1) / per - first + 1;
-        inside = w.at != first * per;
+    __device__ __forceinline__ Shares(const Row& w, const By& per) {
+        first = per(w.at);
+        n = per(w.at + w.steps() - 1) - first + 1;
+        inside = w.at != first * per.d;
     }
     __device__ __forceinline__ uint32_t slot(uint32_t i) const { return 2 * (first + i) + (i == 0 ? inside : 0); }
 };
@@ -108,7 +125,8 @@ struct Division {
     const Attn& a;
     uint32_t len0, total, per;     // length of row `lane`; steps of all rows, of a share
     bool by_row;
-    __device__ __forceinline__ explicit Division(const Attn& attn) : a(attn) {
+    By by;
+    __device__ __forceinline__ explicit Division(const Attn& attn) : a(attn), by(1) {
         const uint32_t lane = threadIdx.x & 63;
         uint32_t sum = 0, longest = 0;
         len0 = length(lane);
@@ -118,11 +136,12 @@ struct Division {
             longest = n > longest ? n : longest;
         }
         total = __builtin_amdgcn_readlane(lane_prefix(sum), 63);
-        per = (total + a.shares - 1) / a.shares;
+        per = a.by_shares(total + a.shares - 1);
         // a row has part of its first and last share
         const uint32_t least = (lane_max(longest) + kMostShares - 3) / (kMostShares - 2);
         per = per > least ? per : least;
         by_row = per <= kFewSteps;
+        by = By(per);
     }
     __device__ __forceinline__ uint32_t length(uint32_t r) const {
         return r < a.rows ? kv_length(a.lengths, r, a.max_length) : 0;
@@ -132,7 +151,7 @@ struct Division {
     }
     // what a row takes of the steps: whole shares by row
     __device__ __forceinline__ uint32_t extent(uint32_t steps) const {
-        return by_row ? (steps + per - 1) / per * per : steps;
+        return by_row ? by(steps + per - 1) * per : steps;
     }
     // the row that step `at` belongs to, or row `b`
     template <bool STEPS>
@@ -259,12 +278,11 @@ struct Parts {
     __device__ __forceinline__ void put_ml(uint32_t slot, uint32_t head, float m, float l) const {
         __builtin_amdgcn_raw_buffer_store_b64(u32x2{f2u(m), f2u(l)}, ml, at(slot, head) * 8, 0, kSysCoherent);
     }
-    __device__ __forceinline__ f32x4 get(uint32_t slot, uint32_t head, uint32_t d) const {
-        const uint32_t off = (at(slot, head) * dim + d) * 4;
+    __device__ __forceinline__ f32x4 get(uint32_t off) const {
         return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, off, 0, kSysCoherent));
     }
-    __device__ __forceinline__ float2 get_ml(uint32_t slot, uint32_t head) const {
-        const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(ml, at(slot, head) * 8, 0, kSysCoherent);
+    __device__ __forceinline__ float2 get_ml(uint32_t off) const {
+        const u32x2 r = __builtin_amdgcn_raw_buffer_load_b64(ml, off, 0, kSysCoherent);
         return make_float2(u2f(r[0]), u2f(r[1]));
     }
 
@@ -273,12 +291,12 @@ struct Parts {
         float2 e[kMostShares / 64];
     };
     __device__ __forceinline__ Ends ends(const Shares& w, uint32_t head) const {
-        const uint32_t lane = threadIdx.x & 63;
+        const uint32_t lane = threadIdx.x & 63, slots = units * a.heads * 8, from = at(2 * w.first, head) * 8;
         Ends x;
 #pragma unroll
         for (int j = 0; j < (int)kMostShares / 64; j++) {
             x.e[j] = make_float2(-INFINITY, 0.0f);
-            if (64 * j + lane < w.n) x.e[j] = get_ml(w.slot(64 * j + lane), head);
+            if (64 * j < (int)w.n && 64 * j + lane < w.n) x.e[j] = get_ml(from + (64 * j + lane ? 2 * (64 * j + lane) : w.inside) * slots);
         }
         return x;
     }
@@ -292,10 +310,11 @@ struct Parts {
         top = lane_max(top);
 #pragma unroll
         for (int j = 0; j < (int)kMostShares / 64; j++) {
+            if (64 * j >= (int)w.n) continue;
             const float f = x.e[j].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.e[j].x - top);
             total += f * x.e[j].y;
             plain += x.e[j].y;
-            if (factors && 64 * j < w.n) factors[64 * j + lane] = f;
+            if (factors) factors[64 * j + lane] = f;
         }
         total = lane_sum(total);
         plain = lane_sum(plain);
@@ -311,13 +330,17 @@ struct Parts {
         const uint32_t span = dim <= 64 ? 16 : dim <= 128 ? 32 : 64, ways = 64 / span;
         const uint32_t d = 4 * (lane & (span - 1)), way = lane / span;
         const bool in = d < dim;
+        const uint32_t slots = units * a.heads * dim * 4, from = (at(2 * w.first, head) * dim + (in ? d : 0)) * 4;
         const Ends e = ends(w, head);
         f32x4 v = {};
         float2 st = {};
         for (uint32_t i0 = way; i0 < way + (w.n + ways - 1) / ways * ways; i0 += U * ways) {
             f32x4 x[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) x[u] = get(w.slot(i0 + u * ways < w.n ? i0 + u * ways : 0), head, in ? d : 0);
+            for (int u = 0; u < U; u++) {
+                const uint32_t i = i0 + u * ways < w.n ? i0 + u * ways : w.n - 1;     // (not 0: n > 1)
+                x[u] = get(from + (u == 0 && i == 0 ? w.inside : 2 * i) * slots);
+            }
             if (i0 == way) {
                 st = whole(e, w, factors);
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -335,10 +358,12 @@ struct Parts {
 
     __device__ __forceinline__ void store(uint32_t b, uint32_t hq, uint32_t d, f32x4 v, float inv) const {
         const size_t to = b * a.out_stride + (size_t)hq * dim + d;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (a.out_f32) static_cast<float*>(a.out)[to + j] = v[j] * inv;
-            else static_cast<uint16_t*>(a.out)[to + j] = bf16_out(v[j] * inv);
+        v *= inv;
+        if (a.out_f32) {
+            *reinterpret_cast<f32_store4*>(static_cast<float*>(a.out) + to) = v;
+        } else {
+            *reinterpret_cast<bf16_store4*>(static_cast<uint16_t*>(a.out) + to) =
+                u32x2{bf16x2_out(v[0], v[1]), bf16x2_out(v[2], v[3])};
         }
     }
 };
@@ -398,7 +423,7 @@ k_kv_attn(const KVPool p, const Attn a) {
 
         const uint32_t b = w.b, ends_at = w.at + w.steps() < stop ? w.at + w.steps() : stop;
         const uint32_t first = (at - w.at) * STEP, upto = (ends_at - w.at) * STEP, last = upto < w.len ? upto : w.len;
-        const Shares shares(w, cut.per);
+        const Shares shares(w, cut.by);
         const uint32_t next_len = ends_at < stop ? cut.length(b + 1) : 0;
 
         f32x4 o[DT] = {};
@@ -449,18 +474,14 @@ k_kv_attn(const KVPool p, const Attn a) {
 
         uint32_t base = first + wave * TILE;
         if (base < last) look(base);
+        // (columns past the tile's heads repeat its last: nothing reads what they give)
+        const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(hq + ((uint32_t)r < nh ? r : nh - 1)) * dim;
         bf16x8 q[KS];
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const uint32_t d = I8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 8 * (g + 4 * s);
-            u32x4 w = {0u, 0u, 0u, 0u};
-            if ((uint32_t)r < nh && d < dim) {
-                const uint16_t* src = a.q + b * a.q_stride + (size_t)(hq + r) * dim + d;
-                if (a.q_aligned) w = *reinterpret_cast<const u32x4*>(src);
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
-            }
+            u32x4 w = *reinterpret_cast<const bf16_load8*>(qh + (FULL || d < dim ? d : 0));
+            if (!FULL && d >= dim) w = u32x4{0u, 0u, 0u, 0u};
             q[s] = __builtin_bit_cast(bf16x8, w);
         }
 
@@ -672,7 +693,7 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
 
     if (blockIdx.x < joins) {
         const Division cut(a);
-        const Shares w(cut.find<false>(b), cut.per);
+        const Shares w(cut.find<false>(b), cut.by);
         if (w.n > 1)
             for (uint32_t j = 4 * blockIdx.x + wave; j < group; j += 4 * joins)
                 parts(j).join(w, b, j % 16, h * group + j, factors[wave]);
@@ -690,7 +711,7 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
     for (int j = 0; j < G; j++) v[j] = s[(size_t)((uint32_t)j < group ? j : 0) * a.logit_stride];
     if (ok) before = p.weights[row];
     const Division cut(a);
-    const Shares w(cut.find<false>(b), cut.per);
+    const Shares w(cut.find<false>(b), cut.by);
     for (uint32_t j0 = 0; j0 < group; j0 += 256) {
         const uint32_t nj = group - j0 < 256 ? group - j0 : 256;
         __syncthreads();
@@ -757,7 +778,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     const size_t logit_stride = accumulate ? steps * STEP : 0, logits = rows * q_heads * logit_stride * sizeof(float);
     const size_t whole = accumulate ? rows * q_heads * sizeof(float2) : 0;
     // (a grid has below 2^32 threads; offsets of the parts and counts of steps are of 32 bits)
-    if (blocks > 0xffffff || part > 0xffffffffu || steps * rows > 0x7fffffffu || steps >= 0x1000000) {
+    if (blocks > 0xffffff || part > 0xffffffffu || steps * rows > 0x7fff0000u || steps >= 0x1000000) {
         snx_set_error("kv_attention: %zu rows of up to %zu tokens are too many", rows, max_length);
         return -1;
     }
@@ -793,11 +814,11 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.heads = (uint32_t)heads;
     a.by_eights = divider(8 * tiles);
     a.by_heads = divider(c->kv_heads);
+    a.by_shares = divider(shares);
     a.shares = (uint32_t)shares;
     a.logit_stride = (uint32_t)logit_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.out_f32 = out_f32;
-    a.q_aligned = ((uintptr_t)q & 15u) == 0 && (rows < 2 || q_stride % 8 == 0);
     if (c->dtype == SNEPPX_INT8) launch<true>((unsigned)blocks, accumulate != 0, p, a, S(st));
     else launch<false>((unsigned)blocks, accumulate != 0, p, a, S(st));
     if (snx_launch_check("k_kv_attn")) return -1;
