@@ -151,38 +151,32 @@ __device__ __forceinline__ uint32_t rank_key(float w, int32_t pos, int32_t recen
 
 constexpr int kCutWaves = 16;
 constexpr int kCutThreads = 64 * kCutWaves;
-constexpr int kPasses = 4;               // digits of 9, 8, 8 and 7 bits: sign and exponent first
-constexpr int kShift[kPasses] = {23, 15, 7, 0}, kBins[kPasses] = {512, 256, 256, 256};
-constexpr uint32_t kSome = 4096;         // keys that share the first digit and are kept apart
+constexpr int kDigit = 11;               // digits of 11, 11 and 10 bits, from the top
+constexpr int kBins = 1 << kDigit;
+constexpr uint32_t kChunk = 4 * kCutThreads;         // slots of a long row that a workgroup has
+constexpr size_t kLong = 16384;          // longer rows are cut by several workgroups
 constexpr uint32_t kMoveAtOnce = 64;     // moves that the workgroup which finds them makes itself
 
-// two counts per wave -> their exclusive prefixes over the waves, and the totals
-__device__ __forceinline__ void wave_prefix(uint32_t& x, uint32_t& y, uint2* sh, uint2& total) {
-    const int w = threadIdx.x >> 6;
+// a count per wave -> its exclusive prefix over the waves, and the total
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x, uint32_t* sh, uint32_t& total) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[w] = make_uint2(x, y);
+    if (lane == 0) sh[w] = x;
     __syncthreads();
-    x = y = 0;
-    total = make_uint2(0, 0);
-#pragma unroll
-    for (int i = 0; i < kCutWaves; i++) {
-        const uint2 v = sh[i];
-        if (i < w) {
-            x += v.x;
-            y += v.y;
-        }
-        total.x += v.x;
-        total.y += v.y;
-    }
+    const uint32_t upto = lane_prefix(lane < kCutWaves ? sh[lane] : 0u);
+    total = __builtin_amdgcn_readlane(upto, kCutWaves - 1);
+    return __builtin_amdgcn_readlane(upto, w) - x;
 }
 
 // rows of the pool (k, v and the planes) of slots of[i] to those of slots
-// to[i], for `n` moves, by `threads` threads of which this is `me`
+// to[i], for `n` moves, by `threads` threads of which this is `me`, with U of a
+// thread's 16-byte loads in flight
+template <int U>
 __device__ __forceinline__ void move_rows(const KVPool& p, uint32_t b, uint32_t h, uint32_t row_bytes,
                                           const uint32_t* to, const uint32_t* of, uint32_t n, uint32_t me,
                                           uint32_t threads) {
     const uint32_t per = row_bytes / 16, chunks = n * per;
-    constexpr int U = 4;
+#pragma unroll 1
     for (uint32_t i0 = me; i0 < chunks; i0 += U * threads) {
         u32x4 x[U], y[U];
         uint32_t src[U], dst[U], c[U];
@@ -226,267 +220,454 @@ __device__ __forceinline__ void move_rows(const KVPool& p, uint32_t b, uint32_t 
     }
 }
 
+// What the workgroups of a long row find about it, one after the other
+struct Chunk {
+    uint32_t cands, low_cands;     // its keys with the first digit of the threshold; those below the budget
+    uint32_t sure, low_sure;       // its keys above them
+};
 struct Cut {
     const int32_t *lengths, *next_pos;
     int32_t* new_lengths;
-    uint32_t max_length, budget, recent, most, row_bytes;
+    uint32_t rows, max_length, budget, recent, most, row_bytes;
     uint32_t* counts;          // [rows * heads] moves of each row and head (unless moved at once)
     uint32_t* moves;           // [rows * heads][2][most] slots: targets, then sources
-    uint32_t* keys;            // [rows * heads][max_length] where they do not fit in LDS
+    uint32_t chunks;           // the rest of long rows, [rows * heads] of each
+    uint32_t* keys;            // [chunks][kChunk]
+    uint32_t* cands;           // [chunks][kChunk]: `cands` keys of each chunk, in the order of their slots
+    uint32_t* firsts;          // [chunks][kBins / 2]: the chunk's keys by first digit, 16 bits each
+    Chunk* found;              // [chunks]
+    uint32_t* absent;          // [chunks]: whether a page is not there
 };
 
-// One workgroup per (row, head): the budget-th largest key by its digits from
-// the top (each time a histogram of the keys that agree with the digits found
-// so far, read by every wave for itself), then the free slots below the budget
-// and the kept ones from it on, both in ascending order.  Each wave has
-// consecutive slots, so that order by (wave, step, lane) is order by slot.
-// KEYS: up to 4 of each thread in registers (16 x 8 of 2049 slots: 8.5 us, in LDS
-// 10.5), up to 32 in LDS, else in a workspace.  MOVE: with so few moves that the
-// workgroup makes them at once.
-enum { kRegisters, kLds, kWorkspace };
-template <int KEYS, bool MOVE>
-__global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
-    // most keys share a few exponents: with many, the first histogram is in copies
-    constexpr int kCopies = KEYS == kRegisters ? 1 : 4;
-    constexpr int kHist = kCopies * kBins[0] + kBins[1] + kBins[2] + kBins[3];
-    extern __shared__ uint32_t near_keys[];
-    __shared__ __attribute__((aligned(16))) uint32_t hist[kHist];
-    __shared__ uint32_t some[KEYS == kRegisters ? 1 : kSome], some_n;
-    __shared__ uint2 sh[kCutWaves];
-    __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
-    const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t L = kv_length(a.lengths, b, a.max_length), budget = a.budget;
-    const uint32_t steps = (L + 4 * kCutThreads - 1) / (4 * kCutThreads) * 4;       // slots of a thread, by fours
-    const uint32_t w0 = wave * steps * 64, t0 = w0 + lane;
-    uint32_t* const keys = KEYS == kLds ? near_keys : a.keys + (size_t)blockIdx.x * a.max_length;
-
-    for (int i = tid; i < kHist; i += kCutThreads) hist[i] = 0;
-    if (tid == 0) some_n = 0;
+// The keys of a lane's slots, every 64th from `t` on
+struct Ranks {
+    const KVPool& p;
+    const int32_t* table;
+    uint32_t L, t, page, slot, pages64, slots64, last_page, first_row, page_rows;
+    int32_t from;
     bool gone = false;
-    uint32_t own_keys[4];
-    if (L > budget) {
+    __device__ __forceinline__ Ranks(const KVPool& pool, const Cut& a, uint32_t b, uint32_t h, uint32_t len, uint32_t start)
+        : p(pool), table(pool.tables + (size_t)b * pool.width), L(len), t(start) {
         const int64_t from64 = (int64_t)a.next_pos[b] - (int64_t)a.recent;
-        const int32_t from = (int32_t)(from64 < INT32_MIN ? INT32_MIN : from64);
-        // G slots at once (past the length: its last one), so that their look-ups
-        // and loads are in flight together; key 0 past the length
-        constexpr int G = KEYS == kRegisters ? 4 : 8;
-        for (uint32_t i0 = 0; i0 < (KEYS == kRegisters ? 4 : steps); i0 += G) {
-            uint32_t rows[G];
-            float w[G];
-            int32_t pos[G];
+        from = (int32_t)(from64 < INT32_MIN ? INT32_MIN : from64);
+        pages64 = p.page_of(64);
+        slots64 = 64 - pages64 * p.page_size;
+        last_page = p.page_of(L - 1);
+        first_row = h * p.page_size;
+        page_rows = p.heads * p.page_size;
+        page = p.page_of(t);
+        slot = t - page * p.page_size;
+    }
+    // G at once (past the length: of its last page), so that their look-ups and
+    // loads are in flight together; 0 past the length
+    template <int G>
+    __device__ __forceinline__ void next(uint32_t (&q)[G]) {
+        uint32_t rows[G];
+        float w[G];
+        int32_t pos[G];
 #pragma unroll
-            for (int i = 0; i < G; i++) {
-                const uint32_t t = t0 + 64 * (i0 + i);
-                const bool there = p.row(b, h, t < L ? t : L - 1, rows[i]);
-                gone |= !there;
-                if (!there) rows[i] = 0;
-            }
-#pragma unroll
-            for (int i = 0; i < G; i++) {
-                w[i] = p.weights[rows[i]];
-                pos[i] = p.positions[rows[i]];
-            }
-#pragma unroll
-            for (int i = 0; i < G; i++) {
-                const uint32_t t = t0 + 64 * (i0 + i), q = t < L ? rank_key(w[i], pos[i], from) : 0u;
-                if (KEYS == kRegisters) own_keys[i & 3] = q;
-                else if (i0 + i < steps && (KEYS == kLds || t < L)) keys[t] = q;
+        for (int i = 0; i < G; i++) {
+            const uint32_t e = (uint32_t)table[page < last_page ? page : last_page];
+            const bool there = e < p.pages;
+            gone |= !there;
+            rows[i] = there ? e * page_rows + first_row + slot : 0;
+            page += pages64;
+            slot += slots64;
+            if (slot >= p.page_size) {
+                slot -= p.page_size;
+                page++;
             }
         }
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            w[i] = p.weights[rows[i]];
+            pos[i] = p.positions[rows[i]];
+        }
+#pragma unroll
+        for (int i = 0; i < G; i++, t += 64) q[i] = t < L ? rank_key(w[i], pos[i], from) : 0u;
     }
+};
+
+__device__ __forceinline__ uint32_t lane_rank(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// The budget-th largest key by its digits from the top: each time a histogram of
+// the keys that agree with the digits found so far.
+struct Threshold {
+    uint32_t prefix = 0, known = 0;      // the digits found so far, their bits
+    uint32_t want, tied = 0;             // it is the want-th largest of the `tied` keys that share them
+    int shift = 32 - kDigit;             // of the next digit (the last has a known bit in it, alike in all)
+    __device__ __forceinline__ explicit Threshold(uint32_t budget) : want(budget) {}
+
+    // counts U keys of each lane
+    template <int U>
+    __device__ __forceinline__ void tally(uint32_t* hist, const uint32_t (&q)[U], const bool (&there)[U]) const {
+        bool mine[U], other = false;
+        uint32_t digit[U], n = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            mine[u] = there[u] && ((q[u] ^ prefix) & known) == 0;
+            digit[u] = (q[u] >> shift) & (kBins - 1);
+        }
+        // many alike (zeros, recent ones) are counted at once
+        const uint32_t first = __builtin_amdgcn_readfirstlane(digit[0]);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            other |= mine[u] && digit[u] != first;
+            n += __popcll(__ballot(mine[u]));
+        }
+        if (__ballot(other) == 0) {
+            if ((threadIdx.x & 63) == 0 && n) atomicAdd(&hist[first], n);
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (mine[u]) atomicAdd(&hist[digit[u]], 1u);
+    }
+    // The digit, by all threads: from the top the wave's 128 bins (the first wave has the
+    // highest) where the number passes `want`, then, in every wave, the bin of them.
+    __device__ __forceinline__ void find(const uint32_t* hist, uint32_t* sh) {
+        const int tid = threadIdx.x, lane = tid & 63;
+        const u32x2* const pairs = reinterpret_cast<const u32x2*>(hist) + kBins / 2 - 1;
+        const u32x2 mine = *(pairs - tid);
+        const uint32_t here = last_lane(lane_prefix(mine[0] + mine[1]));
+        if (lane == 0) sh[tid >> 6] = here;
+        __syncthreads();
+        const uint32_t n = lane < kCutWaves ? sh[lane] : 0u, upto = lane_prefix(n);
+        const int w = __builtin_ctzll(__ballot(upto >= want));
+        const uint32_t before = __builtin_amdgcn_readlane(upto - n, w);
+        const u32x2 pair = *(pairs - (64 * w + lane));
+        const uint32_t upto2 = before + lane_prefix(pair[0] + pair[1]), upto1 = upto2 - pair[0];
+        const int at = __builtin_ctzll(__ballot(upto2 >= want));
+        const uint32_t high = __builtin_amdgcn_readlane(upto1, at);       // with the pair's higher bin
+        const uint32_t n0 = __builtin_amdgcn_readlane(pair[0], at), n1 = __builtin_amdgcn_readlane(pair[1], at);
+        const bool lower = want > high;
+        tied = lower ? n0 : n1;
+        want -= lower ? high : high - n1;
+        prefix |= (uint32_t)(kBins - 1 - 2 * (64 * w + at) - lower) << shift;
+        known = ~0u << shift;
+        shift = shift > kDigit ? shift - kDigit : 0;
+    }
+    __device__ __forceinline__ bool done() const { return want == tied || known == ~0u; }
+    // Above the prefix all stay, of those equal to it the first `want` in the order of
+    // the slots: where all of them do, whatever their other digits are, the prefix
+    // goes below them (it is not 0: some key is left out).
+    __device__ __forceinline__ void settle() {
+        if (want != tied) return;
+        prefix -= 1;
+        want = 0;
+    }
+};
+
+// Lists the free slots below the budget and those from it on that stay, both in
+// ascending order, of `steps` x 1024 slots from `slot0` on whose keys are in LDS;
+// so many ties, free slots and ones to move come before.  Each wave has consecutive
+// slots, so that order by (wave, step, lane) is order by slot.  (Slots past the
+// length have the lowest key and come after all others.)
+__device__ __forceinline__ uint32_t list_slots(const uint32_t* keys, uint32_t slot0, uint32_t steps, uint32_t budget,
+                                               const Threshold& at, uint32_t ties, uint32_t holes0, uint32_t fars0,
+                                               uint32_t* sh, uint32_t* to, uint32_t* of) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t mine = wave * steps * 64, w0 = slot0 + mine;
+    const uint32_t* const q = keys + mine + lane;
+    uint32_t total, n = 0;
+    if (at.want) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < steps; i++) n += __popcll(__ballot(q[64 * i] == at.prefix));
+        ties += wave_prefix(n, sh, total);
+    }
+    // lane i has step i: the free slots, those that stay, and the numbers of both before
+    // them (the latter in the upper half)
+    uint32_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < steps; i++) {
+        uint64_t s = __ballot(q[64 * i] > at.prefix);
+        if (at.want) {
+            const uint64_t tb = __ballot(q[64 * i] == at.prefix);
+            s |= __ballot((__builtin_amdgcn_inverse_ballot_w64(tb)) && ties + lane_rank(tb) < at.want);
+            ties += __popcll(tb);
+        }
+        lo = lane == i ? (uint32_t)s : lo;
+        hi = lane == i ? (uint32_t)(s >> 32) : hi;
+    }
+    const uint64_t s = (uint64_t)hi << 32 | lo;
+    const uint32_t first = w0 + 64 * lane;
+    const uint64_t part = ((uint64_t)1 << ((budget - first) & 63)) - 1;
+    const uint64_t low = lane >= steps || first >= budget ? 0 : budget - first >= 64 ? ~0ull : part;
+    const uint64_t hole = low & ~s, far = s & ~low;
+    const uint32_t own = __popcll(hole) | __popcll(far) << 16, upto = lane_prefix(own), before = upto - own;
+    const uint32_t both = __builtin_amdgcn_readlane(upto, 63);
+    const uint32_t fars = fars0 + wave_prefix(both >> 16, sh, total) + (before >> 16);
+    const uint32_t holes = holes0 + wave_prefix(both & 0xFFFF, sh, total) + (before & 0xFFFF);
+#pragma unroll 1
+    for (uint32_t i = 0; i < steps; i++) {
+        auto write = [&](uint64_t mine, uint32_t first, uint32_t* to) {
+            const uint64_t m = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(mine >> 32), i) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane((uint32_t)mine, i);
+            const uint32_t at = __builtin_amdgcn_readlane(first, i) + lane_rank(m);
+            if (__builtin_amdgcn_inverse_ballot_w64(m)) to[at] = w0 + 64 * i + lane;
+        };
+        // a step lies below the budget, or from it on, or has it within
+        if (w0 + 64 * i < budget) write(hole, holes, to);
+        if (w0 + 64 * i + 64 > budget) write(far, fars, of);
+    }
+    return total;
+}
+
+// One workgroup per (row, head) of up to kLong slots.  A call runs through the code
+// about once, and fetching that is much of its time (16 x 8 of 2049: 8.4 us; unrolled and
+// specialised, with keys in registers, twice the code, 8.5): the
+// loops are left rolled.
+// MOVE: with so few moves that the workgroup makes them at once.
+template <bool MOVE>
+__global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
+    extern __shared__ uint32_t keys[];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
+    __shared__ uint32_t sh[kCutWaves];
+    __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
+    const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
+    const int tid = threadIdx.x;
+    const uint32_t L = kv_length(a.lengths, b, a.max_length), budget = a.budget;
+    const uint32_t steps = (L + kCutThreads - 1) / kCutThreads;       // slots of a thread
+    const uint32_t t0 = (tid & ~63) * steps + (tid & 63);
+    u32x2* const bins = reinterpret_cast<u32x2*>(hist) + tid;
+
+    bool gone = false;
+    if (L > budget) {
+        Ranks ranks(p, a, b, h, L, t0);
+#pragma unroll 1
+        for (uint32_t i = 0; i < steps; i += 4) {
+            uint32_t q[4];
+            ranks.next<4>(q);
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++)
+                if (i + u < steps) keys[t0 + 64 * (i + u)] = q[u];
+        }
+        gone = ranks.gone;
+    }
+    *bins = u32x2{0u, 0u};
     gone = __syncthreads_or(gone);
     if (tid == 0 && h == 0 && a.new_lengths) a.new_lengths[b] = (int32_t)(L > budget && !gone ? budget : L);
     if (L <= budget || gone) {
         if (!MOVE && tid == 0) a.counts[blockIdx.x] = 0;
         return;
     }
-    // Slots past the length have the lowest key and come after all others: no
-    // test keeps them out below.  (Keys are read by the thread that wrote them.)
-    auto each_of = [&](uint32_t i0, uint32_t end, auto f) {
-        for (uint32_t i = i0; i < (KEYS == kRegisters ? 4 : end); i += 4) {
-            uint32_t q[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const uint32_t t = t0 + 64 * (i + u);
-                q[u] = KEYS == kRegisters ? own_keys[u] : KEYS == kLds || t < L ? keys[t] : 0u;
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++) f(i + u, q[u]);
-        }
-    };
-    auto each = [&](auto f) { each_of(0, steps, f); };
-
-    auto lane_rank = [&](uint64_t m) {
-        return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-    };
-
-    uint32_t prefix = 0, want = budget, tied = 0;    // the want-th largest of the `tied` keys that share the prefix
-    bool few = false;                                // these are in `some`
-    uint32_t* hp = hist;
-#pragma unroll
-    for (int pass = 0; pass < kPasses; pass++) {
-        if (want == tied) break;                     // all of them stay, whatever their other digits are
-        const int shift = kShift[pass], bins = kBins[pass], width = pass == 0 ? 9 : pass == 3 ? 7 : 8;
-        const uint32_t digits = (1u << width) - 1u, above_shift = (shift + width) & 31;
-        // One pass over all keys puts those that are left aside, if there is room
-        // (16 of 30001 slots: 39 -> 31 us).
-        if (KEYS != kRegisters && pass == 1 && tied <= kSome) {
-            few = true;
-            uint32_t own = 0;
-            each([&](uint32_t, uint32_t q) { own += __popcll(__ballot(q >> above_shift == prefix >> above_shift)); });
-            uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(&some_n, own);
-            at = __builtin_amdgcn_readfirstlane(at);
-            each([&](uint32_t, uint32_t q) {
-                const uint64_t who = __ballot(q >> above_shift == prefix >> above_shift);
-                if (who >> lane & 1) some[at + lane_rank(who)] = q;
-                at += __popcll(who);
-            });
-            __syncthreads();
-        }
-        if (few) {
-            for (uint32_t i = tid; i < kSome && i < some_n; i += kCutThreads) {
-                const uint32_t q = some[i];
-                if (q >> above_shift == prefix >> above_shift) atomicAdd(&hp[(q >> shift) & digits], 1u);
-            }
-        } else {
-            each([&](uint32_t, uint32_t q) {
-                const uint32_t digit = (q >> shift) & digits;
-                const uint32_t to = pass == 0 ? digit * kCopies + lane % kCopies : digit;
-                const uint64_t who = pass == 0 ? ~0ull : __ballot(q >> above_shift == prefix >> above_shift);
-                if (who == 0) return;
-                // many alike (zeros, recent ones) are counted at once
-                if (who == ~0ull && __ballot(digit != (uint32_t)__builtin_amdgcn_readfirstlane(digit)) == 0) {
-                    if (lane == 0) atomicAdd(&hp[to], 64u);
-                } else if (who >> lane & 1) {
-                    atomicAdd(&hp[to], 1u);
-                }
-            });
-        }
+    Threshold at(budget);
+#pragma unroll 1
+    for (;;) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < steps; i++) at.tally<1>(hist, {keys[t0 + 64 * i]}, {t0 + 64 * i < L});
         __syncthreads();
-        // from the top: lane i has the i-th bins / 64 of them, the last the highest
-        constexpr int most = 8;
-        uint32_t n[most];
-        const int per = bins / 64;
-        uint32_t sum = 0;
-        if (pass == 0 && kCopies == 4) {             // a bin's copies at once
-#pragma unroll
-            for (int j = 0; j < per; j++) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(hp + 4 * (bins - per * (lane + 1) + j));
-                n[j] = v[0] + v[1] + v[2] + v[3];
-                sum += n[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < per; j += 4) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(hp + bins - per * (lane + 1) + j);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    n[j + e] = v[e];
-                    sum += v[e];
-                }
-            }
-        }
-        const uint32_t upto = lane_prefix(sum);
-        uint32_t above = upto - sum, digit = 0, count = 0, rest = 0;
-        const uint64_t mine = __ballot(above < want && want <= upto);
-#pragma unroll
-        for (int j = per - 1; j >= 0; j--) {
-            if (above < want && want <= above + n[j]) {
-                digit = bins - per * (lane + 1) + j;
-                rest = want - above;
-                count = n[j];
-            }
-            above += n[j];
-        }
-        const int at = __builtin_ctzll(mine);
-        prefix |= (uint32_t)__builtin_amdgcn_readlane(digit, at) << shift;
-        want = __builtin_amdgcn_readlane(rest, at);
-        tied = __builtin_amdgcn_readlane(count, at);
-        hp += pass == 0 ? kCopies * bins : bins;
+        at.find(hist, sh);
+        if (at.done()) break;
+        __syncthreads();
+        *bins = u32x2{0u, 0u};
+        __syncthreads();
     }
-
-    // of the keys equal to the threshold the first `want` stay
-    uint2 total;
-    uint32_t ties = 0, none = 0;
-    if (want < tied) {
-        each([&](uint32_t, uint32_t q) { ties += __popcll(__ballot(q == prefix)); });
-        wave_prefix(ties, none, sh, total);
-    }
-    uint32_t seen = ties;
-    // lanes whose slot stays
-    const bool ranked = want < tied;
-    auto stay = [&](uint32_t q) -> uint64_t {
-        if (!ranked) return __ballot(q >= prefix);
-        const uint64_t tb = __ballot(q == prefix);
-        const uint64_t s = __ballot(q > prefix || (q == prefix && seen + lane_rank(tb) < want));
-        seen += __popcll(tb);
-        return s;
-    };
-    // Up to 64 steps from i0 at once, lane i with step i0 + i: the slots below the
-    // budget that are left free, those from it on that stay, and the numbers of
-    // both before them in the block (the latter in the upper half).
-    auto block = [&](uint32_t i0, uint64_t& hole, uint64_t& far) {
-        uint32_t lo = 0, hi = 0;
-        each_of(i0, i0 + 64 < steps ? i0 + 64 : steps, [&](uint32_t i, uint32_t q) {
-            const uint64_t s = stay(q);
-            const bool me = (uint32_t)lane == i - i0;
-            lo = me ? (uint32_t)s : lo;
-            hi = me ? (uint32_t)(s >> 32) : hi;
-        });
-        const uint64_t s = (uint64_t)hi << 32 | lo;
-        const uint32_t at = w0 + 64 * (i0 + lane);
-        const uint64_t part = ((uint64_t)1 << ((budget - at) & 63)) - 1;
-        const uint64_t low = i0 + lane >= steps || at >= budget ? 0 : budget - at >= 64 ? ~0ull : part;
-        hole = low & ~s;
-        far = s & ~low;
-    };
-    uint32_t holes = 0, fars = 0;
-    uint64_t hole, far;
-    for (uint32_t i0 = 0; i0 < steps; i0 += 64) {
-        block(i0, hole, far);
-        const uint32_t sum = __builtin_amdgcn_readlane(lane_prefix(__popcll(hole) | __popcll(far) << 16), 63);
-        holes += sum & 0xFFFF;
-        fars += sum >> 16;
-    }
-    wave_prefix(holes, fars, sh, total);
-    seen = ties;
+    at.settle();
     uint32_t* const to = MOVE ? list : a.moves + (size_t)blockIdx.x * 2 * a.most;
     uint32_t* const of = to + (MOVE ? kMoveAtOnce : a.most);
-    for (uint32_t i0 = 0; i0 < steps; i0 += 64) {
-        if (KEYS == kWorkspace && steps > 64) block(i0, hole, far);      // (else it is the one above)
-        const uint32_t own = __popcll(hole) | __popcll(far) << 16, upto = lane_prefix(own), before = upto - own;
-        const uint32_t end = i0 + 64 < steps ? 64 : steps - i0;
-        for (uint32_t i = 0; i < end; i++) {
-            const uint32_t t = t0 + 64 * (i0 + i), before_i = __builtin_amdgcn_readlane(before, i);
-            auto write = [&](uint64_t mine, uint32_t* to, uint32_t at) {
-                const uint64_t m = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(mine >> 32), i) << 32 |
-                                   (uint32_t)__builtin_amdgcn_readlane((uint32_t)mine, i);
-                if (m >> lane & 1) to[at + lane_rank(m)] = t;
-            };
-            // a step lies below the budget, or from it on, or has it within
-            if (w0 + 64 * (i0 + i) < budget) write(hole, to, holes + (before_i & 0xFFFF));
-            if (w0 + 64 * (i0 + i) + 64 > budget) write(far, of, fars + (before_i >> 16));
-        }
-        const uint32_t sum = __builtin_amdgcn_readlane(upto, 63);
-        holes += sum & 0xFFFF;
-        fars += sum >> 16;
-    }
+    const uint32_t total = list_slots(keys, 0, steps, budget, at, 0, 0, 0, sh, to, of);
     if (MOVE) {
         __syncthreads();
-        move_rows(p, b, h, a.row_bytes, to, of, total.x, tid, kCutThreads);
+        move_rows<1>(p, b, h, a.row_bytes, to, of, total, tid, kCutThreads);
     } else if (tid == 0) {
-        a.counts[blockIdx.x] = total.x;
+        a.counts[blockIdx.x] = total;
     }
 }
 
-// The moves that k_kv_cut listed.  Sources lie in slots from the budget on and
+// ------------------------------------------------------------- of long rows
+// A workgroup has kChunk slots, in three kernels: k_kv_rank counts their keys by
+// first digit; with all chunks' counts k_kv_part finds the threshold's and puts
+// the keys that share it apart; k_kv_list finds the threshold among these, and
+// where its own slots stand in the lists.  (us of a call that cuts so, and with one
+// workgroup for each row and head: 2 rows of 30001 and 8 heads 32 and 41, 4 of 60000
+// 70 and 113; 1 of 16384 30 and 30, of 12288 29 and 26, of 8192 27 and 21, and one
+// token too many in 8 of 16384 29 and 22.)
+__device__ __forceinline__ bool long_row(const KVPool& p, const Cut& a, uint32_t& bh, uint32_t& b, uint32_t& h, uint32_t& L) {
+    bh = blockIdx.y + blockIdx.z * 65535u;
+    b = bh / p.heads;
+    h = bh - b * p.heads;
+    if (b >= a.rows) return false;
+    L = kv_length(a.lengths, b, a.max_length);
+    return L > a.budget && blockIdx.x * kChunk < L;
+}
+// a page of the row that is not there
+__device__ __forceinline__ bool row_absent(const Cut& a, uint32_t bh, uint32_t chunks) {
+    bool gone = false;
+    for (uint32_t c = threadIdx.x; c < chunks; c += kCutThreads) gone |= a.absent[(size_t)bh * a.chunks + c] != 0;
+    return __syncthreads_or(gone);
+}
+
+__global__ void __launch_bounds__(kCutThreads) k_kv_rank(const KVPool p, const Cut a) {
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
+    const int tid = threadIdx.x;
+    uint32_t bh, b, h, L;
+    if (!long_row(p, a, bh, b, h, L)) return;
+    reinterpret_cast<u32x2*>(hist)[tid] = u32x2{0u, 0u};
+    __syncthreads();
+    const size_t chunk = (size_t)bh * a.chunks + blockIdx.x;
+    const uint32_t mine = (tid & ~63) * 4 + (tid & 63), t0 = blockIdx.x * kChunk + mine;
+    Ranks ranks(p, a, b, h, L, t0);
+    uint32_t q[4];
+    ranks.next<4>(q);
+    const bool there[4] = {t0 < L, t0 + 64 < L, t0 + 128 < L, t0 + 192 < L};
+#pragma unroll
+    for (int u = 0; u < 4; u++) a.keys[chunk * kChunk + mine + 64 * u] = q[u];
+    Threshold(0).tally<4>(hist, q, there);
+    const bool gone = __syncthreads_or(ranks.gone);
+    const u32x2 n = reinterpret_cast<const u32x2*>(hist)[tid];
+    a.firsts[chunk * (kBins / 2) + tid] = n[0] | n[1] << 16;
+    if (tid == 0) a.absent[chunk] = gone;
+}
+
+// the threshold's first digit, from the chunks' counts
+__device__ __forceinline__ Threshold first_digit(const Cut& a, uint32_t bh, uint32_t chunks, uint32_t* hist, uint32_t* sh) {
+    u32x2 bins = {0u, 0u};
+    const uint32_t* const firsts = a.firsts + (size_t)bh * a.chunks * (kBins / 2) + threadIdx.x;
+#pragma unroll 8
+    for (uint32_t c = 0; c < chunks; c++) {
+        const uint32_t n = firsts[(size_t)c * (kBins / 2)];
+        bins += u32x2{n & 0xFFFF, n >> 16};
+    }
+    reinterpret_cast<u32x2*>(hist)[threadIdx.x] = bins;
+    __syncthreads();
+    Threshold at(a.budget);
+    at.find(hist, sh);
+    return at;
+}
+
+__global__ void __launch_bounds__(kCutThreads) k_kv_part(const KVPool p, const Cut a) {
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
+    __shared__ uint32_t sh[kCutWaves];
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    uint32_t bh, b, h, L, q[4];
+    if (!long_row(p, a, bh, b, h, L)) return;
+    const uint32_t chunks = (L + kChunk - 1) / kChunk;
+    const size_t chunk = (size_t)bh * a.chunks + blockIdx.x;
+    const uint32_t mine = (tid & ~63u) * 4 + lane, t0 = blockIdx.x * kChunk + mine;
+#pragma unroll
+    for (int u = 0; u < 4; u++) q[u] = a.keys[chunk * kChunk + mine + 64 * u];
+    if (row_absent(a, bh, chunks)) return;
+    const Threshold at = first_digit(a, bh, chunks, hist, sh);
+
+    uint64_t who[4];
+    uint32_t cands = 0, low_cands = 0, sure = 0, low_sure = 0, total, low_total;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const bool there = t0 + 64 * u < L, low = t0 + 64 * u < a.budget;
+        who[u] = __ballot(there && (q[u] & at.known) == at.prefix);
+        const uint64_t above = __ballot(there && (q[u] & at.known) > at.prefix), below = __ballot(low);
+        cands += __popcll(who[u]);
+        low_cands += __popcll(who[u] & below);
+        sure += __popcll(above);
+        low_sure += __popcll(above & below);
+    }
+    uint32_t to = wave_prefix(cands | low_cands << 16, sh, total) & 0xFFFF;
+    (void)wave_prefix(sure | low_sure << 16, sh, low_total);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        if (__builtin_amdgcn_inverse_ballot_w64(who[u])) a.cands[chunk * kChunk + to + lane_rank(who[u])] = q[u];
+        to += __popcll(who[u]);
+    }
+    if (tid == 0) a.found[chunk] = Chunk{total & 0xFFFF, total >> 16, low_total & 0xFFFF, low_total >> 16};
+}
+
+__global__ void __launch_bounds__(kCutThreads) k_kv_list(const KVPool p, const Cut a) {
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kBins], keys[kChunk];
+    __shared__ uint32_t sh[kCutWaves], sums[4][kCutWaves];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t bh, b, h, L;
+    const bool cut = long_row(p, a, bh, b, h, L);
+    if (b >= a.rows) return;
+    const uint32_t chunks = (L + kChunk - 1) / kChunk, chunk = blockIdx.x;
+    const size_t row = (size_t)bh * a.chunks;
+    if (cut)
+        for (uint32_t i = tid; i < kChunk / 4; i += kCutThreads)
+            reinterpret_cast<u32x4*>(keys)[i] = reinterpret_cast<const u32x4*>(a.keys + (row + chunk) * kChunk)[i];
+    const bool gone = L > a.budget && row_absent(a, bh, chunks);
+    if (chunk == 0 && tid == 0 && h == 0 && a.new_lengths) a.new_lengths[b] = (int32_t)(L > a.budget && !gone ? a.budget : L);
+    if (!cut || gone) {
+        if (chunk == 0 && tid == 0) a.counts[bh] = 0;
+        return;
+    }
+    Threshold at = first_digit(a, bh, chunks, hist, sh);
+    // each wave has every 16th chunk's, four of a lane at once
+    auto each = [&](auto f) {
+#pragma unroll 1
+        for (uint32_t c = wave; c < chunks; c += kCutWaves) {
+            const uint32_t n = a.found[row + c].cands;
+            const uint32_t* const cands = a.cands + (row + c) * kChunk;
+#pragma unroll 1
+            for (uint32_t i = lane; i < n + lane; i += 256) {
+                uint32_t q[4];
+                bool there[4];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; u++) {
+                    there[u] = i + 64 * u < n;
+                    q[u] = cands[there[u] ? i + 64 * u : 0];
+                }
+                f(c, i, q, there);
+            }
+        }
+    };
+#pragma unroll 1
+    while (!at.done()) {
+        __syncthreads();
+        reinterpret_cast<u32x2*>(hist)[tid] = u32x2{0u, 0u};
+        __syncthreads();
+        each([&](uint32_t, uint32_t, uint32_t (&q)[4], bool (&there)[4]) { at.tally<4>(hist, q, there); });
+        __syncthreads();
+        at.find(hist, sh);
+    }
+    at.settle();
+    // of the slots before this chunk and of those below the budget: how many keys are
+    // above the threshold, how many equal to it
+    uint32_t more = 0, ties = 0, low_more = 0, low_ties = 0;
+    for (uint32_t c = tid; c < chunks; c += kCutThreads) {
+        const Chunk f = a.found[row + c];
+        more += c < chunk ? f.sure : 0;
+        low_more += f.low_sure;
+    }
+    each([&](uint32_t c, uint32_t i, uint32_t (&q)[4], bool (&there)[4]) {
+        const uint32_t low = a.found[row + c].low_cands;
+#pragma unroll
+        for (uint32_t u = 0; u < 4; u++) {
+            const bool above = there[u] && q[u] > at.prefix, tie = there[u] && q[u] == at.prefix, is_low = i + 64 * u < low;
+            more += c < chunk && above;
+            ties += c < chunk && tie;
+            low_more += is_low && above;
+            low_ties += is_low && tie;
+        }
+    });
+    auto sum = [&](uint32_t x, int k) {
+        x = last_lane(lane_prefix(x));
+        if (lane == 0) sums[k][wave] = x;
+    };
+    sum(more, 0);
+    sum(ties, 1);
+    sum(low_more, 2);
+    sum(low_ties, 3);
+    __syncthreads();
+    auto all = [&](int k) { return last_lane(lane_prefix(lane < kCutWaves ? sums[k][lane] : 0u)); };
+    ties = all(1);
+    low_ties = all(3);
+    const uint32_t kept = all(0) + (ties < at.want ? ties : at.want);                      // before this chunk
+    const uint32_t low_kept = all(2) + (low_ties < at.want ? low_ties : at.want);          // below the budget
+    const uint32_t slot0 = chunk * kChunk;
+    uint32_t* const to = a.moves + (size_t)bh * 2 * a.most;
+    (void)list_slots(keys, slot0, kChunk / kCutThreads, a.budget, at, ties, slot0 < a.budget ? slot0 - kept : 0,
+                     slot0 > a.budget ? kept - low_kept : 0, sh, to, to + a.most);
+    if (chunk == 0 && tid == 0) a.counts[bh] = a.budget - low_kept;
+}
+
+// The moves that k_kv_cut or k_kv_list listed.  Sources lie in slots from the budget on and
 // targets below it, so all are independent.
 __global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a, uint32_t first) {
     const uint32_t bh = first + blockIdx.y, b = bh / p.heads, n = a.counts[bh];
     const uint32_t* to = a.moves + (size_t)bh * 2 * a.most;
-    move_rows(p, b, bh - b * p.heads, a.row_bytes, to, to + a.most, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    move_rows<4>(p, b, bh - b * p.heads, a.row_bytes, to, to + a.most, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 template <int LR>
@@ -495,22 +676,17 @@ void append(bool i8, unsigned blocks, const KVPool& p, const NewRows& n, hipStre
     else k_kv_append<false, LR><<<blocks, 256, 0, s>>>(p, n);
 }
 
-template <int KEYS, bool MOVE>
+template <bool MOVE>
 int cut(unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
-    constexpr uint32_t four = 4 * kCutThreads;
-    const int bytes = KEYS == kLds ? (int)((a.max_length + four - 1) / four * four * sizeof(uint32_t)) : 0;
+    // (rows that nothing is cut from need no keys)
+    const size_t keys = a.most ? ((size_t)a.max_length + kCutThreads - 1) / kCutThreads * kCutThreads : 0;
     static std::atomic<uint64_t> done{0};
-    const void* fn = reinterpret_cast<const void*>(&k_kv_cut<KEYS, MOVE>);
-    if (bytes && lds_optin(fn, 8 * four * sizeof(uint32_t), done) != hipSuccess) {
-        snx_set_error("kv_evict: cannot reserve %d bytes of LDS", bytes);
+    if (lds_optin(reinterpret_cast<const void*>(&k_kv_cut<MOVE>), (int)(kLong * sizeof(uint32_t)), done) != hipSuccess) {
+        snx_set_error("kv_evict: cannot reserve %zu bytes of LDS", kLong * sizeof(uint32_t));
         return -1;
     }
-    k_kv_cut<KEYS, MOVE><<<blocks, kCutThreads, bytes, s>>>(p, a);
+    k_kv_cut<MOVE><<<blocks, kCutThreads, keys * sizeof(uint32_t), s>>>(p, a);
     return snx_launch_check("k_kv_cut");
-}
-template <int KEYS>
-int cut(bool at_once, unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
-    return at_once ? cut<KEYS, true>(blocks, p, a, s) : cut<KEYS, false>(blocks, p, a, s);
 }
 
 uint32_t most_moves(size_t max_length, size_t budget) {
@@ -555,13 +731,14 @@ int snx_k_kv_append(const SNEPPXKVCache* c, const uint16_t* k, size_t k_stride, 
     return snx_launch_check("k_kv_append");
 }
 
-// keys that do not fit in the LDS of a workgroup
-static bool keys_far(size_t max_length) { return max_length > 32 * (size_t)kCutThreads; }
+static bool is_long(size_t max_length, size_t most) { return most && max_length > kLong; }
+static size_t chunks_of(size_t max_length) { return (max_length + kChunk - 1) / kChunk; }
 
 size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, size_t budget) {
-    const size_t most = most_moves(max_length, budget), bh = rows * c->kv_heads;
-    return bh * sizeof(uint32_t) *
-           ((most > kMoveAtOnce ? 1 + 2 * most : 0) + (keys_far(max_length) && most ? max_length : 0));
+    const size_t most = most_moves(max_length, budget), bh = rows * c->kv_heads, chunks = chunks_of(max_length);
+    if (is_long(max_length, most))
+        return bh * (chunks * ((2 * kChunk + kBins / 2 + 1) * sizeof(uint32_t) + sizeof(Chunk)) + (1 + 2 * most) * sizeof(uint32_t));
+    return most > kMoveAtOnce ? bh * (1 + 2 * most) * sizeof(uint32_t) : 0;
 }
 
 int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, const int32_t* lengths,
@@ -578,19 +755,35 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
     a.recent = (uint32_t)(recent < INT32_MAX ? recent : INT32_MAX);
     a.most = most_moves(max_length, budget);
     a.row_bytes = (uint32_t)(c->head_dim * (c->dtype == SNEPPX_INT8 ? 1 : 2));
-    const bool at_once = a.most <= kMoveAtOnce;
-    a.counts = static_cast<uint32_t*>(ws);
-    a.moves = a.counts + bh;
-    a.keys = at_once ? a.counts : a.moves + bh * 2 * a.most;
-    const int rc = !a.most || max_length <= 4 * (size_t)kCutThreads ? cut<kRegisters>(at_once, (unsigned)bh, p, a, S(st))
-                   : !keys_far(max_length)                          ? cut<kLds>(at_once, (unsigned)bh, p, a, S(st))
-                                                                    : cut<kWorkspace>(at_once, (unsigned)bh, p, a, S(st));
-    if (rc) return -1;
-    if (at_once) return 0;
+    a.rows = (uint32_t)rows;
+    a.chunks = (uint32_t)chunks_of(max_length);
+    const hipStream_t s = S(st);
+    if (is_long(max_length, a.most)) {
+        const size_t all = bh * a.chunks;
+        a.found = static_cast<Chunk*>(ws);
+        a.keys = reinterpret_cast<uint32_t*>(a.found + all);
+        a.cands = a.keys + all * kChunk;
+        a.firsts = a.cands + all * kChunk;
+        a.absent = a.firsts + all * (kBins / 2);
+        a.counts = a.absent + all;
+        a.moves = a.counts + bh;
+        const dim3 grid(a.chunks, (unsigned)(bh < 65535 ? bh : 65535), (unsigned)((bh + 65534) / 65535));
+        k_kv_rank<<<grid, kCutThreads, 0, s>>>(p, a);
+        if (snx_launch_check("k_kv_rank")) return -1;
+        k_kv_part<<<grid, kCutThreads, 0, s>>>(p, a);
+        if (snx_launch_check("k_kv_part")) return -1;
+        k_kv_list<<<grid, kCutThreads, 0, s>>>(p, a);
+        if (snx_launch_check("k_kv_list")) return -1;
+    } else {
+        a.counts = static_cast<uint32_t*>(ws);
+        a.moves = a.counts + bh;
+        if (a.most <= kMoveAtOnce) return cut<true>((unsigned)bh, p, a, s);
+        if (cut<false>((unsigned)bh, p, a, s)) return -1;
+    }
     const size_t chunks = (size_t)a.most * (a.row_bytes / 16), gx = (chunks + 1023) / 1024;
     for (size_t at = 0; at < bh; at += 65535) {
         const size_t n = bh - at < 65535 ? bh - at : 65535;
-        k_kv_move<<<dim3((unsigned)(gx < 65536 ? gx : 65536), (unsigned)n), 256, 0, S(st)>>>(p, a, (uint32_t)at);
+        k_kv_move<<<dim3((unsigned)(gx < 65536 ? gx : 65536), (unsigned)n), 256, 0, s>>>(p, a, (uint32_t)at);
         if (snx_launch_check("k_kv_move")) return -1;
     }
     return 0;

@@ -231,6 +231,25 @@ def test_evict_long(lib, length, budget):
     cut(lib, [length], 2, 16, 64, "bf16", budget, budget // 9, uniform, seed=length)
 
 
+@pytest.mark.parametrize("weights", [uniform, few_values, all_alike, odd_numbers])
+@pytest.mark.parametrize("lengths,budget,recent,page", [
+    ([20000, 8200, 0, 4097], 4096, 300, 64),     # the budget ends a chunk of 4096 slots
+    ([17000, 16999, 16384], 16998, 0, 24),       # one or two too many
+    ([20481, 20480], 8193, 8193, 5),             # the newest alone
+    ([16385, 3], 1, 1, 7),
+])
+def test_evict_long_rows_by_weights(lib, lengths, budget, recent, page, weights):
+    """Rows that several workgroups cut: many keys alike, ties in several chunks."""
+    print(f"[gpu] kv_evict long rows {lengths} {budget} {recent} {page} {weights.__name__}", flush=True)
+    cut(lib, lengths, 2, 16, page, "int8", budget, recent, weights, seed=budget + page)
+
+
+def test_evict_long_rows_with_absent_pages(lib):
+    print("[gpu] kv_evict long rows, absent pages", flush=True)
+    cut(lib, [20000, 18000, 17000], 2, 16, 64, "bf16", 9000, 100, uniform, seed=8, absent=[(0, 200, -1), (2, 0, 1 << 29)])
+    cut(lib, [20000, 18000, 17000], 2, 16, 64, "bf16", 9000, 100, few_values, seed=8, most=17500)
+
+
 def test_evict_after_an_eviction(lib):
     """Positions in any order, and more recent ones than the budget holds."""
     print("[gpu] kv_evict positions", flush=True)
