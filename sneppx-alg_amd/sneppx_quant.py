@@ -793,6 +793,9 @@ class _KVCacheStruct(C.Structure):
                 ("dtype", C.c_int), ("pages", _sz), ("page_size", _sz), ("kv_heads", _sz), ("head_dim", _sz)]
 
 
+_BF16, _BF16_OR_F32 = ((torch.bfloat16,), (torch.bfloat16, torch.float32)) if torch else ((), ())
+
+
 class KVCache:
     """A paged key-value pool (include/sneppx_kv.h): k, v [pages, kv_heads,
     page_size, head_dim] in bf16 or int8; k_scales, v_scales (int8), weights
@@ -833,64 +836,68 @@ class KVCache:
         # of it, 2.8 us where this takes 0.2
         return stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device.index or 0)
 
+    # (the checks are on the way of every call: few look-ups of a tensor's attributes,
+    # which take 0.1 us each)
     def _check(self, t, name, dtype, shape):
-        """A contiguous tensor of this type and shape on the cache's device."""
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != self.device \
-                or not t.is_contiguous():
-            got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
-            raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {self.device}, got {got}")
-        return t.data_ptr()
+        """The address of a contiguous tensor of this type and shape on the cache's device."""
+        try:
+            if t.dtype is dtype and t.shape == shape and t.device == self.device and t.is_contiguous():
+                return t.data_ptr()
+        except AttributeError:
+            pass
+        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
+        raise ValueError(f"{name} must be a contiguous {dtype} {tuple(shape)} tensor on {self.device}, got {got}")
 
     def _rows(self, t, name, heads, dtypes):
-        """[n, heads, head_dim] whose rows are contiguous; returns the row stride."""
+        """[n, heads, head_dim] whose rows are contiguous: its address, row stride, n and heads."""
         try:
             (n, h, d), (step, s1, s2) = t.shape, t.stride()
-            good = d == self.head_dim and s2 == 1 and (s1 == d or h == 1) and (h == heads or not heads) \
-                and t.dtype in dtypes and t.device == self.device
-        except (AttributeError, ValueError):
-            good = False
-        if not good:
-            got = f"{t.dtype} {tuple(t.shape)} (strides {t.stride()}) on {t.device}" \
-                if isinstance(t, torch.Tensor) else repr(t)
-            raise ValueError(f"{name} must be [n, {heads or 'q_heads'}, {self.head_dim}] with contiguous rows, "
-                             f"{' or '.join(map(str, dtypes))}, on {self.device}; got {got}")
-        return step
+            if d == self.head_dim and s2 == 1 and (s1 == d or h == 1) and (h == heads or not heads) \
+                    and t.dtype in dtypes and t.device == self.device:
+                return t.data_ptr(), step, n, h
+        except (AttributeError, TypeError, ValueError):
+            pass
+        got = f"{t.dtype} {tuple(t.shape)} (strides {t.stride()}) on {t.device}" \
+            if isinstance(t, torch.Tensor) else repr(t)
+        raise ValueError(f"{name} must be [n, {heads or 'q_heads'}, {self.head_dim}] with contiguous rows, "
+                         f"{' or '.join(map(str, dtypes))}, on {self.device}; got {got}")
 
     def _tables(self, tables, lengths):
         if not isinstance(tables, torch.Tensor) or tables.dim() != 2:
             raise ValueError("tables must be an int32 tensor [rows, width]")
-        n, width = tables.shape
-        return self._check(tables, "tables", torch.int32, (n, width)), width, \
+        shape = n, width = tables.shape
+        return self._check(tables, "tables", torch.int32, shape), width, \
             self._check(lengths, "lengths", torch.int32, (n,)), n
 
     def append(self, k, v, tables, lengths, next_pos=None, starts=None, k_stored=None, v_stored=None, stream=None):
         """SNEPPX_kv_append: k, v bf16 [tokens, kv_heads, head_dim], slices of
         wider rows among them; starts int32 [rows + 1], without it one token
         per row; k_stored, v_stored bf16 [tokens, kv_heads, head_dim]."""
-        ks, vs = (self._rows(t, n, self.kv_heads, (torch.bfloat16,)) for t, n in ((k, "k"), (v, "v")))
+        kp, ks, tokens, heads = self._rows(k, "k", self.kv_heads, _BF16)
+        vp, vs, v_tokens, _ = self._rows(v, "v", self.kv_heads, _BF16)
         tb, width, ln, n = self._tables(tables, lengths)
-        if v.shape != k.shape:
+        if v_tokens != tokens:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
         np_ = None if next_pos is None else self._check(next_pos, "next_pos", torch.int32, (n,))
         st = None if starts is None else self._check(starts, "starts", torch.int32, (n + 1,))
-        ko, vo = (None if t is None else self._check(t, name, torch.bfloat16, k.shape)
-                  for t, name in ((k_stored, "k_stored"), (v_stored, "v_stored")))
-        self.L.check(self._append(self._p, k.data_ptr(), ks, v.data_ptr(), vs, k.shape[0], st, ko, vo, tb, width, ln,
-                                  np_, n, self._stream(stream)), "kv_append")
+        stored = tokens, heads, self.head_dim
+        ko = None if k_stored is None else self._check(k_stored, "k_stored", torch.bfloat16, stored)
+        vo = None if v_stored is None else self._check(v_stored, "v_stored", torch.bfloat16, stored)
+        self.L.check(self._append(self._p, kp, ks, vp, vs, tokens, st, ko, vo, tb, width, ln, np_, n,
+                                  self._stream(stream)), "kv_append")
 
     def attention(self, q, out, tables, lengths, max_length, scale=None, accumulate=False, stream=None):
         """SNEPPX_kv_attention: q bf16 [rows, q_heads, head_dim], out the same
         in bf16 or fp32; scale 1 / sqrt(head_dim) unless given."""
-        qs = self._rows(q, "q", 0, (torch.bfloat16,))
-        os_ = self._rows(out, "out", q.shape[1], (torch.bfloat16, torch.float32))
+        qp, qs, rows, heads = self._rows(q, "q", 0, _BF16)
+        op, os_, out_rows, _ = self._rows(out, "out", heads, _BF16_OR_F32)
         tb, width, ln, n = self._tables(tables, lengths)
-        if q.shape[0] != n or out.shape[0] != n:
-            raise ValueError(f"q has {q.shape[0]} rows and out {out.shape[0]}, tables {n}")
+        if rows != n or out_rows != n:
+            raise ValueError(f"q has {rows} rows and out {out_rows}, tables {n}")
         self.L.check(self._attention(
-            self._p, q.data_ptr(), qs, out.data_ptr(), os_,
-            SNEPPX_FLOAT32 if out.dtype == torch.float32 else SNEPPX_BFLOAT16, tb, width, ln, n, q.shape[1],
-            max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate), self._stream(stream)),
-            "kv_attention")
+            self._p, qp, qs, op, os_, SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, tb, width, ln,
+            n, heads, max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate),
+            self._stream(stream)), "kv_attention")
 
     def evict(self, tables, lengths, next_pos, new_lengths, max_length, budget, recent, stream=None):
         """SNEPPX_kv_evict; new_lengths int32 [rows] or None."""
