@@ -392,6 +392,7 @@ k_kv_attn(const KVPool p, const Attn a) {
     __shared__ float2 ends[WAVES][16];
     __shared__ uint32_t arrived;
 
+    ask_for(p.tables, p.heads, a.rows, a.scale_log2);
     // The heads of a share, then the next share: workgroups go to the XCDs in turn,
     // and so every XCD gets shares of all rows.  The tiles of one head and share
     // are 8 workgroups apart, on one XCD, whose L2 has their tokens then (16 rows of
@@ -684,6 +685,7 @@ k_kv_attn(const KVPool p, const Attn a) {
 __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, uint32_t joins) {
     __shared__ float2 stat[256];      // of a head: maximum, 1 / sum
     __shared__ float factors[4][kMostShares];
+    ask_for(p.tables, p.heads, a.rows, a.scale_log2);
     const uint32_t bh = blockIdx.y + blockIdx.z * 65535u;
     if (bh >= a.rows * p.heads) return;
     const uint32_t b = bh / p.heads, h = bh - b * p.heads;

@@ -41,6 +41,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // at a prompt the reads and writes.
 template <bool I8, int LR>
 __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows n) {
+    ask_for(p.tables, p.heads, n.starts, n.tokens);
     const uint64_t first = (uint64_t)blockIdx.x * (256 / LR);
     const uint32_t per = 2 * p.heads, t0 = (uint32_t)(first / per);
     const uint32_t rest = (uint32_t)(first - (uint64_t)t0 * per) + threadIdx.x / LR;
@@ -426,6 +427,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
     __shared__ uint32_t sh[kCutWaves];
     __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
+    ask_for(p.tables, p.heads, a.budget, a.counts);
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
     const int tid = threadIdx.x;
     const uint32_t L = kv_length(a.lengths, b, a.max_length), budget = a.budget;
@@ -486,6 +488,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
 // 70 and 113; 1 of 16384 30 and 30, of 12288 29 and 26, of 8192 27 and 21, and one
 // token too many in 8 of 16384 29 and 22.)
 __device__ __forceinline__ bool long_row(const KVPool& p, const Cut& a, uint32_t& bh, uint32_t& b, uint32_t& h, uint32_t& L) {
+    ask_for(p.tables, p.heads, a.counts, a.absent);
     bh = blockIdx.y + blockIdx.z * 65535u;
     b = bh / p.heads;
     h = bh - b * p.heads;
@@ -665,6 +668,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_list(const KVPool p, const C
 // The moves that k_kv_cut or k_kv_list listed.  Sources lie in slots from the budget on and
 // targets below it, so all are independent.
 __global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a, uint32_t first) {
+    ask_for(p.tables, p.heads, a.budget, a.counts);
     const uint32_t bh = first + blockIdx.y, b = bh / p.heads, n = a.counts[bh];
     const uint32_t* to = a.moves + (size_t)bh * 2 * a.most;
     move_rows<4>(p, b, bh - b * p.heads, a.row_bytes, to, to + a.most, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
