@@ -22,6 +22,18 @@ hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 // max over non-NaN values, as the reference's `if (a > m) m = a`
 __device__ __forceinline__ float nanless_max(float a, float b) { return b > a ? b : a; }
 
+// of LR lanes, to all of them: exchanges of neighbours, pairs, halves of 8, of 16 and
+// of 32 lanes
+template <int LR>
+__device__ __forceinline__ float row_max(float m) {
+    m = nanless_max(m, lane_step<0xB1, 0xf>(m, m));
+    m = nanless_max(m, lane_step<0x4E, 0xf>(m, m));
+    m = nanless_max(m, lane_step<0x141, 0xf>(m, m));
+    if (LR >= 16) m = nanless_max(m, lane_step<0x140, 0xf>(m, m));
+    if (LR >= 32) m = nanless_max(m, __shfl_xor(m, 16));
+    return m;
+}
+
 // ------------------------------------------------------------------- append
 struct NewRows {
     const uint16_t *k, *v;
@@ -102,8 +114,7 @@ __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) m = nanless_max(m, fabsf(f[e]));
-#pragma unroll
-        for (int o = LR / 2; o > 0; o >>= 1) m = nanless_max(m, __shfl_xor(m, o));
+        m = row_max<LR>(m);
         const float s = m < FLT_MIN ? 1.0f : m / 127.0f, inv = 1.0f / s;
         // Numbers below 128 round half away by adding the number below 1/2 and
         // cutting; what the rule gives for others (an infinity or NaN in the row, a
