@@ -83,11 +83,11 @@ struct Attn {
 // All rows' steps (one at least for each row), one row after the other, are cut
 // into equal shares; a workgroup takes one, with the end of a row, whole rows
 // and the beginning of another in it, and so all end together.  Where a share is
-// only a few steps, changing the row costs more than that evens out, and every
-// row begins with a new share.  The lengths are known on the device alone, so
+// only a few steps, or as many shares are enough so, changing the row costs more
+// than that evens out, and every row begins with a new share.  The lengths are known on the device alone, so
 // every wave works this out for itself.  (us of shares across rows / by rows, 8 heads
 // of 128 in bf16: 16 rows of 0 to 4096 tokens, 4 steps a share, 32 / 28; 24 rows, 6
-// steps, 46 / 54; 64 rows, 16 steps, 100 / 118.  A grid for the longest row that
+// steps, 46 / 54; 64 rows, 16 steps, 100 / 118; 16 of 2049, 5 steps, 33 / 30.  A grid for the longest row that
 // the host allows for leaves most of it idle: 45 for the first.)
 struct Row {
     uint32_t b, at, len;           // the row, its first step, its length in tokens
@@ -137,11 +137,14 @@ struct Division {
         }
         total = __builtin_amdgcn_readlane(lane_prefix(sum), 63);
         per = a.by_shares(total + a.shares - 1);
-        // a row has part of its first and last share
-        const uint32_t least = (lane_max(longest) + kMostShares - 3) / (kMostShares - 2);
-        per = per > least ? per : least;
-        by_row = per <= kFewSteps;
+        if (a.shares > kMostShares - 2) {            // a row has part of its first and last share
+            const uint32_t least = (lane_max(longest) + kMostShares - 3) / (kMostShares - 2);
+            per = per > least ? per : least;
+        }
         by = By(per);
+        by_row = per <= kFewSteps;
+        if (!by_row && a.rows <= 64)
+            by_row = (uint32_t)__builtin_amdgcn_readlane(lane_prefix(by(steps(lane, len0) + per - 1)), 63) <= a.shares;
     }
     __device__ __forceinline__ uint32_t length(uint32_t r) const {
         return r < a.rows ? kv_length(a.lengths, r, a.max_length) : 0;
