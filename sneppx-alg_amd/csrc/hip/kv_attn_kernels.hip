@@ -84,11 +84,12 @@ struct Attn {
 // into equal shares; a workgroup takes one, with the end of a row, whole rows
 // and the beginning of another in it, and so all end together.  Where a share is
 // only a few steps, or as many shares are enough so, changing the row costs more
-// than that evens out, and every row begins with a new share.  The lengths are known on the device alone, so
-// every wave works this out for itself.  (us of shares across rows / by rows, 8 heads
-// of 128 in bf16: 16 rows of 0 to 4096 tokens, 4 steps a share, 32 / 28; 24 rows, 6
-// steps, 46 / 54; 64 rows, 16 steps, 100 / 118; 16 of 2049, 5 steps, 33 / 30.  A grid for the longest row that
-// the host allows for leaves most of it idle: 45 for the first.)
+// than that evens out, and every row begins with a new share.  The lengths are
+// known on the device alone, so every wave works this out for itself.  (us of
+// shares across rows / by rows, 8 heads of 128 in bf16: 16 rows of 0 to 4096
+// tokens, 4 steps a share, 32 / 28; 24 rows, 6 steps, 46 / 54; 64 rows, 16 steps,
+// 100 / 118; 16 of 2049, 5 steps, as many shares, 33 / 30.  A grid for the longest
+// row that the host allows for leaves most of it idle: 45 for the first.)
 struct Row {
     uint32_t b, at, len;           // the row, its first step, its length in tokens
     __device__ __forceinline__ uint32_t steps() const { return len > STEP ? (len + STEP - 1) / STEP : 1; }

@@ -144,6 +144,18 @@ def test_division_of_rows(lib, lengths, heads, dim, dtype):
     lib.fn["SNEPPX_qlinear_release_workspaces"](st.cuda_stream)
 
 
+@pytest.mark.parametrize("lengths,heads,dim,dtype", [
+    ([2500, 2500], 64, 16, "bf16"),              # 8 shares of 5 steps: four for each row
+    ([2304, 2176, 0], 64, 16, "int8"),           # one more row than fits
+    ([1990] * 4, 64, 24, "bf16"),
+    ([7000, 6700], 64, 16, "int8"),
+    ([3000, 900, 2100], 33, 8, "bf16"),
+])
+def test_division_of_rows_in_as_many_shares(lib, lengths, heads, dim, dtype):
+    """Long shares: rows begin them where no more are needed for it."""
+    test_division_of_rows(lib, lengths, heads, dim, dtype)
+
+
 def test_calls_of_many_divisions_in_turn(lib):
     """One stream's scratch and counters serve calls of every size in turn."""
     print("[gpu] kv_attention sizes in turn", flush=True)
