@@ -16,8 +16,8 @@
 //  * A row in several shares is joined, in the order of its shares, by the last of
 //    them to arrive, or by k_kv_join after them, which also adds the attention
 //    weights, from the logits that the first kernel wrote.
-// Reached: 131072 tokens of 8 heads of 128 in bf16 (537 MB) 98 us, 5.5 TB/s, where a
-// copy of 256 MB runs at 5.4; 64 rows of 0 to 8192 in int8 (532 MB) 105 us.  A call
+// Reached: 131072 tokens of 8 heads of 128 in bf16 (537 MB) 97 us, 5.5 TB/s, where a
+// copy of 256 MB runs at 5.4; 64 rows of 0 to 8192 in int8 (532 MB) 103 us.  A call
 // is about 8 us and what it reads at 5.8 TB/s: the look-ups, the first tile, the
 // meeting and the join follow one another.
 #include <hip/hip_runtime.h>
