@@ -428,9 +428,9 @@ __device__ __forceinline__ uint32_t list_slots(const uint32_t* keys, uint32_t sl
 }
 
 // One workgroup per (row, head) of up to kLong slots.  A call runs through the code
-// about once, and fetching that is much of its time (16 x 8 of 2049: 8.4 us; unrolled and
-// specialised, with keys in registers, twice the code, 8.5): the
-// loops are left rolled.
+// about once, and its instructions one after the other are its time: the loops are
+// left rolled (16 x 8 of 2049: 8.4 us; unrolled, with keys in registers, twice the
+// code, 8.5).
 // MOVE: with so few moves that the workgroup makes them at once.
 template <bool MOVE>
 __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
@@ -682,7 +682,10 @@ __global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a, ui
     ask_for(p.tables, p.heads, a.budget, a.counts);
     const uint32_t bh = first + blockIdx.y, b = bh / p.heads, n = a.counts[bh];
     const uint32_t* to = a.moves + (size_t)bh * 2 * a.most;
-    move_rows<4>(p, b, bh - b * p.heads, a.row_bytes, to, to + a.most, n, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    constexpr uint32_t most = 1u << 24;          // (16-byte pieces are counted in 32 bits)
+    for (uint32_t m = 0; m < n; m += most)
+        move_rows<4>(p, b, bh - b * p.heads, a.row_bytes, to + m, to + a.most + m, n - m < most ? n - m : most,
+                     blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 template <int LR>
