@@ -165,7 +165,7 @@ constexpr int kCutWaves = 16;
 constexpr int kCutThreads = 64 * kCutWaves;
 constexpr int kDigit = 11;               // digits of 11, 11 and 10 bits, from the top
 constexpr int kBins = 1 << kDigit;
-constexpr uint32_t kChunk = 4 * kCutThreads;         // slots of a long row that a workgroup has
+constexpr uint32_t kLogChunk = 12, kMostLog = 15;    // of the slots of a long row that a workgroup has
 constexpr size_t kLong = 16384;          // longer rows are cut by several workgroups
 constexpr uint32_t kMoveAtOnce = 64;     // moves that the workgroup which finds them makes itself
 
@@ -237,15 +237,17 @@ struct Chunk {
     uint32_t cands, low_cands;     // its keys with the first digit of the threshold; those below the budget
     uint32_t sure, low_sure;       // its keys above them
 };
+__host__ __device__ __forceinline__ uint32_t chunks_of(uint32_t slots, uint32_t log) { return (slots + (1u << log) - 1) >> log; }
+
 struct Cut {
     const int32_t *lengths, *next_pos;
     int32_t* new_lengths;
     uint32_t rows, max_length, budget, recent, most, row_bytes;
     uint32_t* counts;          // [rows * heads] moves of each row and head (unless moved at once)
     uint32_t* moves;           // [rows * heads][2][most] slots: targets, then sources
-    uint32_t chunks;           // the rest of long rows, [rows * heads] of each
-    uint32_t* keys;            // [chunks][kChunk]
-    uint32_t* cands;           // [chunks][kChunk]: `cands` keys of each chunk, in the order of their slots
+    uint32_t chunks, log;      // the rest of long rows, [rows * heads] of each; log2 of a chunk's slots
+    uint32_t* keys;            // [chunks][1 << log]
+    uint32_t* cands;           // [chunks][1 << log]: `cands` keys of each chunk, in the order of their slots
     uint32_t* firsts;          // [chunks][kBins / 2]: the chunk's keys by first digit, 16 bits each
     Chunk* found;              // [chunks]
     uint32_t* absent;          // [chunks]: whether a page is not there
@@ -434,7 +436,7 @@ __device__ __forceinline__ uint32_t list_slots(const uint32_t* keys, uint32_t sl
 // MOVE: with so few moves that the workgroup makes them at once.
 template <bool MOVE>
 __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
-    extern __shared__ uint32_t keys[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t keys[];
     __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
     __shared__ uint32_t sh[kCutWaves];
     __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
@@ -491,13 +493,15 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
 }
 
 // ------------------------------------------------------------- of long rows
-// A workgroup has kChunk slots, in three kernels: k_kv_rank counts their keys by
+// A workgroup has 4096 slots, up to 32768 where there are many, in three kernels: k_kv_rank counts their keys by
 // first digit; with all chunks' counts k_kv_part finds the threshold's and puts
 // the keys that share it apart; k_kv_list finds the threshold among these, and
 // where its own slots stand in the lists.  (us of a call that cuts so, and with one
 // workgroup for each row and head: 2 rows of 30001 and 8 heads 32 and 41, 4 of 60000
 // 70 and 113; 1 of 16384 30 and 30, of 12288 29 and 26, of 8192 27 and 21, and one
-// token too many in 8 of 16384 29 and 22.)
+// token too many in 8 of 16384 29 and 22.  Every workgroup adds up the counts of all
+// chunks: one token too many in 8 rows of 131072 takes 85 us in chunks for two
+// workgroups a CU, 121 in 4096s; in 1 of 1000000 94 and 248.)
 __device__ __forceinline__ bool long_row(const KVPool& p, const Cut& a, uint32_t& bh, uint32_t& b, uint32_t& h, uint32_t& L) {
     ask_for(p.tables, p.heads, a.counts, a.absent);
     bh = blockIdx.y + blockIdx.z * 65535u;
@@ -505,7 +509,7 @@ __device__ __forceinline__ bool long_row(const KVPool& p, const Cut& a, uint32_t
     h = bh - b * p.heads;
     if (b >= a.rows) return false;
     L = kv_length(a.lengths, b, a.max_length);
-    return L > a.budget && blockIdx.x * kChunk < L;
+    return L > a.budget && blockIdx.x << a.log < L;
 }
 // a page of the row that is not there
 __device__ __forceinline__ bool row_absent(const Cut& a, uint32_t bh, uint32_t chunks) {
@@ -522,14 +526,19 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_rank(const KVPool p, const C
     reinterpret_cast<u32x2*>(hist)[tid] = u32x2{0u, 0u};
     __syncthreads();
     const size_t chunk = (size_t)bh * a.chunks + blockIdx.x;
-    const uint32_t mine = (tid & ~63) * 4 + (tid & 63), t0 = blockIdx.x * kChunk + mine;
-    Ranks ranks(p, a, b, h, L, t0);
-    uint32_t q[4];
-    ranks.next<4>(q);
-    const bool there[4] = {t0 < L, t0 + 64 < L, t0 + 128 < L, t0 + 192 < L};
+    const uint32_t steps = (1u << a.log) / kCutThreads, mine = (tid & ~63) * steps + (tid & 63);
+    uint32_t* const keys = a.keys + (chunk << a.log) + mine;
+    Ranks ranks(p, a, b, h, L, (blockIdx.x << a.log) + mine);
+#pragma unroll 1
+    for (uint32_t i = 0; i < steps; i += 4) {
+        const uint32_t t = ranks.t;
+        uint32_t q[4];
+        ranks.next<4>(q);
+        const bool there[4] = {t < L, t + 64 < L, t + 128 < L, t + 192 < L};
 #pragma unroll
-    for (int u = 0; u < 4; u++) a.keys[chunk * kChunk + mine + 64 * u] = q[u];
-    Threshold(0).tally<4>(hist, q, there);
+        for (int u = 0; u < 4; u++) keys[64 * (i + u)] = q[u];
+        Threshold(0).tally<4>(hist, q, there);
+    }
     const bool gone = __syncthreads_or(ranks.gone);
     const u32x2 n = reinterpret_cast<const u32x2*>(hist)[tid];
     a.firsts[chunk * (kBins / 2) + tid] = n[0] | n[1] << 16;
@@ -558,48 +567,63 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_part(const KVPool p, const C
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     uint32_t bh, b, h, L, q[4];
     if (!long_row(p, a, bh, b, h, L)) return;
-    const uint32_t chunks = (L + kChunk - 1) / kChunk;
+    const uint32_t chunks = chunks_of(L, a.log);
     const size_t chunk = (size_t)bh * a.chunks + blockIdx.x;
-    const uint32_t mine = (tid & ~63u) * 4 + lane, t0 = blockIdx.x * kChunk + mine;
+    const uint32_t steps = (1u << a.log) / kCutThreads, mine = (tid & ~63u) * steps + lane;
+    const uint32_t t0 = (blockIdx.x << a.log) + mine;
+    const uint32_t* const keys = a.keys + (chunk << a.log) + mine;
+    uint32_t* const cands_at = a.cands + (chunk << a.log);
+    auto four = [&](uint32_t i) {
 #pragma unroll
-    for (int u = 0; u < 4; u++) q[u] = a.keys[chunk * kChunk + mine + 64 * u];
+        for (int u = 0; u < 4; u++) q[u] = keys[64 * (i + u)];
+    };
+    four(0);
     if (row_absent(a, bh, chunks)) return;
     const Threshold at = first_digit(a, bh, chunks, hist, sh);
 
-    uint64_t who[4];
-    uint32_t cands = 0, low_cands = 0, sure = 0, low_sure = 0, total, low_total;
+    uint32_t cands = 0, low_cands = 0, sure = 0, low_sure = 0, total, low_total, to = 0;
+    // first the numbers, then the keys
+#pragma unroll 1
+    for (int listing = 0; listing < 2; listing++) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < steps; i += 4) {
+            if (steps > 4) four(i);
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const bool there = t0 + 64 * u < L, low = t0 + 64 * u < a.budget;
-        who[u] = __ballot(there && (q[u] & at.known) == at.prefix);
-        const uint64_t above = __ballot(there && (q[u] & at.known) > at.prefix), below = __ballot(low);
-        cands += __popcll(who[u]);
-        low_cands += __popcll(who[u] & below);
-        sure += __popcll(above);
-        low_sure += __popcll(above & below);
-    }
-    uint32_t to = wave_prefix(cands | low_cands << 16, sh, total) & 0xFFFF;
-    (void)wave_prefix(sure | low_sure << 16, sh, low_total);
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-        if (__builtin_amdgcn_inverse_ballot_w64(who[u])) a.cands[chunk * kChunk + to + lane_rank(who[u])] = q[u];
-        to += __popcll(who[u]);
+            for (int u = 0; u < 4; u++) {
+                const uint32_t t = t0 + 64 * (i + u), digit = q[u] & at.known;
+                const uint64_t who = __ballot(t < L && digit == at.prefix);
+                if (listing) {
+                    if (__builtin_amdgcn_inverse_ballot_w64(who)) cands_at[to + lane_rank(who)] = q[u];
+                    to += __popcll(who);
+                    continue;
+                }
+                const uint64_t above = __ballot(t < L && digit > at.prefix), below = __ballot(t < a.budget);
+                cands += __popcll(who);
+                low_cands += __popcll(who & below);
+                sure += __popcll(above);
+                low_sure += __popcll(above & below);
+            }
+        }
+        if (listing) break;
+        to = wave_prefix(cands | low_cands << 16, sh, total) & 0xFFFF;
+        (void)wave_prefix(sure | low_sure << 16, sh, low_total);
     }
     if (tid == 0) a.found[chunk] = Chunk{total & 0xFFFF, total >> 16, low_total & 0xFFFF, low_total >> 16};
 }
 
 __global__ void __launch_bounds__(kCutThreads) k_kv_list(const KVPool p, const Cut a) {
-    __shared__ __attribute__((aligned(16))) uint32_t hist[kBins], keys[kChunk];
+    extern __shared__ __attribute__((aligned(16))) uint32_t keys[];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
     __shared__ uint32_t sh[kCutWaves], sums[4][kCutWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint32_t bh, b, h, L;
     const bool cut = long_row(p, a, bh, b, h, L);
     if (b >= a.rows) return;
-    const uint32_t chunks = (L + kChunk - 1) / kChunk, chunk = blockIdx.x;
+    const uint32_t chunks = chunks_of(L, a.log), chunk = blockIdx.x, size = 1u << a.log;
     const size_t row = (size_t)bh * a.chunks;
     if (cut)
-        for (uint32_t i = tid; i < kChunk / 4; i += kCutThreads)
-            reinterpret_cast<u32x4*>(keys)[i] = reinterpret_cast<const u32x4*>(a.keys + (row + chunk) * kChunk)[i];
+        for (uint32_t i = tid; i < size / 4; i += kCutThreads)
+            reinterpret_cast<u32x4*>(keys)[i] = reinterpret_cast<const u32x4*>(a.keys + ((row + chunk) << a.log))[i];
     const bool gone = L > a.budget && row_absent(a, bh, chunks);
     if (chunk == 0 && tid == 0 && h == 0 && a.new_lengths) a.new_lengths[b] = (int32_t)(L > a.budget && !gone ? a.budget : L);
     if (!cut || gone) {
@@ -612,7 +636,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_list(const KVPool p, const C
 #pragma unroll 1
         for (uint32_t c = wave; c < chunks; c += kCutWaves) {
             const uint32_t n = a.found[row + c].cands;
-            const uint32_t* const cands = a.cands + (row + c) * kChunk;
+            const uint32_t* const cands = a.cands + ((row + c) << a.log);
 #pragma unroll 1
             for (uint32_t i = lane; i < n + lane; i += 256) {
                 uint32_t q[4];
@@ -669,9 +693,9 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_list(const KVPool p, const C
     low_ties = all(3);
     const uint32_t kept = all(0) + (ties < at.want ? ties : at.want);                      // before this chunk
     const uint32_t low_kept = all(2) + (low_ties < at.want ? low_ties : at.want);          // below the budget
-    const uint32_t slot0 = chunk * kChunk;
+    const uint32_t slot0 = chunk << a.log;
     uint32_t* const to = a.moves + (size_t)bh * 2 * a.most;
-    (void)list_slots(keys, slot0, kChunk / kCutThreads, a.budget, at, ties, slot0 < a.budget ? slot0 - kept : 0,
+    (void)list_slots(keys, slot0, size / kCutThreads, a.budget, at, ties, slot0 < a.budget ? slot0 - kept : 0,
                      slot0 > a.budget ? kept - low_kept : 0, sh, to, to + a.most);
     if (chunk == 0 && tid == 0) a.counts[bh] = a.budget - low_kept;
 }
@@ -694,15 +718,18 @@ void append(bool i8, unsigned blocks, const KVPool& p, const NewRows& n, hipStre
     else k_kv_append<false, LR><<<blocks, 256, 0, s>>>(p, n);
 }
 
+int reserve_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    if (lds_optin(kernel, (int)bytes, done) == hipSuccess) return 0;
+    snx_set_error("kv_evict: cannot reserve %zu bytes of LDS", bytes);
+    return -1;
+}
+
 template <bool MOVE>
 int cut(unsigned blocks, const KVPool& p, const Cut& a, hipStream_t s) {
     // (rows that nothing is cut from need no keys)
     const size_t keys = a.most ? ((size_t)a.max_length + kCutThreads - 1) / kCutThreads * kCutThreads : 0;
     static std::atomic<uint64_t> done{0};
-    if (lds_optin(reinterpret_cast<const void*>(&k_kv_cut<MOVE>), (int)(kLong * sizeof(uint32_t)), done) != hipSuccess) {
-        snx_set_error("kv_evict: cannot reserve %zu bytes of LDS", kLong * sizeof(uint32_t));
-        return -1;
-    }
+    if (reserve_lds(reinterpret_cast<const void*>(&k_kv_cut<MOVE>), kLong * sizeof(uint32_t), done)) return -1;
     k_kv_cut<MOVE><<<blocks, kCutThreads, keys * sizeof(uint32_t), s>>>(p, a);
     return snx_launch_check("k_kv_cut");
 }
@@ -750,12 +777,20 @@ int snx_k_kv_append(const SNEPPXKVCache* c, const uint16_t* k, size_t k_stride, 
 }
 
 static bool is_long(size_t max_length, size_t most) { return most && max_length > kLong; }
-static size_t chunks_of(size_t max_length) { return (max_length + kChunk - 1) / kChunk; }
+// log2 of a chunk's slots: no more workgroups than two for a CU, if that is few slots
+static uint32_t chunk_log(size_t bh, size_t max_length) {
+    uint32_t log = kLogChunk;
+    while (log < kMostLog && bh * chunks_of((uint32_t)max_length, log) > 2 * (size_t)cu_count()) log++;
+    return log;
+}
 
 size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, size_t budget) {
-    const size_t most = most_moves(max_length, budget), bh = rows * c->kv_heads, chunks = chunks_of(max_length);
-    if (is_long(max_length, most))
-        return bh * (chunks * ((2 * kChunk + kBins / 2 + 1) * sizeof(uint32_t) + sizeof(Chunk)) + (1 + 2 * most) * sizeof(uint32_t));
+    const size_t most = most_moves(max_length, budget), bh = rows * c->kv_heads;
+    if (is_long(max_length, most)) {
+        const uint32_t log = chunk_log(bh, max_length);
+        const size_t chunk = ((2u << log) + kBins / 2 + 1) * sizeof(uint32_t) + sizeof(Chunk);
+        return bh * (chunks_of((uint32_t)max_length, log) * chunk + (1 + 2 * most) * sizeof(uint32_t));
+    }
     return most > kMoveAtOnce ? bh * (1 + 2 * most) * sizeof(uint32_t) : 0;
 }
 
@@ -774,14 +809,15 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
     a.most = most_moves(max_length, budget);
     a.row_bytes = (uint32_t)(c->head_dim * (c->dtype == SNEPPX_INT8 ? 1 : 2));
     a.rows = (uint32_t)rows;
-    a.chunks = (uint32_t)chunks_of(max_length);
     const hipStream_t s = S(st);
     if (is_long(max_length, a.most)) {
+        a.log = chunk_log(bh, max_length);
+        a.chunks = chunks_of(a.max_length, a.log);
         const size_t all = bh * a.chunks;
         a.found = static_cast<Chunk*>(ws);
         a.keys = reinterpret_cast<uint32_t*>(a.found + all);
-        a.cands = a.keys + all * kChunk;
-        a.firsts = a.cands + all * kChunk;
+        a.cands = a.keys + (all << a.log);
+        a.firsts = a.cands + (all << a.log);
         a.absent = a.firsts + all * (kBins / 2);
         a.counts = a.absent + all;
         a.moves = a.counts + bh;
@@ -790,7 +826,9 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
         if (snx_launch_check("k_kv_rank")) return -1;
         k_kv_part<<<grid, kCutThreads, 0, s>>>(p, a);
         if (snx_launch_check("k_kv_part")) return -1;
-        k_kv_list<<<grid, kCutThreads, 0, s>>>(p, a);
+        static std::atomic<uint64_t> done{0};
+        if (reserve_lds(reinterpret_cast<const void*>(&k_kv_list), sizeof(uint32_t) << kMostLog, done)) return -1;
+        k_kv_list<<<grid, kCutThreads, sizeof(uint32_t) << a.log, s>>>(p, a);
         if (snx_launch_check("k_kv_list")) return -1;
     } else {
         a.counts = static_cast<uint32_t*>(ws);

@@ -244,6 +244,14 @@ def test_evict_long_rows_by_weights(lib, lengths, budget, recent, page, weights)
     cut(lib, lengths, 2, 16, page, "int8", budget, recent, weights, seed=budget + page)
 
 
+@pytest.mark.parametrize("weights", [uniform, few_values])
+@pytest.mark.parametrize("lengths,heads,budget", [([17000], 130, 8192), ([16900, 16385], 130, 16384), ([17000], 260, 6000)])
+def test_evict_long_rows_of_many_heads(lib, lengths, heads, budget, weights):
+    """Workgroups that have more slots each where rows and heads are many."""
+    print(f"[gpu] kv_evict long rows of many heads {lengths} {heads} {budget} {weights.__name__}", flush=True)
+    cut(lib, lengths, heads, 8, 64, "bf16", budget, 99, weights, seed=heads)
+
+
 def test_evict_long_rows_with_absent_pages(lib):
     print("[gpu] kv_evict long rows, absent pages", flush=True)
     cut(lib, [20000, 18000, 17000], 2, 16, 64, "bf16", 9000, 100, uniform, seed=8, absent=[(0, 200, -1), (2, 0, 1 << 29)])
