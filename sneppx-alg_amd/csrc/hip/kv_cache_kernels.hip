@@ -700,16 +700,20 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_list(const KVPool p, const C
     if (chunk == 0 && tid == 0) a.counts[bh] = a.budget - low_kept;
 }
 
-// The moves that k_kv_cut or k_kv_list listed.  Sources lie in slots from the budget on and
-// targets below it, so all are independent.
-__global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a, uint32_t first) {
+// The moves that k_kv_cut or k_kv_list listed.  Sources lie in slots from the budget
+// on and targets below it, so all are independent.  Rows of head_dim values in any
+// order bound it: 8 x 8 of 8192 halved, 134 MB read and written, 33 us.  Heads go side
+// by side, whose tokens share pages (one after the other: 36 us; 16 x 8 of 2049
+// halved 27 and 30.5 us in all), and a workgroup's loads in flight lie far apart in
+// the list (54 us in all; side by side 59).
+__global__ void __launch_bounds__(256) k_kv_move(const KVPool p, const Cut a) {
     ask_for(p.tables, p.heads, a.budget, a.counts);
-    const uint32_t bh = first + blockIdx.y, b = bh / p.heads, n = a.counts[bh];
+    const uint32_t bh = blockIdx.x, b = bh / p.heads, n = a.counts[bh];
     const uint32_t* to = a.moves + (size_t)bh * 2 * a.most;
     constexpr uint32_t most = 1u << 24;          // (16-byte pieces are counted in 32 bits)
     for (uint32_t m = 0; m < n; m += most)
         move_rows<4>(p, b, bh - b * p.heads, a.row_bytes, to + m, to + a.most + m, n - m < most ? n - m : most,
-                     blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+                     blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
 }
 
 template <int LR>
@@ -837,12 +841,8 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
         if (cut<false>((unsigned)bh, p, a, s)) return -1;
     }
     const size_t chunks = (size_t)a.most * (a.row_bytes / 16), gx = (chunks + 1023) / 1024;
-    for (size_t at = 0; at < bh; at += 65535) {
-        const size_t n = bh - at < 65535 ? bh - at : 65535;
-        k_kv_move<<<dim3((unsigned)(gx < 65536 ? gx : 65536), (unsigned)n), 256, 0, s>>>(p, a, (uint32_t)at);
-        if (snx_launch_check("k_kv_move")) return -1;
-    }
-    return 0;
+    k_kv_move<<<dim3((unsigned)bh, (unsigned)(gx < 65536 ? gx : 65535)), 256, 0, s>>>(p, a);
+    return snx_launch_check("k_kv_move");
 }
 
 }  // extern "C"
