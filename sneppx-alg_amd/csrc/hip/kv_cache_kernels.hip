@@ -251,6 +251,7 @@ struct Cut {
     uint32_t* firsts;          // [chunks][kBins / 2]: the chunk's keys by first digit, 16 bits each
     Chunk* found;              // [chunks]
     uint32_t* absent;          // [chunks]: whether a page is not there
+    uint2* least;              // [chunks], instead: the lowest key and its slot
 };
 
 // The keys of a lane's slots, every 64th from `t` on
@@ -429,6 +430,32 @@ __device__ __forceinline__ uint32_t list_slots(const uint32_t* keys, uint32_t sl
     return total;
 }
 
+// Of one token too many no threshold is needed: the lowest key goes, of equal ones
+// the one in the highest slot, and the last slot's token moves there.
+struct Least {
+    uint32_t key = ~0u, slot = 0;
+    __device__ __forceinline__ void add(uint32_t q, uint32_t t) {       // slots in ascending order
+        slot = q <= key ? t : slot;
+        key = q <= key ? q : key;
+    }
+    __device__ __forceinline__ void of_wave() {
+        const uint32_t least = ~lane_max(~key);
+        slot = lane_max(key == least ? slot : 0u);
+        key = least;
+    }
+    // of `waves` waves, to all of them
+    __device__ __forceinline__ void of_group(uint2* sh, uint32_t waves) {
+        const uint32_t lane = threadIdx.x & 63;
+        of_wave();
+        if (lane == 0) sh[threadIdx.x >> 6] = make_uint2(key, slot);
+        __syncthreads();
+        const uint2 v = sh[lane < waves ? lane : 0];
+        key = v.x;
+        slot = v.y;
+        of_wave();
+    }
+};
+
 // One workgroup per (row, head) of up to kLong slots.  A call runs through the code
 // about once, and its instructions one after the other are its time: the loops are
 // left rolled (16 x 8 of 2049: 8.4 us; unrolled, with keys in registers, twice the
@@ -439,6 +466,7 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     extern __shared__ __attribute__((aligned(16))) uint32_t keys[];
     __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
     __shared__ uint32_t sh[kCutWaves];
+    __shared__ uint2 sh2[kCutWaves];
     __shared__ uint32_t list[MOVE ? 2 * kMoveAtOnce : 1];
     ask_for(p.tables, p.heads, a.budget, a.counts);
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads;
@@ -468,22 +496,36 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
         if (!MOVE && tid == 0) a.counts[blockIdx.x] = 0;
         return;
     }
-    Threshold at(budget);
-#pragma unroll 1
-    for (;;) {
-#pragma unroll 1
-        for (uint32_t i = 0; i < steps; i++) at.tally<1>(hist, {keys[t0 + 64 * i]}, {t0 + 64 * i < L});
-        __syncthreads();
-        at.find(hist, sh);
-        if (at.done()) break;
-        __syncthreads();
-        *bins = u32x2{0u, 0u};
-        __syncthreads();
-    }
-    at.settle();
     uint32_t* const to = MOVE ? list : a.moves + (size_t)blockIdx.x * 2 * a.most;
     uint32_t* const of = to + (MOVE ? kMoveAtOnce : a.most);
-    const uint32_t total = list_slots(keys, 0, steps, budget, at, 0, 0, 0, sh, to, of);
+    uint32_t total;
+    if (L - budget == 1) {                           // (16 x 8 of 2049: 5.7 us, 8.4 the other way)
+        Least least;
+#pragma unroll 1
+        for (uint32_t i = 0; i < steps; i++)
+            if (t0 + 64 * i < L) least.add(keys[t0 + 64 * i], t0 + 64 * i);
+        least.of_group(sh2, kCutWaves);
+        total = least.slot != budget;
+        if (tid == 0 && total) {
+            to[0] = least.slot;
+            of[0] = budget;
+        }
+    } else {
+        Threshold at(budget);
+#pragma unroll 1
+        for (;;) {
+#pragma unroll 1
+            for (uint32_t i = 0; i < steps; i++) at.tally<1>(hist, {keys[t0 + 64 * i]}, {t0 + 64 * i < L});
+            __syncthreads();
+            at.find(hist, sh);
+            if (at.done()) break;
+            __syncthreads();
+            *bins = u32x2{0u, 0u};
+            __syncthreads();
+        }
+        at.settle();
+        total = list_slots(keys, 0, steps, budget, at, 0, 0, 0, sh, to, of);
+    }
     if (MOVE) {
         __syncthreads();
         move_rows<1>(p, b, h, a.row_bytes, to, of, total, tid, kCutThreads);
@@ -498,9 +540,9 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
 // the keys that share it apart; k_kv_list finds the threshold among these, and
 // where its own slots stand in the lists.  (us of a call that cuts so, and with one
 // workgroup for each row and head: 2 rows of 30001 and 8 heads 32 and 41, 4 of 60000
-// 70 and 113; 1 of 16384 30 and 30, of 12288 29 and 26, of 8192 27 and 21, and one
-// token too many in 8 of 16384 29 and 22.  Every workgroup adds up the counts of all
-// chunks: one token too many in 8 rows of 131072 takes 85 us in chunks for two
+// 70 and 113; 1 of 16384 30 and 30, of 12288 29 and 26, of 8192 27 and 21.  Every
+// workgroup adds up the counts of all
+// chunks: two tokens too many in 8 rows of 131072 take 83 us in chunks for two
 // workgroups a CU, 121 in 4096s; in 1 of 1000000 94 and 248.)
 __device__ __forceinline__ bool long_row(const KVPool& p, const Cut& a, uint32_t& bh, uint32_t& b, uint32_t& h, uint32_t& L) {
     ask_for(p.tables, p.heads, a.counts, a.absent);
@@ -516,6 +558,58 @@ __device__ __forceinline__ bool row_absent(const Cut& a, uint32_t bh, uint32_t c
     bool gone = false;
     for (uint32_t c = threadIdx.x; c < chunks; c += kCutThreads) gone |= a.absent[(size_t)bh * a.chunks + c] != 0;
     return __syncthreads_or(gone);
+}
+
+// One token too many at most in long rows: the lowest key of each chunk, then of all
+// (us of the call, and by the kernels below: 1 row of 30000 11.6 and 25, 8 of 131072
+// 45 and 85).
+__global__ void __launch_bounds__(kCutThreads) k_kv_least(const KVPool p, const Cut a) {
+    __shared__ uint2 sh[kCutWaves];
+    const int tid = threadIdx.x;
+    uint32_t bh, b, h, L;
+    if (!long_row(p, a, bh, b, h, L)) return;
+    const size_t chunk = (size_t)bh * a.chunks + blockIdx.x;
+    const uint32_t steps = (1u << a.log) / kCutThreads, mine = (tid & ~63) * steps + (tid & 63);
+    Ranks ranks(p, a, b, h, L, (blockIdx.x << a.log) + mine);
+    Least least;
+#pragma unroll 1
+    for (uint32_t i = 0; i < steps; i += 4) {
+        const uint32_t t = ranks.t;
+        uint32_t q[4];
+        ranks.next<4>(q);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (t + 64 * u < L) least.add(q[u], t + 64 * u);
+    }
+    const bool gone = __syncthreads_or(ranks.gone);
+    least.of_group(sh, kCutWaves);
+    if (tid == 0) {
+        a.least[chunk] = make_uint2(least.key, least.slot);
+        a.absent[chunk] = gone;
+    }
+}
+__global__ void __launch_bounds__(kCutThreads) k_kv_drop(const KVPool p, const Cut a) {
+    __shared__ uint2 sh[kCutWaves];
+    __shared__ uint32_t list[2];
+    ask_for(p.tables, p.heads, a.budget, a.absent);
+    const uint32_t tid = threadIdx.x, bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads;
+    const uint32_t L = kv_length(a.lengths, b, a.max_length), chunks = chunks_of(L, a.log);
+    const bool gone = L > a.budget && row_absent(a, bh, chunks);
+    if (tid == 0 && h == 0 && a.new_lengths) a.new_lengths[b] = (int32_t)(L > a.budget && !gone ? a.budget : L);
+    if (L <= a.budget || gone) return;
+    Least least;
+    for (uint32_t c = tid; c < chunks; c += kCutThreads) {
+        const uint2 v = a.least[(size_t)bh * a.chunks + c];
+        least.add(v.x, v.y);
+    }
+    least.of_group(sh, kCutWaves);
+    if (least.slot == a.budget) return;
+    if (tid == 0) {
+        list[0] = least.slot;
+        list[1] = a.budget;
+    }
+    __syncthreads();
+    move_rows<1>(p, b, h, a.row_bytes, list, list + 1, 1, tid, kCutThreads);
 }
 
 __global__ void __launch_bounds__(kCutThreads) k_kv_rank(const KVPool p, const Cut a) {
@@ -792,6 +886,7 @@ size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, s
     const size_t most = most_moves(max_length, budget), bh = rows * c->kv_heads;
     if (is_long(max_length, most)) {
         const uint32_t log = chunk_log(bh, max_length);
+        if (max_length - budget == 1) return bh * chunks_of((uint32_t)max_length, log) * (sizeof(uint2) + sizeof(uint32_t));
         const size_t chunk = ((2u << log) + kBins / 2 + 1) * sizeof(uint32_t) + sizeof(Chunk);
         return bh * (chunks_of((uint32_t)max_length, log) * chunk + (1 + 2 * most) * sizeof(uint32_t));
     }
@@ -803,7 +898,7 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
                    size_t recent, void* ws, void* st) {
     const KVPool p = kv_pool(c, tables, width);
     const size_t bh = rows * c->kv_heads;
-    Cut a;
+    Cut a = {};
     a.lengths = lengths;
     a.next_pos = next_pos;
     a.new_lengths = new_lengths;
@@ -818,6 +913,15 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
         a.log = chunk_log(bh, max_length);
         a.chunks = chunks_of(a.max_length, a.log);
         const size_t all = bh * a.chunks;
+        const dim3 grid(a.chunks, (unsigned)(bh < 65535 ? bh : 65535), (unsigned)((bh + 65534) / 65535));
+        if (max_length - budget == 1) {
+            a.least = static_cast<uint2*>(ws);
+            a.absent = reinterpret_cast<uint32_t*>(a.least + all);
+            k_kv_least<<<grid, kCutThreads, 0, s>>>(p, a);
+            if (snx_launch_check("k_kv_least")) return -1;
+            k_kv_drop<<<(unsigned)bh, kCutThreads, 0, s>>>(p, a);
+            return snx_launch_check("k_kv_drop");
+        }
         a.found = static_cast<Chunk*>(ws);
         a.keys = reinterpret_cast<uint32_t*>(a.found + all);
         a.cands = a.keys + (all << a.log);
@@ -825,7 +929,6 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
         a.absent = a.firsts + all * (kBins / 2);
         a.counts = a.absent + all;
         a.moves = a.counts + bh;
-        const dim3 grid(a.chunks, (unsigned)(bh < 65535 ? bh : 65535), (unsigned)((bh + 65534) / 65535));
         k_kv_rank<<<grid, kCutThreads, 0, s>>>(p, a);
         if (snx_launch_check("k_kv_rank")) return -1;
         k_kv_part<<<grid, kCutThreads, 0, s>>>(p, a);

@@ -252,6 +252,27 @@ def test_evict_long_rows_of_many_heads(lib, lengths, heads, budget, weights):
     cut(lib, lengths, heads, 8, 64, "bf16", budget, 99, weights, seed=heads)
 
 
+@pytest.mark.parametrize("weights", [uniform, few_values, all_alike, odd_numbers])
+@pytest.mark.parametrize("lengths,heads,budget,page", [
+    ([2, 1, 0], 3, 1, 16),
+    ([600, 599, 3], 3, 599, 24),
+    ([17001, 17000, 400], 2, 17000, 64),
+    ([40001], 2, 40000, 7),
+])
+def test_evict_one_token_too_many(lib, lengths, heads, budget, page, weights):
+    print(f"[gpu] kv_evict one too many {lengths} {heads} {budget} {page} {weights.__name__}", flush=True)
+    cut(lib, lengths, heads, 16, page, "int8", budget, budget // 8, weights, seed=budget, most=budget + 1)
+
+
+def test_evict_one_token_too_many_of_many_heads(lib):
+    """Longer chunks, absent pages, all tokens recent."""
+    print("[gpu] kv_evict one too many, many heads", flush=True)
+    cut(lib, [17001, 16900], 150, 8, 64, "bf16", 17000, 1, few_values, seed=3, most=17001)
+    cut(lib, [17001, 17001], 2, 8, 64, "bf16", 17000, 0, uniform, seed=4, most=17001, absent=[(1, 100, -1)])
+    cut(lib, [17001, 17001], 2, 8, 64, "bf16", 17000, 17000, uniform, seed=4, most=17001,
+        positions=lambda rng, pos, tables: np.full_like(pos, 10 ** 6))
+
+
 def test_evict_long_rows_with_absent_pages(lib):
     print("[gpu] kv_evict long rows, absent pages", flush=True)
     cut(lib, [20000, 18000, 17000], 2, 16, 64, "bf16", 9000, 100, uniform, seed=8, absent=[(0, 200, -1), (2, 0, 1 << 29)])
