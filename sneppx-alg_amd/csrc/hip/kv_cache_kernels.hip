@@ -458,8 +458,8 @@ struct Least {
 
 // One workgroup per (row, head) of up to kLong slots.  A call runs through the code
 // about once, and its instructions one after the other are its time: the loops are
-// left rolled (16 x 8 of 2049: 8.4 us; unrolled, with keys in registers, twice the
-// code, 8.5).
+// left rolled (the threshold of 16 x 8 of 2049: 8.4 us; unrolled, with keys in
+// registers, twice the code, 8.5).
 // MOVE: with so few moves that the workgroup makes them at once.
 template <bool MOVE>
 __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cut a) {
@@ -479,8 +479,16 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
     bool gone = false;
     if (L > budget) {
         Ranks ranks(p, a, b, h, L, t0);
+        uint32_t i = 0;
 #pragma unroll 1
-        for (uint32_t i = 0; i < steps; i += 4) {
+        for (; i + 4 < steps; i += 8) {              // (by fours 8 x 8 of 16000 15.2 us, so 14.2)
+            uint32_t q[8];
+            ranks.next<8>(q);
+#pragma unroll
+            for (uint32_t u = 0; u < 8; u++)
+                if (i + u < steps) keys[t0 + 64 * (i + u)] = q[u];
+        }
+        if (i < steps) {
             uint32_t q[4];
             ranks.next<4>(q);
 #pragma unroll
@@ -535,15 +543,15 @@ __global__ void __launch_bounds__(kCutThreads) k_kv_cut(const KVPool p, const Cu
 }
 
 // ------------------------------------------------------------- of long rows
-// A workgroup has 4096 slots, up to 32768 where there are many, in three kernels: k_kv_rank counts their keys by
-// first digit; with all chunks' counts k_kv_part finds the threshold's and puts
-// the keys that share it apart; k_kv_list finds the threshold among these, and
-// where its own slots stand in the lists.  (us of a call that cuts so, and with one
-// workgroup for each row and head: 2 rows of 30001 and 8 heads 32 and 41, 4 of 60000
-// 70 and 113; 1 of 16384 30 and 30, of 12288 29 and 26, of 8192 27 and 21.  Every
-// workgroup adds up the counts of all
-// chunks: two tokens too many in 8 rows of 131072 take 83 us in chunks for two
-// workgroups a CU, 121 in 4096s; in 1 of 1000000 94 and 248.)
+// A workgroup has 4096 slots, up to 32768 where there are many, in three kernels:
+// k_kv_rank counts their keys by first digit; with all chunks' counts k_kv_part
+// finds the threshold's and puts the keys that share it apart; k_kv_list finds the
+// threshold among these, and where its own slots stand in the lists.  (us of a call
+// that cuts so, and with one workgroup for each row and head: 2 rows of 30001 and 8
+// heads 32 and 41, 4 of 60000 70 and 113; 1 of 16384 30 and 30, of 12288 29 and 26,
+// of 8192 27 and 21.  Every workgroup adds up the counts of all chunks: two tokens
+// too many in 8 rows of 131072 take 83 us in chunks for two workgroups a CU, 121 in
+// 4096s; in 1 of 1000000 94 and 248.)
 __device__ __forceinline__ bool long_row(const KVPool& p, const Cut& a, uint32_t& bh, uint32_t& b, uint32_t& h, uint32_t& L) {
     ask_for(p.tables, p.heads, a.counts, a.absent);
     bh = blockIdx.y + blockIdx.z * 65535u;
