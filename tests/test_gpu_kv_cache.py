@@ -341,3 +341,40 @@ def test_evict_in_a_graph(lib):
         assert new.tolist() == [budget] * rows
     lib.graph_destroy(rec)
     lib.fn["SNEPPX_qlinear_release_workspaces"](st.cuda_stream)
+
+
+@pytest.mark.parametrize("budget", [9000, 17000])
+def test_evict_long_rows_in_a_graph(lib, budget):
+    """Rows that several workgroups cut, and one token too many of them, recorded:
+    the lengths are those of each replay."""
+    print(f"[gpu] kv_evict long rows graph {budget}", flush=True)
+    rows, L, wide = 2, 17001, 266
+    c = lib.kv_cache(rows * wide, 64, 2, 16, weights=True, positions=True)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    tab = torch.randperm(rows * wide, device=DEV, generator=g).to(torch.int32).view(rows, wide)
+    planes = (c.k, c.v, c.weights, c.positions)
+    for t in planes[:3]:
+        t.copy_(torch.rand(t.shape, device=DEV, generator=g))
+    dlen = torch.full((rows,), L, dtype=torch.int32, device=DEV)
+    new = torch.zeros_like(dlen)
+    before = [t.clone() for t in planes]
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    call = lambda: c.evict(tab, dlen, dlen, new, L, budget, 40, stream=st.cuda_stream)   # noqa: E731
+    rec = lib.capture(call, stream=st.cuda_stream)
+    for i, lengths in enumerate(([L, L], [budget, L], [L, 300], [L, L])):
+        dlen.copy_(torch.tensor(lengths, dtype=torch.int32))
+        results = []
+        for run in (call, lambda: lib.graph_launch(rec, stream=st.cuda_stream)):
+            for t, x in zip(planes, before):
+                t.copy_(x)
+            new.zero_()
+            torch.cuda.synchronize()
+            run()
+            st.synchronize()
+            results.append([bits(t).copy() for t in planes] + [new.cpu().numpy().copy()])
+        for x, y in zip(*results):
+            assert np.array_equal(x, y), i
+        assert results[1][-1].tolist() == [min(n, budget) for n in lengths]
+    lib.graph_destroy(rec)
+    lib.fn["SNEPPX_qlinear_release_workspaces"](st.cuda_stream)
