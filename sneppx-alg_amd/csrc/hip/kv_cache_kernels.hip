@@ -882,7 +882,13 @@ int snx_k_kv_append(const SNEPPXKVCache* c, const uint16_t* k, size_t k_stride, 
     return snx_launch_check("k_kv_append");
 }
 
-static bool is_long(size_t max_length, size_t most) { return most && max_length > kLong; }
+// Pages of a few tokens scatter a row's keys, which takes a CU longer (us by one
+// workgroup a row and head / by several, 3 rows of 14899 and 12 heads cut to 5598:
+// pages of 1 87 / 63, of 4 54 / 49, of 8 46 / 46, of 16 40 / 42; 2 of 8000 and 8 heads
+// halved, pages of 1: 37 / 38).
+static bool is_long(size_t max_length, size_t most, size_t page_size) {
+    return most && max_length > (page_size < 8 ? kLong / 2 : kLong);
+}
 // log2 of a chunk's slots: no more workgroups than two for a CU, if that is few slots
 static uint32_t chunk_log(size_t bh, size_t max_length) {
     uint32_t log = kLogChunk;
@@ -892,7 +898,7 @@ static uint32_t chunk_log(size_t bh, size_t max_length) {
 
 size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, size_t budget) {
     const size_t most = most_moves(max_length, budget), bh = rows * c->kv_heads;
-    if (is_long(max_length, most)) {
+    if (is_long(max_length, most, c->page_size)) {
         const uint32_t log = chunk_log(bh, max_length);
         if (max_length - budget == 1) return bh * chunks_of((uint32_t)max_length, log) * (sizeof(uint2) + sizeof(uint32_t));
         const size_t chunk = ((2u << log) + kBins / 2 + 1) * sizeof(uint32_t) + sizeof(Chunk);
@@ -917,7 +923,7 @@ int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, 
     a.row_bytes = (uint32_t)(c->head_dim * (c->dtype == SNEPPX_INT8 ? 1 : 2));
     a.rows = (uint32_t)rows;
     const hipStream_t s = S(st);
-    if (is_long(max_length, a.most)) {
+    if (is_long(max_length, a.most, c->page_size)) {
         a.log = chunk_log(bh, max_length);
         a.chunks = chunks_of(a.max_length, a.log);
         const size_t all = bh * a.chunks;

@@ -273,6 +273,12 @@ def test_evict_one_token_too_many_of_many_heads(lib):
         positions=lambda rng, pos, tables: np.full_like(pos, 10 ** 6))
 
 
+@pytest.mark.parametrize("length,budget,page", [(8193, 4096, 1), (9000, 8999, 3), (8200, 4100, 7), (8192, 8000, 2)])
+def test_evict_long_rows_in_small_pages(lib, length, budget, page):
+    print(f"[gpu] kv_evict small pages {length} {budget} {page}", flush=True)
+    cut(lib, [length, length - 200], 3, 16, page, "int8", budget, budget // 9, few_values, seed=length)
+
+
 def test_evict_long_rows_with_absent_pages(lib):
     print("[gpu] kv_evict long rows, absent pages", flush=True)
     cut(lib, [20000, 18000, 17000], 2, 16, 64, "bf16", 9000, 100, uniform, seed=8, absent=[(0, 200, -1), (2, 0, 1 << 29)])
