@@ -73,7 +73,7 @@ struct Attn {
     float2* ml;               // [2 * shares][kv_heads * tiles][heads]: maximum, sum
     float* logits;            // [rows][q_heads][logit_stride], or NULL
     float2* whole;            // with logits, [rows][q_heads] of rows in one share: maximum, 1 / sum
-    uint32_t rows, q_heads, max_length, tiles, heads, shares, logit_stride;
+    uint32_t rows, q_heads, max_length, tiles, heads, shares, few, logit_stride;
     Divider by_eights, by_heads, by_shares;      // by 8 tiles, kv_heads and shares
     float scale_log2;
     int out_f32;
@@ -120,7 +120,10 @@ struct Shares {
 };
 constexpr uint32_t kMostShares = 256;     // of a row
 
-constexpr uint32_t kFewSteps = 4;         // of a share
+// Steps of a share that are few: with one workgroup to a CU what passes a round waits
+// for whole shares (19 rows of 653, heads of 256 in bf16, 4 steps a share: by rows 45
+// us, across rows 27; 40 of 0 to 500, 3 steps, 33 and 25).
+constexpr uint32_t few_steps(int of_cu) { return of_cu > 1 ? 4 : 2; }
 
 struct Division {
     const Attn& a;
@@ -143,7 +146,7 @@ struct Division {
             per = per > least ? per : least;
         }
         by = By(per);
-        by_row = per <= kFewSteps;
+        by_row = per <= a.few;
         if (!by_row && a.rows <= 64)
             by_row = (uint32_t)__builtin_amdgcn_readlane(lane_prefix(by(steps(lane, len0) + per - 1)), 63) <= a.shares;
     }
@@ -772,12 +775,12 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     const size_t heads = group < 16 ? group : 16;
     // As many shares as the CUs hold workgroups at once; where rows begin shares, one
     // more for each row, but a row has a step at least, and they are up to
-    // kFewSteps for each share then.  No more than there are steps.
+    // few_steps for each share then.  No more than there are steps.
     const size_t steps = (max_length + STEP - 1) / STEP;
     const int of_cu = shares_of_cu(padded(c->head_dim), c->dtype == SNEPPX_INT8);
     const size_t shares = ((size_t)of_cu * cu_count() + units - 1) / units;
     size_t blocks = shares + rows;
-    if (blocks > kFewSteps * shares) blocks = kFewSteps * shares;
+    if (blocks > few_steps(of_cu) * shares) blocks = few_steps(of_cu) * shares;
     if (blocks > rows * (steps ? steps : 1)) blocks = rows * (steps ? steps : 1);
     blocks = (blocks * c->kv_heads + 7) / 8 * 8 * tiles;
     const size_t part = 2 * blocks * heads * c->head_dim * sizeof(float), ml = 2 * blocks * heads * sizeof(float2);
@@ -822,6 +825,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.by_heads = divider(c->kv_heads);
     a.by_shares = divider(shares);
     a.shares = (uint32_t)shares;
+    a.few = few_steps(of_cu);
     a.logit_stride = (uint32_t)logit_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.out_f32 = out_f32;

@@ -150,6 +150,8 @@ def test_division_of_rows(lib, lengths, heads, dim, dtype):
     ([1990] * 4, 64, 24, "bf16"),
     ([7000, 6700], 64, 16, "int8"),
     ([3000, 900, 2100], 33, 8, "bf16"),
+    ([653] * 5, 32, 256, "bf16"),                # one workgroup to a CU: across rows from three steps a share on
+    ([500, 20, 0, 333, 480, 77, 129], 32, 256, "bf16"),
 ])
 def test_division_of_rows_in_as_many_shares(lib, lengths, heads, dim, dtype):
     """Long shares: rows begin them where no more are needed for it."""
