@@ -73,7 +73,8 @@ struct Attn {
     float2* ml;               // [2 * shares][kv_heads * tiles][heads]: maximum, sum
     float* logits;            // [rows][q_heads][logit_stride], or NULL
     float2* whole;            // with logits, [rows][q_heads] of rows in one share: maximum, 1 / sum
-    uint32_t rows, q_heads, max_length, tiles, heads, shares, few, logit_stride;
+    uint32_t rows, q_heads, max_length, tiles, heads, logit_stride;
+    uint32_t shares, about_shares;    // shares, and what is about as many
     Divider by_eights, by_heads, by_shares;      // by 8 tiles, kv_heads and shares
     float scale_log2;
     int out_f32;
@@ -83,13 +84,17 @@ struct Attn {
 // All rows' steps (one at least for each row), one row after the other, are cut
 // into equal shares; a workgroup takes one, with the end of a row, whole rows
 // and the beginning of another in it, and so all end together.  Where a share is
-// only a few steps, or as many shares are enough so, changing the row costs more
-// than that evens out, and every row begins with a new share.  The lengths are
-// known on the device alone, so every wave works this out for itself.  (us of
-// shares across rows / by rows, 8 heads of 128 in bf16: 16 rows of 0 to 4096
-// tokens, 4 steps a share, 32 / 28; 24 rows, 6 steps, 46 / 54; 64 rows, 16 steps,
-// 100 / 118; 16 of 2049, 5 steps, as many shares, 33 / 30.  A grid for the longest
-// row that the host allows for leaves most of it idle: 45 for the first.)
+// one or two steps, or rows need about as many shares if each begins one (up to an
+// eighth more of three or four steps, for which CUs of two workgroups even out what
+// passes a round, no more of longer ones), changing the row costs more than that
+// evens out, and every row begins with a new share.  The lengths are known on the
+// device alone, so every wave works this out for itself.  (us of shares across rows
+// / by rows, 8 heads of 128 in bf16: 16 rows of 0 to 4096 tokens, 4 steps, 66 shares
+// for 64, 32 / 28; 38 of 653, 4 steps, 76 shares, 24 / 33; 64 of 0 to 700, 4 steps,
+// 80 shares, 28 / 26; 16 of 2049, 5 steps, 64 shares, 33 / 30; 24 of 0 to 4096, 6
+// steps, 74 shares, 46 / 54; 64 of 0 to 8192, 16 steps, 100 / 118; heads of 256, one
+// workgroup to a CU: 19 of 653, 4 steps, 38 shares for 32, 27 / 45.  A grid for the
+// longest row that the host allows for leaves most of it idle: 45 for the first.)
 struct Row {
     uint32_t b, at, len;           // the row, its first step, its length in tokens
     __device__ __forceinline__ uint32_t steps() const { return len > STEP ? (len + STEP - 1) / STEP : 1; }
@@ -120,10 +125,7 @@ struct Shares {
 };
 constexpr uint32_t kMostShares = 256;     // of a row
 
-// Steps of a share that are few: with one workgroup to a CU what passes a round waits
-// for whole shares (19 rows of 653, heads of 256 in bf16, 4 steps a share: by rows 45
-// us, across rows 27; 40 of 0 to 500, 3 steps, 33 and 25).
-constexpr uint32_t few_steps(int of_cu) { return of_cu > 1 ? 4 : 2; }
+constexpr uint32_t kFewSteps = 2;         // of a share
 
 struct Division {
     const Attn& a;
@@ -146,9 +148,11 @@ struct Division {
             per = per > least ? per : least;
         }
         by = By(per);
-        by_row = per <= a.few;
-        if (!by_row && a.rows <= 64)
-            by_row = (uint32_t)__builtin_amdgcn_readlane(lane_prefix(by(steps(lane, len0) + per - 1)), 63) <= a.shares;
+        by_row = per <= kFewSteps;
+        if (!by_row && a.rows <= 64) {
+            const uint32_t n = last_lane(lane_prefix(by(steps(lane, len0) + per - 1)));
+            by_row = n <= (per <= 2 * kFewSteps ? a.about_shares : a.shares);
+        }
     }
     __device__ __forceinline__ uint32_t length(uint32_t r) const {
         return r < a.rows ? kv_length(a.lengths, r, a.max_length) : 0;
@@ -775,12 +779,12 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     const size_t heads = group < 16 ? group : 16;
     // As many shares as the CUs hold workgroups at once; where rows begin shares, one
     // more for each row, but a row has a step at least, and they are up to
-    // few_steps for each share then.  No more than there are steps.
+    // kFewSteps for each share then.  No more than there are steps.
     const size_t steps = (max_length + STEP - 1) / STEP;
     const int of_cu = shares_of_cu(padded(c->head_dim), c->dtype == SNEPPX_INT8);
     const size_t shares = ((size_t)of_cu * cu_count() + units - 1) / units;
     size_t blocks = shares + rows;
-    if (blocks > few_steps(of_cu) * shares) blocks = few_steps(of_cu) * shares;
+    if (blocks > kFewSteps * shares) blocks = kFewSteps * shares;
     if (blocks > rows * (steps ? steps : 1)) blocks = rows * (steps ? steps : 1);
     blocks = (blocks * c->kv_heads + 7) / 8 * 8 * tiles;
     const size_t part = 2 * blocks * heads * c->head_dim * sizeof(float), ml = 2 * blocks * heads * sizeof(float2);
@@ -825,7 +829,7 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.by_heads = divider(c->kv_heads);
     a.by_shares = divider(shares);
     a.shares = (uint32_t)shares;
-    a.few = few_steps(of_cu);
+    a.about_shares = (uint32_t)(of_cu > 1 ? shares + shares / 8 : shares);
     a.logit_stride = (uint32_t)logit_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.out_f32 = out_f32;
