@@ -225,19 +225,26 @@ __device__ __forceinline__ bf16x8 bytes_to_bf16(uint32_t a, uint32_t b) {
 
 // Eight weights (not negative) as three bf16 pieces each, exactly (24 significant
 // bits cut into 8 + 8 + 8): the products with bf16 values then sum as fp32 ones
-// would.  The second and third are 2^-126 at least: a zero among them would make
-// NaN of an infinite value.
+// would.  bf16 values may be infinite, and a zero second or third piece would make
+// NaN of that: they are 2^-40 of the first at least (and normal), which no sum
+// shows, but zero where the weight is zero, so that a token of no weight adds
+// nothing to any value.  Of int8 the codes are finite; where the weight is not (an
+// infinite scale) it is all in the first piece.
+template <bool I8>
 __device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&piece)[3]) {
     u32x4 o[3];
-    const float least = u2f(0x00800000u);
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-        float a = x[e], b = x[e + 1];
+        float a[2] = {x[e], x[e + 1]}, least[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 3; i++) {
-            o[i][e >> 1] = __builtin_amdgcn_perm(f2u(b), f2u(a), 0x07060302u);
-            a = fmaxf(a - u2f(f2u(a) & 0xFFFF0000u), least);
-            b = fmaxf(b - u2f(f2u(b) & 0xFFFF0000u), least);
+            o[i][e >> 1] = __builtin_amdgcn_perm(f2u(a[1]), f2u(a[0]), 0x07060302u);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float high = u2f(f2u(a[j]) & 0xFFFF0000u);
+                if (!I8 && i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
+                a[j] = fmaxf(a[j] - high, least[j]);
+            }
         }
     }
 #pragma unroll
@@ -601,7 +608,7 @@ k_kv_attn(const KVPool p, const Attn a) {
                 if (I8) e[i] *= sc[TILE + 8 * g + i];
             }
             bf16x8 pc[3];
-            split3(e, pc);
+            split3<I8>(e, pc);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
