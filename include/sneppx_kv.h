@@ -10,7 +10,8 @@
  * projection reads.  As there, every pointer is a DEVICE pointer (the cache
  * descriptor itself is a host struct, read during the call), every call is
  * asynchronous on `stream`, allocates no output, and returns 0, or -1 with the
- * reason in SNEPPX_qlinear_last_error().
+ * reason in SNEPPX_qlinear_last_error().  A call of no rows or no tokens does
+ * nothing and returns 0; pointers to what is empty may be NULL then.
  *
  * The pool: pages of page_size tokens each, k and v [pages][kv_heads]
  * [page_size][head_dim], so that a head's tokens of one page lie together.

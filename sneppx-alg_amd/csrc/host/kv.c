@@ -42,8 +42,10 @@ static int cache_ok(const char* who, const SNEPPXKVCache* c) {
     return 0;
 }
 
+/* (of no rows nothing is read, and what holds nothing need not have an address) */
 static int rows_ok(const char* who, const SNEPPXKVCache* c, const int32_t* tables, size_t width,
                    const int32_t* lengths, size_t rows) {
+    if (!rows) return 0;
     REQUIRE(tables && lengths, "%s: NULL block_tables or lengths", who);
     REQUIRE(width, "%s: empty block_tables", who);
     REQUIRE(width <= MAX_SLOTS / c->page_size, "%s: table_width %zu * page_size %zu is too large", who, width,
@@ -58,16 +60,17 @@ int SNEPPX_kv_append(const SNEPPXKVCache* cache, const uint16_t* k, size_t k_str
                      const int32_t* lengths, const int32_t* next_pos, size_t rows, SNEPPXStream stream) {
     static const char who[] = "kv_append";
     if (cache_ok(who, cache) || rows_ok(who, cache, block_tables, table_width, lengths, rows)) return -1;
-    REQUIRE(k && v, "kv_append: NULL pointer");
+    const int none = !tokens || !rows;
+    REQUIRE(none || (k && v), "kv_append: NULL pointer");
     REQUIRE(!k_stored == !v_stored, "kv_append: k_stored and v_stored go together");
-    REQUIRE(!cache->positions || next_pos, "kv_append: a cache with positions needs next_pos");
+    REQUIRE(none || !cache->positions || next_pos, "kv_append: a cache with positions needs next_pos");
     REQUIRE(starts || tokens == rows, "kv_append: %zu tokens for %zu rows without starts", tokens, rows);
     REQUIRE(tokens <= MAX_SLOTS, "kv_append: %zu tokens are too many", tokens);
     const size_t n = cache->kv_heads * cache->head_dim;
     REQUIRE(tokens < 2 || (k_stride >= n && v_stride >= n), "kv_append: strides %zu, %zu are below kv_heads * head_dim = %zu",
             k_stride, v_stride, n);
     snx_clear_error();
-    if (!tokens || !rows) return 0;
+    if (none) return 0;
     return snx_k_kv_append(cache, k, k_stride, v, v_stride, tokens, starts, k_stored, v_stored, block_tables, table_width,
                            lengths, next_pos, rows, stream);
 }
@@ -78,7 +81,7 @@ int SNEPPX_kv_attention(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_
                         size_t max_length, float scale, int accumulate, SNEPPXStream stream) {
     static const char who[] = "kv_attention";
     if (cache_ok(who, cache) || rows_ok(who, cache, block_tables, table_width, lengths, rows)) return -1;
-    REQUIRE(q && out, "kv_attention: NULL pointer");
+    REQUIRE(!rows || (q && out), "kv_attention: NULL pointer");
     REQUIRE(out_dtype == SNEPPX_BFLOAT16 || out_dtype == SNEPPX_FLOAT32, "kv_attention: out_dtype %d is neither bf16 nor fp32",
             (int)out_dtype);
     REQUIRE(q_heads && q_heads % cache->kv_heads == 0 && q_heads <= 65535,
@@ -100,11 +103,11 @@ int SNEPPX_kv_evict(const SNEPPXKVCache* cache, const int32_t* block_tables, siz
                     size_t max_length, size_t budget, size_t recent, SNEPPXStream stream) {
     static const char who[] = "kv_evict";
     if (cache_ok(who, cache) || rows_ok(who, cache, block_tables, table_width, lengths, rows)) return -1;
-    REQUIRE(next_pos, "kv_evict: NULL next_pos");
+    REQUIRE(!rows || next_pos, "kv_evict: NULL next_pos");
     REQUIRE(cache->weights && cache->positions, "kv_evict: needs the cache's weights and positions");
     REQUIRE(budget, "kv_evict: budget == 0");
     REQUIRE(recent <= budget, "kv_evict: recent %zu is beyond the budget %zu", recent, budget);
-    REQUIRE(new_lengths != lengths, "kv_evict: new_lengths must not be lengths");
+    REQUIRE(!rows || new_lengths != lengths, "kv_evict: new_lengths must not be lengths");
     snx_clear_error();
     if (!rows) return 0;
     const size_t slots = table_width * cache->page_size;
