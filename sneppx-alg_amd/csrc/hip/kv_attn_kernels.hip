@@ -50,6 +50,7 @@ hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 constexpr int SLOT_KV_ATTN = 7;       // of the stream's workspaces
 constexpr int TILE = 32;              // tokens of a wave's step
 constexpr int WAVES = 4;
+constexpr int kLag = 8;               // log2 of how far a logit may pass the maximum that weights refer to
 constexpr int STEP = TILE * WAVES;    // tokens of a workgroup's step
 
 // Waves of a SIMD that the registers allow with heads padded to `dim`: of a tile's
@@ -72,11 +73,12 @@ struct Attn {
     float* part;              // [2 * shares][kv_heads * tiles][heads][dim]
     float2* ml;               // [2 * shares][kv_heads * tiles][heads]: maximum, sum
     float* logits;            // [rows][q_heads][logit_stride], or NULL
-    float2* whole;            // with logits, [rows][q_heads] of rows in one share: maximum, 1 / sum
+    float2* whole;            // with logits, [rows][q_heads] of rows in one share: maximum, 1 / sum (as Parts::whole)
     uint32_t rows, q_heads, max_length, tiles, heads, logit_stride;
     uint32_t shares, about_shares;    // shares, and what is about as many
     Divider by_eights, by_heads, by_shares;      // by 8 tiles, kv_heads and shares
     float scale_log2;
+    float room;               // log2 of the most that a row's weights of up to 2^kLag sum up to
     int out_f32;
 };
 
@@ -318,7 +320,7 @@ struct Parts {
         }
         return x;
     }
-    // Their maximum and 1 / sum, by one wave: 0 for no tokens, NaN where there are
+    // Their maximum and 1 / sum (of weights of 2^-room), by one wave: 0 for no tokens, NaN where there are
     // tokens and every logit is -inf; to `factors` each share's weight.
     __device__ __forceinline__ float2 whole(const Ends& x, const Shares& w, float* factors) const {
         const uint32_t lane = threadIdx.x & 63;
@@ -590,9 +592,12 @@ k_kv_attn(const KVPool p, const Attn a) {
             }
             any |= (t0 | t1) != 0;
             top = quad_max(top);
-            // The reference point moves only when a logit passes it by 8 (weights
-            // up to 2^8 are no harm): after the first tile hardly ever.
-            if (__any(top > m + 8.0f)) {
+            // The reference point moves only when a logit passes it by kLag: after the
+            // first tile hardly ever.  Weights are taken 2^-room of what they are, so
+            // that they sum up to 1 at most, however many are 2^kLag: a sum of weighted
+            // values is no larger than the largest value then, and finite if that is.
+            // (The joins divide by the sum of the same weights.)
+            if (__any(top > m + (float)kLag)) {
                 const float to = fmaxf(m, top);
                 const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
                 m = to;
@@ -603,7 +608,7 @@ k_kv_attn(const KVPool p, const Attn a) {
             const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                e[i] = __builtin_amdgcn_exp2f(e[i] - ref);
+                e[i] = __builtin_amdgcn_exp2f((e[i] - ref) - a.room);
                 sum += e[i];
                 if (I8) e[i] *= sc[TILE + 8 * g + i];
             }
@@ -739,7 +744,8 @@ __global__ void __launch_bounds__(256) k_kv_join(const KVPool p, const Attn a, u
             const Parts pt = parts(j0 + j);
             const float2 st = w.n == 1 ? a.whole[(size_t)b * a.q_heads + h * group + j0 + j]
                                        : pt.whole(pt.ends(w, (j0 + j) % 16), w, nullptr);
-            if (lane == 0) stat[j] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y);
+            // (the sum is of weights of 2^-room)
+            if (lane == 0) stat[j] = make_float2(st.x == -INFINITY ? 0.0f : st.x, st.y * __builtin_amdgcn_exp2f(-a.room));
         }
         __syncthreads();
         for (uint32_t j1 = 0; j1 < nj; j1 += G) {
@@ -839,6 +845,9 @@ int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_strid
     a.about_shares = (uint32_t)(of_cu > 1 ? shares + shares / 8 : shares);
     a.logit_stride = (uint32_t)logit_stride;
     a.scale_log2 = scale * 1.44269504088896340736f;
+    uint32_t room = kLag;
+    while (((size_t)1 << (room - kLag)) < max_length) room++;
+    a.room = (float)room;
     a.out_f32 = out_f32;
     if (c->dtype == SNEPPX_INT8) launch<true>((unsigned)blocks, accumulate != 0, p, a, S(st));
     else launch<false>((unsigned)blocks, accumulate != 0, p, a, S(st));
