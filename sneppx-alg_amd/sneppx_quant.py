@@ -808,7 +808,7 @@ class KVCache:
     def __init__(self, lib, k, v, k_scales=None, v_scales=None, weights=None, positions=None):
         if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in (torch.bfloat16, torch.int8):
             raise ValueError("k must be a bf16 or int8 tensor [pages, kv_heads, page_size, head_dim]")
-        self.L, self.device = lib, k.device
+        self.L, self.device, self._on_gpu = lib, k.device, k.is_cuda
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         i8 = k.dtype == torch.int8
         planes = k.shape[:3]
@@ -832,6 +832,8 @@ class KVCache:
             lib.fn[f"SNEPPX_kv_{n}"] for n in ("append", "attention", "evict"))
 
     def _stream(self, stream):
+        if not self._on_gpu:
+            raise ValueError(f"the cache is on {self.device}: its calls run on a GPU")
         # torch's current stream as a number: current_stream() makes an object
         # of it, 2.8 us where this takes 0.2
         return stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device.index or 0)

@@ -1,0 +1,35 @@
+"""What the KVCache binding itself refuses and arranges, on CPU tensors: nothing
+reaches the device."""
+import pytest
+import torch
+
+import sneppx_quant as sq
+
+
+@pytest.fixture(scope="module")
+def L():
+    return sq.load()
+
+
+def i32(*s):
+    return torch.zeros(s, dtype=torch.int32)
+
+
+def bf(*s):
+    return torch.zeros(s, dtype=torch.bfloat16)
+
+
+def calls(c, stream=0, max_length=64, budget=10, recent=3):
+    """Calls whose arguments are right."""
+    tab, ln = i32(3, 4), i32(3)
+    return {"append": lambda: c.append(bf(3, 2, 64), bf(3, 2, 64), tab, ln, ln, stream=stream),
+            "attention": lambda: c.attention(bf(3, 8, 64), bf(3, 8, 64), tab, ln, max_length, stream=stream),
+            "evict": lambda: c.evict(tab, ln, ln, i32(3), max_length, budget, recent, stream=stream)}
+
+
+@pytest.mark.parametrize("call", ["append", "attention", "evict"])
+@pytest.mark.parametrize("stream", [None, 0])
+def test_a_cache_in_host_memory_runs_nothing(L, call, stream):
+    c = L.kv_cache(8, 16, 2, 64, weights=True, positions=True, device="cpu")
+    with pytest.raises(ValueError, match="on cpu"):
+        calls(c, stream)[call]()
