@@ -793,6 +793,15 @@ class _KVCacheStruct(C.Structure):
                 ("dtype", C.c_int), ("pages", _sz), ("page_size", _sz), ("kv_heads", _sz), ("head_dim", _sz)]
 
 
+_COUNTS = 1 << 63       # (ctypes passes a size_t on modulo 2^64)
+
+
+def _no_count(**counts):
+    for name, n in counts.items():
+        if not 0 <= n < _COUNTS:
+            raise ValueError(f"{name} must be a count, got {n!r}")
+
+
 _BF16, _BF16_OR_F32 = ((torch.bfloat16,), (torch.bfloat16, torch.float32)) if torch else ((), ())
 
 
@@ -896,6 +905,8 @@ class KVCache:
         tb, width, ln, n = self._tables(tables, lengths)
         if rows != n or out_rows != n:
             raise ValueError(f"q has {rows} rows and out {out_rows}, tables {n}")
+        if not 0 <= max_length < _COUNTS:
+            _no_count(max_length=max_length)
         self.L.check(self._attention(
             self._p, qp, qs, op, os_, SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, tb, width, ln,
             n, heads, max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate),
@@ -906,6 +917,8 @@ class KVCache:
         tb, width, ln, n = self._tables(tables, lengths)
         np_ = self._check(next_pos, "next_pos", torch.int32, (n,))
         nl = None if new_lengths is None else self._check(new_lengths, "new_lengths", torch.int32, (n,))
+        if not (0 <= max_length < _COUNTS and 0 <= budget < _COUNTS and 0 <= recent < _COUNTS):
+            _no_count(max_length=max_length, budget=budget, recent=recent)
         self.L.check(self._evict(self._p, tb, width, ln, np_, nl, n, max_length, budget, recent,
                                  self._stream(stream)), "kv_evict")
 

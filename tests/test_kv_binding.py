@@ -33,3 +33,17 @@ def test_a_cache_in_host_memory_runs_nothing(L, call, stream):
     c = L.kv_cache(8, 16, 2, 64, weights=True, positions=True, device="cpu")
     with pytest.raises(ValueError, match="on cpu"):
         calls(c, stream)[call]()
+
+
+@pytest.mark.parametrize("kw", [dict(max_length=-1), dict(max_length=1 << 64), dict(budget=-1), dict(budget=(1 << 64) + 10),
+                                dict(recent=-1), dict(recent=1 << 64)], ids=str)
+def test_numbers_that_are_no_counts(L, kw):
+    """Negative numbers and those that 64 bits do not hold (they would reach the library
+    as the largest ones, or as small ones)."""
+    c = L.kv_cache(8, 16, 2, 64, weights=True, positions=True, device="cpu")
+    name = next(iter(kw))
+    with pytest.raises(ValueError, match=f"{name} must be a count"):
+        calls(c, **kw)["evict"]()
+    if name == "max_length":
+        with pytest.raises(ValueError, match="max_length must be a count"):
+            calls(c, **kw)["attention"]()
