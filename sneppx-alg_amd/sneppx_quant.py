@@ -811,13 +811,13 @@ class KVCache:
     (fp32) and positions (int32) [pages, kv_heads, page_size].
 
     Calls take the rows' block tables (int32 [rows, width]) and lengths (int32
-    [rows], the call's new tokens included) on the device, and run on torch's
-    current stream unless one is given."""
+    [rows], the call's new tokens included) on the cache's device, and run there
+    on torch's current stream of that device unless one is given."""
 
     def __init__(self, lib, k, v, k_scales=None, v_scales=None, weights=None, positions=None):
         if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in (torch.bfloat16, torch.int8):
             raise ValueError("k must be a bf16 or int8 tensor [pages, kv_heads, page_size, head_dim]")
-        self.L, self.device, self._on_gpu = lib, k.device, k.is_cuda
+        self.L, self.device, self._index = lib, k.device, k.device.index if k.is_cuda else None
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         i8 = k.dtype == torch.int8
         planes = k.shape[:3]
@@ -841,11 +841,21 @@ class KVCache:
             lib.fn[f"SNEPPX_kv_{n}"] for n in ("append", "attention", "evict"))
 
     def _stream(self, stream):
-        if not self._on_gpu:
+        if self._index is None:
             raise ValueError(f"the cache is on {self.device}: its calls run on a GPU")
         # torch's current stream as a number: current_stream() makes an object
         # of it, 2.8 us where this takes 0.2
-        return stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device.index or 0)
+        return stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index)
+
+    def _run(self, what, fn, *args):
+        # (the library's workspaces and launches are the current device's)
+        if torch._C._cuda_getDevice() == self._index:
+            rc = fn(self._p, *args)
+        else:
+            with torch.cuda.device(self._index):
+                rc = fn(self._p, *args)
+        if rc:
+            self.L.check(rc, what)
 
     # (the checks are on the way of every call: few look-ups of a tensor's attributes,
     # which take 0.1 us each)
@@ -894,8 +904,8 @@ class KVCache:
         stored = tokens, heads, self.head_dim
         ko = None if k_stored is None else self._check(k_stored, "k_stored", torch.bfloat16, stored)
         vo = None if v_stored is None else self._check(v_stored, "v_stored", torch.bfloat16, stored)
-        self.L.check(self._append(self._p, kp, ks, vp, vs, tokens, st, ko, vo, tb, width, ln, np_, n,
-                                  self._stream(stream)), "kv_append")
+        self._run("kv_append", self._append, kp, ks, vp, vs, tokens, st, ko, vo, tb, width, ln, np_, n,
+                  self._stream(stream))
 
     def attention(self, q, out, tables, lengths, max_length, scale=None, accumulate=False, stream=None):
         """SNEPPX_kv_attention: q bf16 [rows, q_heads, head_dim], out the same
@@ -907,10 +917,9 @@ class KVCache:
             raise ValueError(f"q has {rows} rows and out {out_rows}, tables {n}")
         if not 0 <= max_length < _COUNTS:
             _no_count(max_length=max_length)
-        self.L.check(self._attention(
-            self._p, qp, qs, op, os_, SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, tb, width, ln,
-            n, heads, max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate),
-            self._stream(stream)), "kv_attention")
+        self._run("kv_attention", self._attention, qp, qs, op, os_,
+                  SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, tb, width, ln, n, heads, max_length,
+                  self.head_dim ** -0.5 if scale is None else scale, int(accumulate), self._stream(stream))
 
     def evict(self, tables, lengths, next_pos, new_lengths, max_length, budget, recent, stream=None):
         """SNEPPX_kv_evict; new_lengths int32 [rows] or None."""
@@ -919,8 +928,7 @@ class KVCache:
         nl = None if new_lengths is None else self._check(new_lengths, "new_lengths", torch.int32, (n,))
         if not (0 <= max_length < _COUNTS and 0 <= budget < _COUNTS and 0 <= recent < _COUNTS):
             _no_count(max_length=max_length, budget=budget, recent=recent)
-        self.L.check(self._evict(self._p, tb, width, ln, np_, nl, n, max_length, budget, recent,
-                                 self._stream(stream)), "kv_evict")
+        self._run("kv_evict", self._evict, tb, width, ln, np_, nl, n, max_length, budget, recent, self._stream(stream))
 
 
 class QLayer:

@@ -47,3 +47,31 @@ def test_numbers_that_are_no_counts(L, kw):
     if name == "max_length":
         with pytest.raises(ValueError, match="max_length must be a count"):
             calls(c, **kw)["attention"]()
+
+
+@pytest.mark.parametrize("call", ["append", "attention", "evict"])
+@pytest.mark.parametrize("stream", [None, 77])
+@pytest.mark.parametrize("current", [0, 1])
+def test_calls_run_on_the_caches_device(L, monkeypatch, call, stream, current):
+    """The library takes workspaces of the current device, which has to be the cache's
+    whichever it was before, and is that again afterwards.  (Devices by number alone.)"""
+    c = L.kv_cache(8, 16, 2, 64, weights=True, positions=True, device="cpu")
+    now, seen = [current], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *_):
+            now[0] = self.before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    c._index = 1
+    setattr(c, f"_{call}", lambda *args: seen.append((now[0], args[-1])) or 0)
+    calls(c, stream)[call]()
+    assert seen == [(1, 101 if stream is None else 77)] and now == [current]
