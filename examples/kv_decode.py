@@ -38,7 +38,7 @@ class AttentionBlock:
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=device)
         self.kept = torch.zeros_like(self.lengths)      # the eviction's lengths
         self.next_pos = torch.zeros_like(self.lengths)
-        self.longest = 0
+        self.held = [0] * rows                          # what lengths holds
         self.out = torch.empty((rows, q_heads, dim), dtype=torch.bfloat16, device=device)
         self.y = torch.empty((rows, hidden), dtype=torch.bfloat16, device=device)
 
@@ -58,33 +58,41 @@ class AttentionBlock:
         h, kv = self.q_heads, self.kv_heads
         return qkv.unflatten(1, (h + 2 * kv, self.dim)).split((h, kv, kv), 1)
 
+    def _grown(self, counts):
+        """The lengths with so many new tokens."""
+        held = [n + c for n, c in zip(self.held, counts)]
+        if max(held) > self.capacity:
+            raise ValueError(f"a row of {max(held)} tokens is beyond the capacity of {self.capacity}")
+        return held
+
     def prompt(self, x, counts):
         """The rows' prompts, one after the other in x [sum(counts), hidden], into
-        the cache (their own attention is not part of this example)."""
+        the cache behind what it holds (their own attention is not part of this
+        example, and so not of what an eviction ranks by: a prompt's tokens begin
+        with a sum of 0)."""
+        self.held = self._grown(counts)
         _, k, v = self.project(x)
         self.starts = torch.tensor([0] + list(counts), dtype=torch.int32).cumsum(0, dtype=torch.int32).to(x.device)
         n = torch.tensor(counts, dtype=torch.int32, device=x.device)
         self.lengths += n
         self.next_pos += n
-        self.longest = max(counts)
         self.cache.append(k, v, self.tables, self.lengths, self.next_pos, starts=self.starts)
 
     def step(self, x):
         """One new token per row, x [rows, hidden]; returns y [rows, hidden]."""
+        self.held = self._grown([1] * self.rows)
+        longest = max(self.held)
         q, k, v = self.project(x)
         self.lengths += 1
         self.next_pos += 1
-        self.longest += 1
-        if self.longest > self.capacity:
-            raise ValueError(f"a row of {self.longest} tokens is beyond the capacity of {self.capacity}")
         self.cache.append(k, v, self.tables, self.lengths, self.next_pos)
-        self.cache.attention(q, self.out, self.tables, self.lengths, self.longest, accumulate=True)
+        self.cache.attention(q, self.out, self.tables, self.lengths, longest, accumulate=True)
         qw, sc, qz = self.o_w
         self.lib.qlinear_w4a16(self.out.flatten(1), qw, sc, qz, None, sc.shape[1], self.y, 128)
-        if self.longest > self.budget:
-            self.cache.evict(self.tables, self.lengths, self.next_pos, self.kept, self.longest, self.budget, self.recent)
+        if longest > self.budget:
+            self.cache.evict(self.tables, self.lengths, self.next_pos, self.kept, longest, self.budget, self.recent)
             self.lengths, self.kept = self.kept, self.lengths
-            self.longest = min(self.longest, self.budget)
+            self.held = [min(n, self.budget) for n in self.held]
         return self.y
 
 
