@@ -102,3 +102,20 @@ def test_values_near_the_largest(lib, lengths, heads, accumulate, signs, dtype):
     for o in (torch.float32, torch.bfloat16):
         out = torch.empty(q.shape, dtype=o, device=DEV)
         compare(c, ref, tables, dtab, dlen, lengths, q, out, 1 / math.sqrt(64), accumulate=accumulate)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int8"])
+@pytest.mark.parametrize("lengths,heads", [([900, 130], 4), ([5000], 1), ([33000], 1)])
+def test_values_far_below_one(lib, lengths, heads, dtype):
+    """Values of 1e-20: as good in proportion as those near one."""
+    print(f"[gpu] kv_attention values far below one {lengths} {dtype}", flush=True)
+    c, ref, tables, dtab, dlen = build(lib, lengths, heads, 64, 16, dtype, 90 + heads, garbage=False)
+    if dtype == "int8":
+        c.v_scales.mul_(1e-20)
+        ref.vs[:] = c.v_scales.cpu().double().numpy()
+    else:
+        c.v.mul_(1e-20)
+        ref.v[:] = c.v.cpu().double().numpy()
+    q = torch.randn((len(lengths), 4 * heads, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(6)).to(torch.bfloat16)
+    out = torch.empty(q.shape, device=DEV)
+    compare(c, ref, tables, dtab, dlen, lengths, q, out, 1 / math.sqrt(64))
