@@ -92,9 +92,9 @@ int SNEPPX_kv_attention(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_
  * move, in order, into the slots below that are left free, in order, with
  * everything the cache has of them; the others stay where they are, so a step
  * that drops one token moves one.  Slots from the new length on keep what they
- * held.  new_lengths int32 [rows] (not `lengths` itself, or NULL): min(length,
- * budget).  A row with a page that is not there keeps its tokens and length.
- * cache->weights and cache->positions have to be there. */
+ * held.  new_lengths int32 [rows] (or NULL; not in the memory of `lengths` or
+ * `next_pos`): min(length, budget).  A row with a page that is not there keeps its
+ * tokens and length.  cache->weights and cache->positions have to be there. */
 int SNEPPX_kv_evict(const SNEPPXKVCache* cache, const int32_t* block_tables, size_t table_width,
                     const int32_t* lengths, const int32_t* next_pos, int32_t* new_lengths, size_t rows,
                     size_t max_length, size_t budget, size_t recent, SNEPPXStream stream);

@@ -24,6 +24,11 @@
 
 static int aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
+static int overlap(const int32_t* a, const int32_t* b, size_t n) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b, bytes = n * sizeof(int32_t);
+    return a && b && x < y + bytes && y < x + bytes;
+}
+
 static int cache_ok(const char* who, const SNEPPXKVCache* c) {
     REQUIRE(c, "%s: NULL cache", who);
     REQUIRE(c->k && c->v, "%s: NULL pointer in the cache", who);
@@ -107,7 +112,9 @@ int SNEPPX_kv_evict(const SNEPPXKVCache* cache, const int32_t* block_tables, siz
     REQUIRE(cache->weights && cache->positions, "kv_evict: needs the cache's weights and positions");
     REQUIRE(budget, "kv_evict: budget == 0");
     REQUIRE(recent <= budget, "kv_evict: recent %zu is beyond the budget %zu", recent, budget);
-    REQUIRE(!rows || new_lengths != lengths, "kv_evict: new_lengths must not be lengths");
+    /* (written by one head's workgroup while others still read) */
+    REQUIRE(!overlap(new_lengths, lengths, rows), "kv_evict: new_lengths must not be lengths, nor overlap them");
+    REQUIRE(!overlap(new_lengths, next_pos, rows), "kv_evict: new_lengths must not be next_pos, nor overlap it");
     snx_clear_error();
     if (!rows) return 0;
     const size_t slots = table_width * cache->page_size;
