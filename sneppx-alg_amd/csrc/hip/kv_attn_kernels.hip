@@ -55,7 +55,8 @@ constexpr int STEP = TILE * WAVES;    // tokens of a workgroup's step
 
 // Waves of a SIMD that the registers allow with heads padded to `dim`: of a tile's
 // keys, values, queries and outputs.  (bf16 heads of 128 at three spill some:
-// 131072 tokens 138 us, 98 at two.)
+// 131072 tokens 138 us, 98 at two.  What is taken spills in the forms for heads that
+// are no whole 64 or 128: ten registers in bf16 up to 64, two in int8 up to 64 and 128.)
 constexpr int resident(int dim, bool i8) { return dim <= 64 ? 4 : dim <= 128 ? (i8 ? 3 : 2) : i8 ? 2 : 1; }
 // Workgroups of a CU that a call is divided among, at most: us at 2 / 3 / 4 for
 // 131072 tokens of 128 in bf16 98 / 102 / 104, in int8 59 / 63 / 68, 64 rows of 0
@@ -97,6 +98,12 @@ struct Attn {
 // steps, 74 shares, 46 / 54; 64 of 0 to 8192, 16 steps, 100 / 118; heads of 256, one
 // workgroup to a CU: 19 of 653, 4 steps, 38 shares for 32, 27 / 45.  A grid for the
 // longest row that the host allows for leaves most of it idle: 45 for the first.)
+// Between 66 and 80 shares it is not their number alone that decides: the limit is
+// below 76, which by rows loses a third, and so gives away a twentieth at 80.  The
+// shares that rows need are counted with one row to a lane, so more than 64 rows of
+// three and more steps a share are always cut across, which costs some of them: 64 and
+// 65 rows of 4000 tokens and one key-value head 24.9 and 27.4 us, of 1000 and two heads
+// 16.0 and 21.3.
 struct Row {
     uint32_t b, at, len;           // the row, its first step, its length in tokens
     __device__ __forceinline__ uint32_t steps() const { return len > STEP ? (len + STEP - 1) / STEP : 1; }

@@ -166,7 +166,7 @@ constexpr int kCutThreads = 64 * kCutWaves;
 constexpr int kDigit = 11;               // digits of 11, 11 and 10 bits, from the top
 constexpr int kBins = 1 << kDigit;
 constexpr uint32_t kLogChunk = 12, kMostLog = 15;    // of the slots of a long row that a workgroup has
-constexpr size_t kLong = 16384;          // longer rows are cut by several workgroups
+constexpr size_t kLong = 16384;          // longer rows (half of it in small pages) are cut by several workgroups
 constexpr uint32_t kMoveAtOnce = 64;     // moves that the workgroup which finds them makes itself
 
 // a count per wave -> its exclusive prefix over the waves, and the total
@@ -456,7 +456,7 @@ struct Least {
     }
 };
 
-// One workgroup per (row, head) of up to kLong slots.  A call runs through the code
+// One workgroup per (row, head) of rows that are not long (see is_long).  A call runs through the code
 // about once, and its instructions one after the other are its time: the loops are
 // left rolled (the threshold of 16 x 8 of 2049: 8.4 us; unrolled, with keys in
 // registers, twice the code, 8.5).
@@ -890,6 +890,8 @@ static bool is_long(size_t max_length, size_t most, size_t page_size) {
     return most && max_length > (page_size < 8 ? kLong / 2 : kLong);
 }
 // log2 of a chunk's slots: no more workgroups than two for a CU, if that is few slots
+// (for k_kv_part and k_kv_list, which add up all chunks' counts; k_kv_least takes the
+// same chunks)
 static uint32_t chunk_log(size_t bh, size_t max_length) {
     uint32_t log = kLogChunk;
     while (log < kMostLog && bh * chunks_of((uint32_t)max_length, log) > 2 * (size_t)cu_count()) log++;
