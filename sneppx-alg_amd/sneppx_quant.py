@@ -840,22 +840,18 @@ class KVCache:
         self._append, self._attention, self._evict = (
             lib.fn[f"SNEPPX_kv_{n}"] for n in ("append", "attention", "evict"))
 
-    def _stream(self, stream):
+    # (the library's workspaces and launches are the current device's.  Asked in line, as
+    # is torch's current stream by its number: a function around every call takes 0.2 us,
+    # current_stream(), which makes an object, 2.8)
+    def _elsewhere(self, fn):
+        """fn on the cache's device, which is not the current one."""
         if self._index is None:
             raise ValueError(f"the cache is on {self.device}: its calls run on a GPU")
-        # torch's current stream as a number: current_stream() makes an object
-        # of it, 2.8 us where this takes 0.2
-        return stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index)
 
-    def _run(self, what, fn, *args):
-        # (the library's workspaces and launches are the current device's)
-        if torch._C._cuda_getDevice() == self._index:
-            rc = fn(self._p, *args)
-        else:
+        def run(*args):
             with torch.cuda.device(self._index):
-                rc = fn(self._p, *args)
-        if rc:
-            self.L.check(rc, what)
+                return fn(*args)
+        return run
 
     # (the checks are on the way of every call: few look-ups of a tensor's attributes,
     # which take 0.1 us each)
@@ -904,8 +900,12 @@ class KVCache:
         stored = tokens, heads, self.head_dim
         ko = None if k_stored is None else self._check(k_stored, "k_stored", torch.bfloat16, stored)
         vo = None if v_stored is None else self._check(v_stored, "v_stored", torch.bfloat16, stored)
-        self._run("kv_append", self._append, kp, ks, vp, vs, tokens, st, ko, vo, tb, width, ln, np_, n,
-                  self._stream(stream))
+        run = self._append if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._append)
+        rc = run(self._p, kp, ks, vp, vs, tokens, st, ko, vo, tb, width, ln, np_, n,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_append")
 
     def attention(self, q, out, tables, lengths, max_length, scale=None, accumulate=False, stream=None):
         """SNEPPX_kv_attention: q bf16 [rows, q_heads, head_dim], out the same
@@ -917,18 +917,27 @@ class KVCache:
             raise ValueError(f"q has {rows} rows and out {out_rows}, tables {n}")
         if not 0 <= max_length < _COUNTS:
             _no_count(max_length=max_length)
-        self._run("kv_attention", self._attention, qp, qs, op, os_,
-                  SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, tb, width, ln, n, heads, max_length,
-                  self.head_dim ** -0.5 if scale is None else scale, int(accumulate), self._stream(stream))
+        run = self._attention if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._attention)
+        rc = run(self._p, qp, qs, op, os_, SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, tb, width,
+                 ln, n, heads, max_length, self.head_dim ** -0.5 if scale is None else scale, int(accumulate),
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_attention")
 
     def evict(self, tables, lengths, next_pos, new_lengths, max_length, budget, recent, stream=None):
         """SNEPPX_kv_evict; new_lengths int32 [rows] or None."""
         tb, width, ln, n = self._tables(tables, lengths)
         np_ = self._check(next_pos, "next_pos", torch.int32, (n,))
         nl = None if new_lengths is None else self._check(new_lengths, "new_lengths", torch.int32, (n,))
-        if not (0 <= max_length < _COUNTS and 0 <= budget < _COUNTS and 0 <= recent < _COUNTS):
+        if not 0 <= max_length | budget | recent < _COUNTS:      # (the sign and high bits of any)
             _no_count(max_length=max_length, budget=budget, recent=recent)
-        self._run("kv_evict", self._evict, tb, width, ln, np_, nl, n, max_length, budget, recent, self._stream(stream))
+        run = self._evict if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._evict)
+        rc = run(self._p, tb, width, ln, np_, nl, n, max_length, budget, recent,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_evict")
 
 
 class QLayer:
