@@ -466,7 +466,7 @@ k_kv_attn(const KVPool p, const Attn a) {
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 const uint32_t tok = base + 8 * (r >> 2) + 4 * t + (r & 3);
-                entry[t] = tok < last ? (uint32_t)p.tables[(size_t)b * p.width + p.page_of(tok)] : 0xFFFFFFFFu;
+                entry[t] = tok < last ? (uint32_t)p.table(b, h)[p.page_of(tok)] : 0xFFFFFFFFu;
             }
         };
         auto find = [&](uint32_t base) {
@@ -792,9 +792,9 @@ void launch(unsigned grid, bool save, const KVPool& p, const Attn& a, hipStream_
 extern "C" {
 
 int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, void* out, size_t out_stride,
-                       int out_f32, const int32_t* tables, size_t width, const int32_t* lengths, size_t rows,
-                       size_t q_heads, size_t max_length, float scale, int accumulate, void* st) {
-    const KVPool p = kv_pool(c, tables, width);
+                       int out_f32, const int32_t* tables, size_t width, int of_heads, const int32_t* lengths,
+                       size_t rows, size_t q_heads, size_t max_length, float scale, int accumulate, void* st) {
+    const KVPool p = kv_pool(c, tables, width, of_heads != 0);
     const size_t group = q_heads / c->kv_heads, tiles = (group + 15) / 16, units = c->kv_heads * tiles;
     const size_t heads = group < 16 ? group : 16;
     // As many shares as the CUs hold workgroups at once; where rows begin shares, one

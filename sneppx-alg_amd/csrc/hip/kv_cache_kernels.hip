@@ -5,11 +5,11 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
-#include <cfloat>
 #include <cstdint>
 
 #include "codec.h"
 #include "kv_pool.h"
+#include "kv_rows.h"
 #include "launch.h"
 #include "../snx_internal.h"
 
@@ -18,21 +18,6 @@ using namespace snx;
 namespace {
 
 hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
-
-// max over non-NaN values, as the reference's `if (a > m) m = a`
-__device__ __forceinline__ float nanless_max(float a, float b) { return b > a ? b : a; }
-
-// of LR lanes, to all of them: exchanges of neighbours, pairs, halves of 8, of 16 and
-// of 32 lanes
-template <int LR>
-__device__ __forceinline__ float row_max(float m) {
-    m = nanless_max(m, lane_step<0xB1, 0xf>(m, m));
-    m = nanless_max(m, lane_step<0x4E, 0xf>(m, m));
-    m = nanless_max(m, lane_step<0x141, 0xf>(m, m));
-    if (LR >= 16) m = nanless_max(m, lane_step<0x140, 0xf>(m, m));
-    if (LR >= 32) m = nanless_max(m, __shfl_xor(m, 16));
-    return m;
-}
 
 // ------------------------------------------------------------------- append
 struct NewRows {
@@ -106,32 +91,15 @@ __global__ void __launch_bounds__(256) k_kv_append(const KVPool p, const NewRows
     if (slot < 0 || (uint32_t)slot >= n.slots || !p.row(b, h, (uint32_t)slot, r)) return;
 
     if (I8) {
-        float f[8], m = 0.0f;
+        float f[8];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             f[2 * e] = u2f(w[e] << 16);
             f[2 * e + 1] = u2f(w[e] & 0xFFFF0000u);
         }
-#pragma unroll
-        for (int e = 0; e < 8; e++) m = nanless_max(m, fabsf(f[e]));
-        m = row_max<LR>(m);
-        const float s = m < FLT_MIN ? 1.0f : m / 127.0f, inv = 1.0f / s;
-        // Numbers below 128 round half away by adding the number below 1/2 and
-        // cutting; what the rule gives for others (an infinity or NaN in the row, a
-        // scale whose reciprocal is infinite) takes the long way.
-        float all = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) all += fabsf(f[e]);
-        const bool plain = all < INFINITY && m < INFINITY && inv < INFINITY;
-        u32x2 q = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float v = f[e] * inv;
-            const int c = plain ? (int)(v + copysignf(0.49999997f, v)) : clampi(round_i32(v), -128, 127);
-            q[e >> 2] |= (uint32_t)(c & 0xFF) << (8 * (e & 3));
-            f[e] = (float)c * s;
-        }
-        if (in) *reinterpret_cast<u32x2*>((is_v ? p.v : p.k) + (size_t)r * p.dim + d) = q;
+        uint32_t q[2];
+        const float s = quantize_row<LR>(f, q);
+        if (in) *reinterpret_cast<u32x2*>((is_v ? p.v : p.k) + (size_t)r * p.dim + d) = u32x2{q[0], q[1]};
         if (d == 0) (is_v ? p.vs : p.ks)[r] = s;
 #pragma unroll
         for (int e = 0; e < 4; e++) w[e] = bf16x2_out(f[2 * e], f[2 * e + 1]);

@@ -31,18 +31,23 @@ struct KVPool {
     uint32_t width, pages, heads, page_size;
     Divider page_of;           // of a slot (below 2^30)
     uint32_t dim;
+    uint32_t row_tables, head_tables;    // tables of a row, and from a head to the next: 1 and 0, or heads and 1
+
+    __device__ __forceinline__ const int32_t* table(uint32_t b, uint32_t h) const {
+        return tables + ((size_t)b * row_tables + h * head_tables) * width;
+    }
 
     // Row of the pool (of head_dim values, and of each plane) that holds slot
     // `slot` of head h in row b's pages; false where that page is not there.
     __device__ __forceinline__ bool row(uint32_t b, uint32_t h, uint32_t slot, uint32_t& r) const {
         const uint32_t e = page_of(slot);
-        const uint32_t page = (uint32_t)tables[(size_t)b * width + e];
+        const uint32_t page = (uint32_t)table(b, h)[e];
         r = (page * heads + h) * page_size + (slot - e * page_size);
         return page < pages;
     }
 };
 
-inline KVPool kv_pool(const SNEPPXKVCache* c, const int32_t* tables, size_t width) {
+inline KVPool kv_pool(const SNEPPXKVCache* c, const int32_t* tables, size_t width, bool of_heads = false) {
     KVPool p;
     p.k = static_cast<uint8_t*>(c->k);
     p.v = static_cast<uint8_t*>(c->v);
@@ -57,6 +62,8 @@ inline KVPool kv_pool(const SNEPPXKVCache* c, const int32_t* tables, size_t widt
     p.page_size = (uint32_t)c->page_size;
     p.dim = (uint32_t)c->head_dim;
     p.page_of = divider(c->page_size);
+    p.row_tables = of_heads ? p.heads : 1;
+    p.head_tables = of_heads;
     return p;
 }
 

@@ -1,0 +1,626 @@
+// kv_shared_kernels.hip - attention of one new token per row, for rows in groups that
+// begin with the same pages (SNEPPX_kv_attention_shared, include/sneppx_kv.h).
+//
+//   s[t] = scale q . k[t],  p = softmax(s),  out = sum_t p[t] v[t]
+//
+// A group's queries over its prefix are a matrix product: all rows' query heads of a
+// key-value head against the same tokens.  So the work is cut into units, each a tile of
+// up to 128 queries (rows and heads) and a run of tokens that they have in common: of a
+// group's prefix, or of a row's own tokens behind it, for which the queries are the row's
+// alone.  A workgroup takes a unit, stages 64 tokens at a time in LDS for its four
+// waves, and leaves weighted values, maximum and sum of every query; k_kv_shared_join
+// adds up what a query has of its prefix and its own tokens.
+#include <hip/hip_runtime.h>
+
+#include <cfloat>
+#include <cstdint>
+
+#include "codec.h"
+#include "kv_pool.h"
+#include "launch.h"
+#include "../snx_internal.h"
+
+using namespace snx;
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 bf16x8_any __attribute__((aligned(2)));
+typedef u32x2 bf16x4_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef __attribute__((address_space(3))) uint8_t* lds_t;
+
+hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
+
+constexpr int SLOT_KV_SHARED = 10;    // of the stream's workspaces
+constexpr uint32_t STEP = 64;         // tokens of a step
+constexpr uint32_t TILE = 128;        // queries of a unit
+constexpr uint32_t kLeast = 4;        // steps of a unit, where there are so many
+constexpr int kLag = 8;               // log2 of how far a logit may pass the maximum that weights refer to
+
+struct Shared {
+    const uint16_t* q;
+    void* out;
+    size_t q_stride, out_stride;
+    const int32_t *lengths, *starts, *prefix;
+    float *part, *own_part;    // [heads][blocks][columns][dim], [rows][heads][own_tiles][splits][own_columns][dim]
+    float2 *ml, *own_ml;       // maximum and sum of the same
+    uint32_t rows, q_heads, group, groups, max_length;
+    uint32_t about, blocks;    // units of the prefixes of a head: about so many, and so many at most
+    uint32_t columns, own_columns, own_tiles, splits;
+    float scale_log2;          // not negative: `flip` changes the queries' signs instead
+    float room, lift;          // log2 of the most that weights of up to 2^kLag sum up to, and that less kLag
+    uint32_t flip;
+    int out_f32;
+};
+
+// The units of the prefixes, worked out by every wave from what only the device knows:
+// one group to a lane, all cut into spans of equal length, the spans of a tile next to
+// one another.
+struct Prefix {
+    uint32_t first, rows, tokens;      // the group's first row and number of rows, tokens of its prefix
+    uint32_t base, spans, per;         // its first unit, spans of a tile, steps of a span
+};
+struct Groups {
+    const Shared& a;
+    uint32_t most, per;
+    __device__ __forceinline__ Groups(const Shared& s, uint32_t slots) : a(s), most(slots < s.max_length ? slots : s.max_length) {
+        uint32_t total = 0;
+        for (uint32_t g0 = 0; g0 < a.groups; g0 += 64) {
+            const Prefix x = at(g0);
+            total += __builtin_amdgcn_readlane(lane_prefix(tiles(x) * steps(x)), 63);
+        }
+        per = (total + a.about - 1) / (a.about ? a.about : 1);
+        per = per > kLeast ? per : kLeast;
+    }
+    __device__ __forceinline__ Prefix at(uint32_t g0) const {
+        const uint32_t g = g0 + (threadIdx.x & 63);
+        Prefix x = {};
+        if (g < a.groups) {
+            const int32_t r0 = a.starts[g], r1 = a.starts[g + 1];
+            const uint32_t from = r0 < 0 ? 0u : (uint32_t)r0 < a.rows ? (uint32_t)r0 : a.rows;
+            const uint32_t to = r1 < 0 ? 0u : (uint32_t)r1 < a.rows ? (uint32_t)r1 : a.rows;
+            x.first = from;
+            x.rows = to > from ? to - from : 0;
+            x.tokens = kv_length(a.prefix, g, most);
+        }
+        return x;
+    }
+    __device__ __forceinline__ uint32_t steps(const Prefix& x) const { return (x.tokens + STEP - 1) / STEP; }
+    __device__ __forceinline__ uint32_t tiles(const Prefix& x) const {
+        return x.tokens ? (x.rows * a.group + TILE - 1) / TILE : 0;
+    }
+    // the group whose unit x is, or (ROW) that row x is in; false if there is none
+    template <bool ROW>
+    __device__ __forceinline__ bool find(uint32_t i, Prefix& out) const {
+        uint32_t base = 0;
+        for (uint32_t g0 = 0; g0 < a.groups; g0 += 64) {
+            const Prefix x = at(g0);
+            const uint32_t spans = (steps(x) + per - 1) / per, n = tiles(x) * spans, upto = lane_prefix(n);
+            const uint64_t is = ROW ? __ballot(x.tokens && i >= x.first && i - x.first < x.rows)
+                                    : __ballot(n && base + upto > i);
+            if (is) {
+                const int lane = __builtin_ctzll(is);
+                auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane(v, lane); };
+                out = Prefix{of(x.first), of(x.rows), of(x.tokens), base + of(upto - n), of(spans), per};
+                return true;
+            }
+            base += __builtin_amdgcn_readlane(upto, 63);
+        }
+        return false;
+    }
+};
+
+// The row of a group whose table has its prefix: the first that is as long, or the
+// longest (of which none reads more of it).
+__device__ __forceinline__ uint32_t row_with(const Shared& a, const Prefix& x) {
+    uint32_t best = x.first, most = kv_length(a.lengths, x.first, x.tokens);
+    for (uint32_t r0 = 0; r0 < x.rows && most < x.tokens; r0 += 64) {
+        const uint32_t r = r0 + (threadIdx.x & 63), n = r < x.rows ? kv_length(a.lengths, x.first + r, x.tokens) : 0;
+        const uint32_t top = lane_max(n);
+        if (top > most) {
+            most = top;
+            best = x.first + r0 + __builtin_ctzll(__ballot(n == top));
+        }
+    }
+    return best;
+}
+
+// x of this lane and of the one 32 lanes away
+__device__ __forceinline__ float swap32(float x, float& y) {
+    const u32x2 r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+    y = u2f(r[1]);
+    return u2f(r[0]);
+}
+
+// eight int8 as bf16 (exact)
+__device__ __forceinline__ u32x4 bytes_to_bf16(uint32_t a, uint32_t b) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t w = i ? b : a;
+        const float f0 = (float)(int8_t)w, f1 = (float)(int8_t)(w >> 8);
+        const float f2 = (float)(int8_t)(w >> 16), f3 = (float)(int8_t)(w >> 24);
+        o[2 * i] = __builtin_amdgcn_perm(f2u(f1), f2u(f0), 0x07060302u);
+        o[2 * i + 1] = __builtin_amdgcn_perm(f2u(f3), f2u(f2), 0x07060302u);
+    }
+    return o;
+}
+
+// Eight weights (not negative) as N bf16 pieces each, of eight bits one after the
+// other: with fp32 results three, which are all 24; with bf16 results, which keep
+// eight, two.  Where values may be infinite, lower pieces are not zero unless the
+// weight is (0 * infinity): 2^-40 of the first at least.
+template <int N, bool I8>
+__device__ __forceinline__ void split(const float* x, bf16x8 (&piece)[N]) {
+    u32x4 o[N];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        float a[2] = {x[e], x[e + 1]}, least[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            o[i][e >> 1] = __builtin_amdgcn_perm(f2u(a[1]), f2u(a[0]), 0x07060302u);
+            if (i == N - 1) break;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float high = u2f(f2u(a[j]) & 0xFFFF0000u);
+                if (!I8 && i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
+                a[j] = fmaxf(a[j] - high, least[j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) piece[i] = __builtin_bit_cast(bf16x8, o[i]);
+}
+
+template <int DP>
+struct Tiles {
+    static constexpr int KS = DP * 2 + 16, VS = DP * 2 + 16;        // bytes of a token's row
+    static constexpr int K = STEP * KS, V = STEP * VS;
+    static constexpr int OS = DP + 4;                               // floats of a query's row at the end
+    static constexpr int END = 2 * 32 * OS * 4;
+    static constexpr int ALL = K + V > END ? K + V : END;
+};
+
+// Lane l = 32 g + c.  Keys are the A operand of 32x32x16 products (32 token rows), the
+// queries the B operand (column c), so a lane ends up with 16 logits of query c: register
+// 8 p + 4 t + i is token 16 p + 8 t + 4 g + i.  Those of a p are the lane's eight elements
+// of the B operand of the second product as they stand, if its A operand, the values
+// transposed (ds_read_tr), has tokens in that order.  Its result has query c in every
+// lane, so a new maximum rescales by the lane's own factor.
+// With more than 64 queries each wave has 32 of them and all tokens of a step; with
+// fewer, waves w and w + 2 have the same 32 and half of the tokens each.
+template <int DP, bool I8, int PIECES>
+__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPool p, const Shared a) {
+    typedef Tiles<DP> L;
+    constexpr int CH = DP * (I8 ? 1 : 2) / 16;             // 16-byte pieces of a row in the pool
+    constexpr int EACH = STEP * CH / 256;                  // of a tile, for a thread
+    constexpr int KQ = DP / 16, DT = DP / 32;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[L::ALL];
+    __shared__ __attribute__((aligned(16))) float scales[2][STEP];
+    __shared__ float2 ends[2][32];
+    uint8_t* const kt = lds;
+    uint8_t* const vt = lds + L::K;
+
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Groups groups(a, p.width * p.page_size);
+
+    // the unit: its rows' first, their number, tile of queries, tokens
+    uint32_t first, rows, tile, t0, t1, cap, reads;
+    size_t slot;
+    float* part;
+    float2* ml;
+    const uint32_t shared_blocks = a.blocks * p.heads;
+    uint32_t h;
+    if (blockIdx.x < shared_blocks) {
+        const uint32_t i = blockIdx.x / p.heads;
+        h = blockIdx.x - i * p.heads;
+        Prefix x;
+        if (!groups.find<false>(i, x)) return;
+        const uint32_t n = i - x.base, span = n % x.spans;
+        first = x.first;
+        rows = x.rows;
+        reads = row_with(a, x);
+        tile = n / x.spans;
+        t0 = span * x.per * STEP;
+        t1 = t0 + x.per * STEP < x.tokens ? t0 + x.per * STEP : x.tokens;
+        slot = (size_t)h * a.blocks + i;
+        part = a.part;
+        ml = a.ml;
+        cap = a.columns;
+    } else {
+        uint32_t i = blockIdx.x - shared_blocks;
+        const uint32_t pair = i / p.heads, rest = pair / a.splits, span = pair - rest * a.splits;
+        h = i - pair * p.heads;
+        const uint32_t b = rest / a.own_tiles;
+        tile = rest - b * a.own_tiles;
+        first = reads = b;
+        rows = 1;
+        const uint32_t len = kv_length(a.lengths, b, groups.most);
+        Prefix x;
+        const uint32_t begins = !groups.find<true>(b, x) ? 0 : x.tokens < len ? x.tokens : len;
+        const uint32_t steps = (len - begins + STEP - 1) / STEP, per = (steps + a.splits - 1) / a.splits;
+        t0 = begins + span * per * STEP;
+        t0 = t0 < len ? t0 : len;
+        t1 = len - t0 < per * STEP ? len : t0 + per * STEP;
+        slot = (((size_t)b * p.heads + h) * a.own_tiles + tile) * a.splits + span;
+        part = a.own_part;
+        ml = a.own_ml;
+        cap = a.own_columns;
+    }
+    const uint32_t all = rows * a.group - tile * TILE, nq = all < TILE ? all : TILE;
+    const bool wide = nq > 64;
+    const uint32_t q0 = 32 * (wide ? wave : wave & 1);       // this wave's first query
+    const bool busy = q0 < nq;
+    const uint32_t u0 = wide ? 0 : wave >> 1, u1 = wide ? 2 : u0 + 1;      // and halves of a step
+    const int32_t* const table = p.table(reads, h);
+    const uint32_t row_bytes = p.dim * (I8 ? 1 : 2);
+
+    // (columns past the tile's queries repeat its last: nothing reads what they give)
+    bf16x8 q[KQ];
+    uint32_t limit;
+    {
+        const uint32_t mine = q0 + c < nq ? q0 + c : nq - 1, idx = tile * TILE + mine, b = first + idx / a.group;
+        const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(h * a.group + idx % a.group) * p.dim;
+        limit = kv_length(a.lengths, b, t1);
+#pragma unroll
+        for (int s = 0; s < KQ; s++) {
+            const uint32_t d = 16 * s + 8 * g;
+            u32x4 w = {0u, 0u, 0u, 0u};
+            if (d < p.dim) w = *reinterpret_cast<const bf16x8_any*>(qh + d) ^ a.flip;
+            q[s] = __builtin_bit_cast(bf16x8, w);
+        }
+    }
+
+    // this lane's token of a step: the page table's entry, then its row of the pool
+    uint32_t entry, row;
+    bool ok;
+    uint64_t there;
+    auto look = [&](uint32_t base) {
+        const uint32_t tok = base + lane;
+        entry = tok < t1 ? (uint32_t)table[p.page_of(tok)] : 0xFFFFFFFFu;
+    };
+    auto find = [&](uint32_t base) {
+        const uint32_t tok = base + lane;
+        ok = entry < p.pages;
+        row = ok ? (entry * p.heads + h) * p.page_size + (tok - p.page_of(tok) * p.page_size) : 0;
+    };
+    u32x4 kc[EACH], vc[EACH];
+    float ksc = 0.0f, vsc = 0.0f;
+    const uint32_t chunk = tid % CH;
+    auto load = [&] {
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const uint32_t r = __shfl(row, tid / CH + i * (256 / CH));
+            const size_t at = (size_t)r * row_bytes + (16 * chunk < row_bytes ? 16 * chunk : 0);
+            kc[i] = *reinterpret_cast<const u32x4*>(p.k + at);
+            vc[i] = *reinterpret_cast<const u32x4*>(p.v + at);
+        }
+        if (I8 && wave == 0) {
+            ksc = p.ks[row];
+            vsc = p.vs[row];
+        }
+    };
+
+    f32x16 o[DT] = {};
+    float m = -INFINITY, sum = 0.0f;
+    bool any = false;
+    if (t0 < t1) {
+        look(t0);
+        find(t0);
+        look(t0 + STEP);
+        load();
+    }
+    for (uint32_t base = t0; base < t1; base += STEP) {
+        // the step's tiles to LDS: values of absent tokens as zeros (0 * NaN), and zeros
+        // behind the head's end
+        there = __ballot(ok);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const uint32_t t = tid / CH + i * (256 / CH);
+            const bool in = 16 * chunk < row_bytes;
+            if (!in) kc[i] = u32x4{0u, 0u, 0u, 0u};
+            if (!in || !(there >> t & 1)) vc[i] = u32x4{0u, 0u, 0u, 0u};
+            if (I8) {
+                uint8_t* const kd = kt + t * L::KS + 32 * chunk;
+                uint8_t* const vd = vt + t * L::VS + 32 * chunk;
+                *reinterpret_cast<u32x4*>(kd) = bytes_to_bf16(kc[i][0], kc[i][1]);
+                *reinterpret_cast<u32x4*>(kd + 16) = bytes_to_bf16(kc[i][2], kc[i][3]);
+                *reinterpret_cast<u32x4*>(vd) = bytes_to_bf16(vc[i][0], vc[i][1]);
+                *reinterpret_cast<u32x4*>(vd + 16) = bytes_to_bf16(vc[i][2], vc[i][3]);
+            } else {
+                *reinterpret_cast<u32x4*>(kt + t * L::KS + 16 * chunk) = kc[i];
+                *reinterpret_cast<u32x4*>(vt + t * L::VS + 16 * chunk) = vc[i];
+            }
+        }
+        if (I8 && wave == 0) {
+            scales[0][lane] = ksc;
+            scales[1][lane] = ok ? vsc : 0.0f;
+        }
+        __syncthreads();
+        if (base + STEP < t1) {
+            find(base + STEP);
+            look(base + 2 * STEP);
+            load();
+        }
+        for (uint32_t u = u0; u < u1 && busy; u++) {
+            f32x16 s = {};
+#pragma unroll
+            for (int i = 0; i < KQ; i++) {
+                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (32 * u + c) * L::KS + 32 * i + 16 * g);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i], s, 0, 0, 0);
+            }
+            float top = -INFINITY;
+            if (I8)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 k4 = *reinterpret_cast<const f32x4*>(&scales[0][32 * u + 2 * r + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[r + i] *= k4[i];
+                }
+            const uint32_t from = base + 32 * u, mask = (uint32_t)(there >> (32 * u));
+            const bool whole = mask == 0xFFFFFFFFu && __all(from + 32 <= limit);
+            if (!whole) {
+                const uint32_t left = limit > from ? limit - from : 0;
+                const uint32_t mine = left >= 32 ? mask : mask & ((1u << left) - 1);
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (!(mine >> (2 * (r & 12) + (r & 3) + 4 * g) & 1)) s[r] = -INFINITY;
+                any |= mine != 0;
+            } else {
+                any = true;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) top = fmaxf(top, s[r]);
+            float other;
+            top = swap32(top, other);
+            top = fmaxf(top, other) * a.scale_log2;
+            // Weights are 2^(logit - m).  The reference m is a whole number, so that
+            // changing it rounds nothing, and moves when a logit comes within `lift` of
+            // it: after the first steps hardly ever.  It is so far above that weights sum
+            // up to 1 at most, however many there are: no sum of weighted values passes
+            // the largest value, and results are finite if that is.
+            if (__any(top + a.lift > m)) {
+                const float to = fmaxf(m, __builtin_ceilf(top) + a.room);
+                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                sum *= f;
+#pragma unroll
+                for (int i = 0; i < DT; i++) o[i] *= f;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float e[16];
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_log2, -ref));
+                sum += e[r];
+            }
+            if (I8)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 v4 = *reinterpret_cast<const f32x4*>(&scales[1][32 * u + 2 * r + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) e[r + i] *= v4[i];
+                }
+#pragma unroll
+            for (int pr = 0; pr < 2; pr++) {
+                bf16x8 pc[PIECES];
+                split<PIECES, I8>(e + 8 * pr, pc);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    s16x4 w[2];
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const int tok = 32 * u + 16 * pr + 8 * t + 4 * g + ((lane & 15) >> 2);
+                        const lds_t at = (lds_t)(vt + tok * L::VS + 64 * dt + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+                        w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                    }
+                    const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int i = 0; i < PIECES; i++) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pc[i], o[dt], 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+    // a maximum of -inf with tokens there is told from no tokens by a sum of 1
+    {
+        float other;
+        sum = swap32(sum, other);
+        sum += other;
+    }
+    if (m == -INFINITY && any && sum == 0.0f) sum = 1.0f;
+    // waves of the same queries meet
+    if (!wide) {
+        float* const ow = reinterpret_cast<float*>(lds) + (wave & 1) * 32 * L::OS + c * L::OS;
+        if (wave >= 2) {
+            if (g == 0) ends[wave & 1][c] = make_float2(m, sum);
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    *reinterpret_cast<f32x4*>(ow + 32 * dt + 2 * r + 4 * g) = f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]};
+        }
+        __syncthreads();
+        if (wave >= 2) return;
+        const float2 e = ends[wave & 1][c];
+        const float top = fmaxf(m, e.x);
+        const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        const float f1 = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
+        sum = top == -INFINITY ? fmaxf(sum, e.y) : f0 * sum + f1 * e.y;
+        m = top;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(ow + 32 * dt + 2 * r + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[dt][r + i] = f0 * o[dt][r + i] + f1 * x[i];
+            }
+    }
+    if (q0 + c >= nq) return;
+    const size_t at = slot * cap + q0 + c;
+    if (g == 0) ml[at] = make_float2(m, sum);
+    float* const to = part + at * p.dim;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const uint32_t d = 32 * dt + 2 * r + 4 * g;
+            if (d < p.dim) *reinterpret_cast<f32x4*>(to + d) = f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]};
+        }
+}
+
+// A wave for each row and query head: what its prefix's spans and its own tokens' left,
+// added in that order.
+__global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Shared a) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t number = (uint64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (number >= (uint64_t)a.rows * a.q_heads) return;
+    const uint32_t b = (uint32_t)(number / a.q_heads), hq = (uint32_t)(number - (uint64_t)b * a.q_heads);
+    const uint32_t h = hq / a.group, j = hq - h * a.group;
+    const Groups groups(a, p.width * p.page_size);
+    Prefix x = {};
+    const bool shared = groups.find<true>(b, x);
+    const uint32_t idx = shared ? (b - x.first) * a.group + j : 0;
+    const uint32_t unit = x.base + idx / TILE * x.spans;
+    // (spans past the workspace: of groups that overlap)
+    const uint32_t spans = !shared || unit >= a.blocks ? 0 : x.spans < a.blocks - unit ? x.spans : a.blocks - unit;
+    const size_t from = ((size_t)h * a.blocks + unit) * a.columns + idx % TILE;
+    const size_t own = ((((size_t)b * p.heads + h) * a.own_tiles + j / TILE) * a.splits) * a.own_columns + j % TILE;
+    const uint32_t n = spans + a.splits;
+    auto place = [&](uint32_t i) { return i < spans ? from + (size_t)i * a.columns : own + (size_t)(i - spans) * a.own_columns; };
+    auto end = [&](uint32_t i) { return i >= n ? make_float2(-INFINITY, 0.0f) : i < spans ? a.ml[place(i)] : a.own_ml[place(i)]; };
+
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, end(i).x);
+    top = lane_max(top);
+    const uint32_t span = p.dim <= 64 ? 16 : p.dim <= 128 ? 32 : 64, ways = 64 / span;
+    const uint32_t d = 4 * (lane & (span - 1)), way = lane / span;
+    const bool in = d < p.dim;
+    f32x4 v = {};
+    float total = 0.0f, plain = 0.0f;
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+        const float2 e = end(i0 + lane);
+        const float f = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
+        total += f * e.y;
+        plain += e.y;
+        const uint32_t here = n - i0 < 64 ? n - i0 : 64;
+        for (uint32_t k = 0; k < here; k += ways) {
+            const float w = __shfl(f, k + way);
+            const uint32_t i = i0 + k + way;
+            if (k + way < here && w != 0.0f && in)
+                v += w * *reinterpret_cast<const f32x4*>((i < spans ? a.part : a.own_part) + place(i) * p.dim + d);
+        }
+    }
+    total = lane_sum(total);
+    plain = lane_sum(plain);
+    for (uint32_t o = span; o < 64; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] += __shfl_xor(v[k], o);
+    if (way || !in) return;
+    v *= top == -INFINITY ? plain == 0.0f ? 0.0f : NAN : 1.0f / total;
+    const size_t to = b * a.out_stride + (size_t)hq * p.dim + d;
+    if (a.out_f32) *reinterpret_cast<f32x4_any*>(static_cast<float*>(a.out) + to) = v;
+    else *reinterpret_cast<bf16x4_any*>(static_cast<uint16_t*>(a.out) + to) = u32x2{bf16x2_out(v[0], v[1]), bf16x2_out(v[2], v[3])};
+}
+
+template <int DP, bool I8>
+void launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
+    if (a.out_f32) k_kv_shared<DP, I8, 3><<<grid, 256, 0, s>>>(p, a);
+    else k_kv_shared<DP, I8, 2><<<grid, 256, 0, s>>>(p, a);
+}
+template <bool I8>
+void launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
+    if (p.dim <= 64) launch<64, I8>(grid, p, a, s);
+    else if (p.dim <= 128) launch<128, I8>(grid, p, a, s);
+    else launch<256, I8>(grid, p, a, s);
+}
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+
+extern "C" {
+
+int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, void* out, size_t out_stride,
+                              int out_f32, const int32_t* tables, size_t width, const int32_t* lengths, size_t rows,
+                              size_t q_heads, size_t max_length, const int32_t* group_starts,
+                              const int32_t* prefix_lengths, size_t groups, size_t max_prefix, size_t max_own,
+                              float scale, void* st) {
+    const KVPool p = kv_pool(c, tables, width);
+    const size_t group = q_heads / c->kv_heads;
+    const size_t tiles = groups ? rows * group / TILE + groups : 0;      // of a head, at most
+    const size_t prefix_steps = groups ? (max_prefix + STEP - 1) / STEP : 0, own_steps = (max_own + STEP - 1) / STEP;
+    // Units for two workgroups on every CU, shared out by the steps that prefixes and
+    // own tokens take.
+    const size_t target = ((size_t)2 * cu_count() + c->kv_heads - 1) / c->kv_heads;
+    const size_t few = groups ? (rows * group + TILE - 1) / TILE : 0;    // tiles of groups that fill them
+    const size_t shared_work = few * prefix_steps, own_work = rows * own_steps;
+    size_t about = shared_work + own_work ? target * shared_work / (shared_work + own_work) : 0;
+    if (about < 1) about = 1;
+    size_t splits = target > about ? (target - about) / rows : 0;
+    const size_t most_splits = (own_steps + kLeast - 1) / kLeast;
+    if (splits > most_splits) splits = most_splits;
+    if (splits < 1) splits = 1;
+    const size_t blocks = groups ? about + tiles : 0;
+    const size_t columns = rows * group < TILE ? rows * group : TILE, own_columns = group < TILE ? group : TILE;
+    const size_t own_tiles = (group + TILE - 1) / TILE;
+    const size_t slots = blocks * c->kv_heads * columns, own = rows * c->kv_heads * own_tiles * splits * own_columns;
+    const size_t grid = blocks * c->kv_heads + rows * c->kv_heads * own_tiles * splits;
+    // (a grid has below 2^32 threads; steps of all tiles are counted in 32 bits)
+    if (grid > 0xffffff || rows * q_heads / 4 > 0xfffffe || tiles * ((max_length + STEP - 1) / STEP) > 0x7fffffff) {
+        snx_set_error("kv_attention_shared: %zu rows of up to %zu tokens are too many", rows, max_length);
+        return -1;
+    }
+    const size_t b0 = round16(slots * c->head_dim * sizeof(float)), b1 = round16(own * c->head_dim * sizeof(float));
+    const size_t b2 = round16(slots * sizeof(float2)), b3 = round16(own * sizeof(float2));
+    uint8_t* ws = static_cast<uint8_t*>(snx_workspace(b0 + b1 + b2 + b3, SLOT_KV_SHARED, st));
+    if (!ws) return -1;
+    Shared a;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.lengths = lengths;
+    a.starts = group_starts;
+    a.prefix = prefix_lengths;
+    a.part = reinterpret_cast<float*>(ws);
+    a.own_part = reinterpret_cast<float*>(ws + b0);
+    a.ml = reinterpret_cast<float2*>(ws + b0 + b1);
+    a.own_ml = reinterpret_cast<float2*>(ws + b0 + b1 + b2);
+    a.rows = (uint32_t)rows;
+    a.q_heads = (uint32_t)q_heads;
+    a.group = (uint32_t)group;
+    a.groups = (uint32_t)groups;
+    a.max_length = (uint32_t)max_length;
+    a.about = (uint32_t)about;
+    a.blocks = (uint32_t)blocks;
+    a.columns = (uint32_t)columns;
+    a.own_columns = (uint32_t)own_columns;
+    a.own_tiles = (uint32_t)own_tiles;
+    a.splits = (uint32_t)splits;
+    // (a scale of zero must not make NaN of a logit of -inf, which is a token that is not there)
+    a.flip = scale < 0.0f ? 0x80008000u : 0u;
+    a.scale_log2 = (scale < 0.0f ? -scale : scale) * 1.44269504088896340736f;
+    if (a.scale_log2 < FLT_MIN) a.scale_log2 = FLT_MIN;
+    uint32_t room = kLag;
+    while (((size_t)1 << (room - kLag)) < max_length) room++;
+    a.room = (float)room;
+    a.lift = (float)(room - kLag);
+    a.out_f32 = out_f32;
+    if (c->dtype == SNEPPX_INT8) launch<true>((unsigned)grid, p, a, S(st));
+    else launch<false>((unsigned)grid, p, a, S(st));
+    if (snx_launch_check("k_kv_shared")) return -1;
+    k_kv_shared_join<<<(unsigned)((rows * q_heads + 3) / 4), 256, 0, S(st)>>>(p, a);
+    return snx_launch_check("k_kv_shared_join");
+}
+
+}  // extern "C"

@@ -8,6 +8,7 @@
 #include "../snx_internal.h"
 
 #define SLOT_KV_MOVES 8
+#define SLOT_KV_SCORES 9
 
 #define REQUIRE(cond, ...)               \
     do {                                 \
@@ -99,7 +100,7 @@ int SNEPPX_kv_attention(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_
     if (!rows) return 0;
     const size_t slots = table_width * cache->page_size;
     if (max_length > slots) max_length = slots;
-    return snx_k_kv_attention(cache, q, q_stride, out, out_stride, out_dtype == SNEPPX_FLOAT32, block_tables, table_width,
+    return snx_k_kv_attention(cache, q, q_stride, out, out_stride, out_dtype == SNEPPX_FLOAT32, block_tables, table_width, 0,
                               lengths, rows, q_heads, max_length, scale, accumulate != 0, stream);
 }
 
@@ -125,4 +126,184 @@ int SNEPPX_kv_evict(const SNEPPXKVCache* cache, const int32_t* block_tables, siz
     if (bytes && !ws) return -1;
     return snx_k_kv_evict(cache, block_tables, table_width, lengths, next_pos, new_lengths, rows, max_length, budget,
                           recent, ws, stream);
+}
+
+int SNEPPX_kv_append_rotated(const SNEPPXKVCache* cache, const SNEPPXRotary* rotary, const uint16_t* q,
+                             size_t q_stride, uint16_t* q_out, size_t q_out_stride, size_t q_heads,
+                             const uint16_t* k, size_t k_stride, const uint16_t* v, size_t v_stride,
+                             size_t tokens, const int32_t* slots, const int32_t* positions, uint16_t* k_stored,
+                             uint16_t* v_stored, SNEPPXStream stream) {
+    static const char who[] = "kv_append_rotated";
+    if (cache_ok(who, cache) || snx_rotary_check(who, rotary, cache->head_dim)) return -1;
+    REQUIRE(!tokens || (k && v && slots && positions), "%s: NULL pointer", who);
+    REQUIRE(!tokens || !q_heads || (q && q_out), "%s: NULL q or q_out", who);
+    REQUIRE(!k_stored == !v_stored, "%s: k_stored and v_stored go together", who);
+    REQUIRE(q_heads <= 65535, "%s: %zu query heads are too many", who, q_heads);
+    REQUIRE(tokens <= MAX_SLOTS, "%s: %zu tokens are too many", who, tokens);
+    REQUIRE(cache->pages <= (size_t)INT32_MAX / cache->page_size, "%s: slots of %zu pages of %zu pass 31 bits", who,
+            cache->pages, cache->page_size);
+    const size_t n = cache->kv_heads * cache->head_dim, nq = q_heads * cache->head_dim;
+    REQUIRE(tokens < 2 || (k_stride >= n && v_stride >= n && q_stride >= nq && q_out_stride >= nq),
+            "%s: a stride (k %zu, v %zu, q %zu, q_out %zu) is below its row of %zu or %zu", who, k_stride, v_stride,
+            q_stride, q_out_stride, n, nq);
+    REQUIRE(!nq || tokens < 2 || q != q_out || q_stride == q_out_stride, "%s: q in place with another stride", who);
+    snx_clear_error();
+    if (!tokens) return 0;
+    return snx_k_kv_append_rotated(cache, rotary, q, q_stride, q_out, q_out_stride, q_heads, k, k_stride, v, v_stride,
+                                   tokens, slots, positions, k_stored, v_stored, stream);
+}
+
+/* ---- pages ---- */
+static int pages_ok(const char* who, const int32_t* refs, size_t pages, size_t page_size, const int32_t* tables,
+                    size_t width, const int32_t* lengths, size_t rows) {
+    REQUIRE(pages && page_size, "%s: no pages, or none of their size", who);
+    REQUIRE(page_size <= MAX_SLOTS && pages <= (size_t)INT32_MAX / page_size, "%s: slots of %zu pages of %zu pass 31 bits",
+            who, pages, page_size);
+    if (!rows) return 0;
+    REQUIRE(refs && tables && lengths, "%s: NULL refs, block_tables or lengths", who);
+    REQUIRE(width, "%s: empty block_tables", who);
+    REQUIRE(width <= MAX_SLOTS / page_size, "%s: table_width %zu * page_size %zu is too large", who, width, page_size);
+    REQUIRE(rows <= MAX_SLOTS / width, "%s: %zu rows of %zu entries are too many", who, rows, width);
+    return 0;
+}
+
+int SNEPPX_kv_reserve(int32_t* refs, size_t pages, size_t page_size, int32_t* block_tables, size_t table_width,
+                      int32_t* lengths, int32_t* next_pos, const int32_t* counts, size_t rows, int32_t* starts,
+                      int32_t* granted, int32_t* slots, int32_t* positions, size_t tokens, SNEPPXStream stream) {
+    static const char who[] = "kv_reserve";
+    if (pages_ok(who, refs, pages, page_size, block_tables, table_width, lengths, rows)) return -1;
+    REQUIRE(!rows || (starts && granted), "%s: NULL starts or granted", who);
+    REQUIRE(!rows || !tokens || slots, "%s: NULL slots", who);
+    REQUIRE(tokens <= MAX_SLOTS, "%s: %zu tokens are too many", who, tokens);
+    REQUIRE(!overlap(granted, counts, rows) && !overlap(granted, lengths, rows) && !overlap(granted, next_pos, rows) &&
+                !overlap(lengths, counts, rows) && !overlap(lengths, next_pos, rows) && !overlap(next_pos, counts, rows),
+            "%s: lengths, next_pos, counts and granted overlap", who);
+    snx_clear_error();
+    if (!rows) return 0;
+    return snx_k_kv_reserve(refs, pages, page_size, block_tables, table_width, lengths, next_pos, counts, rows, starts,
+                            granted, slots, positions, tokens, stream);
+}
+
+int SNEPPX_kv_release(int32_t* refs, size_t pages, size_t page_size, int32_t* block_tables, size_t table_width,
+                      const int32_t* lengths, size_t rows, SNEPPXStream stream) {
+    if (pages_ok("kv_release", refs, pages, page_size, block_tables, table_width, lengths, rows)) return -1;
+    snx_clear_error();
+    if (!rows) return 0;
+    return snx_k_kv_release(refs, pages, page_size, block_tables, table_width, lengths, rows, stream);
+}
+
+int SNEPPX_kv_share(int32_t* refs, size_t pages, size_t page_size, int32_t* block_tables, size_t table_width,
+                    int32_t* lengths, int32_t* next_pos, const int32_t* sources, const int32_t* counts, size_t rows,
+                    SNEPPXStream stream) {
+    static const char who[] = "kv_share";
+    if (pages_ok(who, refs, pages, page_size, block_tables, table_width, lengths, rows)) return -1;
+    REQUIRE(!rows || (sources && counts), "%s: NULL sources or counts", who);
+    REQUIRE(!overlap(lengths, sources, rows) && !overlap(lengths, counts, rows) && !overlap(lengths, next_pos, rows) &&
+                !overlap(next_pos, sources, rows) && !overlap(next_pos, counts, rows),
+            "%s: lengths or next_pos overlap sources, counts or one another", who);
+    snx_clear_error();
+    if (!rows) return 0;
+    return snx_k_kv_share(refs, pages, page_size, block_tables, table_width, lengths, next_pos, sources, counts, rows,
+                          stream);
+}
+
+/* ---- attention of queries over shared prefixes and picked pages ---- */
+static int queries_ok(const char* who, const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, size_t q_heads,
+                      size_t rows) {
+    REQUIRE(!rows || q, "%s: NULL pointer", who);
+    REQUIRE(q_heads && q_heads % c->kv_heads == 0 && q_heads <= 65535,
+            "%s: %zu query heads are not a multiple of %zu key-value heads", who, q_heads, c->kv_heads);
+    REQUIRE(rows < 2 || q_stride >= q_heads * c->head_dim, "%s: q_stride %zu is below q_heads * head_dim = %zu", who,
+            q_stride, q_heads * c->head_dim);
+    return 0;
+}
+
+static int out_ok(const char* who, const SNEPPXKVCache* c, const void* out, size_t out_stride, SNEPPXDtype dtype,
+                  size_t q_heads, size_t rows) {
+    REQUIRE(!rows || out, "%s: NULL pointer", who);
+    REQUIRE(dtype == SNEPPX_BFLOAT16 || dtype == SNEPPX_FLOAT32, "%s: out_dtype %d is neither bf16 nor fp32", who,
+            (int)dtype);
+    REQUIRE(rows < 2 || out_stride >= q_heads * c->head_dim, "%s: out_stride %zu is below q_heads * head_dim = %zu", who,
+            out_stride, q_heads * c->head_dim);
+    return 0;
+}
+
+int SNEPPX_kv_attention_shared(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_stride, void* out,
+                               size_t out_stride, SNEPPXDtype out_dtype, const int32_t* block_tables,
+                               size_t table_width, const int32_t* lengths, size_t rows, size_t q_heads,
+                               size_t max_length, const int32_t* group_starts, const int32_t* prefix_lengths,
+                               size_t groups, size_t max_prefix, size_t max_own, float scale, SNEPPXStream stream) {
+    static const char who[] = "kv_attention_shared";
+    if (cache_ok(who, cache) || rows_ok(who, cache, block_tables, table_width, lengths, rows) ||
+        queries_ok(who, cache, q, q_stride, q_heads, rows) || out_ok(who, cache, out, out_stride, out_dtype, q_heads, rows))
+        return -1;
+    REQUIRE(!rows || !groups || (group_starts && prefix_lengths), "%s: NULL group_starts or prefix_lengths", who);
+    REQUIRE(groups <= rows, "%s: %zu groups of %zu rows", who, groups, rows);
+    snx_clear_error();
+    if (!rows) return 0;
+    const size_t slots = table_width * cache->page_size;
+    if (max_length > slots) max_length = slots;
+    if (max_prefix > max_length) max_prefix = max_length;
+    if (max_own > max_length) max_own = max_length;
+    return snx_k_kv_attention_shared(cache, q, q_stride, out, out_stride, out_dtype == SNEPPX_FLOAT32, block_tables,
+                                     table_width, lengths, rows, q_heads, max_length, group_starts, prefix_lengths, groups,
+                                     max_prefix, max_own, scale, stream);
+}
+
+int SNEPPX_kv_key_bounds(const SNEPPXKVCache* cache, uint16_t* bounds, const int32_t* block_tables,
+                         size_t table_width, const int32_t* lengths, const int32_t* counts, size_t max_count,
+                         size_t rows, SNEPPXStream stream) {
+    static const char who[] = "kv_key_bounds";
+    if (cache_ok(who, cache) || rows_ok(who, cache, block_tables, table_width, lengths, rows)) return -1;
+    REQUIRE(!rows || bounds, "%s: NULL bounds", who);
+    REQUIRE(aligned16(bounds), "%s: bounds must be 16-byte aligned", who);
+    snx_clear_error();
+    if (!rows || !max_count) return 0;
+    const size_t slots = table_width * cache->page_size;
+    if (!counts) max_count = 1;
+    if (max_count > slots) max_count = slots;
+    return snx_k_kv_key_bounds(cache, bounds, block_tables, table_width, lengths, counts, max_count, rows, stream);
+}
+
+int SNEPPX_kv_pick(const SNEPPXKVCache* cache, const uint16_t* bounds, const uint16_t* q, size_t q_stride,
+                   size_t q_heads, const int32_t* block_tables, size_t table_width, const int32_t* lengths,
+                   size_t rows, size_t max_length, size_t budget, size_t first, size_t recent, int32_t* picked,
+                   int32_t* picked_lengths, SNEPPXStream stream) {
+    static const char who[] = "kv_pick";
+    if (cache_ok(who, cache) || rows_ok(who, cache, block_tables, table_width, lengths, rows) ||
+        queries_ok(who, cache, q, q_stride, q_heads, rows))
+        return -1;
+    REQUIRE(!rows || (bounds && picked && picked_lengths), "%s: NULL bounds, picked or picked_lengths", who);
+    REQUIRE(aligned16(bounds), "%s: bounds must be 16-byte aligned", who);
+    REQUIRE(budget && budget <= MAX_SLOTS / cache->page_size, "%s: budget %zu is 0 or too large", who, budget);
+    REQUIRE(recent && recent <= budget && first <= budget - recent, "%s: first %zu and recent %zu (1 at least) do not fit the budget %zu",
+            who, first, recent, budget);
+    REQUIRE(!overlap(picked_lengths, lengths, rows), "%s: picked_lengths must not be lengths, nor overlap them", who);
+    snx_clear_error();
+    if (!rows) return 0;
+    const size_t slots = table_width * cache->page_size;
+    if (max_length > slots) max_length = slots;
+    const size_t most = (max_length + cache->page_size - 1) / cache->page_size;
+    void* ws = NULL;
+    if (most > budget) {
+        ws = snx_workspace(rows * cache->kv_heads * most * sizeof(uint32_t), SLOT_KV_SCORES, stream);
+        if (!ws) return -1;
+    }
+    return snx_k_kv_pick(cache, bounds, q, q_stride, q_heads, block_tables, table_width, lengths, rows, max_length, budget,
+                         first, recent, picked, picked_lengths, ws, stream);
+}
+
+int SNEPPX_kv_attention_picked(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_stride, void* out,
+                               size_t out_stride, SNEPPXDtype out_dtype, const int32_t* picked, size_t budget,
+                               const int32_t* picked_lengths, size_t rows, size_t q_heads, float scale,
+                               int accumulate, SNEPPXStream stream) {
+    static const char who[] = "kv_attention_picked";
+    if (cache_ok(who, cache) || rows_ok(who, cache, picked, budget, picked_lengths, rows) ||
+        queries_ok(who, cache, q, q_stride, q_heads, rows) || out_ok(who, cache, out, out_stride, out_dtype, q_heads, rows))
+        return -1;
+    REQUIRE(!accumulate || cache->weights, "%s: accumulate needs the cache's weights", who);
+    snx_clear_error();
+    if (!rows) return 0;
+    return snx_k_kv_attention(cache, q, q_stride, out, out_stride, out_dtype == SNEPPX_FLOAT32, picked, budget, 1,
+                              picked_lengths, rows, q_heads, budget * cache->page_size, scale, accumulate != 0, stream);
 }

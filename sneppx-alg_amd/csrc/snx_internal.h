@@ -281,18 +281,52 @@ int snx_k_fp8_gemm(const uint8_t* A, const uint8_t* W, const float* sA, const fl
 /* ---- paged key-value cache (kv_attn_kernels.hip, kv_cache_kernels.hip) ----
  * checked arguments; max_length within the table, budget <= max_length; the
  * attention takes its workspaces itself, the eviction gets one of
- * snx_kv_evict_ws bytes */
+ * snx_kv_evict_ws bytes; of_heads: tables [rows][kv_heads][width] */
 int snx_k_kv_append(const SNEPPXKVCache* c, const uint16_t* k, size_t k_stride, const uint16_t* v, size_t v_stride,
                     size_t tokens, const int32_t* starts, uint16_t* k_stored, uint16_t* v_stored,
                     const int32_t* tables, size_t width, const int32_t* lengths, const int32_t* next_pos,
                     size_t rows, void* stream);
 int snx_k_kv_attention(const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, void* out, size_t out_stride,
-                       int out_f32, const int32_t* tables, size_t width, const int32_t* lengths, size_t rows,
-                       size_t q_heads, size_t max_length, float scale, int accumulate, void* stream);
+                       int out_f32, const int32_t* tables, size_t width, int of_heads, const int32_t* lengths,
+                       size_t rows, size_t q_heads, size_t max_length, float scale, int accumulate, void* stream);
 size_t snx_kv_evict_ws(const SNEPPXKVCache* c, size_t rows, size_t max_length, size_t budget);
 int snx_k_kv_evict(const SNEPPXKVCache* c, const int32_t* tables, size_t width, const int32_t* lengths,
                    const int32_t* next_pos, int32_t* new_lengths, size_t rows, size_t max_length, size_t budget,
                    size_t recent, void* ws, void* stream);
+
+/* ---- rotary positions (rotary_kernels.hip; rotary.c checks a descriptor) ---- */
+int snx_rotary_check(const char* who, const SNEPPXRotary* r, size_t head_dim);
+int snx_k_rotary(const SNEPPXRotary* r, const uint16_t* q, size_t q_stride, uint16_t* q_out, size_t q_out_stride,
+                 size_t q_heads, const uint16_t* k, size_t k_stride, uint16_t* k_out, size_t k_out_stride,
+                 size_t kv_heads, size_t head_dim, const int32_t* positions, size_t tokens, void* stream);
+int snx_k_kv_append_rotated(const SNEPPXKVCache* c, const SNEPPXRotary* r, const uint16_t* q, size_t q_stride,
+                            uint16_t* q_out, size_t q_out_stride, size_t q_heads, const uint16_t* k, size_t k_stride,
+                            const uint16_t* v, size_t v_stride, size_t tokens, const int32_t* slots,
+                            const int32_t* positions, uint16_t* k_stored, uint16_t* v_stored, void* stream);
+
+/* ---- pages (kv_pages_kernels.hip) ---- */
+int snx_k_kv_reserve(int32_t* refs, size_t pages, size_t page_size, int32_t* tables, size_t width, int32_t* lengths,
+                     int32_t* next_pos, const int32_t* counts, size_t rows, int32_t* starts, int32_t* granted,
+                     int32_t* slots, int32_t* positions, size_t tokens, void* stream);
+int snx_k_kv_release(int32_t* refs, size_t pages, size_t page_size, int32_t* tables, size_t width,
+                     const int32_t* lengths, size_t rows, void* stream);
+int snx_k_kv_share(int32_t* refs, size_t pages, size_t page_size, int32_t* tables, size_t width, int32_t* lengths,
+                   int32_t* next_pos, const int32_t* sources, const int32_t* counts, size_t rows, void* stream);
+
+/* ---- attention behind shared prefixes (kv_shared_kernels.hip, takes its workspace
+ * itself) and over picked pages (kv_pick_kernels.hip; ws: 4 bytes for each row, head and
+ * page of max_length where that is more than the budget) ---- */
+int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, void* out, size_t out_stride,
+                              int out_f32, const int32_t* tables, size_t width, const int32_t* lengths, size_t rows,
+                              size_t q_heads, size_t max_length, const int32_t* group_starts,
+                              const int32_t* prefix_lengths, size_t groups, size_t max_prefix, size_t max_own,
+                              float scale, void* stream);
+int snx_k_kv_key_bounds(const SNEPPXKVCache* c, uint16_t* bounds, const int32_t* tables, size_t width,
+                        const int32_t* lengths, const int32_t* counts, size_t max_count, size_t rows, void* stream);
+int snx_k_kv_pick(const SNEPPXKVCache* c, const uint16_t* bounds, const uint16_t* q, size_t q_stride, size_t q_heads,
+                  const int32_t* tables, size_t width, const int32_t* lengths, size_t rows, size_t max_length,
+                  size_t budget, size_t first, size_t recent, int32_t* picked, int32_t* picked_lengths, void* ws,
+                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -147,6 +147,21 @@ EXPORTS = {
     "SNEPPX_kv_attention": (C.c_int, [_vp, _vp, _sz, _vp, _sz, C.c_int, _vp, _sz, _vp, _sz, _sz, _sz, C.c_float,
                                       C.c_int, _vp]),
     "SNEPPX_kv_evict": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp]),
+    "SNEPPX_kv_append_rotated": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _vp,
+                                           _vp, _vp]),
+    "SNEPPX_kv_reserve": (C.c_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "SNEPPX_kv_release": (C.c_int, [_vp, _sz, _sz, _vp, _sz, _vp, _sz, _vp]),
+    "SNEPPX_kv_share": (C.c_int, [_vp, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "SNEPPX_kv_attention_shared": (C.c_int, [_vp, _vp, _sz, _vp, _sz, C.c_int, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp,
+                                             _sz, _sz, _sz, C.c_float, _vp]),
+    "SNEPPX_kv_key_bounds": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp]),
+    "SNEPPX_kv_pick": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _vp]),
+    "SNEPPX_kv_attention_picked": (C.c_int, [_vp, _vp, _sz, _vp, _sz, C.c_int, _vp, _sz, _vp, _sz, _sz, C.c_float,
+                                             C.c_int, _vp]),
+    # rotary positions (include/sneppx_rotary.h)
+    "SNEPPX_rotary_frequencies": (C.c_int, [_vp, C.POINTER(C.c_float), _sz, C.c_double, C.c_int, C.c_double, C.c_double,
+                                            C.c_double, C.c_double]),
+    "SNEPPX_rotary_apply": (C.c_int, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _sz, _vp]),
     # thin HIP ABI
     "snx_hip_device_count": (C.c_int, [C.POINTER(C.c_int)]),
     "snx_hip_event_create": (C.c_int, [C.POINTER(_vp)]),
@@ -618,6 +633,39 @@ class Library:
         """A KVCache over tensors that the caller has (layouts of include/sneppx_kv.h)."""
         return KVCache(self, k, v, k_scales, v_scales, weights, positions)
 
+    def kv_pages(self, pages, page_size, device="cuda"):
+        """KVPages of a pool in which every page is free."""
+        return KVPages(self, torch.zeros(pages, dtype=torch.int32, device=device), page_size)
+
+    def kv_pages_from(self, refs, page_size):
+        """KVPages over counts that the caller has: int32 [pages]."""
+        return KVPages(self, refs, page_size)
+
+    # ---------------- rotary positions ---------------------------------------
+    def rotary_frequencies(self, dims, base=10000.0, scaling=None, factor=1.0, original=0.0, low=1.0, high=4.0):
+        """SNEPPX_rotary_frequencies: (float64 numpy [dims / 2], magnitude); scaling None,
+        "linear", "base", "bands" or "ramp"."""
+        if scaling is not None and scaling not in ROTARY_SCALINGS:
+            raise ValueError(f"scaling must be None or one of {ROTARY_SCALINGS}, got {scaling!r}")
+        _no_count(dims=dims)
+        freqs, magnitude = np.zeros(dims // 2, np.float64), C.c_float(0)
+        self.check(self.fn["SNEPPX_rotary_frequencies"](
+            freqs.ctypes.data_as(_vp), C.byref(magnitude), dims, base,
+            0 if scaling is None else 1 + ROTARY_SCALINGS.index(scaling), factor, original, low, high),
+            "rotary_frequencies")
+        return freqs, magnitude.value
+
+    def rotary(self, head_dim, dims=None, base=10000.0, interleaved=False, q_norm=None, k_norm=None, eps=1e-6,
+               device="cuda", **scaling):
+        """A Rotary of the frequencies that rotary_frequencies(dims, base, **scaling) gives
+        (dims: head_dim unless given)."""
+        freqs, magnitude = self.rotary_frequencies(head_dim if dims is None else dims, base, **scaling)
+        return Rotary(self, torch.from_numpy(freqs).to(device), head_dim, interleaved, magnitude, q_norm, k_norm, eps)
+
+    def rotary_from(self, freqs, head_dim, interleaved=False, magnitude=1.0, q_norm=None, k_norm=None, eps=1e-6):
+        """A Rotary over tensors that the caller has."""
+        return Rotary(self, freqs, head_dim, interleaved, magnitude, q_norm, k_norm, eps)
+
     # ---------------- HIP events on an explicit stream ----------------------
     def event(self):
         e = C.c_void_p()
@@ -661,6 +709,9 @@ class Library:
 
 # SNEPPXMXFormat order (include/sneppx_mx.h = MX_FORMATS of mx_formats.py)
 MX_FORMATS = ["mxfp8_e4m3", "mxfp8_e5m2", "mxfp6_e3m2", "mxfp6_e2m3", "mxfp4_e2m1", "nvfp4_e2m1"]
+
+# SNEPPXRotaryScaling (include/sneppx_rotary.h), without SNEPPX_ROTARY_PLAIN
+ROTARY_SCALINGS = ["linear", "base", "bands", "ramp"]
 
 # dtype codes of include/sneppx_qstore.h (= the reference's SNEPPXSafetensorsDType)
 QST_DTYPES = ["F32", "F16", "F64", "I64", "I32", "I16", "I8", "U8", "BOOL", "BF16", "F8_E5M2",
@@ -805,48 +856,18 @@ def _no_count(**counts):
 _BF16, _BF16_OR_F32 = ((torch.bfloat16,), (torch.bfloat16, torch.float32)) if torch else ((), ())
 
 
-class KVCache:
-    """A paged key-value pool (include/sneppx_kv.h): k, v [pages, kv_heads,
-    page_size, head_dim] in bf16 or int8; k_scales, v_scales (int8), weights
-    (fp32) and positions (int32) [pages, kv_heads, page_size].
+class _OnDevice:
+    """What calls on a handle's device share: self.L, self.device, self._index and self.head_dim."""
 
-    Calls take the rows' block tables (int32 [rows, width]) and lengths (int32
-    [rows], the call's new tokens included) on the cache's device, and run there
-    on torch's current stream of that device unless one is given."""
-
-    def __init__(self, lib, k, v, k_scales=None, v_scales=None, weights=None, positions=None):
-        if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in (torch.bfloat16, torch.int8):
-            raise ValueError("k must be a bf16 or int8 tensor [pages, kv_heads, page_size, head_dim]")
-        self.L, self.device, self._index = lib, k.device, k.device.index if k.is_cuda else None
-        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        i8 = k.dtype == torch.int8
-        planes = k.shape[:3]
-        for t, name, dtype, shape, needed in (
-                (k, "k", k.dtype, k.shape, True), (v, "v", k.dtype, k.shape, True),
-                (k_scales, "k_scales", torch.float32, planes, i8), (v_scales, "v_scales", torch.float32, planes, i8),
-                (weights, "weights", torch.float32, planes, False),
-                (positions, "positions", torch.int32, planes, False)):
-            if t is None and not needed:
-                continue
-            self._check(t, name, dtype, shape)
-        if not i8 and (k_scales is not None or v_scales is not None):
-            raise ValueError("a bf16 cache has no scales")
-        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
-        self.weights, self.positions = weights, positions
-        self._c = _KVCacheStruct(*(None if t is None else t.data_ptr()
-                                   for t in (k, v, k_scales, v_scales, weights, positions)),
-                                 SNEPPX_INT8 if i8 else SNEPPX_BFLOAT16, *(k.shape[i] for i in (0, 2, 1, 3)))
-        self._p = C.cast(C.pointer(self._c), _vp)
-        self._append, self._attention, self._evict = (
-            lib.fn[f"SNEPPX_kv_{n}"] for n in ("append", "attention", "evict"))
+    _what = "handle"
 
     # (the library's workspaces and launches are the current device's.  Asked in line, as
     # is torch's current stream by its number: a function around every call takes 0.2 us,
     # current_stream(), which makes an object, 2.8)
     def _elsewhere(self, fn):
-        """fn on the cache's device, which is not the current one."""
+        """fn on the handle's device, which is not the current one."""
         if self._index is None:
-            raise ValueError(f"the cache is on {self.device}: its calls run on a GPU")
+            raise ValueError(f"the {self._what} is on {self.device}: its calls run on a GPU")
 
         def run(*args):
             with torch.cuda.device(self._index):
@@ -856,7 +877,7 @@ class KVCache:
     # (the checks are on the way of every call: few look-ups of a tensor's attributes,
     # which take 0.1 us each)
     def _check(self, t, name, dtype, shape):
-        """The address of a contiguous tensor of this type and shape on the cache's device."""
+        """The address of a contiguous tensor of this type and shape on the handle's device."""
         try:
             if t.dtype is dtype and t.shape == shape and t.device == self.device and t.is_contiguous():
                 return t.data_ptr()
@@ -885,6 +906,47 @@ class KVCache:
         shape = n, width = tables.shape
         return self._check(tables, "tables", torch.int32, shape), width, \
             self._check(lengths, "lengths", torch.int32, (n,)), n
+
+
+class KVCache(_OnDevice):
+    """A paged key-value pool (include/sneppx_kv.h): k, v [pages, kv_heads,
+    page_size, head_dim] in bf16 or int8; k_scales, v_scales (int8), weights
+    (fp32) and positions (int32) [pages, kv_heads, page_size].
+
+    Calls take the rows' block tables (int32 [rows, width]) and lengths (int32
+    [rows], the call's new tokens included) on the cache's device, and run there
+    on torch's current stream of that device unless one is given."""
+
+    _what = "cache"
+
+    def __init__(self, lib, k, v, k_scales=None, v_scales=None, weights=None, positions=None):
+        if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in (torch.bfloat16, torch.int8):
+            raise ValueError("k must be a bf16 or int8 tensor [pages, kv_heads, page_size, head_dim]")
+        self.L, self.device, self._index = lib, k.device, k.device.index if k.is_cuda else None
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        i8 = k.dtype == torch.int8
+        planes = k.shape[:3]
+        for t, name, dtype, shape, needed in (
+                (k, "k", k.dtype, k.shape, True), (v, "v", k.dtype, k.shape, True),
+                (k_scales, "k_scales", torch.float32, planes, i8), (v_scales, "v_scales", torch.float32, planes, i8),
+                (weights, "weights", torch.float32, planes, False),
+                (positions, "positions", torch.int32, planes, False)):
+            if t is None and not needed:
+                continue
+            self._check(t, name, dtype, shape)
+        if not i8 and (k_scales is not None or v_scales is not None):
+            raise ValueError("a bf16 cache has no scales")
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.weights, self.positions = weights, positions
+        self._c = _KVCacheStruct(*(None if t is None else t.data_ptr()
+                                   for t in (k, v, k_scales, v_scales, weights, positions)),
+                                 SNEPPX_INT8 if i8 else SNEPPX_BFLOAT16, *(k.shape[i] for i in (0, 2, 1, 3)))
+        self._p = C.cast(C.pointer(self._c), _vp)
+        self._append, self._attention, self._evict = (
+            lib.fn[f"SNEPPX_kv_{n}"] for n in ("append", "attention", "evict"))
+        self._append_rotated, self._shared, self._bounds, self._pick, self._picked = (
+            lib.fn[f"SNEPPX_kv_{n}"] for n in ("append_rotated", "attention_shared", "key_bounds", "pick",
+                                               "attention_picked"))
 
     def append(self, k, v, tables, lengths, next_pos=None, starts=None, k_stored=None, v_stored=None, stream=None):
         """SNEPPX_kv_append: k, v bf16 [tokens, kv_heads, head_dim], slices of
@@ -938,6 +1000,236 @@ class KVCache:
                  stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
         if rc:
             self.L.check(rc, "kv_evict")
+
+    def append_rotated(self, rotary, q, k, v, slots, positions, q_out=None, k_stored=None, v_stored=None, stream=None):
+        """SNEPPX_kv_append_rotated: q bf16 [tokens, q_heads, head_dim] turned into q_out
+        (without q_out in place), or None; k, v bf16 [tokens, kv_heads, head_dim], slots and
+        positions int32 [tokens]."""
+        kp, ks, tokens, heads = self._rows(k, "k", self.kv_heads, _BF16)
+        vp, vs, v_tokens, _ = self._rows(v, "v", self.kv_heads, _BF16)
+        qp = qs = op = os_ = None
+        q_heads, q_tokens = 0, tokens
+        if q is not None:
+            qp, qs, q_tokens, q_heads = self._rows(q, "q", 0, _BF16)
+            op, os_ = qp, qs
+            if q_out is not None:
+                op, os_, o_tokens, _ = self._rows(q_out, "q_out", q_heads, _BF16)
+                if o_tokens != tokens:
+                    raise ValueError(f"q_out has {o_tokens} tokens, k {tokens}")
+        if v_tokens != tokens or q_tokens != tokens:
+            raise ValueError(f"k has {tokens} tokens, v {v_tokens}, q {q_tokens}")
+        if not isinstance(rotary, Rotary) or rotary.device != self.device or rotary.head_dim != self.head_dim:
+            raise ValueError(f"rotary must be a Rotary of heads of {self.head_dim} on {self.device}, got {rotary!r}")
+        shape = (tokens,)
+        sl, ps = self._check(slots, "slots", torch.int32, shape), self._check(positions, "positions", torch.int32, shape)
+        stored = tokens, heads, self.head_dim
+        ko = None if k_stored is None else self._check(k_stored, "k_stored", torch.bfloat16, stored)
+        vo = None if v_stored is None else self._check(v_stored, "v_stored", torch.bfloat16, stored)
+        run = self._append_rotated if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._append_rotated)
+        rc = run(self._p, rotary._p, qp, qs or 0, op, os_ or 0, q_heads, kp, ks, vp, vs, tokens, sl, ps, ko, vo,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_append_rotated")
+
+    def attention_shared(self, q, out, tables, lengths, max_length, groups, prefix, max_prefix, max_own, scale=None,
+                         stream=None):
+        """SNEPPX_kv_attention_shared: groups int32 [n + 1] (first rows), prefix int32 [n]
+        (tokens that a group's rows have in common); the others as in attention."""
+        qp, qs, rows, heads = self._rows(q, "q", 0, _BF16)
+        op, os_, out_rows, _ = self._rows(out, "out", heads, _BF16_OR_F32)
+        tb, width, ln, n = self._tables(tables, lengths)
+        if rows != n or out_rows != n:
+            raise ValueError(f"q has {rows} rows and out {out_rows}, tables {n}")
+        if not isinstance(prefix, torch.Tensor) or prefix.dim() != 1:
+            raise ValueError("prefix must be an int32 tensor [groups]")
+        many = prefix.shape[0]
+        pf, gr = self._check(prefix, "prefix", torch.int32, (many,)), self._check(groups, "groups", torch.int32, (many + 1,))
+        if not 0 <= max_length | max_prefix | max_own < _COUNTS:
+            _no_count(max_length=max_length, max_prefix=max_prefix, max_own=max_own)
+        run = self._shared if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._shared)
+        rc = run(self._p, qp, qs, op, os_, SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, tb, width,
+                 ln, n, heads, max_length, gr, pf, many, max_prefix, max_own,
+                 self.head_dim ** -0.5 if scale is None else scale,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_attention_shared")
+
+    def key_bounds(self, bounds, tables, lengths, counts=None, max_count=1, stream=None):
+        """SNEPPX_kv_key_bounds: bounds bf16 [pages, kv_heads, 2, head_dim]; the pages of
+        the last counts tokens (int32 [rows], none larger than max_count), or of one."""
+        tb, width, ln, n = self._tables(tables, lengths)
+        bp = self._check(bounds, "bounds", torch.bfloat16, (self.pages, self.kv_heads, 2, self.head_dim))
+        ct = None if counts is None else self._check(counts, "counts", torch.int32, (n,))
+        if not 0 <= max_count < _COUNTS:
+            _no_count(max_count=max_count)
+        run = self._bounds if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._bounds)
+        rc = run(self._p, bp, tb, width, ln, ct, max_count, n,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_key_bounds")
+
+    def _picks(self, picked, lengths, name):
+        """The addresses of page lists [rows, kv_heads, budget] and of their lengths, rows and budget."""
+        if not isinstance(picked, torch.Tensor) or picked.dim() != 3:
+            raise ValueError("picked must be an int32 tensor [rows, kv_heads, budget]")
+        n, _, budget = picked.shape
+        return self._check(picked, "picked", torch.int32, (n, self.kv_heads, budget)), \
+            self._check(lengths, name, torch.int32, (n,)), n, budget
+
+    def pick(self, q, bounds, tables, lengths, max_length, picked, picked_lengths, first=1, recent=1, stream=None):
+        """SNEPPX_kv_pick: picked int32 [rows, kv_heads, budget], picked_lengths int32
+        [rows]; the first `first` and last `recent` pages are always among them."""
+        qp, qs, rows, heads = self._rows(q, "q", 0, _BF16)
+        tb, width, ln, n = self._tables(tables, lengths)
+        bp = self._check(bounds, "bounds", torch.bfloat16, (self.pages, self.kv_heads, 2, self.head_dim))
+        pk, pl, pn, budget = self._picks(picked, picked_lengths, "picked_lengths")
+        if rows != n or pn != n:
+            raise ValueError(f"q has {rows} rows and picked {pn}, tables {n}")
+        if not 0 <= max_length | first | recent < _COUNTS:
+            _no_count(max_length=max_length, first=first, recent=recent)
+        run = self._pick if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._pick)
+        rc = run(self._p, bp, qp, qs, heads, tb, width, ln, n, max_length, budget, first, recent, pk, pl,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_pick")
+
+    def attention_picked(self, q, out, picked, picked_lengths, scale=None, accumulate=False, stream=None):
+        """SNEPPX_kv_attention_picked: attention over the pages that pick has left."""
+        qp, qs, rows, heads = self._rows(q, "q", 0, _BF16)
+        op, os_, out_rows, _ = self._rows(out, "out", heads, _BF16_OR_F32)
+        pk, pl, n, budget = self._picks(picked, picked_lengths, "picked_lengths")
+        if rows != n or out_rows != n:
+            raise ValueError(f"q has {rows} rows and out {out_rows}, picked {n}")
+        run = self._picked if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._picked)
+        rc = run(self._p, qp, qs, op, os_, SNEPPX_BFLOAT16 if out.dtype is torch.bfloat16 else SNEPPX_FLOAT32, pk, budget,
+                 pl, n, heads, self.head_dim ** -0.5 if scale is None else scale, int(accumulate),
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_attention_picked")
+
+
+class KVPages(_OnDevice):
+    """Which pages of a pool are in use (include/sneppx_kv.h): refs int32 [pages], the
+    number of rows that hold each.  Calls change refs, the rows' tables (int32 [rows,
+    width], -1 where there is no page) and lengths (int32 [rows]) on the device, on
+    torch's current stream unless one is given."""
+
+    _what = "page counts"
+
+    def __init__(self, lib, refs, page_size):
+        if not isinstance(refs, torch.Tensor) or refs.dim() != 1 or refs.dtype != torch.int32 or not refs.is_contiguous():
+            raise ValueError("refs must be a contiguous int32 tensor [pages]")
+        _no_count(page_size=page_size)
+        self.L, self.device, self._index = lib, refs.device, refs.device.index if refs.is_cuda else None
+        self.refs, self.pages, self.page_size = refs, refs.shape[0], page_size
+        self._p = refs.data_ptr()
+        self._reserve, self._release, self._share = (lib.fn[f"SNEPPX_kv_{n}"] for n in ("reserve", "release", "share"))
+
+    def reserve(self, tables, lengths, slots, counts=None, next_pos=None, positions=None, starts=None, granted=None,
+                stream=None):
+        """SNEPPX_kv_reserve: slots (and positions) int32 [tokens]; counts, next_pos,
+        granted int32 [rows], starts int32 [rows + 1].  Returns (starts, granted), new ones
+        where none are given."""
+        tb, width, ln, n = self._tables(tables, lengths)
+        if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
+            raise ValueError("slots must be an int32 tensor [tokens]")
+        tokens, rows = slots.shape, (n,)
+        if starts is None:
+            starts = torch.empty(n + 1, dtype=torch.int32, device=self.device)
+        if granted is None:
+            granted = torch.empty(n, dtype=torch.int32, device=self.device)
+        args = [self._check(starts, "starts", torch.int32, (n + 1,)), self._check(granted, "granted", torch.int32, rows),
+                self._check(slots, "slots", torch.int32, tokens),
+                None if positions is None else self._check(positions, "positions", torch.int32, tokens)]
+        np_ = None if next_pos is None else self._check(next_pos, "next_pos", torch.int32, rows)
+        ct = None if counts is None else self._check(counts, "counts", torch.int32, rows)
+        run = self._reserve if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._reserve)
+        rc = run(self._p, self.pages, self.page_size, tb, width, ln, np_, ct, n, *args, tokens[0],
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_reserve")
+        return starts, granted
+
+    def release(self, tables, lengths, stream=None):
+        """SNEPPX_kv_release: the pages behind the rows' lengths go back."""
+        tb, width, ln, n = self._tables(tables, lengths)
+        run = self._release if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._release)
+        rc = run(self._p, self.pages, self.page_size, tb, width, ln, n,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_release")
+
+    def share(self, tables, lengths, sources, counts, next_pos=None, stream=None):
+        """SNEPPX_kv_share: sources int32 [rows] (a row, or -1), counts int32 [rows]
+        (tokens, of which whole pages are taken)."""
+        tb, width, ln, n = self._tables(tables, lengths)
+        sr, ct = self._check(sources, "sources", torch.int32, (n,)), self._check(counts, "counts", torch.int32, (n,))
+        np_ = None if next_pos is None else self._check(next_pos, "next_pos", torch.int32, (n,))
+        run = self._share if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._share)
+        rc = run(self._p, self.pages, self.page_size, tb, width, ln, np_, sr, ct, n,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "kv_share")
+
+
+class _RotaryStruct(C.Structure):
+    """SNEPPXRotary (include/sneppx_rotary.h)."""
+    _fields_ = [("freqs", _vp), ("dims", _sz), ("interleaved", C.c_int), ("magnitude", C.c_float), ("q_norm", _vp),
+                ("k_norm", _vp), ("eps", C.c_float)]
+
+
+class Rotary(_OnDevice):
+    """The rotation of heads of head_dim to their positions (include/sneppx_rotary.h):
+    freqs float64 [pairs], the first 2 * pairs elements of a head turn; q_norm and
+    k_norm float32 [head_dim] (or None) normalise heads first."""
+
+    _what = "rotary"
+
+    def __init__(self, lib, freqs, head_dim, interleaved=False, magnitude=1.0, q_norm=None, k_norm=None, eps=1e-6):
+        if not isinstance(freqs, torch.Tensor) or freqs.dim() != 1 or freqs.dtype != torch.float64:
+            raise ValueError("freqs must be a float64 tensor [pairs]")
+        self.L, self.device, self._index = lib, freqs.device, freqs.device.index if freqs.is_cuda else None
+        self.head_dim, self.freqs, self.q_norm, self.k_norm = head_dim, freqs, q_norm, k_norm
+        qn, kn = (None if t is None else self._check(t, name, torch.float32, (head_dim,))
+                  for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")))
+        self._c = _RotaryStruct(self._check(freqs, "freqs", torch.float64, freqs.shape), 2 * freqs.shape[0],
+                                int(interleaved), magnitude, qn, kn, eps)
+        self._p = C.cast(C.pointer(self._c), _vp)
+        self._apply = lib.fn["SNEPPX_rotary_apply"]
+
+    def apply(self, q, k, positions, q_out=None, k_out=None, stream=None):
+        """SNEPPX_rotary_apply: q, k bf16 [tokens, heads, head_dim], slices of wider rows
+        among them, or None; in place where no output is given.  positions int32 [tokens]."""
+        if not isinstance(positions, torch.Tensor) or positions.dim() != 1:
+            raise ValueError("positions must be an int32 tensor [tokens]")
+        tokens = positions.shape[0]
+        args = []
+        for x, out, name in ((q, q_out, "q"), (k, k_out, "k")):
+            if x is None:
+                args += [None, 0, None, 0, 0]
+                continue
+            xp, xs, n, heads = self._rows(x, name, 0, _BF16)
+            op, os_, on = xp, xs, n
+            if out is not None:
+                op, os_, on, _ = self._rows(out, name + "_out", heads, _BF16)
+            if n != tokens or on != tokens:
+                raise ValueError(f"{name} has {n} tokens and its output {on}, positions {tokens}")
+            args += [xp, xs, op, os_, heads]
+        ps = self._check(positions, "positions", torch.int32, (tokens,))
+        run = self._apply if self._index is not None and torch._C._cuda_getDevice() == self._index \
+            else self._elsewhere(self._apply)
+        rc = run(self._p, *args, self.head_dim, ps, tokens,
+                 stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
+        if rc:
+            self.L.check(rc, "rotary_apply")
 
 
 class QLayer:
