@@ -12,8 +12,10 @@
 // adds up what a query has of its prefix and its own tokens.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "codec.h"
 #include "kv_pool.h"
@@ -34,8 +36,13 @@ typedef u32x4 bf16x8_any __attribute__((aligned(2)));
 typedef u32x2 bf16x4_any __attribute__((aligned(2)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef __attribute__((address_space(3))) uint8_t* lds_t;
+typedef __attribute__((address_space(1))) uint8_t* glb_t;
 
 hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, -1, 0x00020000);
+}
 
 constexpr int SLOT_KV_SHARED = 10;    // of the stream's workspaces
 constexpr uint32_t STEP = 64;         // tokens of a step
@@ -153,15 +160,16 @@ __device__ __forceinline__ u32x4 bytes_to_bf16(uint32_t a, uint32_t b) {
 }
 
 // Eight weights (not negative) as N bf16 pieces each, of eight bits one after the
-// other: with fp32 results three, which are all 24; with bf16 results, which keep
-// eight, two.  Where values may be infinite, lower pieces are not zero unless the
-// weight is (0 * infinity): 2^-40 of the first at least.
-template <int N, bool I8>
+// other.  With fp32 results three, which are all 24; with bf16 results, which keep
+// eight, two, off by 2^-15 of the weight at most (2^-17 are added, about what cutting the
+// lower one takes away on average).  Values may be infinite, and a zero piece would make
+// NaN of that: no piece is zero unless the weight is, of three by 2^-40 of the first.
+template <int N>
 __device__ __forceinline__ void split(const float* x, bf16x8 (&piece)[N]) {
     u32x4 o[N];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-        float a[2] = {x[e], x[e + 1]}, least[2] = {0.0f, 0.0f};
+        float a[2] = {x[e], x[e + 1]}, least[2];
 #pragma unroll
         for (int i = 0; i < N; i++) {
             o[i][e >> 1] = __builtin_amdgcn_perm(f2u(a[1]), f2u(a[0]), 0x07060302u);
@@ -169,7 +177,11 @@ __device__ __forceinline__ void split(const float* x, bf16x8 (&piece)[N]) {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const float high = u2f(f2u(a[j]) & 0xFFFF0000u);
-                if (!I8 && i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
+                if (N < 3) {
+                    a[j] = __builtin_fmaf(high, -(1.0f - 0x1p-17f), a[j]);
+                    continue;
+                }
+                if (i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
                 a[j] = fmaxf(a[j] - high, least[j]);
             }
         }
@@ -178,13 +190,19 @@ __device__ __forceinline__ void split(const float* x, bf16x8 (&piece)[N]) {
     for (int i = 0; i < N; i++) piece[i] = __builtin_bit_cast(bf16x8, o[i]);
 }
 
+// A step's keys and values in LDS, in two buffers: token rows of DP bf16 each, their
+// 16-byte pieces in an order that spreads what is read at once over all banks: eight
+// rows at one place of the keys, four rows at 64 bytes of the values.
 template <int DP>
 struct Tiles {
-    static constexpr int KS = DP * 2 + 16, VS = DP * 2 + 16;        // bytes of a token's row
-    static constexpr int K = STEP * KS, V = STEP * VS;
+    static constexpr int RB = DP * 2, PIECES = RB / 16, T = STEP * RB, BUF = 2 * T;
     static constexpr int OS = DP + 4;                               // floats of a query's row at the end
-    static constexpr int END = 2 * 32 * OS * 4;
-    static constexpr int ALL = K + V > END ? K + V : END;
+    static constexpr int SCALES = 2 * BUF, ENDS = SCALES + 2 * 2 * STEP * 4, ALL = ENDS + 2 * 32 * 8;
+    static_assert(2 * 32 * OS * 4 <= 2 * BUF, "the queries' rows at the end take the tiles' place");
+    static __device__ __forceinline__ int key_piece(int tok, int c) { return c ^ (tok & 7); }
+    static __device__ __forceinline__ int value_piece(int tok, int c) {
+        return c ^ (PIECES >= 16 ? 4 * (tok & 3) : 4 * ((tok >> 1) & 1));
+    }
 };
 
 // Lane l = 32 g + c.  Keys are the A operand of 32x32x16 products (32 token rows), the
@@ -195,17 +213,19 @@ struct Tiles {
 // lane, so a new maximum rescales by the lane's own factor.
 // With more than 64 queries each wave has 32 of them and all tokens of a step; with
 // fewer, waves w and w + 2 have the same 32 and half of the tokens each.
-template <int DP, bool I8, int PIECES>
+// NEAR: bf16 heads of DP in a pool that 32-bit offsets reach; FAR: other bf16 heads.
+enum Form { NEAR, FAR, INT8 };
+
+template <int DP, Form FORM, int PIECES>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPool p, const Shared a) {
     typedef Tiles<DP> L;
-    constexpr int CH = DP * (I8 ? 1 : 2) / 16;             // 16-byte pieces of a row in the pool
+    constexpr bool I8 = FORM == INT8;
+    constexpr int CH = L::PIECES / (I8 ? 2 : 1);           // 16-byte pieces of a row in the pool
     constexpr int EACH = STEP * CH / 256;                  // of a tile, for a thread
     constexpr int KQ = DP / 16, DT = DP / 32;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[L::ALL];
-    __shared__ __attribute__((aligned(16))) float scales[2][STEP];
-    __shared__ float2 ends[2][32];
-    uint8_t* const kt = lds;
-    uint8_t* const vt = lds + L::K;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    float* const scales = reinterpret_cast<float*>(lds + L::SCALES);       // [buffer][keys, values][STEP]
+    float2* const ends = reinterpret_cast<float2*>(lds + L::ENDS);         // [2][32]
 
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -258,30 +278,29 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
     const bool wide = nq > 64;
     const uint32_t q0 = 32 * (wide ? wave : wave & 1);       // this wave's first query
     const bool busy = q0 < nq;
-    const uint32_t u0 = wide ? 0 : wave >> 1, u1 = wide ? 2 : u0 + 1;      // and halves of a step
     const int32_t* const table = p.table(reads, h);
-    const uint32_t row_bytes = p.dim * (I8 ? 1 : 2);
+    const uint32_t dim = FORM == NEAR ? DP : p.dim, row_bytes = dim * (I8 ? 1 : 2);
 
     // (columns past the tile's queries repeat its last: nothing reads what they give)
     bf16x8 q[KQ];
     uint32_t limit;
     {
         const uint32_t mine = q0 + c < nq ? q0 + c : nq - 1, idx = tile * TILE + mine, b = first + idx / a.group;
-        const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(h * a.group + idx % a.group) * p.dim;
+        const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(h * a.group + idx % a.group) * dim;
         limit = kv_length(a.lengths, b, t1);
 #pragma unroll
         for (int s = 0; s < KQ; s++) {
             const uint32_t d = 16 * s + 8 * g;
             u32x4 w = {0u, 0u, 0u, 0u};
-            if (d < p.dim) w = *reinterpret_cast<const bf16x8_any*>(qh + d) ^ a.flip;
+            if (d < dim) w = *reinterpret_cast<const bf16x8_any*>(qh + d) ^ a.flip;
             q[s] = __builtin_bit_cast(bf16x8, w);
         }
     }
+    const uint32_t least = ~__builtin_amdgcn_readfirstlane(lane_max(~limit));     // of the wave's queries
 
     // this lane's token of a step: the page table's entry, then its row of the pool
     uint32_t entry, row;
     bool ok;
-    uint64_t there;
     auto look = [&](uint32_t base) {
         const uint32_t tok = base + lane;
         entry = tok < t1 ? (uint32_t)table[p.page_of(tok)] : 0xFFFFFFFFu;
@@ -291,134 +310,158 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
         ok = entry < p.pages;
         row = ok ? (entry * p.heads + h) * p.page_size + (tok - p.page_of(tok) * p.page_size) : 0;
     };
+    // A step's tiles: bf16 straight to LDS, each wave 16 tokens (a load's 64 pieces lie
+    // there one after the other, so each lane fetches what belongs in its place); int8
+    // through registers, as bf16.
     u32x4 kc[EACH], vc[EACH];
     float ksc = 0.0f, vsc = 0.0f;
-    const uint32_t chunk = tid % CH;
-    auto load = [&] {
+    const __amdgpu_buffer_rsrc_t rk = rsrc(p.k), rv = rsrc(p.v);
+    auto load = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < EACH; i++) {
-            const uint32_t r = __shfl(row, tid / CH + i * (256 / CH));
-            const size_t at = (size_t)r * row_bytes + (16 * chunk < row_bytes ? 16 * chunk : 0);
-            kc[i] = *reinterpret_cast<const u32x4*>(p.k + at);
-            vc[i] = *reinterpret_cast<const u32x4*>(p.v + at);
+            const int tok = I8 ? tid / CH + i * (256 / CH) : 16 * wave + i * (64 / CH) + lane / CH;
+            const uint32_t r = __shfl(row, tok);
+            if (I8) {
+                const uint32_t piece = tid % CH;
+                const size_t at = (size_t)r * row_bytes + (16 * piece < row_bytes ? 16 * piece : 0);
+                kc[i] = *reinterpret_cast<const u32x4*>(p.k + at);
+                vc[i] = *reinterpret_cast<const u32x4*>(p.v + at);
+                continue;
+            }
+            uint8_t* const to = lds + buf * L::BUF + (16 * wave + i * (64 / CH)) * L::RB;
+            const uint32_t kp = 16 * L::key_piece(tok, lane % CH), vp = 16 * L::value_piece(tok, lane % CH);
+            if (FORM == FAR) {
+                const size_t at = (size_t)r * row_bytes;
+                if (kp < row_bytes) __builtin_amdgcn_global_load_lds((const glb_t)(p.k + at + kp), (lds_t)to, 16, 0, 0);
+                if (vp < row_bytes) __builtin_amdgcn_global_load_lds((const glb_t)(p.v + at + vp), (lds_t)(to + L::T), 16, 0, 0);
+            } else {
+                const uint32_t at = r * row_bytes;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_t)to, 16, at + kp, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_t)(to + L::T), 16, at + vp, 0, 0, 0);
+            }
         }
         if (I8 && wave == 0) {
             ksc = p.ks[row];
             vsc = p.vs[row];
         }
     };
+    // values of absent tokens as zeros (0 * NaN), and int8 tiles to LDS
+    auto settle = [&](int buf, uint64_t there) {
+        uint8_t* const kt = lds + buf * L::BUF;
+        uint8_t* const vt = kt + L::T;
+        if (I8) {
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const int tok = tid / CH + i * (256 / CH), piece = tid % CH;
+                const bool in = 16 * piece < (int)row_bytes;
+                if (!in) kc[i] = u32x4{0u, 0u, 0u, 0u};
+                if (!in || !(there >> tok & 1)) vc[i] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    *reinterpret_cast<u32x4*>(kt + tok * L::RB + 16 * L::key_piece(tok, 2 * piece + j)) =
+                        bytes_to_bf16(kc[i][2 * j], kc[i][2 * j + 1]);
+                    *reinterpret_cast<u32x4*>(vt + tok * L::RB + 16 * L::value_piece(tok, 2 * piece + j)) =
+                        bytes_to_bf16(vc[i][2 * j], vc[i][2 * j + 1]);
+                }
+            }
+            if (wave == 0) {
+                scales[(2 * buf) * STEP + lane] = ksc;
+                scales[(2 * buf + 1) * STEP + lane] = there >> lane & 1 ? vsc : 0.0f;
+            }
+        } else if (there != ~0ull) {
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const int tok = 16 * wave + i * (64 / CH) + lane / CH;
+                if (!(there >> tok & 1)) *reinterpret_cast<u32x4*>(vt + tok * L::RB + 16 * (lane % CH)) = u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+    };
 
     f32x16 o[DT] = {};
     float m = -INFINITY, sum = 0.0f;
     bool any = false;
-    if (t0 < t1) {
-        look(t0);
-        find(t0);
-        look(t0 + STEP);
-        load();
-    }
-    for (uint32_t base = t0; base < t1; base += STEP) {
-        // the step's tiles to LDS: values of absent tokens as zeros (0 * NaN), and zeros
-        // behind the head's end
-        there = __ballot(ok);
+    // N x 32 of a step's tokens, from u0 x 32 on
+    auto attend = [&](auto n_, int u0, int buf, uint32_t base, uint64_t there) {
+        constexpr int N = decltype(n_)::value;
+        const uint8_t* const kt = lds + buf * L::BUF + u0 * 32 * L::RB;
+        const uint8_t* const vt = kt + L::T;
+        const float* const sc = scales + 2 * buf * STEP + 32 * u0;
+        f32x16 s[N] = {};
 #pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const uint32_t t = tid / CH + i * (256 / CH);
-            const bool in = 16 * chunk < row_bytes;
-            if (!in) kc[i] = u32x4{0u, 0u, 0u, 0u};
-            if (!in || !(there >> t & 1)) vc[i] = u32x4{0u, 0u, 0u, 0u};
-            if (I8) {
-                uint8_t* const kd = kt + t * L::KS + 32 * chunk;
-                uint8_t* const vd = vt + t * L::VS + 32 * chunk;
-                *reinterpret_cast<u32x4*>(kd) = bytes_to_bf16(kc[i][0], kc[i][1]);
-                *reinterpret_cast<u32x4*>(kd + 16) = bytes_to_bf16(kc[i][2], kc[i][3]);
-                *reinterpret_cast<u32x4*>(vd) = bytes_to_bf16(vc[i][0], vc[i][1]);
-                *reinterpret_cast<u32x4*>(vd + 16) = bytes_to_bf16(vc[i][2], vc[i][3]);
-            } else {
-                *reinterpret_cast<u32x4*>(kt + t * L::KS + 16 * chunk) = kc[i];
-                *reinterpret_cast<u32x4*>(vt + t * L::VS + 16 * chunk) = vc[i];
-            }
-        }
-        if (I8 && wave == 0) {
-            scales[0][lane] = ksc;
-            scales[1][lane] = ok ? vsc : 0.0f;
-        }
-        __syncthreads();
-        if (base + STEP < t1) {
-            find(base + STEP);
-            look(base + 2 * STEP);
-            load();
-        }
-        for (uint32_t u = u0; u < u1 && busy; u++) {
-            f32x16 s = {};
+        for (int i = 0; i < KQ; i++)
 #pragma unroll
-            for (int i = 0; i < KQ; i++) {
-                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (32 * u + c) * L::KS + 32 * i + 16 * g);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i], s, 0, 0, 0);
+            for (int u = 0; u < N; u++) {
+                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (32 * u + c) * L::RB + 16 * L::key_piece(c, 2 * i + g));
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i], s[u], 0, 0, 0);
             }
-            float top = -INFINITY;
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
             if (I8)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
-                    const f32x4 k4 = *reinterpret_cast<const f32x4*>(&scales[0][32 * u + 2 * r + 4 * g]);
+                    const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * u + 2 * r + 4 * g);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[r + i] *= k4[i];
+                    for (int i = 0; i < 4; i++) s[u][r + i] *= k4[i];
                 }
-            const uint32_t from = base + 32 * u, mask = (uint32_t)(there >> (32 * u));
-            const bool whole = mask == 0xFFFFFFFFu && __all(from + 32 <= limit);
-            if (!whole) {
+            const uint32_t from = base + 32 * (u0 + u), mask = (uint32_t)(there >> (32 * (u0 + u)));
+            if (mask != 0xFFFFFFFFu || from + 32 > least) {
                 const uint32_t left = limit > from ? limit - from : 0;
                 const uint32_t mine = left >= 32 ? mask : mask & ((1u << left) - 1);
 #pragma unroll
                 for (int r = 0; r < 16; r++)
-                    if (!(mine >> (2 * (r & 12) + (r & 3) + 4 * g) & 1)) s[r] = -INFINITY;
+                    if (!(mine >> (2 * (r & 12) + (r & 3) + 4 * g) & 1)) s[u][r] = -INFINITY;
                 any |= mine != 0;
             } else {
                 any = true;
             }
 #pragma unroll
-            for (int r = 0; r < 16; r++) top = fmaxf(top, s[r]);
-            float other;
-            top = swap32(top, other);
-            top = fmaxf(top, other) * a.scale_log2;
-            // Weights are 2^(logit - m).  The reference m is a whole number, so that
-            // changing it rounds nothing, and moves when a logit comes within `lift` of
-            // it: after the first steps hardly ever.  It is so far above that weights sum
-            // up to 1 at most, however many there are: no sum of weighted values passes
-            // the largest value, and results are finite if that is.
-            if (__any(top + a.lift > m)) {
-                const float to = fmaxf(m, __builtin_ceilf(top) + a.room);
-                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
-                m = to;
-                sum *= f;
+            for (int r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
+        }
+        float other;
+        top = swap32(top, other);
+        top = fmaxf(top, other) * a.scale_log2;
+        // Weights are 2^(logit - m).  The reference m is a whole number, so that changing
+        // it rounds nothing, and moves when a logit comes within `lift` of it: after the
+        // first steps hardly ever.  It is so far above that weights sum up to 1 at most,
+        // however many there are: no sum of weighted values passes the largest value, and
+        // results are finite if that is.
+        if (__any(top + a.lift > m)) {
+            const float to = fmaxf(m, __builtin_ceilf(top) + a.room);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            sum *= f;
 #pragma unroll
-                for (int i = 0; i < DT; i++) o[i] *= f;
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
-            float e[16];
+            for (int i = 0; i < DT; i++) o[i] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.scale_log2, -ref));
-                sum += e[r];
-            }
-            if (I8)
-#pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f32x4 v4 = *reinterpret_cast<const f32x4*>(&scales[1][32 * u + 2 * r + 4 * g]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) e[r + i] *= v4[i];
-                }
+        for (int u = 0; u < N; u++)
 #pragma unroll
             for (int pr = 0; pr < 2; pr++) {
+                float e[8];
+#pragma unroll
+                for (int r = 0; r < 8; r++) {
+                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * pr + r], a.scale_log2, -ref));
+                    sum += e[r];
+                }
+                if (I8)
+#pragma unroll
+                    for (int r = 0; r < 8; r += 4) {
+                        const f32x4 v4 = *reinterpret_cast<const f32x4*>(sc + STEP + 32 * u + 16 * pr + 2 * r + 4 * g);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) e[r + i] *= v4[i];
+                    }
                 bf16x8 pc[PIECES];
-                split<PIECES, I8>(e + 8 * pr, pc);
+                split<PIECES>(e, pc);
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
                     s16x4 w[2];
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         const int tok = 32 * u + 16 * pr + 8 * t + 4 * g + ((lane & 15) >> 2);
-                        const lds_t at = (lds_t)(vt + tok * L::VS + 64 * dt + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+                        const int piece = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                        const lds_t at = (lds_t)(vt + tok * L::RB + 16 * L::value_piece(tok, piece) + 8 * (lane & 1));
                         w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
                     }
                     const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -426,9 +469,36 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
                     for (int i = 0; i < PIECES; i++) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pc[i], o[dt], 0, 0, 0);
                 }
             }
-        }
+    };
+
+    if (FORM == FAR && row_bytes < L::RB) {      // what loads do not reach: zeros behind the head's end
+        for (int i = 16 * tid; i < 2 * L::BUF; i += 16 * 256) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0u, 0u, 0u, 0u};
         __syncthreads();
     }
+    if (t0 < t1) {
+        look(t0);
+        find(t0);
+        look(t0 + STEP);
+        load(0);
+    }
+    auto steps = [&](auto n, int u0) {
+        int buf = 0;
+        for (uint32_t base = t0; base < t1; base += STEP, buf ^= 1) {
+            const uint64_t there = __ballot(ok);
+            __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's part of the step is there; its reads of the one before are done
+            settle(buf, there);
+            __syncthreads();
+            if (base + STEP < t1) {
+                find(base + STEP);
+                look(base + 2 * STEP);
+                load(buf ^ 1);
+            }
+            if (busy) attend(n, u0, buf, base, there);
+        }
+    };
+    if (wide) steps(std::integral_constant<int, 2>{}, 0);
+    else steps(std::integral_constant<int, 1>{}, wave >> 1);
+    __syncthreads();
 
     // a maximum of -inf with tokens there is told from no tokens by a sum of 1
     {
@@ -441,7 +511,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
     if (!wide) {
         float* const ow = reinterpret_cast<float*>(lds) + (wave & 1) * 32 * L::OS + c * L::OS;
         if (wave >= 2) {
-            if (g == 0) ends[wave & 1][c] = make_float2(m, sum);
+            if (g == 0) ends[32 * (wave & 1) + c] = make_float2(m, sum);
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -450,7 +520,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
         }
         __syncthreads();
         if (wave >= 2) return;
-        const float2 e = ends[wave & 1][c];
+        const float2 e = ends[32 * (wave & 1) + c];
         const float top = fmaxf(m, e.x);
         const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
         const float f1 = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
@@ -468,13 +538,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
     if (q0 + c >= nq) return;
     const size_t at = slot * cap + q0 + c;
     if (g == 0) ml[at] = make_float2(m, sum);
-    float* const to = part + at * p.dim;
+    float* const to = part + at * dim;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const uint32_t d = 32 * dt + 2 * r + 4 * g;
-            if (d < p.dim) *reinterpret_cast<f32x4*>(to + d) = f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]};
+            if (d < dim) *reinterpret_cast<f32x4*>(to + d) = f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]};
         }
 }
 
@@ -532,16 +602,29 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
     else *reinterpret_cast<bf16x4_any*>(static_cast<uint16_t*>(a.out) + to) = u32x2{bf16x2_out(v[0], v[1]), bf16x2_out(v[2], v[3])};
 }
 
-template <int DP, bool I8>
-void launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
-    if (a.out_f32) k_kv_shared<DP, I8, 3><<<grid, 256, 0, s>>>(p, a);
-    else k_kv_shared<DP, I8, 2><<<grid, 256, 0, s>>>(p, a);
+template <int DP, Form FORM, int PIECES>
+int launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    const auto fn = k_kv_shared<DP, FORM, PIECES>;
+    if (Tiles<DP>::ALL > 65536 && lds_optin(reinterpret_cast<const void*>(fn), Tiles<DP>::ALL, done) != hipSuccess) {
+        snx_set_error("kv_attention_shared: no %d bytes of LDS", Tiles<DP>::ALL);
+        return -1;
+    }
+    fn<<<grid, 256, Tiles<DP>::ALL, s>>>(p, a);
+    return snx_launch_check("k_kv_shared");
 }
-template <bool I8>
-void launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
-    if (p.dim <= 64) launch<64, I8>(grid, p, a, s);
-    else if (p.dim <= 128) launch<128, I8>(grid, p, a, s);
-    else launch<256, I8>(grid, p, a, s);
+template <int DP, int PIECES>
+int launch(unsigned grid, bool i8, const KVPool& p, const Shared& a, hipStream_t s) {
+    if (i8) return launch<DP, INT8, PIECES>(grid, p, a, s);
+    // (loads to LDS by 32-bit offsets count apart from LDS reads, those by address do not)
+    const bool near = p.dim == DP && (uint64_t)p.pages * p.heads * p.page_size * DP * 2 <= 0xFFFFFFFFull;
+    return near ? launch<DP, NEAR, PIECES>(grid, p, a, s) : launch<DP, FAR, PIECES>(grid, p, a, s);
+}
+template <int PIECES>
+int launch(unsigned grid, bool i8, const KVPool& p, const Shared& a, hipStream_t s) {
+    if (p.dim <= 64) return launch<64, PIECES>(grid, i8, p, a, s);
+    if (p.dim <= 128) return launch<128, PIECES>(grid, i8, p, a, s);
+    return launch<256, PIECES>(grid, i8, p, a, s);
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
@@ -616,9 +699,8 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     a.room = (float)room;
     a.lift = (float)(room - kLag);
     a.out_f32 = out_f32;
-    if (c->dtype == SNEPPX_INT8) launch<true>((unsigned)grid, p, a, S(st));
-    else launch<false>((unsigned)grid, p, a, S(st));
-    if (snx_launch_check("k_kv_shared")) return -1;
+    const bool i8 = c->dtype == SNEPPX_INT8;
+    if (out_f32 ? launch<3>((unsigned)grid, i8, p, a, S(st)) : launch<2>((unsigned)grid, i8, p, a, S(st))) return -1;
     k_kv_shared_join<<<(unsigned)((rows * q_heads + 3) / 4), 256, 0, S(st)>>>(p, a);
     return snx_launch_check("k_kv_shared_join");
 }
