@@ -59,7 +59,7 @@ struct Shared {
     float2 *ml, *own_ml;       // maximum and sum of the same
     uint32_t rows, q_heads, group, groups, max_length;
     uint32_t about, blocks;    // units of the prefixes of a head: about so many, and so many at most
-    uint32_t columns, own_columns, own_tiles, splits;
+    uint32_t columns, own_columns, own_tiles, splits, own_span;    // own_span: tokens of a split but the last
     float scale_log2;          // not negative: `flip` changes the queries' signs instead
     float room, lift;          // log2 of the most that weights of up to 2^kLag sum up to, and that less kLag
     uint32_t flip;
@@ -75,11 +75,13 @@ struct Prefix {
 };
 struct Groups {
     const Shared& a;
+    Prefix x0;                 // of group `lane`
     uint32_t most, per;
     __device__ __forceinline__ Groups(const Shared& s, uint32_t slots) : a(s), most(slots < s.max_length ? slots : s.max_length) {
         uint32_t total = 0;
+        x0 = at(0);
         for (uint32_t g0 = 0; g0 < a.groups; g0 += 64) {
-            const Prefix x = at(g0);
+            const Prefix x = g0 ? at(g0) : x0;
             total += __builtin_amdgcn_readlane(lane_prefix(tiles(x) * steps(x)), 63);
         }
         per = (total + a.about - 1) / (a.about ? a.about : 1);
@@ -107,7 +109,7 @@ struct Groups {
     __device__ __forceinline__ bool find(uint32_t i, Prefix& out) const {
         uint32_t base = 0;
         for (uint32_t g0 = 0; g0 < a.groups; g0 += 64) {
-            const Prefix x = at(g0);
+            const Prefix x = g0 ? at(g0) : x0;
             const uint32_t spans = (steps(x) + per - 1) / per, n = tiles(x) * spans, upto = lane_prefix(n);
             const uint64_t is = ROW ? __ballot(x.tokens && i >= x.first && i - x.first < x.rows)
                                     : __ballot(n && base + upto > i);
@@ -141,6 +143,13 @@ __device__ __forceinline__ uint32_t row_with(const Shared& a, const Prefix& x) {
 // x of this lane and of the one 32 lanes away
 __device__ __forceinline__ float swap32(float x, float& y) {
     const u32x2 r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
+    y = u2f(r[1]);
+    return u2f(r[0]);
+}
+
+// and of the one 16 lanes away
+__device__ __forceinline__ float swap16(float x, float& y) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
     y = u2f(r[1]);
     return u2f(r[0]);
 }
@@ -198,12 +207,215 @@ struct Tiles {
     static constexpr int RB = DP * 2, PIECES = RB / 16, T = STEP * RB, BUF = 2 * T;
     static constexpr int OS = DP + 4;                               // floats of a query's row at the end
     static constexpr int SCALES = 2 * BUF, ENDS = SCALES + 2 * 2 * STEP * 4, ALL = ENDS + 2 * 32 * 8;
+    static_assert(4 * (32 * (RB + 32) + 16 + 256) <= ALL, "rows' own tokens take their place");
     static_assert(2 * 32 * OS * 4 <= 2 * BUF, "the queries' rows at the end take the tiles' place");
     static __device__ __forceinline__ int key_piece(int tok, int c) { return c ^ (tok & 7); }
     static __device__ __forceinline__ int value_piece(int tok, int c) {
         return c ^ (PIECES >= 16 ? 4 * (tok & 3) : 4 * ((tok >> 1) & 1));
     }
 };
+
+// NEAR: bf16 heads of DP in a pool that 32-bit offsets reach; FAR: other bf16 heads.
+enum Form { NEAR, FAR, INT8 };
+
+// a lane's logits: as far as their tokens are there, one bit each in `mine`
+template <int N, typename F>
+__device__ __forceinline__ float masked_max(float* s, uint32_t mine, bool whole, F bit) {
+    if (!whole)
+#pragma unroll
+        for (int r = 0; r < N; r++)
+            if (!(mine >> bit(r) & 1)) s[r] = -INFINITY;
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < N; r++) top = fmaxf(top, s[r]);
+    return top;
+}
+
+// A wave's rows of its own tokens' values in LDS: rows of RB bytes, whose stride and order
+// spread the transposed reads (32 bytes of the same columns from eight rows at once) and the
+// writes (16 bytes of 16 rows) over all banks.
+template <int DP>
+struct OwnTile {
+    static constexpr int RB = DP * 2, STRIDE = RB + 32, UPPER = 16, V = 32 * STRIDE + UPPER, ALL = V + 2 * 32 * 4;
+    static __device__ __forceinline__ int row(int tok) {
+        return ((tok & 19) | ((tok >> 1) & 4) | ((tok << 1) & 8)) * STRIDE + (tok >> 4) * UPPER;
+    }
+};
+
+// The tokens of one row from t0 to t1 for up to 16 of its query heads, by one wave: what a
+// wave waits for, the others of the CU make use of.  Lane l = 16 g + r.  Keys are the A
+// operand of 16x16x32 products and the queries the B operand (column r); with product t's
+// row r being token 8 (r / 4) + 4 t + r % 4 of 32, a lane's weights are those of tokens
+// 8 g .. 8 g + 7, the B operand of the product with the values.  Keys and values of the
+// next 32 tokens are on their way meanwhile, keys into the registers that the first product
+// has used, values into those that went to LDS.
+template <int DP, bool I8>
+__device__ __forceinline__ void own_queries(const KVPool& p, const Shared& a, uint32_t b, uint32_t head0, uint32_t nq,
+                                            bf16x8 (&q)[DP / 32]) {
+    const uint32_t r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+    const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(head0 + (r < nq ? r : nq - 1)) * p.dim;
+#pragma unroll
+    for (int s = 0; s < DP / 32; s++) {
+        const uint32_t d = I8 ? 16 * (g + 4 * (s >> 1)) + 8 * (s & 1) : 8 * (g + 4 * s);
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if (d < p.dim) w = *reinterpret_cast<const bf16x8_any*>(qh + d) ^ a.flip;
+        q[s] = __builtin_bit_cast(bf16x8, w);
+    }
+}
+template <int DP, bool I8, int PIECES>
+__device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uint32_t b, uint32_t h, const bf16x8 (&q)[DP / 32],
+                                           uint32_t nq, uint32_t t0, uint32_t t1, size_t slot, uint8_t* vt) {
+    typedef OwnTile<DP> L;
+    constexpr int NC = DP * (I8 ? 1 : 2) / 64, KS = DP / 32, DT = DP / 16;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const uint32_t dim = p.dim, row_bytes = dim * (I8 ? 1 : 2);
+    const int32_t* const table = p.table(b, h);
+    float* const sc = reinterpret_cast<float*>(vt + L::V);
+
+    uint32_t entry[2], row[2];
+    bool ok[2];
+    auto token = [&](int t) { return 8 * (r >> 2) + 4 * t + (r & 3); };
+    auto look = [&](uint32_t base) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint32_t tok = base + token(t);
+            entry[t] = tok < t1 ? (uint32_t)table[p.page_of(tok)] : 0xFFFFFFFFu;
+        }
+    };
+    auto find = [&](uint32_t base) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint32_t tok = base + token(t);
+            ok[t] = entry[t] < p.pages;
+            row[t] = ok[t] ? (entry[t] * p.heads + h) * p.page_size + (tok - p.page_of(tok) * p.page_size) : 0;
+        }
+    };
+    u32x4 kc[2][NC], vc[2][NC];
+    float ksc[2], vsc[2];
+    auto fetch = [&](const uint8_t* pool, const float* scales, u32x4 (&to)[2][NC], float (&s)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const uint32_t x = 16 * (g + 4 * i);
+                to[t][i] = *reinterpret_cast<const u32x4*>(pool + (size_t)row[t] * row_bytes + (x < row_bytes ? x : 0));
+            }
+            if (I8) s[t] = scales[row[t]];
+        }
+    };
+    look(t0);
+    f32x4 o[DT] = {};
+    float m = -INFINITY, sum = 0.0f;
+    bool any = false;
+    if (t0 < t1) {
+        find(t0);
+        look(t0 + 32);
+        fetch(p.k, p.ks, kc, ksc);
+        fetch(p.v, p.vs, vc, vsc);
+    }
+    for (uint32_t base = t0; base < t1; base += 32) {
+        const uint64_t there[2] = {__ballot(ok[0]), __ballot(ok[1])};      // lanes whose tokens are there
+        const bool whole = (there[0] & there[1]) == ~0ull, more = base + 32 < t1;
+        const bool is[2] = {ok[0], ok[1]};
+        float s[8];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            f32x4 x = {};
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                u32x4 w = kc[t][I8 ? i >> 1 : i];
+                if (I8) w = (i & 1) ? bytes_to_bf16(w[2], w[3]) : bytes_to_bf16(w[0], w[1]);
+                // past the head's end the lane has other elements, maybe NaN
+                if ((I8 ? 16 * (g + 4 * (i >> 1)) : 8 * (g + 4 * i)) >= (int)dim) w = u32x4{0u, 0u, 0u, 0u};
+                x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), q[i], x, 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[4 * t + j] = x[j];
+            if (I8 && g == 0) sc[token(t)] = ksc[t];
+        }
+        if (more) {
+            find(base + 32);
+            look(base + 64);
+            fetch(p.k, p.ks, kc, ksc);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int tok = token(t);
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                if (!is[t]) vc[t][i] = u32x4{0u, 0u, 0u, 0u};        // (0 * NaN)
+                uint8_t* const to = vt + L::row(tok) + (I8 ? 32 : 16) * (g + 4 * i);
+                if (I8) {
+                    *reinterpret_cast<u32x4*>(to) = bytes_to_bf16(vc[t][i][0], vc[t][i][1]);
+                    *reinterpret_cast<u32x4*>(to + 16) = bytes_to_bf16(vc[t][i][2], vc[t][i][3]);
+                } else {
+                    *reinterpret_cast<u32x4*>(to) = vc[t][i];
+                }
+            }
+            if (I8 && g == 0) sc[32 + tok] = is[t] ? vsc[t] : 0.0f;
+        }
+        if (more) fetch(p.v, p.vs, vc, vsc);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (I8)
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i] *= sc[8 * g + i];
+        // (bits of the lane's tokens 8 g .. 8 g + 7: product t has tokens 4 t .. 4 t + 3 of them in lanes 4 g ..)
+        const uint32_t mine = ((uint32_t)(there[0] >> (4 * g)) & 15u) | ((uint32_t)(there[1] >> (4 * g)) & 15u) << 4;
+        float top = masked_max<8>(s, mine, whole, [](int i) { return i; });
+        any |= mine != 0;
+        float other;
+        top = swap32(top, other);
+        top = fmaxf(top, other);
+        top = swap16(top, other);
+        top = fmaxf(top, other) * a.scale_log2;
+        if (__any(top + a.lift > m)) {
+            const float to = fmaxf(m, __builtin_ceilf(top) + a.room);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < DT; i++) o[i] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale_log2, -ref));
+            sum += s[i];
+            if (I8) s[i] *= sc[32 + 8 * g + i];
+        }
+        bf16x8 pc[PIECES];
+        split<PIECES>(s, pc);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            s16x4 w[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const lds_t at = (lds_t)(vt + L::row(8 * g + 4 * t + (r >> 2)) + 8 * (r & 3) + 32 * dt);
+                w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+            }
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pc[i], o[dt], 0, 0, 0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    float other;
+    sum = swap32(sum, other);
+    sum += other;
+    sum = swap16(sum, other);
+    sum += other;
+    // (a maximum of -inf with tokens there is told from no tokens by a sum of 1)
+    any = __any(any);
+    if (m == -INFINITY && any && sum == 0.0f) sum = 1.0f;
+    if ((uint32_t)r >= nq) return;
+    if (g == 0) a.own_ml[slot + r] = make_float2(m, sum);
+    float* const to = a.own_part + (slot + r) * dim;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+        if (16 * dt + 4 * g < (int)dim) *reinterpret_cast<f32x4*>(to + 16 * dt + 4 * g) = o[dt];
+}
 
 // Lane l = 32 g + c.  Keys are the A operand of 32x32x16 products (32 token rows), the
 // queries the B operand (column c), so a lane ends up with 16 logits of query c: register
@@ -213,9 +425,6 @@ struct Tiles {
 // lane, so a new maximum rescales by the lane's own factor.
 // With more than 64 queries each wave has 32 of them and all tokens of a step; with
 // fewer, waves w and w + 2 have the same 32 and half of the tokens each.
-// NEAR: bf16 heads of DP in a pool that 32-bit offsets reach; FAR: other bf16 heads.
-enum Form { NEAR, FAR, INT8 };
-
 template <int DP, Form FORM, int PIECES>
 __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPool p, const Shared a) {
     typedef Tiles<DP> L;
@@ -229,74 +438,47 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
 
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Groups groups(a, p.width * p.page_size);
 
-    // the unit: its rows' first, their number, tile of queries, tokens
-    uint32_t first, rows, tile, t0, t1, cap, reads;
-    size_t slot;
-    float* part;
-    float2* ml;
+    // the unit: a tile of a group's queries and a span of its prefix, or by waves a row's own tokens
     const uint32_t shared_blocks = a.blocks * p.heads;
-    uint32_t h;
-    if (blockIdx.x < shared_blocks) {
-        const uint32_t i = blockIdx.x / p.heads;
-        h = blockIdx.x - i * p.heads;
-        Prefix x;
-        if (!groups.find<false>(i, x)) return;
-        const uint32_t n = i - x.base, span = n % x.spans;
-        first = x.first;
-        rows = x.rows;
-        reads = row_with(a, x);
-        tile = n / x.spans;
-        t0 = span * x.per * STEP;
-        t1 = t0 + x.per * STEP < x.tokens ? t0 + x.per * STEP : x.tokens;
-        slot = (size_t)h * a.blocks + i;
-        part = a.part;
-        ml = a.ml;
-        cap = a.columns;
-    } else {
-        uint32_t i = blockIdx.x - shared_blocks;
-        const uint32_t pair = i / p.heads, rest = pair / a.splits, span = pair - rest * a.splits;
-        h = i - pair * p.heads;
-        const uint32_t b = rest / a.own_tiles;
-        tile = rest - b * a.own_tiles;
-        first = reads = b;
-        rows = 1;
-        const uint32_t len = kv_length(a.lengths, b, groups.most);
+    if (blockIdx.x >= shared_blocks) {
+        const uint32_t i = __builtin_amdgcn_readfirstlane((blockIdx.x - shared_blocks) * 4 + wave);
+        // (the rows' first spans, then their second ones, ..: workgroups go to the XCDs in
+        // turn, and so every XCD gets spans of all kinds)
+        const uint32_t pair = i / p.heads, h = i - pair * p.heads, rest = pair / a.own_tiles, tile = pair - rest * a.own_tiles;
+        const uint32_t span = rest / a.rows, b = rest - span * a.rows;
+        if (span >= a.splits) return;
+        // (asked for before what the groups say, which the rest depends on)
+        const uint32_t left = a.group - tile * 16, nq = left < 16 ? left : 16;
+        bf16x8 q[DP / 32];
+        own_queries<DP, I8>(p, a, b, h * a.group + tile * 16, nq, q);
+        uint32_t len = kv_length(a.lengths, b, a.max_length);
+        const Groups groups(a, p.width * p.page_size);
+        len = len < groups.most ? len : groups.most;
         Prefix x;
         const uint32_t begins = !groups.find<true>(b, x) ? 0 : x.tokens < len ? x.tokens : len;
-        const uint32_t steps = (len - begins + STEP - 1) / STEP, per = (steps + a.splits - 1) / a.splits;
-        t0 = begins + span * per * STEP;
-        t0 = t0 < len ? t0 : len;
-        t1 = len - t0 < per * STEP ? len : t0 + per * STEP;
-        slot = (((size_t)b * p.heads + h) * a.own_tiles + tile) * a.splits + span;
-        part = a.own_part;
-        ml = a.own_ml;
-        cap = a.own_columns;
+        const uint32_t t0 = begins + span * a.own_span;
+        if (span && t0 >= len) return;
+        const uint32_t t1 = span + 1 < a.splits && len - t0 > a.own_span ? t0 + a.own_span : len;
+        own_tokens<DP, I8, PIECES>(p, a, b, h, q, nq, t0, t1,
+                                   ((((size_t)b * p.heads + h) * a.own_tiles + tile) * a.splits + span) * a.own_columns,
+                                   lds + wave * OwnTile<DP>::ALL);
+        return;
     }
-    const uint32_t all = rows * a.group - tile * TILE, nq = all < TILE ? all : TILE;
+    const Groups groups(a, p.width * p.page_size);
+    const uint32_t unit = blockIdx.x / p.heads, h = blockIdx.x - unit * p.heads;
+    Prefix x;
+    if (!groups.find<false>(unit, x)) return;
+    const uint32_t tile = (unit - x.base) / x.spans, span = unit - x.base - tile * x.spans;
+    const uint32_t first = x.first, at = tile * TILE, t0 = span * x.per * STEP;
+    const uint32_t t1 = t0 + x.per * STEP < x.tokens ? t0 + x.per * STEP : x.tokens;
+    const size_t slot = ((size_t)h * a.blocks + unit) * a.columns;
+    const uint32_t left = x.rows * a.group - at, nq = left < TILE ? left : TILE;
     const bool wide = nq > 64;
     const uint32_t q0 = 32 * (wide ? wave : wave & 1);       // this wave's first query
     const bool busy = q0 < nq;
-    const int32_t* const table = p.table(reads, h);
+    const int32_t* table = p.table(first, h);
     const uint32_t dim = FORM == NEAR ? DP : p.dim, row_bytes = dim * (I8 ? 1 : 2);
-
-    // (columns past the tile's queries repeat its last: nothing reads what they give)
-    bf16x8 q[KQ];
-    uint32_t limit;
-    {
-        const uint32_t mine = q0 + c < nq ? q0 + c : nq - 1, idx = tile * TILE + mine, b = first + idx / a.group;
-        const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(h * a.group + idx % a.group) * dim;
-        limit = kv_length(a.lengths, b, t1);
-#pragma unroll
-        for (int s = 0; s < KQ; s++) {
-            const uint32_t d = 16 * s + 8 * g;
-            u32x4 w = {0u, 0u, 0u, 0u};
-            if (d < dim) w = *reinterpret_cast<const bf16x8_any*>(qh + d) ^ a.flip;
-            q[s] = __builtin_bit_cast(bf16x8, w);
-        }
-    }
-    const uint32_t least = ~__builtin_amdgcn_readfirstlane(lane_max(~limit));     // of the wave's queries
 
     // this lane's token of a step: the page table's entry, then its row of the pool
     uint32_t entry, row;
@@ -310,34 +492,60 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
         ok = entry < p.pages;
         row = ok ? (entry * p.heads + h) * p.page_size + (tok - p.page_of(tok) * p.page_size) : 0;
     };
-    // A step's tiles: bf16 straight to LDS, each wave 16 tokens (a load's 64 pieces lie
-    // there one after the other, so each lane fetches what belongs in its place); int8
-    // through registers, as bf16.
-    u32x4 kc[EACH], vc[EACH];
+    look(t0);
+    // (columns past the tile's queries repeat its last: nothing reads what they give)
+    bf16x8 q[KQ];
+    uint32_t limit;
+    {
+        const uint32_t idx = at + (q0 + c < nq ? q0 + c : nq - 1), b = first + idx / a.group;
+        const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(h * a.group + idx % a.group) * dim;
+        limit = kv_length(a.lengths, b, t1);
+#pragma unroll
+        for (int s = 0; s < KQ; s++) {
+            const uint32_t d = 16 * s + 8 * g;
+            u32x4 w = {0u, 0u, 0u, 0u};
+            if (d < dim) w = *reinterpret_cast<const bf16x8_any*>(qh + d) ^ a.flip;
+            q[s] = __builtin_bit_cast(bf16x8, w);
+        }
+    }
+    const uint32_t least = ~__builtin_amdgcn_readfirstlane(lane_max(~limit));     // of the wave's queries
+
+    // (looked up above by the first row's table, which nearly always has the prefix)
+    if (const uint32_t reads = row_with(a, x); reads != first) {
+        table = p.table(reads, h);
+        look(t0);
+    }
+
+    // A step's tiles, each wave 16 tokens: bf16 straight to LDS (a load's 64 pieces lie there
+    // one after the other, so each lane fetches what belongs in its place), int8 through
+    // registers, as bf16.
+    constexpr int OF_LOAD = 64 / CH, LOADS = 16 / OF_LOAD;       // tokens of a wave's load, loads of 16 tokens
+    const int in_load = lane / CH, piece = lane % CH;
+    u32x4 kc[I8 ? LOADS : 1], vc[I8 ? LOADS : 1];
     float ksc = 0.0f, vsc = 0.0f;
     const __amdgpu_buffer_rsrc_t rk = rsrc(p.k), rv = rsrc(p.v);
-    auto load = [&](int buf) {
+    const int tok0 = 16 * wave;
+    auto load = [&](uint8_t* kt, uint8_t* vt) {
 #pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int tok = I8 ? tid / CH + i * (256 / CH) : 16 * wave + i * (64 / CH) + lane / CH;
+        for (int i = 0; i < LOADS; i++) {
+            const int tok = tok0 + i * OF_LOAD + in_load;
             const uint32_t r = __shfl(row, tok);
             if (I8) {
-                const uint32_t piece = tid % CH;
-                const size_t at = (size_t)r * row_bytes + (16 * piece < row_bytes ? 16 * piece : 0);
-                kc[i] = *reinterpret_cast<const u32x4*>(p.k + at);
-                vc[i] = *reinterpret_cast<const u32x4*>(p.v + at);
+                const size_t x = (size_t)r * row_bytes + (16 * piece < (int)row_bytes ? 16 * piece : 0);
+                kc[i] = *reinterpret_cast<const u32x4*>(p.k + x);
+                vc[i] = *reinterpret_cast<const u32x4*>(p.v + x);
                 continue;
             }
-            uint8_t* const to = lds + buf * L::BUF + (16 * wave + i * (64 / CH)) * L::RB;
-            const uint32_t kp = 16 * L::key_piece(tok, lane % CH), vp = 16 * L::value_piece(tok, lane % CH);
+            const uint32_t kp = 16 * L::key_piece(tok, piece), vp = 16 * L::value_piece(tok, piece);
+            const lds_t kto = (lds_t)(kt + i * OF_LOAD * L::RB), vto = (lds_t)(vt + i * OF_LOAD * L::RB);
             if (FORM == FAR) {
-                const size_t at = (size_t)r * row_bytes;
-                if (kp < row_bytes) __builtin_amdgcn_global_load_lds((const glb_t)(p.k + at + kp), (lds_t)to, 16, 0, 0);
-                if (vp < row_bytes) __builtin_amdgcn_global_load_lds((const glb_t)(p.v + at + vp), (lds_t)(to + L::T), 16, 0, 0);
+                const size_t x = (size_t)r * row_bytes;
+                if (kp < row_bytes) __builtin_amdgcn_global_load_lds((const glb_t)(p.k + x + kp), kto, 16, 0, 0);
+                if (vp < row_bytes) __builtin_amdgcn_global_load_lds((const glb_t)(p.v + x + vp), vto, 16, 0, 0);
             } else {
-                const uint32_t at = r * row_bytes;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_t)to, 16, at + kp, 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_t)(to + L::T), 16, at + vp, 0, 0, 0);
+                const uint32_t x = r * row_bytes;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, kto, 16, x + kp, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, vto, 16, x + vp, 0, 0, 0);
             }
         }
         if (I8 && wave == 0) {
@@ -345,69 +553,74 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
             vsc = p.vs[row];
         }
     };
-    // values of absent tokens as zeros (0 * NaN), and int8 tiles to LDS
-    auto settle = [&](int buf, uint64_t there) {
-        uint8_t* const kt = lds + buf * L::BUF;
-        uint8_t* const vt = kt + L::T;
+    // then: values of absent tokens as zeros (0 * NaN), and int8 rows to LDS
+    auto settle = [&](uint8_t* kt, uint8_t* vt, float* sc, uint64_t there) {
         if (I8) {
 #pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                const int tok = tid / CH + i * (256 / CH), piece = tid % CH;
+            for (int i = 0; i < LOADS; i++) {
+                const int tok = tok0 + i * OF_LOAD + in_load, to = (i * OF_LOAD + in_load) * L::RB;
                 const bool in = 16 * piece < (int)row_bytes;
                 if (!in) kc[i] = u32x4{0u, 0u, 0u, 0u};
                 if (!in || !(there >> tok & 1)) vc[i] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    *reinterpret_cast<u32x4*>(kt + tok * L::RB + 16 * L::key_piece(tok, 2 * piece + j)) =
+                    *reinterpret_cast<u32x4*>(kt + to + 16 * L::key_piece(tok, 2 * piece + j)) =
                         bytes_to_bf16(kc[i][2 * j], kc[i][2 * j + 1]);
-                    *reinterpret_cast<u32x4*>(vt + tok * L::RB + 16 * L::value_piece(tok, 2 * piece + j)) =
+                    *reinterpret_cast<u32x4*>(vt + to + 16 * L::value_piece(tok, 2 * piece + j)) =
                         bytes_to_bf16(vc[i][2 * j], vc[i][2 * j + 1]);
                 }
             }
             if (wave == 0) {
-                scales[(2 * buf) * STEP + lane] = ksc;
-                scales[(2 * buf + 1) * STEP + lane] = there >> lane & 1 ? vsc : 0.0f;
+                sc[lane] = ksc;
+                sc[STEP + lane] = there >> lane & 1 ? vsc : 0.0f;
             }
         } else if (there != ~0ull) {
 #pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                const int tok = 16 * wave + i * (64 / CH) + lane / CH;
-                if (!(there >> tok & 1)) *reinterpret_cast<u32x4*>(vt + tok * L::RB + 16 * (lane % CH)) = u32x4{0u, 0u, 0u, 0u};
-            }
+            for (int i = 0; i < LOADS; i++)
+                if (!(there >> (tok0 + i * OF_LOAD + in_load) & 1))
+                    *reinterpret_cast<u32x4*>(vt + (i * OF_LOAD + in_load) * L::RB + 16 * piece) = u32x4{0u, 0u, 0u, 0u};
         }
     };
 
     f32x16 o[DT] = {};
     float m = -INFINITY, sum = 0.0f;
     bool any = false;
-    // N x 32 of a step's tokens, from u0 x 32 on
-    auto attend = [&](auto n_, int u0, int buf, uint32_t base, uint64_t there) {
+    // N x 32 tokens from `base` on, whose rows and scales lie at kt, vt, ksc and vsc
+    auto attend = [&](auto n_, const uint8_t* kt, const uint8_t* vt, const float* kscales, const float* vscales, uint32_t base,
+                      uint64_t there) {
         constexpr int N = decltype(n_)::value;
-        const uint8_t* const kt = lds + buf * L::BUF + u0 * 32 * L::RB;
-        const uint8_t* const vt = kt + L::T;
-        const float* const sc = scales + 2 * buf * STEP + 32 * u0;
         f32x16 s[N] = {};
+        // (reads ahead of the products: one after the other they would wait for each)
+        constexpr int AHEAD = DP <= 64 ? KQ : I8 ? (DP <= 128 ? 4 : 2) : DP <= 128 ? KQ : 4;
 #pragma unroll
-        for (int i = 0; i < KQ; i++)
+        for (int i0 = 0; i0 < KQ; i0 += AHEAD) {
+            bf16x8 kf[AHEAD][N];
 #pragma unroll
-            for (int u = 0; u < N; u++) {
-                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (32 * u + c) * L::RB + 16 * L::key_piece(c, 2 * i + g));
-                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[i], s[u], 0, 0, 0);
-            }
+            for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+                for (int u = 0; u < N; u++)
+                    kf[i][u] = *reinterpret_cast<const bf16x8*>(kt + (32 * u + c) * L::RB + 16 * L::key_piece(c, 2 * (i0 + i) + g));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+                for (int u = 0; u < N; u++) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i][u], q[i0 + i], s[u], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < N; u++) {
             if (I8)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
-                    const f32x4 k4 = *reinterpret_cast<const f32x4*>(sc + 32 * u + 2 * r + 4 * g);
+                    const f32x4 k4 = *reinterpret_cast<const f32x4*>(kscales + 32 * u + 2 * r + 4 * g);
 #pragma unroll
                     for (int i = 0; i < 4; i++) s[u][r + i] *= k4[i];
                 }
-            const uint32_t from = base + 32 * (u0 + u), mask = (uint32_t)(there >> (32 * (u0 + u)));
+            const uint32_t from = base + 32 * u, mask = (uint32_t)(there >> (32 * u));
             if (mask != 0xFFFFFFFFu || from + 32 > least) {
-                const uint32_t left = limit > from ? limit - from : 0;
-                const uint32_t mine = left >= 32 ? mask : mask & ((1u << left) - 1);
+                const uint32_t upto = limit > from ? limit - from : 0;
+                const uint32_t mine = upto >= 32 ? mask : mask & ((1u << upto) - 1);
 #pragma unroll
                 for (int r = 0; r < 16; r++)
                     if (!(mine >> (2 * (r & 12) + (r & 3) + 4 * g) & 1)) s[u][r] = -INFINITY;
@@ -435,70 +648,95 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
             for (int i = 0; i < DT; i++) o[i] *= f;
         }
         const float ref = m == -INFINITY ? 0.0f : m;
+        // 16 tokens at a time: the next ones' weights and values while these are multiplied
+        bf16x8 pc[2][PIECES], vf[2][DT];
+        auto weigh = [&](int k) {
+            float e[8];
 #pragma unroll
-        for (int u = 0; u < N; u++)
+            for (int r = 0; r < 8; r++) {
+                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k >> 1][8 * (k & 1) + r], a.scale_log2, -ref));
+                sum += e[r];
+            }
+            if (I8)
 #pragma unroll
-            for (int pr = 0; pr < 2; pr++) {
-                float e[8];
+                for (int r = 0; r < 8; r += 4) {
+                    const f32x4 v4 = *reinterpret_cast<const f32x4*>(vscales + 16 * k + 2 * r + 4 * g);
 #pragma unroll
-                for (int r = 0; r < 8; r++) {
-                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * pr + r], a.scale_log2, -ref));
-                    sum += e[r];
+                    for (int i = 0; i < 4; i++) e[r + i] *= v4[i];
                 }
-                if (I8)
+            split<PIECES>(e, pc[k & 1]);
+        };
+        auto values = [&](int k) {
 #pragma unroll
-                    for (int r = 0; r < 8; r += 4) {
-                        const f32x4 v4 = *reinterpret_cast<const f32x4*>(sc + STEP + 32 * u + 16 * pr + 2 * r + 4 * g);
+            for (int dt = 0; dt < DT; dt++) {
+                s16x4 w[2];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) e[r + i] *= v4[i];
-                    }
-                bf16x8 pc[PIECES];
-                split<PIECES>(e, pc);
+                for (int t = 0; t < 2; t++) {
+                    const int tok = 16 * k + 8 * t + 4 * g + ((lane & 15) >> 2);
+                    const int piece = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                    const lds_t at = (lds_t)(vt + tok * L::RB + 16 * L::value_piece(tok, piece) + 8 * (lane & 1));
+                    w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+                }
+                vf[k & 1][dt] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+        };
+        values(0);
+        weigh(0);
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    s16x4 w[2];
+        for (int k = 0; k < 2 * N; k++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (k + 1 < 2 * N) {
+                values(k + 1);
+                weigh(k + 1);
+            }
 #pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        const int tok = 32 * u + 16 * pr + 8 * t + 4 * g + ((lane & 15) >> 2);
-                        const int piece = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                        const lds_t at = (lds_t)(vt + tok * L::RB + 16 * L::value_piece(tok, piece) + 8 * (lane & 1));
-                        w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-                    }
-                    const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int i = 0; i < PIECES; i++)
 #pragma unroll
-                    for (int i = 0; i < PIECES; i++) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pc[i], o[dt], 0, 0, 0);
+                for (int dt = 0; dt < DT; dt++)
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[k & 1][dt], pc[k & 1][i], o[dt], 0, 0, 0);
+            if (k + 1 < 2 * N) {
+                // the reads first, then a few of the weights' instructions behind each product
+                __builtin_amdgcn_sched_group_barrier(0x100, 2 * DT, 0);
+#pragma unroll
+                for (int i = 0; i < PIECES * DT; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, PIECES == 2 ? 7 : 8, 0);
                 }
             }
+        }
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     if (FORM == FAR && row_bytes < L::RB) {      // what loads do not reach: zeros behind the head's end
         for (int i = 16 * tid; i < 2 * L::BUF; i += 16 * 256) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0u, 0u, 0u, 0u};
         __syncthreads();
     }
-    if (t0 < t1) {
-        look(t0);
-        find(t0);
-        look(t0 + STEP);
-        load(0);
-    }
-    auto steps = [&](auto n, int u0) {
-        int buf = 0;
-        for (uint32_t base = t0; base < t1; base += STEP, buf ^= 1) {
-            const uint64_t there = __ballot(ok);
-            __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's part of the step is there; its reads of the one before are done
-            settle(buf, there);
-            __syncthreads();
-            if (base + STEP < t1) {
-                find(base + STEP);
-                look(base + 2 * STEP);
-                load(buf ^ 1);
+    find(t0);
+    look(t0 + STEP);
+    {
+        auto steps = [&](auto n, int u0) {
+            auto tile = [&](int buf) { return lds + buf * L::BUF + tok0 * L::RB; };
+            load(tile(0), tile(0) + L::T);
+            int buf = 0;
+            for (uint32_t base = t0; base < t1; base += STEP, buf ^= 1) {
+                const uint64_t there = __ballot(ok);
+                __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's part of the step is there; its reads of the one before are done
+                settle(tile(buf), tile(buf) + L::T, scales + 2 * buf * STEP, there);
+                __syncthreads();
+                if (base + STEP < t1) {
+                    find(base + STEP);
+                    look(base + 2 * STEP);
+                    load(tile(buf ^ 1), tile(buf ^ 1) + L::T);
+                }
+                const uint8_t* const kt = lds + buf * L::BUF + u0 * 32 * L::RB;
+                const float* const sc = scales + 2 * buf * STEP + 32 * u0;
+                if (busy) attend(n, kt, kt + L::T, sc, sc + STEP, base + 32 * u0, there >> (32 * u0));
             }
-            if (busy) attend(n, u0, buf, base, there);
-        }
-    };
-    if (wide) steps(std::integral_constant<int, 2>{}, 0);
-    else steps(std::integral_constant<int, 1>{}, wave >> 1);
-    __syncthreads();
+        };
+        if (wide) steps(std::integral_constant<int, 2>{}, 0);
+        else steps(std::integral_constant<int, 1>{}, wave >> 1);
+        __syncthreads();
+    }
 
     // a maximum of -inf with tokens there is told from no tokens by a sum of 1
     {
@@ -536,9 +774,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
             }
     }
     if (q0 + c >= nq) return;
-    const size_t at = slot * cap + q0 + c;
-    if (g == 0) ml[at] = make_float2(m, sum);
-    float* const to = part + at * dim;
+    const size_t place = slot + q0 + c;
+    if (g == 0) a.ml[place] = make_float2(m, sum);
+    float* const to = a.part + place * dim;
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -552,11 +790,12 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
 // added in that order.
 __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Shared a) {
     const uint32_t lane = threadIdx.x & 63;
-    const uint64_t number = (uint64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (number >= (uint64_t)a.rows * a.q_heads) return;
-    const uint32_t b = (uint32_t)(number / a.q_heads), hq = (uint32_t)(number - (uint64_t)b * a.q_heads);
-    const uint32_t h = hq / a.group, j = hq - h * a.group;
+    const uint32_t number = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (number >= a.rows * a.q_heads) return;
+    const uint32_t b = number / a.q_heads, hq = number - b * a.q_heads, h = hq / a.group, j = hq - h * a.group;
+    uint32_t len = kv_length(a.lengths, b, a.max_length);        // (asked for before what the groups say)
     const Groups groups(a, p.width * p.page_size);
+    len = len < groups.most ? len : groups.most;
     Prefix x = {};
     const bool shared = groups.find<true>(b, x);
     const uint32_t idx = shared ? (b - x.first) * a.group + j : 0;
@@ -564,8 +803,10 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
     // (spans past the workspace: of groups that overlap)
     const uint32_t spans = !shared || unit >= a.blocks ? 0 : x.spans < a.blocks - unit ? x.spans : a.blocks - unit;
     const size_t from = ((size_t)h * a.blocks + unit) * a.columns + idx % TILE;
-    const size_t own = ((((size_t)b * p.heads + h) * a.own_tiles + j / TILE) * a.splits) * a.own_columns + j % TILE;
-    const uint32_t n = spans + a.splits;
+    const size_t own = ((((size_t)b * p.heads + h) * a.own_tiles + j / 16) * a.splits) * a.own_columns + j % 16;
+    const uint32_t begins = !shared ? 0 : x.tokens < len ? x.tokens : len;
+    const uint32_t splits = len - begins > a.own_span ? (len - begins + a.own_span - 1) / a.own_span : 1;
+    const uint32_t n = spans + (splits < a.splits ? splits : a.splits);
     auto place = [&](uint32_t i) { return i < spans ? from + (size_t)i * a.columns : own + (size_t)(i - spans) * a.own_columns; };
     auto end = [&](uint32_t i) { return i >= n ? make_float2(-INFINITY, 0.0f) : i < spans ? a.ml[place(i)] : a.own_ml[place(i)]; };
 
@@ -583,11 +824,20 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
         total += f * e.y;
         plain += e.y;
         const uint32_t here = n - i0 < 64 ? n - i0 : 64;
-        for (uint32_t k = 0; k < here; k += ways) {
-            const float w = __shfl(f, k + way);
-            const uint32_t i = i0 + k + way;
-            if (k + way < here && w != 0.0f && in)
-                v += w * *reinterpret_cast<const f32x4*>((i < spans ? a.part : a.own_part) + place(i) * p.dim + d);
+        constexpr int U = 8;              // loads in flight
+        for (uint32_t k0 = 0; k0 < here; k0 += U * ways) {
+            f32x4 part[U];
+            float w[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t k = k0 + u * ways + way, i = i0 + (k < here ? k : here - 1);
+                part[u] = *reinterpret_cast<const f32x4*>((i < spans ? a.part : a.own_part) + place(i) * p.dim + (in ? d : 0));
+                w[u] = __shfl(f, k & 63);
+                if (k >= here) w[u] = 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (w[u] != 0.0f) v += w[u] * part[u];
         }
     }
     total = lane_sum(total);
@@ -642,22 +892,22 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     const size_t group = q_heads / c->kv_heads;
     const size_t tiles = groups ? rows * group / TILE + groups : 0;      // of a head, at most
     const size_t prefix_steps = groups ? (max_prefix + STEP - 1) / STEP : 0, own_steps = (max_own + STEP - 1) / STEP;
-    // Units for two workgroups on every CU, shared out by the steps that prefixes and
-    // own tokens take.
+    // Units for two workgroups on every CU, shared out by what prefixes and own tokens
+    // take.
     const size_t target = ((size_t)2 * cu_count() + c->kv_heads - 1) / c->kv_heads;
     const size_t few = groups ? (rows * group + TILE - 1) / TILE : 0;    // tiles of groups that fill them
-    const size_t shared_work = few * prefix_steps, own_work = rows * own_steps;
+    const size_t own_tiles = (group + 15) / 16;
+    const size_t shared_work = 3 * few * prefix_steps, own_work = rows * own_steps;
     size_t about = shared_work + own_work ? target * shared_work / (shared_work + own_work) : 0;
     if (about < 1) about = 1;
-    size_t splits = target > about ? (target - about) / rows : 0;
-    const size_t most_splits = (own_steps + kLeast - 1) / kLeast;
-    if (splits > most_splits) splits = most_splits;
+    size_t own_span = rows * c->kv_heads * own_tiles * max_own / 1024 / 32 * 32;
+    if (own_span < 64) own_span = 64;
+    size_t splits = (max_own + own_span - 1) / own_span;
     if (splits < 1) splits = 1;
     const size_t blocks = groups ? about + tiles : 0;
-    const size_t columns = rows * group < TILE ? rows * group : TILE, own_columns = group < TILE ? group : TILE;
-    const size_t own_tiles = (group + TILE - 1) / TILE;
+    const size_t columns = rows * group < TILE ? rows * group : TILE, own_columns = group < 16 ? group : 16;
     const size_t slots = blocks * c->kv_heads * columns, own = rows * c->kv_heads * own_tiles * splits * own_columns;
-    const size_t grid = blocks * c->kv_heads + rows * c->kv_heads * own_tiles * splits;
+    const size_t grid = blocks * c->kv_heads + (rows * c->kv_heads * own_tiles * splits + 3) / 4;
     // (a grid has below 2^32 threads; steps of all tiles are counted in 32 bits)
     if (grid > 0xffffff || rows * q_heads / 4 > 0xfffffe || tiles * ((max_length + STEP - 1) / STEP) > 0x7fffffff) {
         snx_set_error("kv_attention_shared: %zu rows of up to %zu tokens are too many", rows, max_length);
@@ -690,6 +940,7 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     a.own_columns = (uint32_t)own_columns;
     a.own_tiles = (uint32_t)own_tiles;
     a.splits = (uint32_t)splits;
+    a.own_span = (uint32_t)own_span;
     // (a scale of zero must not make NaN of a logit of -inf, which is a token that is not there)
     a.flip = scale < 0.0f ? 0x80008000u : 0u;
     a.scale_log2 = (scale < 0.0f ? -scale : scale) * 1.44269504088896340736f;
