@@ -42,11 +42,17 @@ struct Renew {
     uint32_t rows, each;      // each: pages of a row that its new tokens are in, at most
 };
 
-// A workgroup for each page and head: LR lanes a token, eight elements each.
+__device__ __forceinline__ float least_of(float a, float b) { return b < a || b != b ? b : a; }        // (a NaN stays)
+__device__ __forceinline__ float largest_of(float a, float b) { return b > a || b != b ? b : a; }
+
+// A workgroup for each page and head: LR lanes a token, eight elements each; tokens meet
+// over the lanes of a wave, then in LDS.  What bounds it: length, page, keys and result,
+// one after the other (3.7 us for the newest page of 8 heads).
 template <bool I8, int LR>
 __global__ void __launch_bounds__(256) k_kv_key_bounds(const KVPool p, const Renew a) {
     constexpr int TOKENS = 256 / LR;
-    __shared__ float ends[2][TOKENS][LR * 8];
+    __shared__ float ends[2][4][LR * 8];
+    ask_for(p.tables, p.heads, p.page_of.mul, a.rows);
     const uint32_t h = blockIdx.x % p.heads, at = blockIdx.x / p.heads, b = at / a.each, i = at - b * a.each;
     const uint32_t n = kv_length(a.lengths, b, p.width * p.page_size);
     int32_t c = a.counts ? a.counts[b] : 1;
@@ -57,7 +63,7 @@ __global__ void __launch_bounds__(256) k_kv_key_bounds(const KVPool p, const Ren
     const uint32_t page = (uint32_t)p.table(b, h)[e];
     if (page >= p.pages) return;
     const uint32_t left = n - e * p.page_size, used = left < p.page_size ? left : p.page_size;
-    const uint32_t lane = threadIdx.x % LR, first = threadIdx.x / LR, d = 8 * lane;
+    const uint32_t lane = threadIdx.x % LR, d = 8 * lane, wave = threadIdx.x >> 6;
     const bool in = d < p.dim;
     const size_t r0 = ((size_t)page * p.heads + h) * p.page_size;
     float lo[8], hi[8];
@@ -66,38 +72,59 @@ __global__ void __launch_bounds__(256) k_kv_key_bounds(const KVPool p, const Ren
         lo[j] = INFINITY;
         hi[j] = -INFINITY;
     }
-    for (uint32_t t = first; t < used && in; t += TOKENS) {
-        float f[8];
-        if (I8) {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(p.k + (r0 + t) * p.dim + d);
-            const float s = p.ks[r0 + t];
+    constexpr int U = 4;              // tokens in flight
+    for (uint32_t t0 = threadIdx.x / LR; t0 < used; t0 += U * TOKENS) {
+        u32x4 w[U];
+        float s[U];
 #pragma unroll
-            for (int j = 0; j < 8; j++) f[j] = bf16_to_f32(bf16_out((float)(int8_t)(w[j >> 2] >> (8 * (j & 3))) * s));
-        } else {
-            widen(*reinterpret_cast<const u32x4*>(p.k + ((r0 + t) * p.dim + d) * 2), f);
+        for (int u = 0; u < U; u++) {
+            // (past the last token: that one again)
+            const uint32_t t = t0 + u * TOKENS < used ? t0 + u * TOKENS : used - 1;
+            if (I8) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(p.k + (r0 + t) * p.dim + (in ? d : 0));
+                w[u][0] = x[0];
+                w[u][1] = x[1];
+                s[u] = p.ks[r0 + t];
+            } else {
+                w[u] = *reinterpret_cast<const u32x4*>(p.k + ((r0 + t) * p.dim + (in ? d : 0)) * 2);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float f[8];
+            if (I8)
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    f[j] = bf16_to_f32(bf16_out((float)(int8_t)(w[u][j >> 2] >> (8 * (j & 3))) * s[u]));
+            else widen(w[u], f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                lo[j] = least_of(lo[j], f[j]);
+                hi[j] = largest_of(hi[j], f[j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = LR; o < 64; o <<= 1)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            lo[j] = f[j] < lo[j] || f[j] != f[j] ? f[j] : lo[j];       // (a NaN stays)
-            hi[j] = f[j] > hi[j] || f[j] != f[j] ? f[j] : hi[j];
+            lo[j] = least_of(lo[j], __shfl_xor(lo[j], o));
+            hi[j] = largest_of(hi[j], __shfl_xor(hi[j], o));
         }
-    }
+    if ((threadIdx.x & 63) < LR)
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        ends[0][first][d + j] = lo[j];
-        ends[1][first][d + j] = hi[j];
-    }
+        for (int j = 0; j < 8; j++) {
+            ends[0][wave][d + j] = lo[j];
+            ends[1][wave][d + j] = hi[j];
+        }
     __syncthreads();
     uint16_t* const to = a.bounds + ((size_t)page * p.heads + h) * 2 * p.dim;
-    const uint32_t groups = used < TOKENS ? used : TOKENS;
     for (uint32_t x = threadIdx.x; x < 2 * p.dim; x += 256) {
         const bool top = x >= p.dim;
-        const uint32_t at_d = top ? x - p.dim : x;
-        float m = ends[top][0][at_d];
-        for (uint32_t k = 1; k < groups; k++) {
-            const float f = ends[top][k][at_d];
-            m = (top ? f > m : f < m) || f != f ? f : m;
-        }
+        const uint32_t k = top ? x - p.dim : x;
+        float m = ends[top][0][k];
+#pragma unroll
+        for (int j = 1; j < 4; j++) m = top ? largest_of(m, ends[1][j][k]) : least_of(m, ends[0][j][k]);
         to[x] = (uint16_t)(f2u(m) >> 16);          // (bf16 already)
     }
 }
@@ -107,7 +134,7 @@ struct Pick {
     const uint16_t *bounds, *q;
     size_t q_stride;
     const int32_t* lengths;
-    uint32_t* keys;            // [rows][heads][most]
+    uint32_t* keys;            // [rows][heads][most], rows of whole 16 bytes
     int32_t *picked, *picked_lengths;
     uint32_t rows, group, most, max_length, budget, first, recent;
 };
@@ -127,62 +154,113 @@ __device__ __forceinline__ double lane_step64(double x) {
     const uint32_t lo = lane_step<CTRL, 0xf>((uint32_t)u, 0u), hi = lane_step<CTRL, 0xf>((uint32_t)(u >> 32), 0u);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+// Four numbers of LR lanes, each summed over them: lane l gets the sum of number l % 4
+// (neighbours share two of the four each, pairs one, and so on).
 template <int LR>
-__device__ __forceinline__ double row_sum64(double x) {
-    x += lane_step64<0xB1>(x);
-    x += lane_step64<0x4E>(x);
-    x += lane_step64<0x141>(x);
-    if (LR >= 16) x += lane_step64<0x140>(x);
-    if (LR >= 32) x += __shfl_xor(x, 16);
-    return x;
+__device__ __forceinline__ double row_sums64(const double (&x)[4]) {
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+    const double a = (odd ? x[1] : x[0]) + lane_step64<0xB1>(odd ? x[0] : x[1]);
+    const double b = (odd ? x[3] : x[2]) + lane_step64<0xB1>(odd ? x[2] : x[3]);
+    double y = (high ? b : a) + lane_step64<0x4E>(high ? a : b);
+    if (LR == 8) return y + __shfl_xor(y, 4);
+    y += lane_step64<0x124>(y);       // (rotations of 16 lanes by 4 and 8 keep l % 4)
+    y += lane_step64<0x128>(y);
+    if (LR >= 32) y += __shfl_xor(y, 16);
+    return y;
 }
 
-// LR lanes a page, eight elements each; blockIdx.y (and z): row and head.
-template <int LR>
-__global__ void __launch_bounds__(256) k_kv_scores(const KVPool p, const Pick a) {
+// LR lanes a page, eight elements each; blockIdx.y (and z): row and head, whose pages the
+// workgroups of a row take in turn, so that all have the same of a short one.  For finite
+// bounds
+//   max(q least, q largest) = q/2 (largest + least) + |q|/2 (largest - least),
+// two fp64 products and no choice, with the queries' conversions once for all pages (FEW:
+// up to four query heads); a page whose sum is not finite is summed up by the definition.
+// What bounds it: the bounds' bytes and, near them, fp64 conversions and products (see
+// k_kv_pick).
+template <int LR, bool FEW>
+__global__ void __launch_bounds__(256, FEW ? 4 : 2) k_kv_scores(const KVPool p, const Pick a) {
     const uint32_t bh = blockIdx.y + blockIdx.z * 65535u;
     if (bh >= a.rows * p.heads) return;
     const uint32_t b = bh / p.heads, h = bh - b * p.heads;
-    const uint32_t n = kv_length(a.lengths, b, a.max_length), have = p.page_of(n + p.page_size - 1);
-    const uint32_t e = blockIdx.x * (256 / LR) + threadIdx.x / LR;
-    if (have <= a.budget || e >= have) return;
-    uint32_t* const key = a.keys + (size_t)bh * a.most + e;
     const uint32_t lane = threadIdx.x % LR, d = 8 * lane;
-    const bool always = e < a.first || e >= have - a.recent;
-    const uint32_t page = (uint32_t)p.table(b, h)[e];
-    if (always || page >= p.pages) {
-        if (lane == 0) *key = always ? 0xFFFFFFFFu : 0u;
-        return;
-    }
     const bool in = d < p.dim;
-    float lo[8] = {}, hi[8] = {};
-    if (in) {
-        const uint16_t* const x = a.bounds + ((size_t)page * p.heads + h) * 2 * p.dim + d;
-        widen(*reinterpret_cast<const u32x4*>(x), lo);
-        widen(*reinterpret_cast<const u32x4*>(x + p.dim), hi);
-    }
-    float best = -INFINITY;
-    for (uint32_t g0 = 0; g0 < a.group; g0 += kHeadsAtOnce) {
-        double sum[kHeadsAtOnce];
+    const uint32_t stride = gridDim.x * (256 / LR);
+    const uint32_t n = kv_length(a.lengths, b, a.max_length), have = p.page_of(n + p.page_size - 1);
+    uint32_t e = blockIdx.x * (256 / LR) + threadIdx.x / LR;
+    if (have <= a.budget || e >= have) return;
+    const int32_t* const table = p.table(b, h);
+    uint32_t* const keys = a.keys + (size_t)bh * a.most;
+
+    double x[kHeadsAtOnce][8];        // q / 2
+    auto queries = [&](uint32_t g0) {
 #pragma unroll
         for (int g = 0; g < kHeadsAtOnce; g++) {
-            sum[g] = 0.0;
             const uint32_t j = g0 + g < a.group ? g0 + g : a.group - 1;
-            float q[8] = {};
-            if (in) widen(*reinterpret_cast<const bf16x8_any*>(a.q + b * a.q_stride + (size_t)(h * a.group + j) * p.dim + d), q);
+            u32x4 w = {0u, 0u, 0u, 0u};
+            if (in) w = *reinterpret_cast<const bf16x8_any*>(a.q + b * a.q_stride + (size_t)(h * a.group + j) * p.dim + d);
+            float q[8];
+            widen(w, q);
 #pragma unroll
-            for (int k = 0; k < 8; k++) sum[g] += (double)q[k] * (double)(q[k] > 0.0f ? hi[k] : lo[k]);
+            for (int k = 0; k < 8; k++) x[g][k] = (double)(0.5f * q[k]);
         }
+    };
+    u32x4 next_lo, next_hi;
+    auto fetch = [&](uint32_t page) {
+        const uint16_t* const at = a.bounds + ((size_t)(page < p.pages ? page : 0) * p.heads + h) * 2 * p.dim + (in ? d : 0);
+        next_lo = *reinterpret_cast<const u32x4*>(at);
+        next_hi = *reinterpret_cast<const u32x4*>(at + p.dim);
+    };
+    uint32_t page = (uint32_t)table[e], next = e + stride < have ? (uint32_t)table[e + stride] : 0u;
+    fetch(page);
+    if (FEW) queries(0);
+#pragma unroll 1
+    for (; e < have; e += stride) {
+        float l[8], u[8];
+        widen(next_lo, l);
+        widen(next_hi, u);
+        const bool there = page < p.pages;
+        page = next;
+        if (e + stride < have) {
+            fetch(page);
+            if (e + 2 * stride < have) next = (uint32_t)table[e + 2 * stride];
+        }
+        float best = -INFINITY;
+#pragma unroll 1
+        for (uint32_t g0 = 0; g0 < (FEW ? 1u : a.group); g0 += kHeadsAtOnce) {
+            if (!FEW) queries(g0);
+            double sum[kHeadsAtOnce] = {};
 #pragma unroll
-        for (int g = 0; g < kHeadsAtOnce; g++) {
-            const float s = (float)row_sum64<LR>(sum[g]);
-            best = s > best || s != s ? s : best;             // (a NaN stays)
+            for (int k = 0; k < 8; k++) {
+                const double mid = (double)u[k] + (double)l[k], half = (double)u[k] - (double)l[k];
+#pragma unroll
+                for (int g = 0; g < kHeadsAtOnce; g++) {
+                    sum[g] = __builtin_fma(x[g][k], mid, sum[g]);
+                    sum[g] = __builtin_fma(__builtin_fabs(x[g][k]), half, sum[g]);
+                }
+            }
+            double s = row_sums64<LR>(sum);
+            if (__any(!(__builtin_fabs(s) < INFINITY))) {
+#pragma unroll
+                for (int g = 0; g < kHeadsAtOnce; g++) {
+                    sum[g] = 0.0;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) sum[g] += 2.0 * x[g][k] * (double)(x[g][k] > 0.0 ? u[k] : l[k]);
+                }
+                s = row_sums64<LR>(sum);
+            }
+            // the largest of the four heads (a NaN stays)
+            float f = (float)s;
+            f = largest_of(f, lane_step<0xB1, 0xf>(f, 0.0f));
+            f = largest_of(f, lane_step<0x4E, 0xf>(f, 0.0f));
+            best = largest_of(best, f);
         }
+        if (lane == 0) keys[e] = there ? score_key(best) : 0u;
     }
-    if (lane == 0) *key = score_key(best);
 }
 
 constexpr int kWaves = 16, kThreads = 64 * kWaves;
+constexpr uint32_t kChunk = 4 * kThreads;      // pages of a workgroup at a time
+constexpr uint32_t kBins = 2 * kThreads;
 
 // Over the workgroup: inclusive prefixes and the total.
 __device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* sh, uint32_t& total) {
@@ -196,12 +274,16 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* sh, uint3
     return mine + (w ? (uint32_t)__builtin_amdgcn_readlane(upto, w - 1) : 0u);
 }
 
-// A workgroup for each row and head: the budget-th largest key by digits of 8 bits,
-// each a histogram of the keys that agree so far, then the pages above it and the
-// first of those that equal it, in order.
+// A workgroup for each row and head, four pages next to one another to a thread (the first
+// 4096 keys stay in registers).  Scores of a row lie close together, so what is searched for
+// the smallest key that is kept is the range from the smallest to the largest: cut into
+// 2048 equal parts, of the part that it is in again, until all of a part are kept or it
+// has one key.  Then the pages that are kept, in order; of those that equal that key the
+// first.
 __global__ void __launch_bounds__(kThreads) k_kv_pick(const KVPool p, const Pick a) {
-    __shared__ uint32_t bins[256], sh[kWaves], chosen[2];
+    __shared__ uint32_t bins[kBins], sh[kWaves], ends[2][kWaves], chosen[3];
     const uint32_t tid = threadIdx.x, bh = blockIdx.x, b = bh / p.heads, h = bh - b * p.heads;
+    ask_for(p.tables, p.heads, a.rows, a.keys);
     const uint32_t n = kv_length(a.lengths, b, a.max_length), have = p.page_of(n + p.page_size - 1);
     const int32_t* const table = p.table(b, h);
     int32_t* const to = a.picked + (size_t)bh * a.budget;
@@ -211,38 +293,94 @@ __global__ void __launch_bounds__(kThreads) k_kv_pick(const KVPool p, const Pick
         for (uint32_t i = tid; i < a.budget; i += kThreads) to[i] = i < have ? table[i] : -1;
         return;
     }
-    const uint32_t* const keys = a.keys + (size_t)bh * a.most;
-    uint32_t left = a.budget, prefix = 0;       // of the keys that agree so far, how many are to be kept
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) bins[tid] = 0;
-        __syncthreads();
-        for (uint32_t e = tid; e < have; e += kThreads) {
-            const uint32_t k = keys[e];
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[(k >> shift) & 255], 1u);
+    const u32x4* const keys = reinterpret_cast<const u32x4*>(a.keys + (size_t)bh * a.most);
+    const uint32_t last = have - a.recent;         // pages from a.first to here are picked among
+    auto load = [&](uint32_t c0) { return c0 + 4 * tid < have ? keys[c0 / 4 + tid] : u32x4{0u, 0u, 0u, 0u}; };
+    const u32x4 first = load(0);
+    auto each = [&](auto&& f) {
+        f(0u, first);
+        for (uint32_t c0 = kChunk; c0 < have; c0 += kChunk) f(c0, load(c0));
+    };
+    auto among = [&](uint32_t e) { return e >= a.first && e < last; };
+
+    uint32_t left = a.budget - a.first - a.recent, from = 0xFFFFFFFFu, trim = 0;      // keys from `from` on are kept, of equal ones `trim`
+    if (left) {
+        uint32_t lo = 0xFFFFFFFFu, hi = 0u;
+        each([&](uint32_t c0, u32x4 k) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (among(c0 + 4 * tid + j)) {
+                    lo = lo < k[j] ? lo : k[j];
+                    hi = hi > k[j] ? hi : k[j];
+                }
+        });
+        lo = ~lane_max(~lo);
+        hi = lane_max(hi);
+        if ((tid & 63) == 0) {
+            ends[0][tid >> 6] = lo;
+            ends[1][tid >> 6] = hi;
         }
+        bins[tid] = bins[tid + kThreads] = 0;
         __syncthreads();
-        // the digit in which the left-th largest is: counts from the top
-        uint32_t total;
-        const uint32_t c = tid < 256 ? bins[255 - tid] : 0, upto = block_prefix(c, sh, total);
-        if (tid < 256 && upto >= left && upto - c < left) {
-            chosen[0] = 255 - tid;
-            chosen[1] = left - (upto - c);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            lo = lo < ends[0][w] ? lo : ends[0][w];
+            hi = hi > ends[1][w] ? hi : ends[1][w];
         }
-        __syncthreads();
-        prefix |= chosen[0] << shift;
-        left = chosen[1];
+        for (;;) {
+            const uint32_t range = hi - lo, bits = range ? 32 - __builtin_clz(range) : 0, shift = bits > 11 ? bits - 11 : 0;
+            each([&](uint32_t c0, u32x4 k) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (among(c0 + 4 * tid + j) && k[j] >= lo && k[j] <= hi) atomicAdd(&bins[(k[j] - lo) >> shift], 1u);
+            });
+            __syncthreads();
+            // the part that has the left-th largest: two parts to a thread, from the top
+            const uint32_t c1 = bins[kBins - 1 - 2 * tid], c0 = bins[kBins - 2 - 2 * tid];
+            uint32_t total;
+            const uint32_t before = block_prefix(c0 + c1, sh, total) - c0 - c1;
+            if (before < left && before + c0 + c1 >= left) {
+                const bool upper = before + c1 >= left;
+                chosen[0] = kBins - 1 - 2 * tid - !upper;
+                chosen[1] = left - before - (upper ? 0 : c1);
+                chosen[2] = upper ? c1 : c0;
+            }
+            bins[tid] = bins[tid + kThreads] = 0;
+            __syncthreads();
+            lo += chosen[0] << shift;
+            left = chosen[1];
+            if (shift == 0 || chosen[2] == left) {
+                from = lo;
+                trim = chosen[2] == left ? 0xFFFFFFFFu : left;
+                break;
+            }
+            hi = hi - lo < (1u << shift) - 1 ? hi : lo + (1u << shift) - 1;
+            __syncthreads();                       // (chosen is read before it is written again)
+        }
     }
-    uint32_t above = 0, equal = 0;              // of the pages before
-    for (uint32_t e0 = 0; e0 < have; e0 += kThreads) {
-        const uint32_t e = e0 + tid, k = e < have ? keys[e] : 0;
-        const uint32_t is_above = e < have && k > prefix, is_equal = e < have && k == prefix;
+    uint32_t above = 0, equal = 0;                 // of the chunks before
+    each([&](uint32_t c0, u32x4 k) {
+        uint32_t is_above[4], is_equal[4], mine = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t e = c0 + 4 * tid + j;
+            const bool in = among(e);
+            is_above[j] = e < have && (!in || (trim == 0xFFFFFFFFu ? k[j] >= from : k[j] > from));
+            is_equal[j] = trim != 0xFFFFFFFFu && in && k[j] == from;
+            mine += is_above[j] | is_equal[j] << 16;
+        }
         uint32_t total;
-        const uint32_t before = block_prefix(is_above | is_equal << 16, sh, total) - (is_above | is_equal << 16);
-        const uint32_t eq = equal + (before >> 16), at = above + (before & 0xFFFFu) + (eq < left ? eq : left);
-        if (is_above || (is_equal && eq < left)) to[at] = table[e];
+        const uint32_t before = block_prefix(mine, sh, total) - mine;
+        uint32_t ab = above + (before & 0xFFFFu), eq = equal + (before >> 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (is_above[j] || (is_equal[j] && eq < trim)) to[ab + (eq < trim ? eq : trim)] = table[c0 + 4 * tid + j];
+            ab += is_above[j];
+            eq += is_equal[j];
+        }
         above += total & 0xFFFFu;
         equal += total >> 16;
-    }
+    });
 }
 
 template <bool I8>
@@ -250,6 +388,12 @@ void bounds(unsigned grid, const KVPool& p, const Renew& a, hipStream_t s) {
     if (p.dim <= 64) k_kv_key_bounds<I8, 8><<<grid, 256, 0, s>>>(p, a);
     else if (p.dim <= 128) k_kv_key_bounds<I8, 16><<<grid, 256, 0, s>>>(p, a);
     else k_kv_key_bounds<I8, 32><<<grid, 256, 0, s>>>(p, a);
+}
+
+template <int LR>
+void scores(dim3 grid, const KVPool& p, const Pick& a, hipStream_t s) {
+    if (a.group <= kHeadsAtOnce) k_kv_scores<LR, true><<<grid, 256, 0, s>>>(p, a);
+    else k_kv_scores<LR, false><<<grid, 256, 0, s>>>(p, a);
 }
 
 }  // namespace
@@ -293,23 +437,26 @@ int snx_k_kv_pick(const SNEPPXKVCache* c, const uint16_t* bounds, const uint16_t
     a.picked_lengths = picked_lengths;
     a.rows = (uint32_t)rows;
     a.group = (uint32_t)(q_heads / c->kv_heads);
-    a.most = (uint32_t)((max_length + c->page_size - 1) / c->page_size);
+    a.most = (uint32_t)((max_length + c->page_size - 1) / c->page_size + 3) / 4 * 4;
     a.max_length = (uint32_t)max_length;
     a.budget = (uint32_t)budget;
     a.first = (uint32_t)first;
     a.recent = (uint32_t)recent;
     const size_t bh = rows * c->kv_heads;
     if (ws) {
+        // As many pages to a lane as leave every CU its waves.
         const int lr = c->head_dim <= 64 ? 8 : c->head_dim <= 128 ? 16 : 32;
-        const size_t gx = ((size_t)a.most * lr + 255) / 256;
+        size_t pages = (size_t)a.most * bh * lr / 64 / (16 * (size_t)cu_count());
+        pages = pages < 1 ? 1 : pages > 8 ? 8 : pages;
+        const size_t gx = ((size_t)a.most * lr + 256 * pages - 1) / (256 * pages);
         if (gx * bh > 0xffffff) {     // a grid has below 2^32 threads
             snx_set_error("kv_pick: %zu rows of up to %zu tokens are too many", rows, max_length);
             return -1;
         }
         const dim3 grid((unsigned)gx, (unsigned)(bh < 65535 ? bh : 65535), (unsigned)((bh + 65534) / 65535));
-        if (lr == 8) k_kv_scores<8><<<grid, 256, 0, S(st)>>>(p, a);
-        else if (lr == 16) k_kv_scores<16><<<grid, 256, 0, S(st)>>>(p, a);
-        else k_kv_scores<32><<<grid, 256, 0, S(st)>>>(p, a);
+        if (lr == 8) scores<8>(grid, p, a, S(st));
+        else if (lr == 16) scores<16>(grid, p, a, S(st));
+        else scores<32>(grid, p, a, S(st));
         if (snx_launch_check("k_kv_scores")) return -1;
     }
     k_kv_pick<<<(unsigned)bh, kThreads, 0, S(st)>>>(p, a);

@@ -285,8 +285,8 @@ int SNEPPX_kv_pick(const SNEPPXKVCache* cache, const uint16_t* bounds, const uin
     if (max_length > slots) max_length = slots;
     const size_t most = (max_length + cache->page_size - 1) / cache->page_size;
     void* ws = NULL;
-    if (most > budget) {
-        ws = snx_workspace(rows * cache->kv_heads * most * sizeof(uint32_t), SLOT_KV_SCORES, stream);
+    if (most > budget) {                              /* (rows of whole 16 bytes) */
+        ws = snx_workspace(rows * cache->kv_heads * ((most + 3) / 4 * 4) * sizeof(uint32_t), SLOT_KV_SCORES, stream);
         if (!ws) return -1;
     }
     return snx_k_kv_pick(cache, bounds, q, q_stride, q_heads, block_tables, table_width, lengths, rows, max_length, budget,

@@ -315,7 +315,7 @@ int snx_k_kv_share(int32_t* refs, size_t pages, size_t page_size, int32_t* table
 
 /* ---- attention behind shared prefixes (kv_shared_kernels.hip, takes its workspace
  * itself) and over picked pages (kv_pick_kernels.hip; ws: 4 bytes for each row, head and
- * page of max_length where that is more than the budget) ---- */
+ * page of max_length, four pages at a time, where that is more than the budget) ---- */
 int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t q_stride, void* out, size_t out_stride,
                               int out_f32, const int32_t* tables, size_t width, const int32_t* lengths, size_t rows,
                               size_t q_heads, size_t max_length, const int32_t* group_starts,
