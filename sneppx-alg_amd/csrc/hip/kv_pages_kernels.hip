@@ -19,9 +19,8 @@ typedef i32x4 i32x4_any __attribute__((aligned(4)));
 
 hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-constexpr int kWaves = 16, kThreads = 64 * kWaves;
 constexpr uint32_t kMost = 0x7FFFFFFFu;              // sums of counts stay here
-constexpr uint32_t kEach = 8, kTurn = kEach * kThreads;       // refs of a thread and of all in a turn
+constexpr uint32_t kEach = 8;                        // refs of a thread in a turn
 constexpr uint32_t kWithin = 4096;                   // tokens that the workgroup which takes pages places itself
 
 struct Pages {
@@ -41,18 +40,31 @@ __device__ __forceinline__ uint32_t pages_of(const Pages& a, uint32_t n) { retur
 
 __device__ __forceinline__ uint32_t add_cut(uint32_t a, uint32_t b) { return a + b < kMost ? a + b : kMost; }
 
-// Over the workgroup: inclusive prefixes of x (sums cut at kMost), and the total.
-// sh: kWaves words, free again after the next barrier.
-__device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* sh, uint32_t& total) {
+// Over a workgroup of W waves: inclusive prefixes (sums cut at kMost) of N numbers, and
+// their totals.  sh: N * W words, free again after the next barrier.
+template <int W, int N>
+__device__ __forceinline__ void block_prefix(uint32_t (&x)[N], uint32_t* sh, uint32_t (&total)[N]) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t mine = lane_scan(x, 0u, add_cut);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = lane_scan(x[i], 0u, add_cut);
     __syncthreads();
-    if (lane == 63) sh[w] = mine;
+    if (lane == 63)
+#pragma unroll
+        for (int i = 0; i < N; i++) sh[i * W + w] = x[i];
     __syncthreads();
-    const uint32_t upto = lane_scan(lane < kWaves ? sh[lane] : 0u, 0u, add_cut);
-    total = __builtin_amdgcn_readlane(upto, kWaves - 1);
-    const uint32_t before = w ? (uint32_t)__builtin_amdgcn_readlane(upto, w - 1) : 0u;
-    return add_cut(before, mine);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t upto = lane_scan(lane < W ? sh[i * W + lane] : 0u, 0u, add_cut);
+        total[i] = __builtin_amdgcn_readlane(upto, W - 1);
+        x[i] = add_cut(w ? (uint32_t)__builtin_amdgcn_readlane(upto, w - 1) : 0u, x[i]);
+    }
+}
+template <int W>
+__device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* sh, uint32_t& total) {
+    uint32_t a[1] = {x}, t[1];
+    block_prefix<W, 1>(a, sh, t);
+    total = t[0];
+    return a[0];
 }
 
 // the last of n ascending numbers (the first at most x) that is at most x
@@ -96,28 +108,33 @@ __device__ __forceinline__ uint32_t free_of(const Pages& a, uint32_t p) {
     return free_bits;
 }
 
-// One workgroup, 1024 rows at a time: what each wants and needs, how far the free
-// pages go, and then every free page of those to the row and entry that its number
-// among them says.  The entries that rows need are numbered one row after the other and
-// shared out among the threads, so that a few rows of many pages go as fast as many
-// of one.
-// What bounds it: one load after the other (lengths, entries, refs), and for pools
-// with few free pages the refs up to the last one taken, at the rate of one CU.
-__global__ void __launch_bounds__(kThreads) k_kv_reserve(const Pages a) {
-    __shared__ uint32_t sh[kWaves], first[kThreads], entry[kThreads], need[kThreads], upto[kThreads], start[kThreads + 1];
-    __shared__ uint32_t length[kThreads], found[kTurn];
-    __shared__ uint8_t given[kThreads];
-    __shared__ int32_t next[kThreads];
+// One workgroup, a row to a thread (and then the next ones): what each wants and needs, how
+// far the free pages go, and then every free page of those to the row and entry that its
+// number among them says.  The entries that rows need are numbered one row after the other
+// and shared out among the threads, so that a few rows of many pages go as fast as many of
+// one.  The first refs are asked for before all else.
+// What bounds it: one load after the other (lengths, entries, new entries again) and some
+// 14 barriers, 6 us for 64 rows by four waves; for pools with few free pages the refs up to
+// the last one taken, at the rate of one CU.
+template <int W>
+__global__ void __launch_bounds__(64 * W) k_kv_reserve(const Pages a) {
+    constexpr uint32_t THREADS = 64 * W, TURN = kEach * THREADS;
+    __shared__ uint32_t sh[2 * W], first[THREADS], entry[THREADS], need[THREADS], upto[THREADS], start[THREADS + 1];
+    __shared__ uint32_t length[THREADS], found[TURN];
+    __shared__ uint8_t given[THREADS];
+    __shared__ int32_t next[THREADS];
+    ask_for(a.tables, a.counts, a.positions, a.page_of.mul);
     const uint32_t tid = threadIdx.x, most = a.width * a.page_size;
     uint32_t carry = 0;        // tokens of the rows before
     uint32_t cursor = 0;       // no page before it is free
     bool spent = false;        // a row was left without pages
 
-    for (uint32_t r0 = 0; r0 < a.rows; r0 += kThreads) {
-        const uint32_t b = r0 + tid, rows = a.rows - r0 < kThreads ? a.rows - r0 : kThreads;
+    for (uint32_t r0 = 0; r0 < a.rows; r0 += THREADS) {
+        const uint32_t b = r0 + tid, rows = a.rows - r0 < THREADS ? a.rows - r0 : THREADS;
         uint32_t n = 0, want = 0, e0 = 0, span = 0;
         int32_t pos = 0;
         bool fits = false;
+        const uint32_t ahead = free_of(a, cursor + kEach * tid);
         if (b < a.rows) {
             const int32_t c = a.counts ? a.counts[b] : 1;
             n = length_of(a, a.lengths[b]);
@@ -127,53 +144,71 @@ __global__ void __launch_bounds__(kThreads) k_kv_reserve(const Pages a) {
             e0 = pages_of(a, n);
             span = fits ? pages_of(a, n + want) - e0 : 0;
         }
-        uint32_t tokens, entries, needed;
-        const uint32_t tokens_upto = block_prefix(want, sh, tokens), entries_upto = block_prefix(span, sh, entries);
-        first[tid] = entries_upto - span;
+        uint32_t sums[2] = {want, span}, totals[2], needed;
+        block_prefix<W, 2>(sums, sh, totals);
+        const uint32_t tokens = totals[0], entries = totals[1];
+        first[tid] = sums[1] - span;
         entry[tid] = e0;
-        need[tid] = 0;
-        start[tid + 1] = add_cut(carry, tokens_upto);
+        need[tid] = span;
+        start[tid + 1] = add_cut(carry, sums[0]);
         if (tid == 0) start[0] = carry;
         length[tid] = n;
         next[tid] = pos;
         __syncthreads();
         if (b < a.rows) a.starts[b] = (int32_t)start[tid];
 
-        // entries that name no page
-        for (uint32_t i = tid; i < entries; i += kThreads) {
-            const uint32_t r = last_upto(first, rows, i);
-            const uint32_t page = (uint32_t)a.tables[(size_t)(r0 + r) * a.width + entry[r] + (i - first[r])];
-            if (page >= a.pages) atomicAdd(&need[r], 1u);
+        // less the entries that name a page (a few, and seldom)
+        constexpr int U = 4;              // loads in flight
+        for (uint32_t i0 = tid; i0 < entries; i0 += U * THREADS) {
+            uint32_t r[U], page[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t i = i0 + u * THREADS < entries ? i0 + u * THREADS : i0;
+                r[u] = last_upto(first, rows, i);
+                page[u] = (uint32_t)a.tables[(size_t)(r0 + r[u]) * a.width + entry[r[u]] + (i - first[r[u]])];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (i0 + u * THREADS < entries && page[u] < a.pages) atomicSub(&need[r[u]], 1u);
         }
         __syncthreads();
-        const uint32_t mine = need[tid], mine_upto = block_prefix(mine, sh, needed);
-        upto[tid] = mine_upto - mine;
+        const uint32_t mine = need[tid];
+        // (with them the free pages of the first turn)
+        uint32_t pair[2] = {mine, (uint32_t)__popc(ahead)}, pair_totals[2];
+        block_prefix<W, 2>(pair, sh, pair_totals);
+        needed = pair_totals[0];
+        upto[tid] = pair[0] - mine;
 
         // the free pages, as far as they are needed
         uint32_t have = 0;
-        if (needed && !spent)
-            for (uint32_t p0 = cursor; p0 < a.pages && have < needed; p0 += 2 * kTurn) {
+        if (needed && !spent) {
+            have = pair_totals[1];
+            for (uint32_t p0 = cursor + TURN; p0 < a.pages && have < needed; p0 += 2 * TURN) {
                 uint32_t sum;
                 const uint32_t p = p0 + kEach * tid;
-                (void)block_prefix(__popc(free_of(a, p)) + __popc(free_of(a, p + kTurn)), sh, sum);
+                (void)block_prefix<W>(__popc(free_of(a, p)) + __popc(free_of(a, p + TURN)), sh, sum);
                 have += sum;
             }
-        const bool ok = b < a.rows && fits && (mine == 0 || mine_upto <= have);
+        }
+        const bool ok = b < a.rows && fits && (mine == 0 || pair[0] <= have);
         given[tid] = ok;
-        __syncthreads();
         // pages that go to rows: those up to the last row whose pages are there
         uint32_t taken = needed;
         if (have < needed) {
             spent = true;
             uint32_t sum;
-            (void)block_prefix(ok ? mine : 0u, sh, sum);
+            (void)block_prefix<W>(ok ? mine : 0u, sh, sum);
             taken = sum;
         }
+        uint32_t bits = ahead, before = pair[1] - __popc(ahead), sum = pair_totals[1];
+        bool turned = false;             // beyond the first turn
         for (uint32_t done = 0; done < taken && cursor < a.pages;) {
             const uint32_t p0 = cursor + kEach * tid;
-            uint32_t bits = free_of(a, p0), sum;
-            uint32_t i = block_prefix(__popc(bits), sh, sum) - __popc(bits);
-            for (; bits; bits &= bits - 1) found[i++] = p0 + __builtin_ctz(bits);
+            if (turned) {
+                bits = free_of(a, p0);
+                before = block_prefix<W>(__popc(bits), sh, sum) - __popc(bits);
+            }
+            for (uint32_t i = before; bits; bits &= bits - 1) found[i++] = p0 + __builtin_ctz(bits);
             __syncthreads();
             // (all entries are chosen before any is written: of a row whose entries name
             // pages here and there, those that name none are counted)
@@ -181,8 +216,8 @@ __global__ void __launch_bounds__(kThreads) k_kv_reserve(const Pages a) {
             uint32_t where[kEach];
 #pragma unroll
             for (uint32_t q = 0; q < kEach; q++) {
-                const uint32_t k = done + tid + q * kThreads;
-                if (tid + q * kThreads >= n_now) break;
+                const uint32_t k = done + tid + q * THREADS;
+                if (tid + q * THREADS >= n_now) break;
                 const uint32_t r = last_upto(upto, rows, k), j = k - upto[r];
                 uint32_t e = entry[r] + j;
                 const uint32_t all = (r + 1 < rows ? first[r + 1] : entries) - first[r];
@@ -197,13 +232,15 @@ __global__ void __launch_bounds__(kThreads) k_kv_reserve(const Pages a) {
             __syncthreads();
 #pragma unroll
             for (uint32_t q = 0; q < kEach; q++) {
-                if (tid + q * kThreads >= n_now) break;
-                const uint32_t page = found[tid + q * kThreads];
+                if (tid + q * THREADS >= n_now) break;
+                const uint32_t page = found[tid + q * THREADS];
                 a.tables[where[q]] = (int32_t)page;
                 a.refs[page] = 1;
             }
             done += sum;
-            if (done <= taken) cursor += kTurn;      // (all of these are taken)
+            if (done > taken) break;
+            cursor += TURN;                          // (all of these are taken)
+            turned = true;
             __syncthreads();
         }
 
@@ -215,9 +252,10 @@ __global__ void __launch_bounds__(kThreads) k_kv_reserve(const Pages a) {
                 if (a.next_pos) a.next_pos[b] = pos + (int32_t)count;
             }
         }
+        __syncthreads();
         const uint32_t end = add_cut(carry, tokens);
         if (a.tokens <= kWithin)
-            for (uint32_t t = carry + tid; t < end && t < a.tokens; t += kThreads) {
+            for (uint32_t t = carry + tid; t < end && t < a.tokens; t += THREADS) {
                 const uint32_t r = last_upto(start, rows, t);
                 place(a, t, r0 + r, t - start[r], given[r], length[r], next[r]);
             }
@@ -226,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_reserve(const Pages a) {
     }
     if (tid == 0) a.starts[a.rows] = (int32_t)carry;
     if (a.tokens <= kWithin)
-        for (uint32_t t = carry + tid; t < a.tokens; t += kThreads) place(a, t, 0, 0, false, 0, 0);
+        for (uint32_t t = carry + tid; t < a.tokens; t += THREADS) place(a, t, 0, 0, false, 0, 0);
 }
 
 // After it, for more tokens: a thread each.
@@ -315,7 +353,10 @@ int snx_k_kv_reserve(int32_t* refs, size_t pages, size_t page_size, int32_t* tab
     a.slots = slots;
     a.positions = positions;
     a.tokens = (uint32_t)tokens;
-    k_kv_reserve<<<1, kThreads, 0, S(st)>>>(a);
+    // Four waves for what a decode step asks for (their barriers take less), sixteen for
+    // more rows, tokens and so pages.
+    if (rows <= 256 && tokens <= 1024) k_kv_reserve<4><<<1, 256, 0, S(st)>>>(a);
+    else k_kv_reserve<16><<<1, 1024, 0, S(st)>>>(a);
     if (snx_launch_check("k_kv_reserve")) return -1;
     if (tokens <= kWithin) return 0;
     k_kv_slots<<<(unsigned)((tokens + 255) / 256), 256, 0, S(st)>>>(a);
