@@ -1138,19 +1138,18 @@ class KVPages(_OnDevice):
         tb, width, ln, n = self._tables(tables, lengths)
         if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
             raise ValueError("slots must be an int32 tensor [tokens]")
-        tokens, rows = slots.shape, (n,)
+        tokens, rows, int32, check = slots.shape, (n,), torch.int32, self._check
         if starts is None:
-            starts = torch.empty(n + 1, dtype=torch.int32, device=self.device)
+            starts = torch.empty(n + 1, dtype=int32, device=self.device)
         if granted is None:
-            granted = torch.empty(n, dtype=torch.int32, device=self.device)
-        args = [self._check(starts, "starts", torch.int32, (n + 1,)), self._check(granted, "granted", torch.int32, rows),
-                self._check(slots, "slots", torch.int32, tokens),
-                None if positions is None else self._check(positions, "positions", torch.int32, tokens)]
-        np_ = None if next_pos is None else self._check(next_pos, "next_pos", torch.int32, rows)
-        ct = None if counts is None else self._check(counts, "counts", torch.int32, rows)
+            granted = torch.empty(n, dtype=int32, device=self.device)
+        st, gr = check(starts, "starts", int32, (n + 1,)), check(granted, "granted", int32, rows)
+        sl, ps = check(slots, "slots", int32, tokens), None if positions is None else check(positions, "positions", int32, tokens)
+        np_ = None if next_pos is None else check(next_pos, "next_pos", int32, rows)
+        ct = None if counts is None else check(counts, "counts", int32, rows)
         run = self._reserve if self._index is not None and torch._C._cuda_getDevice() == self._index \
             else self._elsewhere(self._reserve)
-        rc = run(self._p, self.pages, self.page_size, tb, width, ln, np_, ct, n, *args, tokens[0],
+        rc = run(self._p, self.pages, self.page_size, tb, width, ln, np_, ct, n, st, gr, sl, ps, tokens[0],
                  stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
         if rc:
             self.L.check(rc, "kv_reserve")
@@ -1210,23 +1209,23 @@ class Rotary(_OnDevice):
         among them, or None; in place where no output is given.  positions int32 [tokens]."""
         if not isinstance(positions, torch.Tensor) or positions.dim() != 1:
             raise ValueError("positions must be an int32 tensor [tokens]")
-        tokens = positions.shape[0]
-        args = []
-        for x, out, name in ((q, q_out, "q"), (k, k_out, "k")):
-            if x is None:
-                args += [None, 0, None, 0, 0]
-                continue
-            xp, xs, n, heads = self._rows(x, name, 0, _BF16)
-            op, os_, on = xp, xs, n
-            if out is not None:
-                op, os_, on, _ = self._rows(out, name + "_out", heads, _BF16)
-            if n != tokens or on != tokens:
-                raise ValueError(f"{name} has {n} tokens and its output {on}, positions {tokens}")
-            args += [xp, xs, op, os_, heads]
-        ps = self._check(positions, "positions", torch.int32, (tokens,))
+        shape = tokens, = positions.shape
+        ps = self._check(positions, "positions", torch.int32, shape)
+        qp = qs = qo = qos = kp = ks = ko = kos = None
+        qh = kh = 0
+        qn = qon = kn = kon = tokens
+        if q is not None:
+            qp, qs, qn, qh = self._rows(q, "q", 0, _BF16)
+            qo, qos, qon, _ = (qp, qs, qn, qh) if q_out is None else self._rows(q_out, "q_out", qh, _BF16)
+        if k is not None:
+            kp, ks, kn, kh = self._rows(k, "k", 0, _BF16)
+            ko, kos, kon, _ = (kp, ks, kn, kh) if k_out is None else self._rows(k_out, "k_out", kh, _BF16)
+        if not qn == qon == kn == kon == tokens:
+            raise ValueError(f"q has {qn} tokens and its output {qon}, k has {kn} tokens and its output {kon}, "
+                             f"positions {tokens}")
         run = self._apply if self._index is not None and torch._C._cuda_getDevice() == self._index \
             else self._elsewhere(self._apply)
-        rc = run(self._p, *args, self.head_dim, ps, tokens,
+        rc = run(self._p, qp, qs or 0, qo, qos or 0, qh, kp, ks or 0, ko, kos or 0, kh, self.head_dim, ps, tokens,
                  stream if stream is not None else torch._C._cuda_getCurrentRawStream(self._index))
         if rc:
             self.L.check(rc, "rotary_apply")
