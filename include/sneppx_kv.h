@@ -161,12 +161,12 @@ int SNEPPX_kv_share(int32_t* refs, size_t pages, size_t page_size, int32_t* bloc
  * same pages, which are read once for a group and not once for each row.
  * group_starts int32 [groups + 1] (ascending): group g is the rows group_starts[g] ..
  * group_starts[g + 1], and their first prefix_lengths[g] tokens (int32 [groups]) are
- * the same: they are read by the table of its first row that is as long as that (of its
- * longest row, if none is).  Rows of no group, and rows shorter than their group's
- * prefix, are right as well.  max_length: no row
- * is longer; max_prefix and max_own: about the longest prefix, and the most tokens
- * that a row has behind its prefix (they size the launch; results do not depend on
- * them but for the rounding).  Scratch: a workspace of the calling thread on `stream`. */
+ * the same, read once by the table of its first row that is as long.  Rows of no group,
+ * and rows shorter than their group's prefix, read all their tokens by themselves.
+ * max_length: no row is longer; max_prefix and max_own: about the longest prefix, and
+ * the most tokens that a row has behind its prefix (they size the launch; results do not
+ * depend on them but for the rounding).  Scratch: a workspace of the calling thread on
+ * `stream`. */
 int SNEPPX_kv_attention_shared(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_stride, void* out,
                                size_t out_stride, SNEPPXDtype out_dtype, const int32_t* block_tables,
                                size_t table_width, const int32_t* lengths, size_t rows, size_t q_heads,

@@ -125,19 +125,20 @@ struct Groups {
     }
 };
 
-// The row of a group whose table has its prefix: the first that is as long, or the
-// longest (of which none reads more of it).
-__device__ __forceinline__ uint32_t row_with(const Shared& a, const Prefix& x) {
-    uint32_t best = x.first, most = kv_length(a.lengths, x.first, x.tokens);
-    for (uint32_t r0 = 0; r0 < x.rows && most < x.tokens; r0 += 64) {
-        const uint32_t r = r0 + (threadIdx.x & 63), n = r < x.rows ? kv_length(a.lengths, x.first + r, x.tokens) : 0;
-        const uint32_t top = lane_max(n);
-        if (top > most) {
-            most = top;
-            best = x.first + r0 + __builtin_ctzll(__ballot(n == top));
-        }
+// The row of a group whose table its prefix is read by: the first that is as long.  False
+// if there is none: rows shorter than the prefix have all their tokens for their own (a
+// token that one row has and another has not must not meet the other's weights, not even
+// as 0 * NaN).
+__device__ __forceinline__ bool row_with(const Shared& a, const Prefix& x, uint32_t& row) {
+    row = x.first;
+    if (kv_length(a.lengths, x.first, x.tokens) == x.tokens) return true;
+    for (uint32_t r0 = 0; r0 < x.rows; r0 += 64) {
+        const uint32_t r = r0 + (threadIdx.x & 63);
+        const uint64_t is = __ballot(r < x.rows && kv_length(a.lengths, x.first + (r < x.rows ? r : 0), x.tokens) == x.tokens);
+        row = x.first + r0 + (is ? __builtin_ctzll(is) : 0);
+        if (is) return true;
     }
-    return best;
+    return false;
 }
 
 // x of this lane and of the one 32 lanes away
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
         const Groups groups(a, p.width * p.page_size);
         len = len < groups.most ? len : groups.most;
         Prefix x;
-        const uint32_t begins = !groups.find<true>(b, x) ? 0 : x.tokens < len ? x.tokens : len;
+        const uint32_t begins = groups.find<true>(b, x) && x.tokens <= len ? x.tokens : 0;
         const uint32_t t0 = begins + span * a.own_span;
         if (span && t0 >= len) return;
         const uint32_t t1 = span + 1 < a.splits && len - t0 > a.own_span ? t0 + a.own_span : len;
@@ -495,11 +496,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
     look(t0);
     // (columns past the tile's queries repeat its last: nothing reads what they give)
     bf16x8 q[KQ];
-    uint32_t limit;
     {
         const uint32_t idx = at + (q0 + c < nq ? q0 + c : nq - 1), b = first + idx / a.group;
         const uint16_t* const qh = a.q + b * a.q_stride + (size_t)(h * a.group + idx % a.group) * dim;
-        limit = kv_length(a.lengths, b, t1);
 #pragma unroll
         for (int s = 0; s < KQ; s++) {
             const uint32_t d = 16 * s + 8 * g;
@@ -508,10 +507,10 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
             q[s] = __builtin_bit_cast(bf16x8, w);
         }
     }
-    const uint32_t least = ~__builtin_amdgcn_readfirstlane(lane_max(~limit));     // of the wave's queries
-
     // (looked up above by the first row's table, which nearly always has the prefix)
-    if (const uint32_t reads = row_with(a, x); reads != first) {
+    uint32_t reads;
+    if (!row_with(a, x, reads)) return;
+    if (reads != first) {
         table = p.table(reads, h);
         look(t0);
     }
@@ -585,9 +584,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
     f32x16 o[DT] = {};
     float m = -INFINITY, sum = 0.0f;
     bool any = false;
-    // N x 32 tokens from `base` on, whose rows and scales lie at kt, vt, ksc and vsc
-    auto attend = [&](auto n_, const uint8_t* kt, const uint8_t* vt, const float* kscales, const float* vscales, uint32_t base,
-                      uint64_t there) {
+    // N x 32 tokens, whose rows and scales lie at kt, vt, kscales and vscales
+    auto attend = [&](auto n_, const uint8_t* kt, const uint8_t* vt, const float* kscales, const float* vscales, uint64_t there) {
         constexpr int N = decltype(n_)::value;
         f32x16 s[N] = {};
         // (reads ahead of the products: one after the other they would wait for each)
@@ -617,17 +615,12 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
 #pragma unroll
                     for (int i = 0; i < 4; i++) s[u][r + i] *= k4[i];
                 }
-            const uint32_t from = base + 32 * u, mask = (uint32_t)(there >> (32 * u));
-            if (mask != 0xFFFFFFFFu || from + 32 > least) {
-                const uint32_t upto = limit > from ? limit - from : 0;
-                const uint32_t mine = upto >= 32 ? mask : mask & ((1u << upto) - 1);
+            const uint32_t mask = (uint32_t)(there >> (32 * u));
+            any |= mask != 0;
+            if (mask != 0xFFFFFFFFu)
 #pragma unroll
                 for (int r = 0; r < 16; r++)
-                    if (!(mine >> (2 * (r & 12) + (r & 3) + 4 * g) & 1)) s[u][r] = -INFINITY;
-                any |= mine != 0;
-            } else {
-                any = true;
-            }
+                    if (!(mask >> (2 * (r & 12) + (r & 3) + 4 * g) & 1)) s[u][r] = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; r++) top = fmaxf(top, s[u][r]);
         }
@@ -730,7 +723,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
                 }
                 const uint8_t* const kt = lds + buf * L::BUF + u0 * 32 * L::RB;
                 const float* const sc = scales + 2 * buf * STEP + 32 * u0;
-                if (busy) attend(n, kt, kt + L::T, sc, sc + STEP, base + 32 * u0, there >> (32 * u0));
+                if (busy) attend(n, kt, kt + L::T, sc, sc + STEP, there >> (32 * u0));
             }
         };
         if (wide) steps(std::integral_constant<int, 2>{}, 0);
@@ -797,14 +790,14 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
     const Groups groups(a, p.width * p.page_size);
     len = len < groups.most ? len : groups.most;
     Prefix x = {};
-    const bool shared = groups.find<true>(b, x);
+    const bool shared = groups.find<true>(b, x) && x.tokens <= len;
     const uint32_t idx = shared ? (b - x.first) * a.group + j : 0;
-    const uint32_t unit = x.base + idx / TILE * x.spans;
+    const uint32_t unit = shared ? x.base + idx / TILE * x.spans : 0;
     // (spans past the workspace: of groups that overlap)
     const uint32_t spans = !shared || unit >= a.blocks ? 0 : x.spans < a.blocks - unit ? x.spans : a.blocks - unit;
     const size_t from = ((size_t)h * a.blocks + unit) * a.columns + idx % TILE;
     const size_t own = ((((size_t)b * p.heads + h) * a.own_tiles + j / 16) * a.splits) * a.own_columns + j % 16;
-    const uint32_t begins = !shared ? 0 : x.tokens < len ? x.tokens : len;
+    const uint32_t begins = shared ? x.tokens : 0;
     const uint32_t splits = len - begins > a.own_span ? (len - begins + a.own_span - 1) / a.own_span : 1;
     const uint32_t n = spans + (splits < a.splits ? splits : a.splits);
     auto place = [&](uint32_t i) { return i < spans ? from + (size_t)i * a.columns : own + (size_t)(i - spans) * a.own_columns; };
