@@ -431,7 +431,6 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
     typedef Tiles<DP> L;
     constexpr bool I8 = FORM == INT8;
     constexpr int CH = L::PIECES / (I8 ? 2 : 1);           // 16-byte pieces of a row in the pool
-    constexpr int EACH = STEP * CH / 256;                  // of a tile, for a thread
     constexpr int KQ = DP / 16, DT = DP / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     float* const scales = reinterpret_cast<float*>(lds + L::SCALES);       // [buffer][keys, values][STEP]
