@@ -47,7 +47,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p) {
 constexpr int SLOT_KV_SHARED = 10;    // of the stream's workspaces
 constexpr uint32_t STEP = 64;         // tokens of a step
 constexpr uint32_t TILE = 128;        // queries of a unit
-constexpr uint32_t kLeast = 4;        // steps of a unit, where there are so many
+constexpr uint32_t kLeast = 3;        // steps of a unit at least, of long prefixes
 constexpr int kLag = 8;               // log2 of how far a logit may pass the maximum that weights refer to
 
 struct Shared {
@@ -59,6 +59,7 @@ struct Shared {
     float2 *ml, *own_ml;       // maximum and sum of the same
     uint32_t rows, q_heads, group, groups, max_length;
     uint32_t about, blocks;    // units of the prefixes of a head: about so many, and so many at most
+    uint32_t least;            // steps of one at least
     uint32_t columns, own_columns, own_tiles, splits, own_span;    // own_span: tokens of a split but the last
     float scale_log2;          // not negative: `flip` changes the queries' signs instead
     float room, lift;          // log2 of the most that weights of up to 2^kLag sum up to, and that less kLag
@@ -85,7 +86,7 @@ struct Groups {
             total += __builtin_amdgcn_readlane(lane_prefix(tiles(x) * steps(x)), 63);
         }
         per = (total + a.about - 1) / (a.about ? a.about : 1);
-        per = per > kLeast ? per : kLeast;
+        per = per > a.least ? per : a.least;
     }
     __device__ __forceinline__ Prefix at(uint32_t g0) const {
         const uint32_t g = g0 + (threadIdx.x & 63);
@@ -778,11 +779,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
         }
 }
 
-// A wave for each row and query head: what its prefix's spans and its own tokens' left,
-// added in that order.
+// W waves for each row and query head: what its prefix's spans and its own tokens' left,
+// added in that order by every one for its part of them, and then the waves' sums.
+template <int W>
 __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Shared a) {
-    const uint32_t lane = threadIdx.x & 63;
-    const uint32_t number = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ f32x4 sums[W > 1 ? W - 1 : 1][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t number = blockIdx.x * (4 / W) + (W > 1 ? 0 : wave);
     if (number >= a.rows * a.q_heads) return;
     const uint32_t b = number / a.q_heads, hq = number - b * a.q_heads, h = hq / a.group, j = hq - h * a.group;
     uint32_t len = kv_length(a.lengths, b, a.max_length);        // (asked for before what the groups say)
@@ -802,34 +805,40 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
     auto place = [&](uint32_t i) { return i < spans ? from + (size_t)i * a.columns : own + (size_t)(i - spans) * a.own_columns; };
     auto end = [&](uint32_t i) { return i >= n ? make_float2(-INFINITY, 0.0f) : i < spans ? a.ml[place(i)] : a.own_ml[place(i)]; };
 
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 64) top = fmaxf(top, end(i).x);
-    top = lane_max(top);
-    const uint32_t span = p.dim <= 64 ? 16 : p.dim <= 128 ? 32 : 64, ways = 64 / span;
-    const uint32_t d = 4 * (lane & (span - 1)), way = lane / span;
+    const uint32_t span = p.dim <= 64 ? 16 : p.dim <= 128 ? 32 : 64, ways = 64 / span * W;
+    const uint32_t d = 4 * (lane & (span - 1)), way = (W > 1 ? wave * (64 / span) : 0) + lane / span;
     const bool in = d < p.dim;
+    constexpr int U = 8;              // loads in flight
+    f32x4 part[U];
+    auto fetch = [&](uint32_t i0, uint32_t k0, uint32_t here) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t k = k0 + u * ways + way, i = i0 + (k < here ? k : here - 1);
+            part[u] = *reinterpret_cast<const f32x4*>((i < spans ? a.part : a.own_part) + place(i) * p.dim + (in ? d : 0));
+        }
+    };
+    // (the first values on their way along with the maxima)
+    float2 e = end(lane);
+    fetch(0, 0, n < 64 ? n : 64);
+    float top = e.x;
+    for (uint32_t i = lane + 64; i < n; i += 64) top = fmaxf(top, end(i).x);
+    top = lane_max(top);
     f32x4 v = {};
     float total = 0.0f, plain = 0.0f;
     for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-        const float2 e = end(i0 + lane);
+        if (i0) e = end(i0 + lane);
         const float f = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
         total += f * e.y;
         plain += e.y;
         const uint32_t here = n - i0 < 64 ? n - i0 : 64;
-        constexpr int U = 8;              // loads in flight
         for (uint32_t k0 = 0; k0 < here; k0 += U * ways) {
-            f32x4 part[U];
-            float w[U];
+            if (i0 + k0) fetch(i0, k0, here);
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const uint32_t k = k0 + u * ways + way, i = i0 + (k < here ? k : here - 1);
-                part[u] = *reinterpret_cast<const f32x4*>((i < spans ? a.part : a.own_part) + place(i) * p.dim + (in ? d : 0));
-                w[u] = __shfl(f, k & 63);
-                if (k >= here) w[u] = 0.0f;
+                const uint32_t k = k0 + u * ways + way;
+                const float w = __shfl(f, k & 63);
+                if (k < here && w != 0.0f) v += w * part[u];
             }
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if (w[u] != 0.0f) v += w[u] * part[u];
         }
     }
     total = lane_sum(total);
@@ -837,6 +846,13 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
     for (uint32_t o = span; o < 64; o <<= 1)
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] += __shfl_xor(v[k], o);
+    if (W > 1) {
+        if (wave) sums[wave - 1][lane] = v;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 1; w < W; w++) v += sums[w - 1][lane];
+    }
     if (way || !in) return;
     v *= top == -INFINITY ? plain == 0.0f ? 0.0f : NAN : 1.0f / total;
     const size_t to = b * a.out_stride + (size_t)hq * p.dim + d;
@@ -892,6 +908,11 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     const size_t shared_work = 3 * few * prefix_steps, own_work = rows * own_steps;
     size_t about = shared_work + own_work ? target * shared_work / (shared_work + own_work) : 0;
     if (about < 1) about = 1;
+    // A prefix of up to ten steps a step to each workgroup, of twice that two, of more three:
+    // a span's steps follow one another, but all of them are joined (20 rows behind 500
+    // tokens 15.5 with spans of three, 13.6 of one; five prefixes of up to 8192 18.7 and 19.8).
+    size_t least = (prefix_steps + 9) / 10;
+    least = least < 1 ? 1 : least < kLeast ? least : kLeast;
     size_t own_span = rows * c->kv_heads * own_tiles * max_own / 1024 / 32 * 32;
     if (own_span < 64) own_span = 64;
     size_t splits = (max_own + own_span - 1) / own_span;
@@ -928,6 +949,7 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     a.max_length = (uint32_t)max_length;
     a.about = (uint32_t)about;
     a.blocks = (uint32_t)blocks;
+    a.least = (uint32_t)least;
     a.columns = (uint32_t)columns;
     a.own_columns = (uint32_t)own_columns;
     a.own_tiles = (uint32_t)own_tiles;
@@ -944,7 +966,12 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     a.out_f32 = out_f32;
     const bool i8 = c->dtype == SNEPPX_INT8;
     if (out_f32 ? launch<3>((unsigned)grid, i8, p, a, S(st)) : launch<2>((unsigned)grid, i8, p, a, S(st))) return -1;
-    k_kv_shared_join<<<(unsigned)((rows * q_heads + 3) / 4), 256, 0, S(st)>>>(p, a);
+    // Few rows with much to add up: four waves for each query (48 rows of 4 heads and some 55
+    // parts 21.8 to 18.7 us, one of 32 heads and 63 16.5 to 13.8; with up to 17 parts one
+    // wave is better, 15.6 to 17.1, and with 2048 queries, 32.9 to 37.1).
+    const size_t most = (prefix_steps + least - 1) / least, parts = (few && about / few < most ? about / few : most) + splits;
+    if (rows * q_heads <= 1024 && parts > 32) k_kv_shared_join<4><<<(unsigned)(rows * q_heads), 256, 0, S(st)>>>(p, a);
+    else k_kv_shared_join<1><<<(unsigned)((rows * q_heads + 3) / 4), 256, 0, S(st)>>>(p, a);
     return snx_launch_check("k_kv_shared_join");
 }
 
