@@ -85,7 +85,7 @@ __device__ __forceinline__ void place(const Pages& a, uint32_t t, uint32_t b, ui
     int32_t slot = -1, at = -1;
     if (ok) {
         const uint32_t s = len + i, e = a.page_of(s);
-        const uint32_t page = (uint32_t)a.tables[(size_t)b * a.width + e];
+        const uint32_t page = e < a.width ? (uint32_t)a.tables[(size_t)b * a.width + e] : 0xFFFFFFFFu;
         if (page < a.pages) slot = (int32_t)(page * a.page_size + (s - e * a.page_size));
         at = pos + (int32_t)i;
     }
@@ -114,12 +114,12 @@ __device__ __forceinline__ uint32_t free_of(const Pages& a, uint32_t p) {
 // and shared out among the threads, so that a few rows of many pages go as fast as many of
 // one.  The first refs are asked for before all else.
 // What bounds it: one load after the other (lengths, entries, new entries again) and some
-// 14 barriers, 6 us for 64 rows by four waves; for pools with few free pages the refs up to
+// 14 barriers, 5.3 us for 64 rows by four waves; for pools with few free pages the refs up to
 // the last one taken, at the rate of one CU.
 template <int W>
 __global__ void __launch_bounds__(64 * W) k_kv_reserve(const Pages a) {
     constexpr uint32_t THREADS = 64 * W, TURN = kEach * THREADS;
-    __shared__ uint32_t sh[2 * W], first[THREADS], entry[THREADS], need[THREADS], upto[THREADS], start[THREADS + 1];
+    __shared__ uint32_t sh[3 * W], first[THREADS], entry[THREADS], need[THREADS], upto[THREADS], start[THREADS + 1];
     __shared__ uint32_t length[THREADS], found[TURN];
     __shared__ uint8_t given[THREADS];
     __shared__ int32_t next[THREADS];
@@ -144,12 +144,15 @@ __global__ void __launch_bounds__(64 * W) k_kv_reserve(const Pages a) {
             e0 = pages_of(a, n);
             span = fits ? pages_of(a, n + want) - e0 : 0;
         }
-        uint32_t sums[2] = {want, span}, totals[2], needed;
-        block_prefix<W, 2>(sums, sh, totals);
+        // (a row's first entry by its own thread: a decode step needs no others)
+        uint32_t own = 0xFFFFFFFFu;
+        if (span) own = (uint32_t)a.tables[(size_t)b * a.width + e0];
+        uint32_t sums[3] = {want, span, span > 1}, totals[3], needed;
+        block_prefix<W, 3>(sums, sh, totals);
         const uint32_t tokens = totals[0], entries = totals[1];
         first[tid] = sums[1] - span;
         entry[tid] = e0;
-        need[tid] = span;
+        need[tid] = span - (own < a.pages);
         start[tid + 1] = add_cut(carry, sums[0]);
         if (tid == 0) start[0] = carry;
         length[tid] = n;
@@ -159,13 +162,14 @@ __global__ void __launch_bounds__(64 * W) k_kv_reserve(const Pages a) {
 
         // less the entries that name a page (a few, and seldom)
         constexpr int U = 4;              // loads in flight
-        for (uint32_t i0 = tid; i0 < entries; i0 += U * THREADS) {
+        for (uint32_t i0 = tid; totals[2] && i0 < entries; i0 += U * THREADS) {
             uint32_t r[U], page[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const uint32_t i = i0 + u * THREADS < entries ? i0 + u * THREADS : i0;
                 r[u] = last_upto(first, rows, i);
-                page[u] = (uint32_t)a.tables[(size_t)(r0 + r[u]) * a.width + entry[r[u]] + (i - first[r[u]])];
+                page[u] = 0xFFFFFFFFu;
+                if (i != first[r[u]]) page[u] = (uint32_t)a.tables[(size_t)(r0 + r[u]) * a.width + entry[r[u]] + (i - first[r[u]])];
             }
 #pragma unroll
             for (int u = 0; u < U; u++)
