@@ -67,16 +67,29 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* sh, uint3
     return a[0];
 }
 
-// the last of n ascending numbers (the first at most x) that is at most x
-__device__ __forceinline__ uint32_t last_upto(const uint32_t* at, uint32_t n, uint32_t x) {
-    uint32_t b = 0;
+// the last of n ascending numbers (the first at most x) that is at most x: of N x at once
+// (a look at LDS at a time takes 130 cycles, whether for one or for N)
+template <int N>
+__device__ __forceinline__ void last_upto(const uint32_t* at, uint32_t n, const uint32_t (&x)[N], uint32_t (&b)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) b[i] = 0;
     while (n > 1) {
+        // (the upper half of an odd number has one more, and the lower is looked through as if
+        // it had: what lies behind it is above x)
         const uint32_t half = n / 2;
-        const bool up = at[b + half] <= x;
-        b += up ? half : 0;
-        n = up ? n - half : half;
+        uint32_t seen[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) seen[i] = at[b[i] + half];
+#pragma unroll
+        for (int i = 0; i < N; i++) b[i] += seen[i] <= x[i] ? half : 0;
+        n -= half;
     }
-    return b;
+}
+__device__ __forceinline__ uint32_t last_upto(const uint32_t* at, uint32_t n, uint32_t x) {
+    const uint32_t one[1] = {x};
+    uint32_t b[1];
+    last_upto<1>(at, n, one, b);
+    return b[0];
 }
 
 // slot and position of token i of a row's new ones (granted: its length and next
@@ -163,13 +176,15 @@ __global__ void __launch_bounds__(64 * W) k_kv_reserve(const Pages a) {
         // less the entries that name a page (a few, and seldom)
         constexpr int U = 4;              // loads in flight
         for (uint32_t i0 = tid; totals[2] && i0 < entries; i0 += U * THREADS) {
-            uint32_t r[U], page[U];
+            uint32_t i[U], r[U], page[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) i[u] = i0 + u * THREADS < entries ? i0 + u * THREADS : i0;
+            last_upto<U>(first, rows, i, r);
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const uint32_t i = i0 + u * THREADS < entries ? i0 + u * THREADS : i0;
-                r[u] = last_upto(first, rows, i);
+                const uint32_t j = i[u] - first[r[u]];
                 page[u] = 0xFFFFFFFFu;
-                if (i != first[r[u]]) page[u] = (uint32_t)a.tables[(size_t)(r0 + r[u]) * a.width + entry[r[u]] + (i - first[r[u]])];
+                if (j) page[u] = (uint32_t)a.tables[(size_t)(r0 + r[u]) * a.width + entry[r[u]] + j];
             }
 #pragma unroll
             for (int u = 0; u < U; u++)
@@ -219,19 +234,28 @@ __global__ void __launch_bounds__(64 * W) k_kv_reserve(const Pages a) {
             const uint32_t n_now = sum < taken - done ? sum : taken - done;
             uint32_t where[kEach];
 #pragma unroll
-            for (uint32_t q = 0; q < kEach; q++) {
-                const uint32_t k = done + tid + q * THREADS;
-                if (tid + q * THREADS >= n_now) break;
-                const uint32_t r = last_upto(upto, rows, k), j = k - upto[r];
-                uint32_t e = entry[r] + j;
-                const uint32_t all = (r + 1 < rows ? first[r + 1] : entries) - first[r];
-                if (all != need[r]) {
-                    // (those that earlier turns gave to the row name pages by now)
-                    const int32_t* const t = a.tables + (size_t)(r0 + r) * a.width;
-                    uint32_t left = done > upto[r] ? k - done : j;
-                    for (e = entry[r]; e + 1 < entry[r] + all && ((uint32_t)t[e] < a.pages || left--); e++) {}
+            for (uint32_t q0 = 0; q0 < kEach; q0 += U) {
+                if (tid + q0 * THREADS >= n_now) break;
+                uint32_t k[U], r[U];
+#pragma unroll
+                for (uint32_t u = 0; u < U; u++) {
+                    const uint32_t i = tid + (q0 + u) * THREADS;
+                    k[u] = done + (i < n_now ? i : n_now - 1);
                 }
-                where[q] = (r0 + r) * a.width + e;
+                last_upto<U>(upto, rows, k, r);
+#pragma unroll
+                for (uint32_t u = 0; u < U; u++) {
+                    const uint32_t of = r[u], j = k[u] - upto[of];
+                    uint32_t e = entry[of] + j;
+                    const uint32_t all = (of + 1 < rows ? first[of + 1] : entries) - first[of];
+                    if (all != need[of]) {
+                        // (those that earlier turns gave to the row name pages by now)
+                        const int32_t* const t = a.tables + (size_t)(r0 + of) * a.width;
+                        uint32_t left = done > upto[of] ? k[u] - done : j;
+                        for (e = entry[of]; e + 1 < entry[of] + all && ((uint32_t)t[e] < a.pages || left--); e++) {}
+                    }
+                    where[q0 + u] = (r0 + of) * a.width + e;
+                }
             }
             __syncthreads();
 #pragma unroll
