@@ -66,7 +66,7 @@ def build(lib, groups, loose, heads, dim, page, dtype, seed, std=1.0):
             for t in range(lists[b] * page, min(n, lengths[b])):
                 src, dst = tables[parents[b], t // page], tables[b, t // page]
                 k[dst, :, t % page], v[dst, :, t % page] = k[src, :, t % page], v[src, :, t % page]
-    # (the first row's table is read for the whole prefix, also where that row is shorter)
+    # (pages that a first row shorter than the prefix names behind its end are other rows')
     for (n, mine), r0 in zip(groups, starts):
         if mine:
             t = np.arange(min(n, width * page))
@@ -233,3 +233,17 @@ def test_infinite_and_nan_logits(lib):
     assert (o[0, :, 7] == math.inf).all()
     o[0, :, 7] = 0
     assert torch.isfinite(o[0]).all()
+
+
+@pytest.mark.parametrize("own", [[-100, 20, -1], [-1, -200, -500], [-500, 0, 3]])
+@pytest.mark.parametrize("dtype", ["bf16", "int8"])
+def test_rows_shorter_than_their_prefix(lib, own, dtype):
+    """Entries behind a short row's end name no page: the prefix is read by the table of a
+    row that has it, and by none if none has."""
+    c, ref, tables, lengths, *dev = build(lib, [(500, own)], [70], 2, 64, 16, dtype, 12)
+    for b, n in enumerate(lengths):
+        tables[b, -(-n // 16):] = -1
+    dev[0].copy_(torch.from_numpy(tables))
+    q = torch.randn((4, 8, 64), device=DEV, generator=torch.Generator(device=DEV).manual_seed(6)).to(torch.bfloat16)
+    check(c, ref, tables, lengths, dev, q, "f32", 0.125)
+    check(c, ref, tables, lengths, dev, q, "bf16", 0.125, max_own=1)
