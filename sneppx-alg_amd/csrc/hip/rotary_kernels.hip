@@ -10,7 +10,9 @@
 // maximum).  The work is reading and writing every head once; what stands in its way is
 // the angles, four fp64 products and four sines and cosines to a lane, so a lane takes
 // up to kMostHeads heads of a token with the angles of the first, all their loads in
-// flight over that.
+// flight over that.  2320 tokens of 40 heads of 128, normalised, take 12.3 us (48 MB read
+// and written, 4.9 TB/s behind the launch), into an int8 cache 14.3 (62 MB); 16 tokens 2.4,
+// a chain of position, angle, head and result.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -169,9 +171,11 @@ __global__ void __launch_bounds__(256) k_rotate(const KVPool p, const Heads n) {
 
 template <bool APPEND, bool I8, int LR>
 int launch(const KVPool& p, Heads& n, hipStream_t s, const char* who) {
-    // As many heads to a lane as leave every CU some waves.
+    // Four heads to a lane where that leaves every CU eight waves: 16 tokens of 40 heads 2.35
+    // us with one and 3.4 with four, 600 of them 4.7 either way, 1200 9.6 and 8.7, 2320 15.6
+    // and 13.2 (8 heads to a lane as 4).
     const size_t waves = (size_t)n.tokens * n.heads * LR / 64;
-    const int per = waves >= 4096 * kMostHeads ? kMostHeads : 1;
+    const int per = waves >= 2048 * kMostHeads ? kMostHeads : 1;
     n.groups = (n.heads + per - 1) / per;
     n.by_groups = divider(n.groups);
     const size_t numbers = (size_t)n.tokens * n.groups, blocks = (numbers * LR + 255) / 256;
