@@ -907,27 +907,50 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     const KVPool p = kv_pool(c, tables, width);
     const size_t group = q_heads / c->kv_heads;
     const size_t tiles = groups ? rows * group / TILE + groups : 0;      // of a head, at most
-    const size_t prefix_steps = groups ? (max_prefix + STEP - 1) / STEP : 0, own_steps = (max_own + STEP - 1) / STEP;
-    // Units for two workgroups on every CU (256 rows behind 16384 tokens 125 us, with one 145,
-    // with three 131), shared out by what prefixes and own tokens take: a step of a tile
-    // about three times what a row's has, 64 rows behind 4096 with up to 512 of their own
-    // 30.5 us so, 33.4 at once the row's and 33.1 at six times.
-    const size_t target = ((size_t)2 * cu_count() + c->kv_heads - 1) / c->kv_heads;
-    const size_t few = groups ? (rows * group + TILE - 1) / TILE : 0;    // tiles of groups that fill them
+    const size_t prefix_steps = groups ? (max_prefix + STEP - 1) / STEP : 0;
     const size_t own_tiles = (group + 15) / 16;
-    const size_t shared_work = 3 * few * prefix_steps, own_work = rows * own_steps;
-    size_t about = shared_work + own_work ? target * shared_work / (shared_work + own_work) : 0;
-    if (about < 1) about = 1;
+    const size_t places = (size_t)(c->head_dim <= 128 ? 2 : 1) * cu_count();      // of workgroups that run at once
+    // Own tokens by about 1024 waves, which all run at once (64 rows behind 4096 tokens with up
+    // to 512 of their own 30.5 us so, by 2048 36.7).
+    size_t own_span = rows * c->kv_heads * own_tiles * max_own / 1024 / 32 * 32;
+    if (own_span < 64) own_span = 64;
+    size_t splits = (max_own + own_span - 1) / own_span;
+    if (splits < 1) splits = 1;
     // A prefix of up to ten steps a step to each workgroup, of twice that two, of more three:
     // a span's steps follow one another, but all of them are joined (20 rows behind 500
     // tokens 15.5 with spans of three, 13.6 of one; five prefixes of up to 8192 18.7 and 19.8).
     size_t least = (prefix_steps + 9) / 10;
     least = least < 1 ? 1 : least < kLeast ? least : kLeast;
-    // Own tokens by about 1024 waves, which all run at once (the same 30.5, by 2048 36.7).
-    size_t own_span = rows * c->kv_heads * own_tiles * max_own / 1024 / 32 * 32;
-    if (own_span < 64) own_span = 64;
-    size_t splits = (max_own + own_span - 1) / own_span;
-    if (splits < 1) splits = 1;
+    // As many spans of a prefix as make the launch shortest, by a count of what runs one after
+    // the other in the CUs' places, in steps (3 us): units of `per` steps and one to begin
+    // with, rows' own tokens 40 to a step, in places that units leave free or behind them,
+    // and parts, written and read again.  Against as many units as places, shared out by the
+    // two kinds' work: 112 rows behind 4125 tokens, heads of 256, 64 to 52 us, 32 behind
+    // 2048 with up to 1024 of their own 28.4 to 26.1; 20 prefixes of 5 rows 27.7 to 30.4.
+    const size_t few = groups ? (rows * group + TILE - 1) / TILE : 0;    // tiles of groups that fill them
+    const size_t about_tiles = few > groups ? few : groups;
+    const size_t own_wgs = (rows * c->kv_heads * own_tiles * splits + 3) / 4;
+    const float own_time = max_own ? (float)(own_span < max_own ? own_span : max_own) / 40.0f + 1.0f : 0.0f;
+    const float per_place = 1.0f / (float)places;
+    auto rounds = [&](size_t wgs) { return __builtin_ceilf((float)wgs * per_place); };
+    size_t about = 1;
+    float best = FLT_MAX;
+    for (size_t per = prefix_steps; per >= least;) {
+        const size_t spans = (prefix_steps + per - 1) / per, units = about_tiles * spans * c->kv_heads;
+        if (spans > 1 && (units > 4 * places || spans > 128)) break;
+        const float unit_time = (float)per + 1.0f, all = rounds(units);
+        const float free = all * (float)places - (float)units;       // places of the last round
+        float left = (float)own_wgs;
+        if (own_time > 0.0f) left -= free * __builtin_floorf(unit_time / own_time);
+        const float parts = (float)(rows * q_heads * spans) * (float)c->head_dim * 6e-7f;
+        const float time = all * unit_time + (left > 0.0f ? rounds((size_t)left) * own_time : 0.0f) + parts;
+        if (time < best) {
+            best = time;
+            about = about_tiles * spans;
+        }
+        const size_t next = (prefix_steps + spans) / (spans + 1);        // of one span more
+        per = next < per ? next : per - 1;
+    }
     const size_t blocks = groups ? about + tiles : 0;
     const size_t columns = rows * group < TILE ? rows * group : TILE, own_columns = group < 16 ? group : 16;
     const size_t slots = blocks * c->kv_heads * columns, own = rows * c->kv_heads * own_tiles * splits * own_columns;
