@@ -433,12 +433,15 @@ __device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uin
 // reaches 1.29); without the lower pieces 81, in any order of the instructions 102.  For
 // few the chain of a step (look-up, row, tile, logits, maximum, weights), 3 us, a unit of
 // three steps 15.
-template <int DP, Form FORM, int PIECES>
-__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPool p, const Shared a) {
+// DIM: the head's elements that products are made of, DP those of a row in LDS (heads of 80,
+// 256 rows behind 16384 tokens: 109 us with products of 128 elements, 98 of 96).
+template <int DIM, Form FORM, int PIECES>
+__global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVPool p, const Shared a) {
+    constexpr int DP = DIM <= 64 ? 64 : DIM <= 128 ? 128 : 256;
     typedef Tiles<DP> L;
     constexpr bool I8 = FORM == INT8;
     constexpr int CH = L::PIECES / (I8 ? 2 : 1);           // 16-byte pieces of a row in the pool
-    constexpr int KQ = DP / 16, DT = DP / 32;
+    constexpr int KQ = DIM / 16, DT = DIM / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     float* const scales = reinterpret_cast<float*>(lds + L::SCALES);       // [buffer][keys, values][STEP]
     float2* const ends = reinterpret_cast<float2*>(lds + L::ENDS);         // [2][32]
@@ -595,7 +598,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_kv_shared(const KVPo
         constexpr int N = decltype(n_)::value;
         f32x16 s[N] = {};
         // (reads ahead of the products: one after the other they would wait for each)
-        constexpr int AHEAD = DP <= 64 ? KQ : I8 ? (DP <= 128 ? 4 : 2) : DP <= 128 ? KQ : 4;
+        constexpr int AHEAD = DP <= 64 ? KQ : I8 ? (DP <= 128 ? KQ / 2 : 2) : DP <= 128 ? KQ : 4;
 #pragma unroll
         for (int i0 = 0; i0 < KQ; i0 += AHEAD) {
             bf16x8 kf[AHEAD][N];
@@ -868,27 +871,32 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
     else *reinterpret_cast<bf16x4_any*>(static_cast<uint16_t*>(a.out) + to) = u32x2{bf16x2_out(v[0], v[1]), bf16x2_out(v[2], v[3])};
 }
 
-template <int DP, Form FORM, int PIECES>
+template <int DIM, Form FORM, int PIECES>
 int launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    const auto fn = k_kv_shared<DP, FORM, PIECES>;
-    if (Tiles<DP>::ALL > 65536 && lds_optin(reinterpret_cast<const void*>(fn), Tiles<DP>::ALL, done) != hipSuccess) {
-        snx_set_error("kv_attention_shared: no %d bytes of LDS", Tiles<DP>::ALL);
+    constexpr int LDS = Tiles<DIM <= 64 ? 64 : DIM <= 128 ? 128 : 256>::ALL;
+    const auto fn = k_kv_shared<DIM, FORM, PIECES>;
+    if (LDS > 65536 && lds_optin(reinterpret_cast<const void*>(fn), LDS, done) != hipSuccess) {
+        snx_set_error("kv_attention_shared: no %d bytes of LDS", LDS);
         return -1;
     }
-    fn<<<grid, 256, Tiles<DP>::ALL, s>>>(p, a);
+    fn<<<grid, 256, LDS, s>>>(p, a);
     return snx_launch_check("k_kv_shared");
 }
-template <int DP, int PIECES>
+template <int DIM, int PIECES>
 int launch(unsigned grid, bool i8, const KVPool& p, const Shared& a, hipStream_t s) {
-    if (i8) return launch<DP, INT8, PIECES>(grid, p, a, s);
-    // (loads to LDS by 32-bit offsets count apart from LDS reads, those by address do not)
-    const bool near = p.dim == DP && (uint64_t)p.pages * p.heads * p.page_size * DP * 2 <= 0xFFFFFFFFull;
-    return near ? launch<DP, NEAR, PIECES>(grid, p, a, s) : launch<DP, FAR, PIECES>(grid, p, a, s);
+    if (i8) return launch<DIM, INT8, PIECES>(grid, p, a, s);
+    // (loads to LDS by 32-bit offsets count apart from LDS reads, those by address do not:
+    // 64 rows behind 4096 tokens 30.9 us and 33.6)
+    if constexpr (DIM != 96)
+        if (p.dim == DIM && (uint64_t)p.pages * p.heads * p.page_size * DIM * 2 <= 0xFFFFFFFFull)
+            return launch<DIM, NEAR, PIECES>(grid, p, a, s);
+    return launch<DIM, FAR, PIECES>(grid, p, a, s);
 }
 template <int PIECES>
 int launch(unsigned grid, bool i8, const KVPool& p, const Shared& a, hipStream_t s) {
     if (p.dim <= 64) return launch<64, PIECES>(grid, i8, p, a, s);
+    if (p.dim <= 96) return launch<96, PIECES>(grid, i8, p, a, s);
     if (p.dim <= 128) return launch<128, PIECES>(grid, i8, p, a, s);
     return launch<256, PIECES>(grid, i8, p, a, s);
 }

@@ -146,6 +146,9 @@ CASES = [
     ([(100, [1, 2]), (130, [3])], [], 3, 3, 8, 5, "bf16", "f32"),
     ([(100, [1, 2]), (130, [3])], [], 6, 3, 16, 128, "int8", "f32"),
     ([(32, [1, 2])] * 70, [5], 4, 1, 64, 16, "bf16", "f32"),             # more groups than a wave has lanes
+    ([(320, list(range(17)))], [], 8, 1, 96, 16, "bf16", "f32"),         # heads between 64 and 128, 136 queries
+    ([(320, list(range(17)))], [], 8, 1, 80, 16, "int8", "bf16"),
+    ([(200, [3, 0, 90])], [4], 8, 2, 72, 16, "bf16", "f32"),
     ([(5000, [10, 20, 30])], [], 8, 2, 64, 16, "bf16", "f32"),           # many spans
 ]
 
