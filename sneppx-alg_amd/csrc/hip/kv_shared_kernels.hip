@@ -927,8 +927,12 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     // A prefix of up to ten steps a step to each workgroup, of twice that two, of more three:
     // a span's steps follow one another, but all of them are joined (20 rows behind 500
     // tokens 15.5 with spans of three, 13.6 of one; five prefixes of up to 8192 18.7 and 19.8).
-    size_t least = (prefix_steps + 9) / 10;
-    least = least < 1 ? 1 : least < kLeast ? least : kLeast;
+    // Steps of heads beyond 128 are twice as long: one of up to 40, else two (2 rows behind
+    // 2217 tokens 23.3 with three, 17.2 so; behind 5052 21.1, 17.8 and with one 19.3).
+    const bool large = c->head_dim > 128;
+    size_t least = large ? (prefix_steps + 39) / 40 : (prefix_steps + 9) / 10;
+    const size_t most_least = large ? 2 : kLeast;
+    least = least < 1 ? 1 : least < most_least ? least : most_least;
     // As many spans of a prefix as make the launch shortest, by a count of what runs one after
     // the other in the CUs' places, in steps (3 us): units of `per` steps and one to begin
     // with, rows' own tokens 40 to a step, in places that units leave free or behind them,
