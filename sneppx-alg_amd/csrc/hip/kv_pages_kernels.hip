@@ -70,7 +70,7 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t x, uint32_t* sh, uint3
 }
 
 // the last of n ascending numbers (the first at most x) that is at most x: of N x at once
-// (a look at LDS at a time takes 130 cycles, whether for one or for N)
+// (looks at LDS, each waiting for the one before)
 template <int N>
 __device__ __forceinline__ void last_upto(const uint32_t* at, uint32_t n, const uint32_t (&x)[N], uint32_t (&b)[N]) {
 #pragma unroll
@@ -129,7 +129,7 @@ __device__ __forceinline__ uint32_t free_of(const Pages& a, uint32_t p) {
 // and shared out among the threads, so that a few rows of many pages go as fast as many of
 // one.  The first refs are asked for before all else.
 // What bounds it: one load after the other (lengths, entries, new entries again) and some
-// 14 barriers, 5.3 us for 64 rows by four waves; 11 for 48 prompts of up to 4096 tokens, of
+// 14 barriers, 5 us for 64 rows by four waves; 11 for 48 prompts of up to 4096 tokens, of
 // which a third is looking for the entries that need pages and a third giving them out; for pools with few free pages the refs up to
 // the last one taken, at the rate of one CU.
 template <int W>
@@ -177,7 +177,9 @@ __global__ void __launch_bounds__(64 * W) k_kv_reserve(const Pages a) {
         if (b < a.rows) a.starts[b] = (int32_t)start[tid];
 
         // less the entries that name a page (a few, and seldom)
-        constexpr int U = 4;              // loads in flight
+        // (at once: 48 prompts of up to 600 tokens 10.7 us with one, 11.1 with two, 12.2 with four,
+        // of up to 4096 22.1, 20.3 and 20.3)
+        constexpr int U = 2;
         for (uint32_t i0 = tid; totals[2] && i0 < entries; i0 += U * THREADS) {
             uint32_t i[U], r[U], page[U];
 #pragma unroll
@@ -386,8 +388,8 @@ int snx_k_kv_reserve(int32_t* refs, size_t pages, size_t page_size, int32_t* tab
     a.slots = slots;
     a.positions = positions;
     a.tokens = (uint32_t)tokens;
-    // Four waves for what a decode step asks for (their barriers take less: 64 rows 7.0 us,
-    // by sixteen 7.9, a copy of their state included), sixteen for more rows, tokens and so
+    // Four waves for what a decode step asks for (their barriers take less: 64 rows 6.7 us,
+    // by sixteen 7.6, a copy of their state included), sixteen for more rows, tokens and so
     // pages (512 rows 9.1 and by four 12.4, 16 prompts of up to 256 tokens 9.3 and 11.1).
     if (rows <= 256 && tokens <= 1024) k_kv_reserve<4><<<1, 256, 0, S(st)>>>(a);
     else k_kv_reserve<16><<<1, 1024, 0, S(st)>>>(a);
