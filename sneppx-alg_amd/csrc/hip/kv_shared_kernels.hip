@@ -764,7 +764,9 @@ __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVP
         const float top = fmaxf(m, e.x);
         const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
         const float f1 = e.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
-        sum = top == -INFINITY ? fmaxf(sum, e.y) : f0 * sum + f1 * e.y;
+        // (without a finite logit in either: 0, 1 or NaN each, of which the sum keeps what the
+        // join asks for, no tokens, tokens, and NaN)
+        sum = top == -INFINITY ? sum + e.y : f0 * sum + f1 * e.y;
         m = top;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
