@@ -175,7 +175,9 @@ __device__ __forceinline__ u32x4 bytes_to_bf16(uint32_t a, uint32_t b) {
 // eight, two, off by 2^-15 of the weight at most (2^-17 are added, about what cutting the
 // lower one takes away on average).  Values may be infinite, and a zero piece would make
 // NaN of that: no piece is zero unless the weight is, of three by 2^-40 of the first.
-template <int N>
+// Of int8 the codes are finite; where the weight is not (an infinite scale) it is all in
+// the first piece.
+template <int N, bool I8>
 __device__ __forceinline__ void split(const float* x, bf16x8 (&piece)[N]) {
     u32x4 o[N];
 #pragma unroll
@@ -190,10 +192,12 @@ __device__ __forceinline__ void split(const float* x, bf16x8 (&piece)[N]) {
                 const float high = u2f(f2u(a[j]) & 0xFFFF0000u);
                 if (N < 3) {
                     a[j] = __builtin_fmaf(high, -(1.0f - 0x1p-17f), a[j]);
+                    if (I8) a[j] = a[j] == a[j] ? a[j] : 0.0f;
                     continue;
                 }
-                if (i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
-                a[j] = fmaxf(a[j] - high, least[j]);
+                const float low = a[j] - high;
+                if (!I8 && i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
+                a[j] = I8 ? (low == low ? low : 0.0f) : fmaxf(low, least[j]);
             }
         }
     }
@@ -388,7 +392,7 @@ __device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uin
             if (I8) s[i] *= sc[32 + 8 * g + i];
         }
         bf16x8 pc[PIECES];
-        split<PIECES>(s, pc);
+        split<PIECES, I8>(s, pc);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             s16x4 w[2];
@@ -666,7 +670,7 @@ __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVP
 #pragma unroll
                     for (int i = 0; i < 4; i++) e[r + i] *= v4[i];
                 }
-            split<PIECES>(e, pc[k & 1]);
+            split<PIECES, I8>(e, pc[k & 1]);
         };
         auto values = [&](int k) {
 #pragma unroll
