@@ -170,39 +170,35 @@ __device__ __forceinline__ u32x4 bytes_to_bf16(uint32_t a, uint32_t b) {
     return o;
 }
 
-// Eight weights (not negative) as N bf16 pieces each, of eight bits one after the
-// other.  With fp32 results three, which are all 24; with bf16 results, which keep
-// eight, two, off by 2^-15 of the weight at most (2^-17 are added, about what cutting the
-// lower one takes away on average).  Values may be infinite, and a zero piece would make
-// NaN of that: no piece is zero unless the weight is, of three by 2^-40 of the first.
-// Of int8 the codes are finite; where the weight is not (an infinite scale) it is all in
-// the first piece.
-template <int N, bool I8>
-__device__ __forceinline__ void split(const float* x, bf16x8 (&piece)[N]) {
-    u32x4 o[N];
+// Eight weights (not negative) as three bf16 pieces each, exactly (24 significant bits
+// cut into 8 + 8 + 8): the products with bf16 values then sum as fp32 ones would, whatever
+// the results' type.  bf16 values may be infinite, and a zero second or third piece would
+// make NaN of that: they are 2^-40 of the first at least (and normal), which no sum shows,
+// but zero where the weight is zero, so that a token of no weight adds nothing to any
+// value.  Of int8 the codes are finite; where the weight is not (an infinite scale) it is
+// all in the first piece.  (Two pieces for bf16 results, 2^-15 of a weight off, put
+// some results on the other side of a rounding: 256 rows behind 16384 tokens take 154 us
+// with three and 125 with two, 64 behind 4096 33.4 and 32.7.)
+template <bool I8>
+__device__ __forceinline__ void split3(const float* x, bf16x8 (&piece)[3]) {
+    u32x4 o[3];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
         float a[2] = {x[e], x[e + 1]}, least[2];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
+        for (int i = 0; i < 3; i++) {
             o[i][e >> 1] = __builtin_amdgcn_perm(f2u(a[1]), f2u(a[0]), 0x07060302u);
-            if (i == N - 1) break;
+            if (i == 2) break;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float high = u2f(f2u(a[j]) & 0xFFFF0000u);
-                if (N < 3) {
-                    a[j] = __builtin_fmaf(high, -(1.0f - 0x1p-17f), a[j]);
-                    if (I8) a[j] = a[j] == a[j] ? a[j] : 0.0f;
-                    continue;
-                }
-                const float low = a[j] - high;
+                const float high = u2f(f2u(a[j]) & 0xFFFF0000u), low = a[j] - high;
                 if (!I8 && i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
                 a[j] = I8 ? (low == low ? low : 0.0f) : fmaxf(low, least[j]);
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < N; i++) piece[i] = __builtin_bit_cast(bf16x8, o[i]);
+    for (int i = 0; i < 3; i++) piece[i] = __builtin_bit_cast(bf16x8, o[i]);
 }
 
 // A step's keys and values in LDS, in two buffers: token rows of DP bf16 each, their
@@ -269,7 +265,7 @@ __device__ __forceinline__ void own_queries(const KVPool& p, const Shared& a, ui
         q[s] = __builtin_bit_cast(bf16x8, w);
     }
 }
-template <int DP, bool I8, int PIECES>
+template <int DP, bool I8>
 __device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uint32_t b, uint32_t h, const bf16x8 (&q)[DP / 32],
                                            uint32_t nq, uint32_t t0, uint32_t t1, size_t slot, uint8_t* vt) {
     typedef OwnTile<DP> L;
@@ -391,8 +387,8 @@ __device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uin
             sum += s[i];
             if (I8) s[i] *= sc[32 + 8 * g + i];
         }
-        bf16x8 pc[PIECES];
-        split<PIECES, I8>(s, pc);
+        bf16x8 pc[3];
+        split3<I8>(s, pc);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             s16x4 w[2];
@@ -403,7 +399,7 @@ __device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uin
             }
             const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-            for (int i = 0; i < PIECES; i++) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pc[i], o[dt], 0, 0, 0);
+            for (int i = 0; i < 3; i++) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pc[i], o[dt], 0, 0, 0);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -433,13 +429,14 @@ __device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uin
 // With more than 64 queries each wave has 32 of them and all tokens of a step; with
 // fewer, waves w and w + 2 have the same 32 and half of the tokens each.
 // What bounds it: for many queries the products.  1024 queries of a head over 16384 tokens,
-// 8 heads: 102 us, 103 GFLOP with two pieces of a weight, 1.0 PFLOP/s (a plain product
-// reaches 1.29); without the lower pieces 81, in any order of the instructions 102.  For
+// 8 heads: 145 us, 137 GFLOP with the three pieces of a weight, 0.95 PFLOP/s (a plain
+// product reaches 1.29); without the lower two 81, in any order of the instructions.  For
 // few the chain of a step (look-up, row, tile, logits, maximum, weights), 3 us, a unit of
 // three steps 15.
 // DIM: the head's elements that products are made of, DP those of a row in LDS (heads of 80,
-// 256 rows behind 16384 tokens: 109 us with products of 128 elements, 98 of 96).
-template <int DIM, Form FORM, int PIECES>
+// 256 rows behind 16384 tokens: 109 us with products of 128 elements, 98 of 96, both with
+// two pieces of a weight; 140 of 96 with three).
+template <int DIM, Form FORM>
 __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVPool p, const Shared a) {
     constexpr int DP = DIM <= 64 ? 64 : DIM <= 128 ? 128 : 256;
     typedef Tiles<DP> L;
@@ -474,7 +471,7 @@ __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVP
         const uint32_t t0 = begins + span * a.own_span;
         if (span && t0 >= len) return;
         const uint32_t t1 = span + 1 < a.splits && len - t0 > a.own_span ? t0 + a.own_span : len;
-        own_tokens<DP, I8, PIECES>(p, a, b, h, q, nq, t0, t1,
+        own_tokens<DP, I8>(p, a, b, h, q, nq, t0, t1,
                                    ((((size_t)b * p.heads + h) * a.own_tiles + tile) * a.splits + span) * a.own_columns,
                                    lds + wave * OwnTile<DP>::ALL);
         return;
@@ -655,7 +652,7 @@ __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVP
         }
         const float ref = m == -INFINITY ? 0.0f : m;
         // 16 tokens at a time: the next ones' weights and values while these are multiplied
-        bf16x8 pc[2][PIECES], vf[2][DT];
+        bf16x8 pc[2][3], vf[2][DT];
         auto weigh = [&](int k) {
             float e[8];
 #pragma unroll
@@ -670,7 +667,7 @@ __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVP
 #pragma unroll
                     for (int i = 0; i < 4; i++) e[r + i] *= v4[i];
                 }
-            split<PIECES, I8>(e, pc[k & 1]);
+            split3<I8>(e, pc[k & 1]);
         };
         auto values = [&](int k) {
 #pragma unroll
@@ -696,7 +693,7 @@ __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVP
                 weigh(k + 1);
             }
 #pragma unroll
-            for (int i = 0; i < PIECES; i++)
+            for (int i = 0; i < 3; i++)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
                     o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[k & 1][dt], pc[k & 1][i], o[dt], 0, 0, 0);
@@ -704,9 +701,9 @@ __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVP
                 // the reads first, then a few of the weights' instructions behind each product
                 __builtin_amdgcn_sched_group_barrier(0x100, 2 * DT, 0);
 #pragma unroll
-                for (int i = 0; i < PIECES * DT; i++) {
+                for (int i = 0; i < 3 * DT; i++) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x402, PIECES == 2 ? 7 : 8, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, 8, 0);
                 }
             }
         }
@@ -877,11 +874,11 @@ __global__ void __launch_bounds__(256) k_kv_shared_join(const KVPool p, const Sh
     else *reinterpret_cast<bf16x4_any*>(static_cast<uint16_t*>(a.out) + to) = u32x2{bf16x2_out(v[0], v[1]), bf16x2_out(v[2], v[3])};
 }
 
-template <int DIM, Form FORM, int PIECES>
+template <int DIM, Form FORM>
 int launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr int LDS = Tiles<DIM <= 64 ? 64 : DIM <= 128 ? 128 : 256>::ALL;
-    const auto fn = k_kv_shared<DIM, FORM, PIECES>;
+    const auto fn = k_kv_shared<DIM, FORM>;
     if (LDS > 65536 && lds_optin(reinterpret_cast<const void*>(fn), LDS, done) != hipSuccess) {
         snx_set_error("kv_attention_shared: no %d bytes of LDS", LDS);
         return -1;
@@ -889,22 +886,21 @@ int launch(unsigned grid, const KVPool& p, const Shared& a, hipStream_t s) {
     fn<<<grid, 256, LDS, s>>>(p, a);
     return snx_launch_check("k_kv_shared");
 }
-template <int DIM, int PIECES>
+template <int DIM>
 int launch(unsigned grid, bool i8, const KVPool& p, const Shared& a, hipStream_t s) {
-    if (i8) return launch<DIM, INT8, PIECES>(grid, p, a, s);
+    if (i8) return launch<DIM, INT8>(grid, p, a, s);
     // (loads to LDS by 32-bit offsets count apart from LDS reads, those by address do not:
     // 64 rows behind 4096 tokens 30.9 us and 33.6)
     if constexpr (DIM != 96)
         if (p.dim == DIM && (uint64_t)p.pages * p.heads * p.page_size * DIM * 2 <= 0xFFFFFFFFull)
-            return launch<DIM, NEAR, PIECES>(grid, p, a, s);
-    return launch<DIM, FAR, PIECES>(grid, p, a, s);
+            return launch<DIM, NEAR>(grid, p, a, s);
+    return launch<DIM, FAR>(grid, p, a, s);
 }
-template <int PIECES>
 int launch(unsigned grid, bool i8, const KVPool& p, const Shared& a, hipStream_t s) {
-    if (p.dim <= 64) return launch<64, PIECES>(grid, i8, p, a, s);
-    if (p.dim <= 96) return launch<96, PIECES>(grid, i8, p, a, s);
-    if (p.dim <= 128) return launch<128, PIECES>(grid, i8, p, a, s);
-    return launch<256, PIECES>(grid, i8, p, a, s);
+    if (p.dim <= 64) return launch<64>(grid, i8, p, a, s);
+    if (p.dim <= 96) return launch<96>(grid, i8, p, a, s);
+    if (p.dim <= 128) return launch<128>(grid, i8, p, a, s);
+    return launch<256>(grid, i8, p, a, s);
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
@@ -1017,7 +1013,7 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     a.lift = (float)(room - kLag);
     a.out_f32 = out_f32;
     const bool i8 = c->dtype == SNEPPX_INT8;
-    if (out_f32 ? launch<3>((unsigned)grid, i8, p, a, S(st)) : launch<2>((unsigned)grid, i8, p, a, S(st))) return -1;
+    if (launch((unsigned)grid, i8, p, a, S(st))) return -1;
     // Few rows with much to add up: four waves for each query (48 rows of 4 heads and some 55
     // parts 21.8 to 18.7 us, one of 32 heads and 63 16.5 to 13.8; with up to 17 parts one
     // wave is better, 15.6 to 17.1, and with 2048 queries, 32.9 to 37.1).
