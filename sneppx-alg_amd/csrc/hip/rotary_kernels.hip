@@ -8,7 +8,7 @@
 // 8, 16 or 32 lanes have a head, eight of its elements each: of the part that turns
 // four pairs, so that nothing is exchanged but the sum of squares (and for int8 the
 // maximum).  The work is reading and writing every head once; what stands in its way is
-// the angles, four fp64 products and four sines and cosines to a lane, so a lane takes
+// the angles, four fp64 sines and cosines to a lane, so a lane takes
 // up to kMostHeads heads of a token with the angles of the first, all their loads in
 // flight over that.  2320 tokens of 40 heads of 128, normalised, take 12.3 us (48 MB read
 // and written, 4.9 TB/s behind the launch), into an int8 cache 14.3 (62 MB); 16 tokens 2.4,
@@ -50,6 +50,31 @@ struct Heads {
 
 constexpr int kMostHeads = 4;
 
+// Sine and cosine times m, both in fp64 and rounded to fp32 once.  The angle in turns,
+// without the whole ones (one rounding, by the product's own), then without the quarters:
+// what is left, x of up to pi / 4, goes into the series of Taylor up to x^13 and x^12, whose
+// next terms are below 2^-45 and 2^-41.  (An fp32 fraction with sines in fp32 is up to two units
+// of 2^-24 further off, which codes of an int8 cache next to a border show, and takes as
+// long: 2320 tokens 12.4 us so and 12.3; the library's fp64 sines 12.8, into an int8 cache
+// 15.3 against 14.5.)
+__device__ __forceinline__ void sine_cosine(double angle, double m, float& s, float& c) {
+    constexpr double by_turn = 0.15915494309189533577, turn = 6.28318530717958647693;
+    const double part = __builtin_fma(angle, by_turn, -__builtin_rint(angle * by_turn));
+    const double quarters = __builtin_rint(4.0 * part), x = turn * __builtin_fma(quarters, -0.25, part), y = x * x;
+    constexpr double of_sine[6] = {-1.0 / 6, 1.0 / 120, -1.0 / 5040, 1.0 / 362880, -1.0 / 39916800, 1.0 / 6227020800.0};
+    constexpr double of_cosine[6] = {-1.0 / 2, 1.0 / 24, -1.0 / 720, 1.0 / 40320, -1.0 / 3628800, 1.0 / 479001600};
+    double a = of_sine[5], b = of_cosine[5];
+#pragma unroll
+    for (int i = 4; i >= 0; i--) {
+        a = __builtin_fma(a, y, of_sine[i]);
+        b = __builtin_fma(b, y, of_cosine[i]);
+    }
+    const float s0 = (float)(__builtin_fma(a * y, x, x) * m), c0 = (float)(__builtin_fma(b, y, 1.0) * m);
+    const uint32_t q = (uint32_t)(int)quarters;
+    s = u2f(f2u((q & 1u) ? c0 : s0) ^ (q & 2u) << 30);
+    c = u2f(f2u((q & 1u) ? s0 : c0) ^ ((q + 1u) & 2u) << 30);
+}
+
 template <bool APPEND, bool I8, int LR, int HEADS>
 __global__ void __launch_bounds__(256) k_rotate(const KVPool p, const Heads n) {
     const uint32_t number = blockIdx.x * (256 / LR) + threadIdx.x / LR, t = n.by_groups(number);
@@ -86,12 +111,7 @@ __global__ void __launch_bounds__(256) k_rotate(const KVPool p, const Heads n) {
         const double f[4] = {f0[0], f0[1], f1[0], f1[1]};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            // in half turns, without the whole turns
-            const double turns64 = (double)pos * f[e] * 0.15915494309189533577;
-            const float half = 2.0f * (float)(turns64 - __builtin_rint(turns64));
-            sincospif(half, &sn[e], &cs[e]);
-            sn[e] *= n.magnitude;
-            cs[e] *= n.magnitude;
+            sine_cosine((double)pos * f[e], (double)n.magnitude, sn[e], cs[e]);
         }
     }
 
