@@ -245,8 +245,11 @@ __global__ void __launch_bounds__(256, FEW ? 4 : 2) k_kv_scores(const KVPool p, 
                 for (int g = 0; g < kHeadsAtOnce; g++) {
                     sum[g] = 0.0;
 #pragma unroll
-                    for (int k = 0; k < 8; k++)      // (lanes past the head's end have others' bounds)
-                        sum[g] += in ? 2.0 * x[g][k] * (double)(x[g][k] > 0.0 ? u[k] : l[k]) : 0.0;
+                    for (int k = 0; k < 8; k++) {
+                        // (a NaN of either stays: 0 * inf; lanes past the head's end have others' bounds)
+                        const double q = 2.0 * x[g][k], low = q * (double)l[k], high = q * (double)u[k];
+                        sum[g] += !in ? 0.0 : high > low || high != high ? high : low;
+                    }
                 }
                 s = row_sums64<LR>(sum);
             }

@@ -42,3 +42,20 @@ def test_infinite_bounds(lib, dim, group):
     b[16, :, 1, 1] = math.inf                    # (and all take this)
     for budget in (2, 10, 20, 28):
         check(lib, b.to(torch.bfloat16), q.to(torch.bfloat16).to(DEV), budget)
+
+
+@pytest.mark.parametrize("group", [1, 3, 7])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_zeros_of_a_query_against_infinite_bounds(lib, dim, group):
+    """0 * inf is NaN at either end, and ranks the page below every number."""
+    g = torch.Generator().manual_seed(dim)
+    pages = 30
+    b = torch.randn((pages, 1, 2, dim), generator=g).sort(2)[0]
+    q = torch.randn((1, group, dim), generator=g)
+    q[..., 5] = 0.0
+    b[3, :, 1, 5] = math.inf
+    b[7, :, 0, 5] = -math.inf
+    b[11, :, 1, 6] = math.inf              # (a number against infinity: infinite, and first)
+    b[13, :, 0, 5], b[13, :, 1, 5] = -math.inf, math.inf
+    for budget in (2, 10, 28, 29):
+        check(lib, b.to(torch.bfloat16), q.to(torch.bfloat16).to(DEV), budget)
