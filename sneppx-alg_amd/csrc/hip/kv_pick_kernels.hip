@@ -14,6 +14,7 @@
 
 #include "codec.h"
 #include "kv_pool.h"
+#include "kv_rows.h"
 #include "launch.h"
 #include "../snx_internal.h"
 
@@ -174,12 +175,17 @@ __device__ __forceinline__ double row_sums64(const double (&x)[4]) {
 // bounds
 //   max(q least, q largest) = q/2 (largest + least) + |q|/2 (largest - least),
 // two fp64 products and no choice, with the queries' conversions once for all pages (FEW:
-// up to four query heads); a page whose sum is not finite is summed up by the definition.
+// up to four query heads).  The end that a query does not take is in both sums and costs
+// bits where it is far the larger: a page with a lane whose second sum is beyond 2^20 of what
+// is left (below that 33 of 53 bits stand, and 24 are kept), or not finite, is summed up by
+// the definition.  (The sums apart need more registers than four waves a SIMD have, which
+// would spill 22: one row of 2048 pages 28.7 us with its attention, 30.4 with four waves, 16
+// of up to 1024 in int8 45 and 52.6; without that check and four waves 27.9 and 44.3.)
 // What bounds it: the bounds' bytes and, near them, fp64 conversions and products: 16 rows
-// of up to 1024 pages and 8 heads 14 us (38 MB, 2.7 TB/s), with fp32 sums 11.5; one row of
-// 2048 pages 6.3.
+// of up to 1024 pages and 8 heads 15 us (38 MB, 2.5 TB/s), with fp32 sums 11.5; one row of
+// 2048 pages 6.9.
 template <int LR, bool FEW>
-__global__ void __launch_bounds__(256, FEW ? 4 : 2) k_kv_scores(const KVPool p, const Pick a) {
+__global__ void __launch_bounds__(256, FEW ? 3 : 2) k_kv_scores(const KVPool p, const Pick a) {
     const uint32_t bh = blockIdx.y + blockIdx.z * 65535u;
     if (bh >= a.rows * p.heads) return;
     const uint32_t b = bh / p.heads, h = bh - b * p.heads;
@@ -193,73 +199,90 @@ __global__ void __launch_bounds__(256, FEW ? 4 : 2) k_kv_scores(const KVPool p, 
     uint32_t* const keys = a.keys + (size_t)bh * a.most;
 
     double x[kHeadsAtOnce][8];        // q / 2
+    auto query = [&](uint32_t g) {
+        const uint32_t j = g < a.group ? g : a.group - 1;
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if (in) w = *reinterpret_cast<const bf16x8_any*>(a.q + b * a.q_stride + (size_t)(h * a.group + j) * p.dim + d);
+        return w;
+    };
     auto queries = [&](uint32_t g0) {
 #pragma unroll
         for (int g = 0; g < kHeadsAtOnce; g++) {
-            const uint32_t j = g0 + g < a.group ? g0 + g : a.group - 1;
-            u32x4 w = {0u, 0u, 0u, 0u};
-            if (in) w = *reinterpret_cast<const bf16x8_any*>(a.q + b * a.q_stride + (size_t)(h * a.group + j) * p.dim + d);
             float q[8];
-            widen(w, q);
+            widen(query(g0 + g), q);
 #pragma unroll
             for (int k = 0; k < 8; k++) x[g][k] = (double)(0.5f * q[k]);
         }
     };
     u32x4 next_lo, next_hi;
-    auto fetch = [&](uint32_t page) {
+    auto fetch = [&](uint32_t page, u32x4& lo, u32x4& hi) {
         const uint16_t* const at = a.bounds + ((size_t)(page < p.pages ? page : 0) * p.heads + h) * 2 * p.dim + (in ? d : 0);
-        next_lo = *reinterpret_cast<const u32x4*>(at);
-        next_hi = *reinterpret_cast<const u32x4*>(at + p.dim);
+        lo = *reinterpret_cast<const u32x4*>(at);
+        hi = *reinterpret_cast<const u32x4*>(at + p.dim);
+    };
+    // a page's sums of four heads by the definition, from memory again
+    auto by_definition = [&](uint32_t page, uint32_t g0, double (&sum)[kHeadsAtOnce]) {
+        asm volatile("" : "+v"(page), "+v"(g0));       // (nothing is kept for it in registers)
+        u32x4 lo, hi;
+        fetch(page, lo, hi);
+#pragma unroll
+        for (int g = 0; g < kHeadsAtOnce; g++) {
+            float q[8], l[8], u[8];
+            widen(query(g0 + g), q);
+            widen(lo, l);
+            widen(hi, u);
+            sum[g] = 0.0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                // (a NaN of either stays: 0 * inf; lanes past the head's end have others' bounds)
+                const double low = (double)q[k] * (double)l[k], high = (double)q[k] * (double)u[k];
+                sum[g] += !in ? 0.0 : high > low || high != high ? high : low;
+            }
+        }
     };
     uint32_t page = (uint32_t)table[e], next = e + stride < have ? (uint32_t)table[e + stride] : 0u;
-    fetch(page);
+    fetch(page, next_lo, next_hi);
     if (FEW) queries(0);
 #pragma unroll 1
     for (; e < have; e += stride) {
         float l[8], u[8];
         widen(next_lo, l);
         widen(next_hi, u);
-        const bool there = page < p.pages;
+        const uint32_t seen = page;
         page = next;
         if (e + stride < have) {
-            fetch(page);
+            fetch(page, next_lo, next_hi);
             if (e + 2 * stride < have) next = (uint32_t)table[e + 2 * stride];
         }
         float best = -INFINITY;
 #pragma unroll 1
         for (uint32_t g0 = 0; g0 < (FEW ? 1u : a.group); g0 += kHeadsAtOnce) {
             if (!FEW) queries(g0);
-            double sum[kHeadsAtOnce] = {};
+            double sum[kHeadsAtOnce] = {}, wide[kHeadsAtOnce] = {};
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const double mid = (double)u[k] + (double)l[k], half = (double)u[k] - (double)l[k];
 #pragma unroll
                 for (int g = 0; g < kHeadsAtOnce; g++) {
                     sum[g] = __builtin_fma(x[g][k], mid, sum[g]);
-                    sum[g] = __builtin_fma(__builtin_fabs(x[g][k]), half, sum[g]);
+                    wide[g] = __builtin_fma(__builtin_fabs(x[g][k]), half, wide[g]);
                 }
             }
-            double s = row_sums64<LR>(sum);
-            if (__any(!(__builtin_fabs(s) < INFINITY))) {
+            bool fine = true;
 #pragma unroll
-                for (int g = 0; g < kHeadsAtOnce; g++) {
-                    sum[g] = 0.0;
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        // (a NaN of either stays: 0 * inf; lanes past the head's end have others' bounds)
-                        const double q = 2.0 * x[g][k], low = q * (double)l[k], high = q * (double)u[k];
-                        sum[g] += !in ? 0.0 : high > low || high != high ? high : low;
-                    }
-                }
-                s = row_sums64<LR>(sum);
+            for (int g = 0; g < kHeadsAtOnce; g++) {
+                sum[g] += wide[g];
+                fine &= wide[g] <= 0x1p20 * __builtin_fabs(sum[g]) && __builtin_fabs(sum[g]) < INFINITY;
             }
+            if (__any(!fine)) by_definition(seen, g0, sum);
+            const double s = row_sums64<LR>(sum);
             // the largest of the four heads (a NaN stays)
             float f = (float)s;
             f = largest_of(f, lane_step<0xB1, 0xf>(f, 0.0f));
             f = largest_of(f, lane_step<0x4E, 0xf>(f, 0.0f));
             best = largest_of(best, f);
         }
-        if (lane == 0) keys[e] = there ? score_key(best) : 0u;
+        if (lane == 0) keys[e] = seen < p.pages ? score_key(best) : 0u;
     }
 }
 

@@ -59,3 +59,19 @@ def test_zeros_of_a_query_against_infinite_bounds(lib, dim, group):
     b[13, :, 0, 5], b[13, :, 1, 5] = -math.inf, math.inf
     for budget in (2, 10, 28, 29):
         check(lib, b.to(torch.bfloat16), q.to(torch.bfloat16).to(DEV), budget)
+
+
+@pytest.mark.parametrize("group", [1, 3, 7])
+@pytest.mark.parametrize("dim", [8, 64, 128, 256])
+@pytest.mark.parametrize("power", [10, 30, 60, 100])
+def test_bounds_far_apart(lib, power, dim, group):
+    """Where a query takes the smaller end of a wide range, the other end does not count."""
+    g = torch.Generator().manual_seed(power + dim)
+    pages = 40
+    b = torch.randn((pages, 2, 2, dim), generator=g).sort(2)[0]
+    q = torch.randn((1, 2 * group, dim), generator=g)
+    # element 1 reaches far down, and all queries point up there; element 2 the other way
+    b[::2, :, 0, 1] = -(2.0 ** power)
+    b[::3, :, 1, 2] = 2.0 ** power
+    q[..., 1], q[..., 2] = q[..., 1].abs() + 0.1, -q[..., 2].abs() - 0.1
+    check(lib, b.to(torch.bfloat16), q.to(torch.bfloat16).to(DEV), 9)
