@@ -173,7 +173,7 @@ __device__ __forceinline__ double row_sums64(const double (&x)[4]) {
 // LR lanes a page, eight elements each; blockIdx.y (and z): row and head, whose pages the
 // workgroups of a row take in turn, so that all have the same of a short one.  For finite
 // bounds
-//   max(q least, q largest) = q/2 (largest + least) + |q|/2 (largest - least),
+//   max(q least, q largest) = q/2 (largest + least) + |q|/2 |largest - least|,
 // two fp64 products and no choice, with the queries' conversions once for all pages (FEW:
 // up to four query heads).  The end that a query does not take is in both sums and costs
 // bits where it is far the larger: a page with a lane whose second sum is beyond 2^20 of what
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(256, FEW ? 3 : 2) k_kv_scores(const KVPool p, 
 #pragma unroll
                 for (int g = 0; g < kHeadsAtOnce; g++) {
                     sum[g] = __builtin_fma(x[g][k], mid, sum[g]);
-                    wide[g] = __builtin_fma(__builtin_fabs(x[g][k]), half, wide[g]);
+                    wide[g] = __builtin_fma(__builtin_fabs(x[g][k]), __builtin_fabs(half), wide[g]);
                 }
             }
             bool fine = true;

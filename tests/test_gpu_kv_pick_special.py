@@ -75,3 +75,12 @@ def test_bounds_far_apart(lib, power, dim, group):
     b[::3, :, 1, 2] = 2.0 ** power
     q[..., 1], q[..., 2] = q[..., 1].abs() + 0.1, -q[..., 2].abs() - 0.1
     check(lib, b.to(torch.bfloat16), q.to(torch.bfloat16).to(DEV), 9)
+
+
+@pytest.mark.parametrize("dim", [64, 80])
+def test_bounds_in_no_order(lib, dim):
+    """Pages whose bounds were never written are ranked by what they hold, the larger product
+    of each element, whichever end it is of."""
+    g = torch.Generator().manual_seed(dim)
+    b, q = torch.randn((50, 2, 2, dim), generator=g), torch.randn((1, 6, dim), generator=g)
+    check(lib, b.to(torch.bfloat16), q.to(torch.bfloat16).to(DEV), 12)
