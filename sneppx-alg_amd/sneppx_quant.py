@@ -1130,19 +1130,27 @@ class KVPages(_OnDevice):
         self._p = refs.data_ptr()
         self._reserve, self._release, self._share = (lib.fn[f"SNEPPX_kv_{n}"] for n in ("reserve", "release", "share"))
 
+    # (memory of torch's current stream may still be in use there)
+    def _new(self, n, stream):
+        """int32 [n] of the memory of the stream that a call writes it on."""
+        if stream is None or self._index is None or stream == torch._C._cuda_getCurrentRawStream(self._index):
+            return torch.empty(n, dtype=torch.int32, device=self.device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
+            return torch.empty(n, dtype=torch.int32, device=self.device)
+
     def reserve(self, tables, lengths, slots, counts=None, next_pos=None, positions=None, starts=None, granted=None,
                 stream=None):
         """SNEPPX_kv_reserve: slots (and positions) int32 [tokens]; counts, next_pos,
-        granted int32 [rows], starts int32 [rows + 1].  Returns (starts, granted), new ones
-        where none are given."""
+        granted int32 [rows], starts int32 [rows + 1].  Returns (starts, granted), new ones of
+        the stream's memory where none are given."""
         tb, width, ln, n = self._tables(tables, lengths)
         if not isinstance(slots, torch.Tensor) or slots.dim() != 1:
             raise ValueError("slots must be an int32 tensor [tokens]")
         tokens, rows, int32, check = slots.shape, (n,), torch.int32, self._check
         if starts is None:
-            starts = torch.empty(n + 1, dtype=int32, device=self.device)
+            starts = self._new(n + 1, stream)
         if granted is None:
-            granted = torch.empty(n, dtype=int32, device=self.device)
+            granted = self._new(n, stream)
         st, gr = check(starts, "starts", int32, (n + 1,)), check(granted, "granted", int32, rows)
         sl, ps = check(slots, "slots", int32, tokens), None if positions is None else check(positions, "positions", int32, tokens)
         np_ = None if next_pos is None else check(next_pos, "next_pos", int32, rows)
