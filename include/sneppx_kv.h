@@ -136,7 +136,8 @@ int SNEPPX_kv_append_rotated(const SNEPPXKVCache* cache, const SNEPPXRotary* rot
  * page * page_size + offset, or -1 for tokens that are not granted, whose page is not
  * there, or past starts[rows]; positions (int32 [tokens], or NULL) the row's next_pos
  * (without it, its length) from before the call on, -1 for those not granted and past
- * the end.  With tokens below starts[rows] the others are left out. */
+ * the end.  With tokens below starts[rows] the others are left out.  None of these arrays
+ * overlaps another. */
 int SNEPPX_kv_reserve(int32_t* refs, size_t pages, size_t page_size, int32_t* block_tables, size_t table_width,
                       int32_t* lengths, int32_t* next_pos, const int32_t* counts, size_t rows, int32_t* starts,
                       int32_t* granted, int32_t* slots, int32_t* positions, size_t tokens, SNEPPXStream stream);
@@ -194,8 +195,9 @@ int SNEPPX_kv_key_bounds(const SNEPPXKVCache* cache, uint16_t* bounds, const int
  * there, rank below every number.  picked int32 [rows][kv_heads][budget]: the pages in the
  * order of the row, -1 behind the last; picked_lengths int32 [rows]: the tokens in them
  * (the row's last page is the last one picked).  A row of no more than `budget` pages has
- * them all.  q as in SNEPPX_kv_attention; max_length: no row is longer.  Scratch: a
- * workspace of the calling thread on `stream`. */
+ * them all.  picked and picked_lengths do not overlap what is read.  q as in
+ * SNEPPX_kv_attention; max_length: no row is longer.  Scratch: a workspace of the calling
+ * thread on `stream`. */
 int SNEPPX_kv_pick(const SNEPPXKVCache* cache, const uint16_t* bounds, const uint16_t* q, size_t q_stride,
                    size_t q_heads, const int32_t* block_tables, size_t table_width, const int32_t* lengths,
                    size_t rows, size_t max_length, size_t budget, size_t first, size_t recent, int32_t* picked,

@@ -25,10 +25,13 @@
 
 static int aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-static int overlap(const int32_t* a, const int32_t* b, size_t n) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b, bytes = n * sizeof(int32_t);
-    return a && b && x < y + bytes && y < x + bytes;
+/* of arrays of m and n entries */
+static int meet(const int32_t* a, size_t m, const int32_t* b, size_t n) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + n * sizeof(int32_t) && y < x + m * sizeof(int32_t);
 }
+
+static int overlap(const int32_t* a, const int32_t* b, size_t n) { return meet(a, n, b, n); }
 
 static int cache_ok(const char* who, const SNEPPXKVCache* c) {
     REQUIRE(c, "%s: NULL cache", who);
@@ -175,9 +178,13 @@ int SNEPPX_kv_reserve(int32_t* refs, size_t pages, size_t page_size, int32_t* bl
     REQUIRE(!rows || (starts && granted), "%s: NULL starts or granted", who);
     REQUIRE(!rows || !tokens || slots, "%s: NULL slots", who);
     REQUIRE(tokens <= MAX_SLOTS, "%s: %zu tokens are too many", who, tokens);
-    REQUIRE(!overlap(granted, counts, rows) && !overlap(granted, lengths, rows) && !overlap(granted, next_pos, rows) &&
-                !overlap(lengths, counts, rows) && !overlap(lengths, next_pos, rows) && !overlap(next_pos, counts, rows),
-            "%s: lengths, next_pos, counts and granted overlap", who);
+    /* (written while other threads still read, or what others write) */
+    const int32_t* const arrays[] = {lengths, next_pos, counts, granted, starts, slots, positions};
+    const size_t entries[] = {rows, rows, rows, rows, rows + 1, tokens, tokens};
+    for (int i = 1; i < 7; i++)
+        for (int j = 0; j < i; j++)
+            REQUIRE(!rows || !meet(arrays[i], entries[i], arrays[j], entries[j]),
+                    "%s: lengths, next_pos, counts, granted, starts, slots and positions must not overlap", who);
     snx_clear_error();
     if (!rows) return 0;
     return snx_k_kv_reserve(refs, pages, page_size, block_tables, table_width, lengths, next_pos, counts, rows, starts,
@@ -279,6 +286,10 @@ int SNEPPX_kv_pick(const SNEPPXKVCache* cache, const uint16_t* bounds, const uin
     REQUIRE(recent && recent <= budget && first <= budget - recent, "%s: first %zu and recent %zu (1 at least) do not fit the budget %zu",
             who, first, recent, budget);
     REQUIRE(!overlap(picked_lengths, lengths, rows), "%s: picked_lengths must not be lengths, nor overlap them", who);
+    const size_t all = rows * cache->kv_heads * budget;
+    REQUIRE(!rows || !(meet(picked, all, block_tables, rows * table_width) || meet(picked, all, lengths, rows) ||
+                       meet(picked, all, picked_lengths, rows) || meet(picked_lengths, rows, block_tables, rows * table_width)),
+            "%s: picked and picked_lengths must not overlap block_tables, lengths or one another", who);
     snx_clear_error();
     if (!rows) return 0;
     const size_t slots = table_width * cache->page_size;
