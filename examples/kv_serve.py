@@ -25,8 +25,9 @@ I32, BF16 = torch.int32, torch.bfloat16
 
 class ServeBlock:
     """Row 0 holds the common prompt and does not decode; rows 1 .. rows - 1 are
-    streams.  The host keeps how long each row is (`held`), which it needs for the
-    launches alone: lengths, tables and free pages stay on the device."""
+    streams.  The host keeps how long each row is (`held`) and how much of the prompt it
+    shares, which it needs for the launches alone: lengths, tables and free pages stay on
+    the device."""
 
     def __init__(self, lib, rows, pages, width, hidden=4096, q_heads=32, kv_heads=8, dim=128, page=16, dtype="bf16",
                  pick=0, seed=0, device="cuda"):
@@ -43,8 +44,8 @@ class ServeBlock:
         ints = lambda *shape: torch.zeros(shape, dtype=I32, device=device)  # noqa: E731
         self.tables = ints(rows, width) - 1
         self.lengths, self.next_pos, self.granted, self.starts = ints(rows), ints(rows), ints(rows), ints(rows + 1)
-        self.groups, self.prefix = torch.tensor([1, rows], dtype=I32, device=device), ints(1)
-        self.held, self.common = [0] * rows, 0
+        self.held, self.common, self.shared = [0] * rows, 0, [0] * rows
+        self._group()
         if pick:
             self.bounds = torch.zeros((pages, kv_heads, 2, dim), dtype=BF16, device=device)
             self.picked, self.picked_lengths = ints(rows, kv_heads, pick), ints(rows)
@@ -82,13 +83,20 @@ class ServeBlock:
             self.cache.key_bounds(self.bounds, self.tables, self.lengths, self.counts, max(counts))
         return q
 
+    def _group(self):
+        """Streams next to one another that share as much of the prompt are a group."""
+        mine = self.shared
+        first = [b for b in range(1, self.rows) if b == 1 or mine[b] != mine[b - 1]]
+        self.groups = torch.tensor([b - 1 for b in first] + [self.rows - 1], dtype=I32).to(self.tables.device)
+        self.prefix = torch.tensor([mine[b] for b in first], dtype=I32).to(self.tables.device)
+
     def share(self, rows):
         """Has rows begin with row 0's prompt, as far as it fills pages."""
         self.common = self.held[0] // self.page * self.page
         sources = torch.tensor([0 if b in rows else -1 for b in range(self.rows)], dtype=I32).to(self.tables.device)
         self.free.share(self.tables, self.lengths, sources, torch.full_like(sources, self.common), next_pos=self.next_pos)
-        self.prefix.fill_(self.common)
-        self.held = [self.common if b in rows else n for b, n in enumerate(self.held)]
+        self.held, self.shared = ([self.common if b in rows else n for b, n in enumerate(x)] for x in (self.held, self.shared))
+        self._group()
 
     def end(self, rows):
         """Rows that have ended give their pages back."""
@@ -96,7 +104,8 @@ class ServeBlock:
         for t in (self.lengths, self.next_pos):
             t.masked_fill_(gone, 0)
         self.free.release(self.tables, self.lengths)
-        self.held = [0 if b in rows else n for b, n in enumerate(self.held)]
+        self.held, self.shared = ([0 if b in rows else n for b, n in enumerate(x)] for x in (self.held, self.shared))
+        self._group()
 
     def step(self, x):
         """One new token of each stream, x [rows, hidden] (row 0 is not looked at);
@@ -108,8 +117,8 @@ class ServeBlock:
             self.cache.pick(q, self.bounds, tables, lengths, longest, self.picked[1:], self.picked_lengths[1:], 1, 2)
             self.cache.attention_picked(q, out, self.picked[1:], self.picked_lengths[1:])
         else:
-            self.cache.attention_shared(q, out, tables, lengths, longest, self.groups - 1, self.prefix, self.common,
-                                        longest - self.common)
+            self.cache.attention_shared(q, out, tables, lengths, longest, self.groups, self.prefix, max(self.shared),
+                                        max(n - s for n, s in zip(self.held[1:], self.shared[1:])))
         qw, sc, qz = self.o_w
         self.lib.qlinear_w4a16(self.out.flatten(1), qw, sc, qz, None, sc.shape[1], self.y, 128)
         return self.y
