@@ -25,6 +25,7 @@
 #include <cstdint>
 
 #include "codec.h"
+#include "kv_pieces.h"
 #include "kv_pool.h"
 #include "launch.h"
 #include "../snx_internal.h"
@@ -33,10 +34,7 @@ using namespace snx;
 
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 // of any alignment that their elements have
@@ -193,16 +191,6 @@ struct Division {
 };
 
 // max / sum over the four lanes that differ in bits 4 and 5
-__device__ __forceinline__ float swap32(float x, float& y) {
-    const u32x2 r = __builtin_amdgcn_permlane32_swap(f2u(x), f2u(x), false, false);
-    y = u2f(r[1]);
-    return u2f(r[0]);
-}
-__device__ __forceinline__ float swap16(float x, float& y) {
-    const u32x2 r = __builtin_amdgcn_permlane16_swap(f2u(x), f2u(x), false, false);
-    y = u2f(r[1]);
-    return u2f(r[0]);
-}
 __device__ __forceinline__ float quad_max(float x) {
     float y;
     x = swap32(x, y);
@@ -216,48 +204,6 @@ __device__ __forceinline__ float quad_sum(float x) {
     x += y;
     x = swap16(x, y);
     return x + y;
-}
-
-// eight int8 as bf16 (exact)
-__device__ __forceinline__ bf16x8 bytes_to_bf16(uint32_t a, uint32_t b) {
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint32_t w = i ? b : a;
-        const float f0 = (float)(int8_t)w, f1 = (float)(int8_t)(w >> 8);
-        const float f2 = (float)(int8_t)(w >> 16), f3 = (float)(int8_t)(w >> 24);
-        o[2 * i] = __builtin_amdgcn_perm(f2u(f1), f2u(f0), 0x07060302u);
-        o[2 * i + 1] = __builtin_amdgcn_perm(f2u(f3), f2u(f2), 0x07060302u);
-    }
-    return __builtin_bit_cast(bf16x8, o);
-}
-
-// Eight weights (not negative) as three bf16 pieces each, exactly (24 significant
-// bits cut into 8 + 8 + 8): the products with bf16 values then sum as fp32 ones
-// would.  bf16 values may be infinite, and a zero second or third piece would make
-// NaN of that: they are 2^-40 of the first at least (and normal), which no sum
-// shows, but zero where the weight is zero, so that a token of no weight adds
-// nothing to any value.  Of int8 the codes are finite; where the weight is not (an
-// infinite scale) it is all in the first piece.
-template <bool I8>
-__device__ __forceinline__ void split3(const float (&x)[8], bf16x8 (&piece)[3]) {
-    u32x4 o[3];
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-        float a[2] = {x[e], x[e + 1]}, least[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-            o[i][e >> 1] = __builtin_amdgcn_perm(f2u(a[1]), f2u(a[0]), 0x07060302u);
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const float high = u2f(f2u(a[j]) & 0xFFFF0000u);
-                if (!I8 && i == 0) least[j] = __builtin_amdgcn_fmed3f(high, high * 0x1p-40f, 0x1p-126f);
-                a[j] = fmaxf(a[j] - high, least[j]);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 3; i++) piece[i] = __builtin_bit_cast(bf16x8, o[i]);
 }
 
 // A wave's value tile in LDS: token rows of RB bytes.  The transposed reads take
@@ -535,7 +481,7 @@ k_kv_attn(const KVPool p, const Attn a) {
                     // (or the compiler converts when it loads, and keeps twice the registers)
                     if (I8) asm volatile("" : "+v"(w));
                     bf16x8 kf;
-                    if (I8) kf = (i & 1) ? bytes_to_bf16(w[2], w[3]) : bytes_to_bf16(w[0], w[1]);
+                    if (I8) kf = __builtin_bit_cast(bf16x8, (i & 1) ? bytes_to_bf16(w[2], w[3]) : bytes_to_bf16(w[0], w[1]));
                     else kf = __builtin_bit_cast(bf16x8, w);
                     // past the head's end the lane has other elements, maybe NaN
                     if (!FULL && (I8 ? 16 * (g + 4 * (i >> 1)) : 8 * (g + 4 * i)) >= (int)dim)
@@ -629,7 +575,7 @@ k_kv_attn(const KVPool p, const Attn a) {
                     const int tok = 8 * g + (r >> 1);
                     const lds_t at = (lds_t)(vt + L::row(tok) + 8 * (r & 1) + 16 * dt);
                     const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)at);
-                    vf = bytes_to_bf16((uint32_t)w[0], (uint32_t)w[1]);
+                    vf = __builtin_bit_cast(bf16x8, bytes_to_bf16((uint32_t)w[0], (uint32_t)w[1]));
                 } else {
                     s16x4 w[2];
 #pragma unroll
