@@ -152,7 +152,8 @@ int SNEPPX_kv_release(int32_t* refs, size_t pages, size_t page_size, int32_t* bl
  * first counts[r] / page_size entries of row sources[r] (whole pages within that row's
  * length), each one's refs one more, and gives back what its own entries there named;
  * its length becomes what it took, and so does next_pos (or NULL).  Other rows are
- * left as they are, as is a row whose source is itself or takes pages in this call. */
+ * left as they are, as is a row whose source is itself, or has a source of its own among
+ * the other rows in this call (whether or not it takes pages by it). */
 int SNEPPX_kv_share(int32_t* refs, size_t pages, size_t page_size, int32_t* block_tables, size_t table_width,
                     int32_t* lengths, int32_t* next_pos, const int32_t* sources, const int32_t* counts, size_t rows,
                     SNEPPXStream stream);
@@ -162,11 +163,15 @@ int SNEPPX_kv_share(int32_t* refs, size_t pages, size_t page_size, int32_t* bloc
  * same pages, which are read once for a group and not once for each row.
  * group_starts int32 [groups + 1] (ascending): group g is the rows group_starts[g] ..
  * group_starts[g + 1], and their first prefix_lengths[g] tokens (int32 [groups]) are
- * the same, read once by the table of its first row that is as long.  Rows of no group,
- * and rows shorter than their group's prefix, read all their tokens by themselves.
- * max_length: no row is longer; max_prefix and max_own: about the longest prefix, and
- * the most tokens that a row has behind its prefix (they size the launch; results do not
- * depend on them but for the rounding).  Scratch: a workspace of the calling thread on
+ * the same, read once by the table of its first row that is as long; a row is in one
+ * group at most, and there are no more groups than rows.  Rows of no group, and rows
+ * shorter than their group's prefix, read all their tokens by themselves.  max_length: no
+ * row is longer; max_prefix and max_own: about the longest prefix, and the most tokens that
+ * a row reads by itself, behind its prefix or all of them.  The last two size the launch:
+ * results depend on them by their rounding only, but the time does, for what a row reads
+ * by itself beyond max_own is read by one wave for each key-value head and 16 query heads
+ * (16 rows behind 16384 tokens 26 us; with one of them a token shorter than that 900 with a
+ * max_own of 128 and 137 with one of 16384).  Scratch: a workspace of the calling thread on
  * `stream`. */
 int SNEPPX_kv_attention_shared(const SNEPPXKVCache* cache, const uint16_t* q, size_t q_stride, void* out,
                                size_t out_stride, SNEPPXDtype out_dtype, const int32_t* block_tables,
@@ -183,7 +188,8 @@ int SNEPPX_kv_attention_shared(const SNEPPXKVCache* cache, const uint16_t* q, si
 /* Renews the bounds of the pages that the last counts[row] (NULL: one) tokens of each
  * row are in, from all tokens of the row in them.  max_count: no count is larger.  Keys
  * count as the cache gives them back (int8: code * scale in fp32, rounded to bf16); a
- * NaN makes both bounds of its element NaN. */
+ * NaN makes both bounds of its element NaN.  Rows that share a page here have the same
+ * number of tokens in it. */
 int SNEPPX_kv_key_bounds(const SNEPPXKVCache* cache, uint16_t* bounds, const int32_t* block_tables,
                          size_t table_width, const int32_t* lengths, const int32_t* counts, size_t max_count,
                          size_t rows, SNEPPXStream stream);
@@ -191,7 +197,8 @@ int SNEPPX_kv_key_bounds(const SNEPPXKVCache* cache, uint16_t* bounds, const int
 /* Picks `budget` pages of each row and key-value head: the first `first` and last
  * `recent` of the row's pages (recent >= 1, first + recent <= budget), and the others by
  * their score: the largest sum above over the query heads of the key-value head, taken in
- * fp64 and rounded to fp32.  Of equal ones the earlier page; a NaN, and a page that is not
+ * fp64 and rounded to fp32 (a product of either bound that is NaN, 0 * inf too, makes it
+ * NaN).  Of equal ones the earlier page; a NaN, and a page that is not
  * there, rank below every number.  picked int32 [rows][kv_heads][budget]: the pages in the
  * order of the row, -1 behind the last; picked_lengths int32 [rows]: the tokens in them
  * (the row's last page is the last one picked).  A row of no more than `budget` pages has

@@ -9,8 +9,9 @@
  * for the dims / 2 pairs (a, b) of the head's first `dims` elements, by the angle
  * position * freqs[pair]; the elements behind them are left as they are.  Angles
  * and their sines and cosines are taken in fp64 (a position of 10^6 has no fraction of a
- * turn left in fp32) and rounded to fp32 with the magnitude; everything else is fp32, with
- * one rounding at the end.
+ * turn left in fp32) and rounded to fp32 with the magnitude; everything else is fp32
+ * (elements whose squares pass its range, from 10^19 on, have an infinite mean), with one
+ * rounding at the end.
  *
  * The reference has rotary positions on the CPU (SNEPPX_rope_precompute, called at
  * kernel/inference/inference_engine.c:247).

@@ -189,8 +189,9 @@ struct OwnTile {
 // row r being token 8 (r / 4) + 4 t + r % 4 of 32, a lane's weights are those of tokens
 // 8 g .. 8 g + 7, the B operand of the product with the values.  Keys and values of the
 // next 32 tokens are on their way meanwhile, keys into the registers that the first product
-// has used, values into those that went to LDS.  64 rows of 512 tokens and 8 heads run at 5.4
-// TB/s, of 0 to 512 at 4.2.
+// has used, values into those that went to LDS.  64 rows of 512 tokens and 8 heads (134 MB)
+// take 27 us, of 0 to 512 (67 MB) 20: spans are cut by the longest row that the host allows
+// for, not by what rows have, so the longest wave has twice an equal share.
 template <int DP, bool I8>
 __device__ __forceinline__ void own_queries(const KVPool& p, const Shared& a, uint32_t b, uint32_t head0, uint32_t nq,
                                             bf16x8 (&q)[DP / 32]) {
@@ -376,8 +377,7 @@ __device__ __forceinline__ void own_tokens(const KVPool& p, const Shared& a, uin
 // other side of a rounding: 256 rows behind 16384 tokens take 154 us with three pieces and
 // 125 with two, 64 behind 4096 33.4 and 32.7.)
 // DIM: the head's elements that products are made of, DP those of a row in LDS (heads of 80,
-// 256 rows behind 16384 tokens: 109 us with products of 128 elements, 98 of 96, both with
-// two pieces of a weight; 140 of 96 with three).
+// 256 rows behind 16384 tokens: 135 us with products of 128 elements, 122 of 96).
 template <int DIM, Form FORM>
 __global__ void __launch_bounds__(256, DIM <= 128 ? 2 : 1) k_kv_shared(const KVPool p, const Shared a) {
     constexpr int DP = DIM <= 64 ? 64 : DIM <= 128 ? 128 : 256;
@@ -832,7 +832,7 @@ template <int DIM>
 int launch(unsigned grid, bool i8, const KVPool& p, const Shared& a, hipStream_t s) {
     if (i8) return launch<DIM, INT8>(grid, p, a, s);
     // (loads to LDS by 32-bit offsets count apart from LDS reads, those by address do not:
-    // 64 rows behind 4096 tokens 30.9 us and 33.6)
+    // 64 rows behind 4096 tokens 32.1 us and 36.7)
     if constexpr (DIM != 96)
         if (p.dim == DIM && (uint64_t)p.pages * p.heads * p.page_size * DIM * 2 <= 0xFFFFFFFFull)
             return launch<DIM, NEAR>(grid, p, a, s);
@@ -863,16 +863,16 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     const size_t own_tiles = (group + 15) / 16;
     const size_t places = (size_t)(c->head_dim <= 128 ? 2 : 1) * cu_count();      // of workgroups that run at once
     // Own tokens by about 1024 waves, which all run at once (64 rows behind 4096 tokens with up
-    // to 512 of their own 30.5 us so, by 2048 36.7).
+    // to 512 of their own 32.1 us so, by 2048 35.4).
     size_t own_span = rows * c->kv_heads * own_tiles * max_own / 1024 / 32 * 32;
     if (own_span < 64) own_span = 64;
     size_t splits = (max_own + own_span - 1) / own_span;
     if (splits < 1) splits = 1;
     // A prefix of up to ten steps a step to each workgroup, of twice that two, of more three:
     // a span's steps follow one another, but all of them are joined (20 rows behind 500
-    // tokens 15.5 with spans of three, 13.6 of one; five prefixes of up to 8192 18.7 and 19.8).
-    // Steps of heads beyond 128 are twice as long: one of up to 40, else two (2 rows behind
-    // 2217 tokens 23.3 with three, 17.2 so; behind 5052 21.1, 17.8 and with one 19.3).
+    // tokens 15.3 with spans of three, 13.4 of one; five prefixes of up to 8192 17.6 and 19.4).
+    // Steps of heads beyond 128 are twice as long: one of up to 40, else two (2 rows and one
+    // key-value head behind 2217 tokens 19.4 with three, 17.7 so; behind 5052 21.0 and 17.4).
     const bool large = c->head_dim > 128;
     size_t least = large ? (prefix_steps + 39) / 40 : (prefix_steps + 9) / 10;
     const size_t most_least = large ? 2 : kLeast;
@@ -880,9 +880,11 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     // As many spans of a prefix as make the launch shortest, by a count of what runs one after
     // the other in the CUs' places, in steps (3 us): units of `per` steps and one to begin
     // with, rows' own tokens 40 to a step, in places that units leave free or behind them,
-    // and parts, written and read again.  Against as many units as places, shared out by the
-    // two kinds' work: 112 rows behind 4125 tokens, heads of 256, 64 to 52 us, 32 behind
-    // 2048 with up to 1024 of their own 28.4 to 26.1; 20 prefixes of 5 rows 27.7 to 30.4.
+    // and parts, written and read again, at 4.4 TB/s.  (These numbers were chosen among others
+    // by timing fifteen calls of 4 to 256 rows.)  Against as many units as places, shared out by the two kinds' work: 112 rows behind 4125 tokens,
+    // heads of 256, 77 to 68 us, 64 behind 8192 83 to 61, 32 of 128 behind 2048 with up to
+    // 1024 of their own 29.2 to 27.4; what it loses: 20 prefixes of 5 rows 29.8 to 31.0, 64
+    // rows behind 4096 31.7 to 32.5.
     const size_t few = groups ? (rows * group + TILE - 1) / TILE : 0;    // tiles of groups that fill them
     const size_t about_tiles = few > groups ? few : groups;
     const size_t own_wgs = (rows * c->kv_heads * own_tiles * splits + 3) / 4;
@@ -957,8 +959,8 @@ int snx_k_kv_attention_shared(const SNEPPXKVCache* c, const uint16_t* q, size_t 
     const bool i8 = c->dtype == SNEPPX_INT8;
     if (launch((unsigned)grid, i8, p, a, S(st))) return -1;
     // Few rows with much to add up: four waves for each query (48 rows of 4 heads and some 55
-    // parts 21.8 to 18.7 us, one of 32 heads and 63 16.5 to 13.8; with up to 17 parts one
-    // wave is better, 15.6 to 17.1, and with 2048 queries, 32.9 to 37.1).
+    // parts 20.0 to 17.7 us, one of 32 heads and 44 17.0 to 15.9; with up to 17 parts one
+    // wave is better, 13.5 to 15.1, and with 2048 queries, 32.2 to 36.5).
     const size_t most = (prefix_steps + least - 1) / least, parts = (few && about / few < most ? about / few : most) + splits;
     if (rows * q_heads <= 1024 && parts > 32) k_kv_shared_join<4><<<(unsigned)(rows * q_heads), 256, 0, S(st)>>>(p, a);
     else k_kv_shared_join<1><<<(unsigned)((rows * q_heads + 3) / 4), 256, 0, S(st)>>>(p, a);
