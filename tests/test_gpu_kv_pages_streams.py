@@ -45,3 +45,21 @@ def test_the_current_stream_by_its_number(lib):
         torch.cuda.synchronize()
         assert starts.tolist() == [0, 1, 2] and granted.tolist() == [1, 1]
     assert lengths.tolist() == [3, 3]
+
+
+def test_recorded_without_outputs_of_the_callers(lib):
+    """A stream that nothing was allocated for: nothing is allocated while it is recorded
+    that the recording could not bear."""
+    p = lib.kv_pages(80, 4)
+    tables, lengths = torch.full((2, 9), -1, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    slots, st = torch.zeros(2, dtype=torch.int32, device=DEV), torch.cuda.Stream()
+    spare = [torch.empty(3, dtype=torch.int32, device=DEV) for _ in range(4)]
+    del spare
+    torch.cuda.synchronize()
+    kept = []
+    graph = lib.capture(lambda: kept.append(p.reserve(tables, lengths, slots, stream=st.cuda_stream)), stream=st.cuda_stream)
+    for i in range(1, 6):
+        lib.graph_launch(graph, stream=st.cuda_stream)
+        torch.cuda.synchronize()
+        assert lengths.tolist() == [i, i] and kept[0][0].tolist() == [0, 1, 2] and kept[0][1].tolist() == [1, 1]
+    lib.graph_destroy(graph)
