@@ -11,8 +11,8 @@
 // the angles, four fp64 sines and cosines to a lane, so a lane takes
 // up to kMostHeads heads of a token with the angles of the first, all their loads in
 // flight over that.  2320 tokens of 40 heads of 128, normalised, take 12.3 us (48 MB read
-// and written, 4.9 TB/s behind the launch), into an int8 cache 14.3 (62 MB); 16 tokens 2.4,
-// a chain of position, angle, head and result.
+// and written, 4.9 TB/s behind the launch), into an int8 cache 14.5 (62 MB); 16 tokens 2.3
+// in a graph, a chain of position, angle, head and result.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -191,9 +191,9 @@ __global__ void __launch_bounds__(256) k_rotate(const KVPool p, const Heads n) {
 
 template <bool APPEND, bool I8, int LR>
 int launch(const KVPool& p, Heads& n, hipStream_t s, const char* who) {
-    // Four heads to a lane where that leaves every CU eight waves: 16 tokens of 40 heads 2.35
-    // us with one and 3.4 with four, 600 of them 4.7 either way, 1200 9.6 and 8.7, 2320 15.6
-    // and 13.2 (8 heads to a lane as 4).
+    // Four heads to a lane where that leaves every CU eight waves: in a graph 16 tokens of 40
+    // heads take 2.3 us with one and 3.4 with four, 600 of them 4.9 and 4.6, 1200 7.8 and 6.2,
+    // 2320 13.0 and 9.9 (8 heads to a lane as 4).
     const size_t waves = (size_t)n.tokens * n.heads * LR / 64;
     const int per = waves >= 2048 * kMostHeads ? kMostHeads : 1;
     n.groups = (n.heads + per - 1) / per;
