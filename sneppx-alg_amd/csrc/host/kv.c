@@ -28,7 +28,7 @@ static int aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 /* of arrays of m and n entries */
 static int meet(const int32_t* a, size_t m, const int32_t* b, size_t n) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && x < y + n * sizeof(int32_t) && y < x + m * sizeof(int32_t);
+    return a && b && m && n && x < y + n * sizeof(int32_t) && y < x + m * sizeof(int32_t);
 }
 
 static int overlap(const int32_t* a, const int32_t* b, size_t n) { return meet(a, n, b, n); }

@@ -3,6 +3,7 @@ read, before they touch the device.  CPU only (the pointers are never dereferenc
 import ctypes as C
 
 import pytest
+import torch
 
 from test_kv_serve_args import L, pick, reserve  # noqa: F401
 
@@ -23,6 +24,13 @@ def test_reserve(L, a, b):  # noqa: F811
     for to in (AT[b], AT[b] + 4 * (ENTRIES[b] - 1), AT[b] - 4 * (ENTRIES[a] - 1)):
         assert reserve(L, tokens=5, **args(**{a: to})) == -1
         assert "overlap" in L.last_error()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the call goes on to a launch, which only a machine without a GPU refuses")
+def test_arrays_of_no_entries_meet_nothing(L):  # noqa: F811
+    """No tokens: where slots and positions would be does not matter."""
+    assert reserve(L, tokens=0, **args(slots=AT["counts"] + 4, pos=AT["starts"] + 4)) == -1
+    assert "overlap" not in L.last_error()
 
 
 def test_pick(L):  # noqa: F811
