@@ -122,7 +122,9 @@ int SNEPPX_kv_append_rotated(const SNEPPXKVCache* cache, const SNEPPXRotary* rot
  * and -1 in every entry of its block tables.)  The three calls below change refs,
  * block tables and lengths in the order of the stream, without asking the device, so a
  * program can record them into a graph together with the rest of a step.  A row holds
- * the pages that its table names; an entry outside [0, pages) names none. */
+ * the pages that its table names; an entry outside [0, pages) names none.  Tokens go into
+ * the pages that a row holds behind its length before it is given others, so what it shares
+ * there (a row cut, or begun anew by kv_share) is given back by kv_release first. */
 
 /* Room for new tokens: counts int32 [rows] of them for each row (NULL: one each; below
  * 0 counts as 0), behind its lengths[row].  Entries of the table that they need beyond
@@ -188,7 +190,8 @@ int SNEPPX_kv_attention_shared(const SNEPPXKVCache* cache, const uint16_t* q, si
 /* Renews the bounds of the pages that the last counts[row] (NULL: one) tokens of each
  * row are in, from all tokens of the row in them.  max_count: no count is larger.  Keys
  * count as the cache gives them back (int8: code * scale in fp32, rounded to bf16); a
- * NaN makes both bounds of its element NaN.  Rows that share a page here have the same
+ * NaN makes both bounds of its element NaN.  An eviction moves tokens between pages: what
+ * a row has left is renewed behind it (counts of the new lengths).  Rows that share a page here have the same
  * number of tokens in it. */
 int SNEPPX_kv_key_bounds(const SNEPPXKVCache* cache, uint16_t* bounds, const int32_t* block_tables,
                          size_t table_width, const int32_t* lengths, const int32_t* counts, size_t max_count,
