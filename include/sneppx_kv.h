@@ -191,8 +191,8 @@ int SNEPPX_kv_attention_shared(const SNEPPXKVCache* cache, const uint16_t* q, si
  * row are in, from all tokens of the row in them.  max_count: no count is larger.  Keys
  * count as the cache gives them back (int8: code * scale in fp32, rounded to bf16); a
  * NaN makes both bounds of its element NaN.  An eviction moves tokens between pages: what
- * a row has left is renewed behind it (counts of the new lengths).  Rows that share a page here have the same
- * number of tokens in it. */
+ * a row has left is renewed behind it (counts of the new lengths).  Rows that share a page
+ * here have the same number of tokens in it. */
 int SNEPPX_kv_key_bounds(const SNEPPXKVCache* cache, uint16_t* bounds, const int32_t* block_tables,
                          size_t table_width, const int32_t* lengths, const int32_t* counts, size_t max_count,
                          size_t rows, SNEPPXStream stream);
